@@ -38,7 +38,9 @@ enum {
 
 /* ---- element types of activations ---------------------------------------------------------- */
 enum { MSNH_B200_F32 = 0,  /* fp32 storage, tf32 tensor-core contraction, fp32 accumulate       */
-       MSNH_B200_F16 = 1 };/* fp16 storage, fp16 tensor-core contraction, fp32 accumulate       */
+       MSNH_B200_F16 = 1,  /* fp16 storage, fp16 tensor-core contraction, fp32 accumulate       */
+       MSNH_B200_BF16 = 2, /* token operators only                                              */
+       MSNH_B200_E4M3 = 3 };/* token operators only: 8 bits (4 exponent, 3 mantissa, no infinity, largest 448) */
 
 /* ---- activations: same set and formulas as include/Msnhnet/layers/MsnhActivations.h:39-168 -- */
 enum {
@@ -320,6 +322,126 @@ int  msnh_b200_yolo_collect_static(const float *dev_decoded, int n_images, int g
                                    int max_rows_per_image, int *dev_counts, void *stream);
 /* Text of the last failure of msnh_b200_yolo_collect_static on this thread (static buffer). */
 const char *msnh_b200_static_last_error(void);
+
+/* ---- operators for decoding tokens --------------------------------------------------------------
+ * No counterpart in the reference, which answers with classes and boxes. For programs that read a net's features out as
+ * tokens (captions, text in images): the norm, products and attention of one decoding step and the cache it reads.
+ * All of them work on device memory of the caller and enqueue on the caller's stream (NULL = the legacy stream): no
+ * allocation, no synchronisation, so they can be captured in a CUDA graph. Text of a failure: msnh_b200_last_error.
+ * Strides are in elements; where a struct names none, rows lie one behind the other. Memory of the call must stay valid
+ * until the stream has passed it. Two calls may run at the same time on two streams if neither writes what the other uses.
+ * A call with nothing to do (no rows, no sequences) returns MSNH_B200_OK. */
+
+/* y = h * rsqrt(mean(h^2) + eps) * weight, h = x + residual (x alone without a residual), over rows of `cols` values.
+ * h is held in fp32; residual_out (may be NULL; may be x's or the residual's memory) receives it rounded to `dtype`.
+ * out_dtype = dtype, or MSNH_B200_E4M3: y_scale[row] = max|y| / 448 and y holds y / y_scale to the nearest (ties to even);
+ * a row of zeros has scale 0 and codes 0, a row whose y is not finite scale NaN and codes 0. y may be x's, the residual's or
+ * residual_out's memory only where types and strides agree (y then overwrites what lay there). */
+typedef struct MsnhB200RmsNorm {
+    const void *x, *residual, *weight;
+    void *residual_out, *y;
+    float *y_scale;                    /* rows values; for out_dtype MSNH_B200_E4M3 only           */
+    int64_t rows;
+    int32_t cols;
+    int32_t dtype;                     /* of x, residual, residual_out: F32, F16, BF16             */
+    int32_t weight_dtype;              /* dtype or F32                                             */
+    int32_t out_dtype;
+    int64_t x_stride, residual_stride, residual_out_stride, y_stride;
+    float   eps;
+} MsnhB200RmsNorm;
+int  msnh_b200_rms_norm(MsnhB200Ctx *ctx, const MsnhB200RmsNorm *args, void *stream);
+
+/* Products with 4-bit weights. A weight row n of k values is stored as codes 0..15 with a scale and a zero point for every
+ * `group` values (a multiple of 32; the last group may be shorter): w = (code - zero) * scale, zero = 8 without `zeros`.
+ * w4_pack lays codes, scales and zeros out as the kernels read them, once, into `packed` (w4_pack_bytes of them, 16-byte
+ * aligned):
+ *   codes  : [n][codes_stride] bytes, value 2i in the low and 2i+1 in the high half of byte i
+ *   scales : [n][ceil(k / group)], F16, BF16 or F32;  zeros : the same shape, one byte each, values 0..15 (or NULL) */
+typedef struct MsnhB200W4 {
+    const void *packed;
+    int32_t n, k, group;
+    int32_t scale_dtype;               /* as given to w4_pack                                      */
+    int32_t has_zeros;
+} MsnhB200W4;
+int  msnh_b200_w4_pack_bytes(MsnhB200Ctx *ctx, const MsnhB200W4 *weights, size_t *bytes);
+int  msnh_b200_w4_pack(MsnhB200Ctx *ctx, const MsnhB200W4 *weights, const uint8_t *codes, int64_t codes_stride, const void *scales,
+                       const uint8_t *zeros, void *packed, void *stream);
+/* y[row][n] = x_scale[row] * sum_k x[row][k] w[n][k] + bias[n], summed in fp32 and rounded once. At most
+ * MSNH_B200_W4_MAX_ROWS rows (a product of more rows is not bound by its weights). */
+#define MSNH_B200_W4_MAX_ROWS 64
+typedef struct MsnhB200W4Linear {
+    const void *x;
+    void *y;
+    const float *x_scale;              /* rows values or NULL                                      */
+    const float *bias;                 /* n values or NULL                                         */
+    int32_t rows;
+    int32_t dtype;                     /* of x: F32, F16, BF16, E4M3                               */
+    int32_t out_dtype;                 /* of y: F32, F16, BF16                                     */
+    int64_t x_stride, y_stride;
+    void   *workspace;                 /* w4_linear_workspace bytes, 16-byte aligned; NULL if 0     */
+    size_t  workspace_bytes;
+} MsnhB200W4Linear;
+int  msnh_b200_w4_linear_workspace(MsnhB200Ctx *ctx, const MsnhB200W4 *weights, const MsnhB200W4Linear *args, size_t *bytes);
+int  msnh_b200_w4_linear(MsnhB200Ctx *ctx, const MsnhB200W4 *weights, const MsnhB200W4Linear *args, void *stream);
+
+/* A cache of keys and values in pages of page_size tokens. Token t of sequence s lies in page page_table[s][t / page_size] at
+ * place t % page_size. Sequences may share full pages (refs counts the sequences that hold a page; 0 = free); a page that is not
+ * full belongs to one sequence. All of it is the caller's memory; a fresh cache has lengths and refs of 0.
+ * An operation that finds no free page, no place left in a table row, or a sequence number that is none leaves that sequence
+ * as it was and adds one to *refused. */
+typedef struct MsnhB200KvCache {
+    void *k_pages, *v_pages;           /* [n_pages][page_size][n_kv_heads][head_dim] in the order of the strides */
+    int64_t k_page_stride, k_token_stride, k_head_stride;
+    int64_t v_page_stride, v_token_stride, v_head_stride;
+    int32_t *page_table;               /* [n_seqs][max_pages], rows table_stride apart             */
+    int32_t *lengths;                  /* [n_seqs] tokens                                          */
+    int32_t *refs;                     /* [n_pages]                                                */
+    int32_t *refused;                  /* one counter                                              */
+    int64_t table_stride;
+    int32_t n_pages, page_size, n_kv_heads, head_dim, n_seqs, max_pages;
+    int32_t dtype;                     /* F32, F16, BF16                                           */
+} MsnhB200KvCache;
+
+/* Attention of one query token a row over the cached tokens of its sequence: out[row][h] = sum_t p_t v_t, p = softmax(scale *
+ * q[row][h] . k_t) over the sequence's last `window` tokens (0: all), with keys and values of kv head h / (n_heads / n_kv_heads).
+ * Statistics and sums are fp32. Table entries outside [0, n_pages) are holes: their tokens are left out. Where no token is
+ * left, out is 0 and lse -infinity. head_dim: a multiple of 16 bytes, at most 256 values; the pages' rows 16-byte aligned. */
+typedef struct MsnhB200AttnDecode {
+    const void *q;                     /* [rows][n_heads][head_dim], the cache's type              */
+    void *out;                         /* same shape and type                                      */
+    float *lse;                        /* [rows][n_heads] log of the softmax's sum, or NULL         */
+    const int32_t *seqs;               /* [rows] sequence of each row, or NULL: row i is sequence i */
+    int32_t rows, n_heads;
+    int64_t q_row_stride, q_head_stride, out_row_stride, out_head_stride;
+    float   scale;
+    int32_t window;
+    void   *workspace;                 /* attn_decode_workspace bytes, 16-byte aligned; NULL if 0   */
+    size_t  workspace_bytes;
+} MsnhB200AttnDecode;
+int  msnh_b200_attn_decode_workspace(MsnhB200Ctx *ctx, const MsnhB200KvCache *cache, const MsnhB200AttnDecode *args, size_t *bytes);
+int  msnh_b200_attn_decode(MsnhB200Ctx *ctx, const MsnhB200KvCache *cache, const MsnhB200AttnDecode *args, void *stream);
+
+/* Upkeep of the cache; sequence numbers and counts lie on the device. A sequence is named at most once in a call (fork: as
+ * dst; it may be src of several, but not src and dst). `workspace`: kv_workspace bytes, 16-byte aligned.
+ *   append : tokens behind each sequence's own: starts (n + 1 offsets into k_new / v_new's rows) or NULL = one token each;
+ *            the pages that opens are the lowest free ones, in the order of the call
+ *   fork   : dst (empty before) becomes a copy of src: full pages are shared, the tokens of a last page that is not full are
+ *            copied to the lowest free page
+ *   free   : the sequence's pages are given back, its length is 0
+ *   compact: the i-th free page below the number of live pages takes the i-th live page from there on, contents, refs and
+ *            table entries; afterwards live pages are 0..live-1. table_out / refs_out: where the new table (rows
+ *            table_stride apart) and refs go, the cache's own or memory beside them (all entries are written)
+ *   copy   : page src[i] to page dst[i]; no page is dst twice or src and dst */
+int  msnh_b200_kv_workspace(MsnhB200Ctx *ctx, const MsnhB200KvCache *cache, int n, size_t *bytes);
+int  msnh_b200_kv_append(MsnhB200Ctx *ctx, const MsnhB200KvCache *cache, const int32_t *seqs, const int32_t *starts, int n,
+                         const void *k_new, const void *v_new, int64_t new_token_stride, int64_t new_head_stride, int n_tokens,
+                         void *workspace, size_t workspace_bytes, void *stream);
+int  msnh_b200_kv_fork(MsnhB200Ctx *ctx, const MsnhB200KvCache *cache, const int32_t *src, const int32_t *dst, int n,
+                       void *workspace, size_t workspace_bytes, void *stream);
+int  msnh_b200_kv_free(MsnhB200Ctx *ctx, const MsnhB200KvCache *cache, const int32_t *seqs, int n, void *stream);
+int  msnh_b200_kv_compact(MsnhB200Ctx *ctx, const MsnhB200KvCache *cache, int32_t *table_out, int32_t *refs_out,
+                          void *workspace, size_t workspace_bytes, void *stream);
+int  msnh_b200_kv_copy_pages(MsnhB200Ctx *ctx, const MsnhB200KvCache *cache, const int32_t *src, const int32_t *dst, int n, void *stream);
 
 #ifdef __cplusplus
 }

@@ -15,7 +15,7 @@ MAX_IN = 8
 
 # status codes / enums (include/msnh_b200.h)
 OK = 0
-F32, F16 = 0, 1
+F32, F16, BF16, E4M3 = 0, 1, 2, 3
 (ACT_NONE, ACT_LOGISTIC, ACT_LOGGY, ACT_RELU, ACT_RELU6, ACT_HARD_SWISH, ACT_ELU, ACT_SELU, ACT_RELIE, ACT_RAMP,
  ACT_LEAKY, ACT_TANH, ACT_STAIR, ACT_HARDTAN, ACT_SOFT_PLUS, ACT_PLSE, ACT_LHTAN, ACT_MISH, ACT_SWISH) = range(19)
 (OP_CONV, OP_BATCHNORM, OP_ACTIVATION, OP_MAXPOOL, OP_AVGPOOL, OP_UPSAMPLE, OP_CONCAT, OP_ADD, OP_SLICE, OP_PAD,
@@ -75,6 +75,39 @@ def make_op(kind, inputs, **kw):
     return op
 
 
+class RmsNorm(C.Structure):
+    """MsnhB200RmsNorm"""
+    _fields_ = [("x", C.c_void_p), ("residual", C.c_void_p), ("weight", C.c_void_p), ("residual_out", C.c_void_p), ("y", C.c_void_p), ("y_scale", C.c_void_p),
+                ("rows", C.c_int64), ("cols", C.c_int32), ("dtype", C.c_int32), ("weight_dtype", C.c_int32), ("out_dtype", C.c_int32),
+                ("x_stride", C.c_int64), ("residual_stride", C.c_int64), ("residual_out_stride", C.c_int64), ("y_stride", C.c_int64), ("eps", C.c_float)]
+
+
+class W4(C.Structure):
+    """MsnhB200W4"""
+    _fields_ = [("packed", C.c_void_p), ("n", C.c_int32), ("k", C.c_int32), ("group", C.c_int32), ("scale_dtype", C.c_int32), ("has_zeros", C.c_int32)]
+
+
+class W4Linear(C.Structure):
+    """MsnhB200W4Linear"""
+    _fields_ = [("x", C.c_void_p), ("y", C.c_void_p), ("x_scale", C.c_void_p), ("bias", C.c_void_p), ("rows", C.c_int32), ("dtype", C.c_int32),
+                ("out_dtype", C.c_int32), ("x_stride", C.c_int64), ("y_stride", C.c_int64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class KvCache(C.Structure):
+    """MsnhB200KvCache"""
+    _fields_ = [("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("k_page_stride", C.c_int64), ("k_token_stride", C.c_int64), ("k_head_stride", C.c_int64),
+                ("v_page_stride", C.c_int64), ("v_token_stride", C.c_int64), ("v_head_stride", C.c_int64), ("page_table", C.c_void_p), ("lengths", C.c_void_p),
+                ("refs", C.c_void_p), ("refused", C.c_void_p), ("table_stride", C.c_int64), ("n_pages", C.c_int32), ("page_size", C.c_int32),
+                ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("n_seqs", C.c_int32), ("max_pages", C.c_int32), ("dtype", C.c_int32)]
+
+
+class AttnDecode(C.Structure):
+    """MsnhB200AttnDecode"""
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p), ("seqs", C.c_void_p), ("rows", C.c_int32), ("n_heads", C.c_int32),
+                ("q_row_stride", C.c_int64), ("q_head_stride", C.c_int64), ("out_row_stride", C.c_int64), ("out_head_stride", C.c_int64), ("scale", C.c_float),
+                ("window", C.c_int32), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 _kernel = None
 _host = None
 
@@ -126,6 +159,20 @@ def kernel_lib():
     f64p = C.POINTER(C.c_double)
     lib.msnh_b200_clock_probe_start.argtypes = [i32, i32, C.POINTER(vp)]
     lib.msnh_b200_clock_probe_stop.argtypes = [vp, f64p, f64p, f64p, C.POINTER(i32)]
+    i64, szp = C.c_int64, C.POINTER(C.c_size_t)
+    lib.msnh_b200_rms_norm.argtypes = [vp, C.POINTER(RmsNorm), vp]
+    lib.msnh_b200_w4_pack_bytes.argtypes = [vp, C.POINTER(W4), szp]
+    lib.msnh_b200_w4_pack.argtypes = [vp, C.POINTER(W4), vp, i64, vp, vp, vp, vp]
+    lib.msnh_b200_w4_linear_workspace.argtypes = [vp, C.POINTER(W4), C.POINTER(W4Linear), szp]
+    lib.msnh_b200_w4_linear.argtypes = [vp, C.POINTER(W4), C.POINTER(W4Linear), vp]
+    lib.msnh_b200_attn_decode_workspace.argtypes = [vp, C.POINTER(KvCache), C.POINTER(AttnDecode), szp]
+    lib.msnh_b200_attn_decode.argtypes = [vp, C.POINTER(KvCache), C.POINTER(AttnDecode), vp]
+    lib.msnh_b200_kv_workspace.argtypes = [vp, C.POINTER(KvCache), i32, szp]
+    lib.msnh_b200_kv_append.argtypes = [vp, C.POINTER(KvCache), vp, vp, i32, vp, vp, i64, i64, i32, vp, C.c_size_t, vp]
+    lib.msnh_b200_kv_fork.argtypes = [vp, C.POINTER(KvCache), vp, vp, i32, vp, C.c_size_t, vp]
+    lib.msnh_b200_kv_free.argtypes = [vp, C.POINTER(KvCache), vp, i32, vp]
+    lib.msnh_b200_kv_compact.argtypes = [vp, C.POINTER(KvCache), vp, vp, vp, C.c_size_t, vp]
+    lib.msnh_b200_kv_copy_pages.argtypes = [vp, C.POINTER(KvCache), vp, vp, i32, vp]
     _kernel = lib
     return lib
 
@@ -141,6 +188,9 @@ KERNEL_SYMBOLS = [
     "msnh_b200_plan_profile", "msnh_b200_plan_read_trace", "msnh_b200_plan_destroy",
     "msnh_b200_yolo_collect_static", "msnh_b200_static_last_error",
     "msnh_b200_clock_probe_start", "msnh_b200_clock_probe_stop",
+    "msnh_b200_rms_norm", "msnh_b200_w4_pack_bytes", "msnh_b200_w4_pack", "msnh_b200_w4_linear_workspace", "msnh_b200_w4_linear",
+    "msnh_b200_attn_decode_workspace", "msnh_b200_attn_decode", "msnh_b200_kv_workspace", "msnh_b200_kv_append", "msnh_b200_kv_fork",
+    "msnh_b200_kv_free", "msnh_b200_kv_compact", "msnh_b200_kv_copy_pages",
 ]
 
 
