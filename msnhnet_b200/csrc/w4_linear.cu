@@ -1,60 +1,67 @@
 // Products with 4-bit weights (msnh_b200_w4_pack, msnh_b200_w4_linear).
+#include <cooperative_groups.h>
+#include "common.cuh"
 #include "token_ops.h"
 #include "token_types.cuh"
 
 namespace msnh {
 namespace {
 
-// Packed weights: codes in blocks of 16 rows by 64 values (512 bytes), the blocks of a 16-row tile one behind the other; then the
-// scales [tile][group][16 rows] (fp16 or fp32), then the zero points in the same order, a byte each. Codes beyond n and k are 0.
-// Inside a block, 16 bytes belong to a lane of the warp that reads it: lane l has rows l / 4 and l / 4 + 8, and in its word j the
-// four values from 32 * (j / 2) + 8 * (l % 4) + 4 * (j % 2) on. That is the A operand of m16n8k16 with the 16 values of a k-step in an
-// order that the B operand follows, so nothing is moved between lanes. Half-bytes of a word, from the lowest: value 0 of both rows,
-// value 2 of both rows, value 1 of both, value 3 of both (pairs 16 bits apart are neighbours in k).
-constexpr int kTileRows = 16, kBlockK = 64, kBlockBytes = 512;
+// Packed weights: units of 16 rows by 128 values, the units of a 16-row tile one behind the other. A unit is 1024 bytes of codes, then
+// for each of its 1, 2 or 4 spans (128, 64 or 32 values: the most that always lie in one group) eight records of the scales (fp16 or
+// fp32) and zero points (a byte each) of rows r and r + 8, 8 or 16 bytes. Codes beyond n and k are 0.
+// Of the codes, 16 bytes of each half (64 values, 512 bytes) belong to a lane of the warp that reads it: lane l has rows l / 4 and
+// l / 4 + 8, and in its words 2 s and 2 s + 1 (one for either row) the eight values from 32 * s + 8 * (l % 4) on: byte i has value i in its
+// low and value 4 + i in its high half. Two masks make 8-bit A operands of m16n8k32 of a word, four make 16-bit ones of m16n8k16, with k in
+// an order that the B operand follows, so nothing is moved between lanes.
+constexpr int kTileRows = 16, kUnitK = 128, kCodeBytes = 1024;
 
 struct W4Layout {
-    int n, k, group, tiles, blocks, groups;
-    size_t scale_size, scales_at, zeros_at, bytes;
+    int n, k, group, tiles, units, groups, wide, spans;          // units: of a tile; wide: scales in fp32; spans: of a unit
+    size_t unit_bytes, bytes;
     W4Layout(const MsnhB200W4 &w)
-        : n(w.n), k(w.k), group(w.group), tiles((w.n + kTileRows - 1) / kTileRows), blocks((w.k + kBlockK - 1) / kBlockK),
-          groups((w.k + w.group - 1) / w.group) {
-        scale_size = w.scale_dtype == MSNH_B200_F16 ? 2 : 4;
-        scales_at = static_cast<size_t>(tiles) * blocks * kBlockBytes;
-        zeros_at = scales_at + static_cast<size_t>(tiles) * groups * kTileRows * scale_size;
-        bytes = zeros_at + (w.has_zeros ? static_cast<size_t>(tiles) * groups * kTileRows : 0);
+        : n(w.n), k(w.k), group(w.group), tiles((w.n + kTileRows - 1) / kTileRows), units((w.k + kUnitK - 1) / kUnitK),
+          groups((w.k + w.group - 1) / w.group), wide(w.scale_dtype != MSNH_B200_F16), spans(w.group % 128 == 0 ? 1 : w.group % 64 == 0 ? 2 : 4) {
+        unit_bytes = kCodeBytes + static_cast<size_t>(spans) * 8 * (wide ? 16 : 8);
+        bytes = static_cast<size_t>(tiles) * units * unit_bytes;
     }
 };
+
+template <typename S> struct Record { S scale[2]; uint8_t zero[2], rest[sizeof(S) * 2 - 2]; };
 
 __device__ __forceinline__ int code_at(const uint8_t *codes, long long stride, int n, int k, int row, int at) {
     if (row >= n || at >= k) return 0;
     return codes[row * stride + at / 2] >> (at % 2 * 4) & 15;
 }
 
-__global__ void w4_pack_codes_kernel(const uint8_t *codes, long long stride, int n, int k, int blocks, long long words, uint32_t *out) {
+__global__ void w4_pack_codes_kernel(const uint8_t *codes, long long stride, int n, int k, int units, size_t unit_bytes, long long words, uint8_t *out) {
     for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < words; i += static_cast<long long>(gridDim.x) * blockDim.x) {
-        const int j = static_cast<int>(i % 4), lane = static_cast<int>(i / 4 % 32);
-        const long long block = i / 128;
-        const int row = static_cast<int>(block / blocks) * kTileRows + lane / 4;
-        const int at = static_cast<int>(block % blocks) * kBlockK + 32 * (j / 2) + 8 * (lane % 4) + 4 * (j % 2);
+        const int in_unit = static_cast<int>(i % 256), half = in_unit / 128, lane = in_unit / 4 % 32, word_of = in_unit % 4;
+        const long long unit = i / 256;
+        const int row = static_cast<int>(unit / units) * kTileRows + lane / 4 + word_of % 2 * 8;
+        const int at = static_cast<int>(unit % units) * kUnitK + 64 * half + 32 * (word_of / 2) + 8 * (lane % 4);
         uint32_t word = 0;
 #pragma unroll
-        for (int v = 0; v < 4; ++v)
-#pragma unroll
-            for (int half = 0; half < 2; ++half)
-                word |= static_cast<uint32_t>(code_at(codes, stride, n, k, row + 8 * half, at + v)) << (16 * (v % 2) + 8 * (v / 2) + 4 * half);
-        out[i] = word;
+        for (int v = 0; v < 8; ++v) word |= static_cast<uint32_t>(code_at(codes, stride, n, k, row, at + v)) << (v % 4 * 8 + v / 4 * 4);
+        *reinterpret_cast<uint32_t *>(out + unit * unit_bytes + in_unit * 4) = word;
     }
 }
 
 template <typename S, typename Out>
-__global__ void w4_pack_scales_kernel(const S *scales, const uint8_t *zeros, int n, int groups, long long count, Out *scales_out, uint8_t *zeros_out) {
+__global__ void w4_pack_records_kernel(const S *scales, const uint8_t *zeros, int n, int k, int units, int spans, int group, int groups, size_t unit_bytes,
+                                       long long count, uint8_t *out) {
     for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < count; i += static_cast<long long>(gridDim.x) * blockDim.x) {
-        const long long tile_group = i / kTileRows;
-        const long long row = tile_group / groups * kTileRows + i % kTileRows, group = tile_group % groups;
-        const bool inside = row < n;
-        scales_out[i] = inside ? static_cast<Out>(to_float(scales[row * groups + group])) : static_cast<Out>(0.f);
-        if (zeros) zeros_out[i] = inside ? zeros[row * groups + group] : 0;
+        const int pair = static_cast<int>(i % 8), span = static_cast<int>(i / 8 % spans);
+        const long long unit = i / 8 / spans, at = unit % units * kUnitK + span * (kUnitK / spans);
+        const long long g = at / group;
+        Record<Out> r = {};
+        for (int half = 0; half < 2; ++half) {
+            const long long row = unit / units * kTileRows + pair + 8 * half;
+            const bool there = row < n && at < k;
+            r.scale[half] = there ? static_cast<Out>(to_float(scales[row * groups + g])) : static_cast<Out>(0.f);
+            r.zero[half] = there && zeros ? zeros[row * groups + g] & 15 : 8;
+        }
+        reinterpret_cast<Record<Out> *>(out + unit * unit_bytes + kCodeBytes)[span * 8 + pair] = r;
     }
 }
 
@@ -64,49 +71,807 @@ struct W4Params {
     void *y;
     const float *x_scale, *bias;
     long long x_stride, y_stride;
-    size_t scales_at, zeros_at;
-    int n, k, group, blocks, groups, rows, scale_size, has_zeros;
+    long long unit_bytes;
+    int n, k, tiles, units, rows;
+    int dtype, wide, spans, vectors, out_dtype;
+    int split, share, block_units;           // warps that share a tile's k in a block; units of k of each, of the block at most
+    int ring_at, x_at, meta_at;              // of the rings and the activations, in shared memory
+    uint8_t *digits_made, *meta_made;        // in the workspace, or null
+    int *error;                              // where the host learns of a wait that ran out
+    uint32_t exponents;                      // of the operands' type (a parameter, so that the compiler takes it for a variable)
 };
 
-__device__ __forceinline__ float scale_at(const W4Params &p, size_t i) {
-    return p.scale_size == 2 ? __half2float(reinterpret_cast<const __half *>(p.packed + p.scales_at)[i])
-                             : reinterpret_cast<const float *>(p.packed + p.scales_at)[i];
+constexpr int kWarps = 16, kSummers = 4, kThreads = (kWarps + kSummers) * 32;      // warps that multiply, and that add up
+
+__device__ __forceinline__ void copy16(uint32_t to, const void *from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
+
+// The A operand's element type for activations of type X, and how many operands of that type an activation becomes: fp16, bf16 and 8-bit
+// values are operands themselves, an fp32 value is the sum of three bf16 ones (8 bits of it each), whose products with a code are exact.
+template <typename X> struct Operand { using Type = X; static constexpr int kParts = 1; };
+template <> struct Operand<__nv_fp8_e4m3> { using Type = __half; static constexpr int kParts = 1; };
+template <> struct Operand<float> { using Type = __nv_bfloat16; static constexpr int kParts = 3; };
+
+template <typename H> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+    H v[2] = {from_float<H>(a), from_float<H>(b)};
+    uint32_t r;
+    memcpy(&r, v, 4);
+    return r;
+}
+// the three bf16 parts of two fp32 values
+__device__ __forceinline__ void split2(float a, float b, uint32_t &high, uint32_t &middle, uint32_t &low) {
+    high = pack2<__nv_bfloat16>(a, b);
+    // (what is left of an infinity or NaN is 0: the first part carries it)
+    const float ra = fabsf(a) <= 3.3e38f ? a - __uint_as_float(high << 16) : 0.f, rb = fabsf(b) <= 3.3e38f ? b - __uint_as_float(high & 0xffff0000u) : 0.f;
+    middle = pack2<__nv_bfloat16>(ra, rb);
+    low = pack2<__nv_bfloat16>(ra - __uint_as_float(middle << 16), rb - __uint_as_float(middle & 0xffff0000u));
 }
 
-// A warp an output value.
-template <typename T, typename Out>
-__global__ void w4_dot_kernel(W4Params p) {
-    const long long i = (blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x) / 32;
-    if (i >= static_cast<long long>(p.n) * p.rows) return;
-    const int row = static_cast<int>(i / p.rows), m = static_cast<int>(i % p.rows), lane = threadIdx.x % 32;
-    const int tile = row / kTileRows, in_tile = row % kTileRows;
-    const T *x = static_cast<const T *>(p.x) + m * p.x_stride;
-    float sum = 0.f;
-    for (int at = lane; at < p.k; at += 32) {
-        const int in_block = at % kBlockK, word = in_block / 32 * 2 + in_block / 4 % 2, v = at % 4;
-        const size_t byte = (static_cast<size_t>(tile) * p.blocks + at / kBlockK) * kBlockBytes + (in_tile % 8 * 4 + in_block % 32 / 8) * 16 + word * 4 + v % 2 * 2 + v / 2;
-        const int code = p.packed[byte] >> (in_tile / 8 * 4) & 15;
-        const size_t g = (static_cast<size_t>(tile) * p.groups + at / p.group) * kTileRows + in_tile;
-        const int zero = p.has_zeros ? p.packed[p.zeros_at + g] : 8;
-        sum += (code - zero) * scale_at(p, g) * to_float(x[at]);
-    }
+// pairs 01 23 45 67 to 02 13 46 57
+__device__ __forceinline__ void interleave(uint32_t (&v)[4]) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-    if (lane == 0) {
-        const float y = sum * (p.x_scale ? p.x_scale[m] : 1.f) + (p.bias ? p.bias[row] : 0.f);
-        static_cast<Out *>(p.y)[m * p.y_stride + row] = from_float<Out>(y);
+    for (int i = 0; i < 4; i += 2) {
+        const uint32_t a = v[i], b = v[i + 1];
+        v[i] = __byte_perm(a, b, 0x5410);
+        v[i + 1] = __byte_perm(a, b, 0x7632);
     }
 }
 
-template <typename T, typename Out>
-cudaError_t launch(const W4Params &p, void *stream) {
-    const long long warps = static_cast<long long>(p.n) * p.rows;
-    return launch_token_kernel(w4_dot_kernel<T, Out>, dim3(static_cast<unsigned>((warps + 7) / 8)), 256, 0, stream, false, p);
+// Eight values of a row, `left` of which are there (all and aligned: kFast), as operands: two k-steps of two registers a part, values 0 and 2,
+// 1 and 3, 4 and 6, 5 and 7.
+template <typename X, bool kFast> __device__ __forceinline__ void load_x(const X *row, int left, uint32_t (&out)[Operand<X>::kParts][4]) {
+    if constexpr (std::is_same<X, float>::value) {
+        float v[8];
+        if (kFast) {
+            const float4 a = __ldg(reinterpret_cast<const float4 *>(row)), b = __ldg(reinterpret_cast<const float4 *>(row) + 1);
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = i < left ? row[i] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) split2(v[i / 2 * 4 + i % 2], v[i / 2 * 4 + i % 2 + 2], out[0][i], out[1][i], out[2][i]);
+    } else if constexpr (std::is_same<X, __nv_fp8_e4m3>::value) {
+        uint16_t raw[4];
+        if (kFast) {
+            const uint2 a = __ldg(reinterpret_cast<const uint2 *>(row));
+            memcpy(raw, &a, 8);
+        } else {
+            const uint8_t *bytes = reinterpret_cast<const uint8_t *>(row);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                raw[i] = 2 * i < left ? bytes[2 * i] : 0;
+                if (2 * i + 1 < left) raw[i] |= static_cast<uint16_t>(bytes[2 * i + 1] << 8);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(raw[i], __NV_E4M3);
+            memcpy(&out[0][i], &h, 4);
+        }
+        interleave(out[0]);
+    } else {
+        if (kFast) {
+            const uint4 a = __ldg(reinterpret_cast<const uint4 *>(row));
+            out[0][0] = a.x; out[0][1] = a.y; out[0][2] = a.z; out[0][3] = a.w;
+        } else {
+            X v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = i < left ? row[i] : from_float<X>(0.f);
+            memcpy(out[0], v, 16);
+        }
+        interleave(out[0]);
+    }
 }
 
-template <typename T>
-cudaError_t launch(const W4Params &p, int out_dtype, void *stream) {
-    return out_dtype == MSNH_B200_F32 ? launch<T, float>(p, stream) : out_dtype == MSNH_B200_F16 ? launch<T, __half>(p, stream) : launch<T, __nv_bfloat16>(p, stream);
+// (w & mask) | exponents in one instruction, which takes one constant at most: the exponents come in a register
+template <uint32_t kMask> __device__ __forceinline__ uint32_t masked_or(uint32_t w, uint32_t exponents) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "n"(kMask), "r"(exponents));
+    return r;
+}
+// The 16-bit operands of a word of codes, less their row's zero point: values 0 and 2, 1 and 3, 4 and 6, 5 and 7. fp16: a half-byte below
+// the exponent of 1024 is 1024 + code, one four bits higher 1024 + 16 code; bf16 has seven bits behind its leading one, so every half-byte
+// is moved to the lowest place: 128 + code. All exact.
+template <typename H> struct Zero;
+template <> struct Zero<__half> {
+    static constexpr uint32_t kExponents = 0x64006400u;
+    __half2 low, high;
+    __device__ __forceinline__ void set(uint32_t z) {
+        const uint32_t a = (0xe400u + z) * 0x10001u, b = (0xd400u + 16 * z) * 0x10001u;        // -(1024 + zero), -(64 + zero)
+        memcpy(&low, &a, 4);
+        memcpy(&high, &b, 4);
+    }
+    __device__ __forceinline__ void operand(uint32_t w, uint32_t exponents, uint32_t (&out)[4]) const {
+        const __half2 sixteenth = __half2half2(__float2half_rn(0.0625f));
+        const uint32_t above = w >> 8;
+        const uint32_t raw[4] = {masked_or<0x000f000fu>(w, exponents), masked_or<0x000f000fu>(above, exponents), masked_or<0x00f000f0u>(w, exponents),
+                                 masked_or<0x00f000f0u>(above, exponents)};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            __half2 v;
+            memcpy(&v, &raw[i], 4);
+            v = i / 2 ? __hfma2(v, sixteenth, high) : __hadd2(v, low);
+            memcpy(&out[i], &v, 4);
+        }
+    }
+};
+template <> struct Zero<__nv_bfloat16> {
+    static constexpr uint32_t kExponents = 0x43004300u;
+    __nv_bfloat162 low;
+    __device__ __forceinline__ void set(uint32_t z) {
+        const uint32_t a = (0xc300u + z) * 0x10001u;                                           // -(128 + zero)
+        memcpy(&low, &a, 4);
+    }
+    __device__ __forceinline__ void operand(uint32_t w, uint32_t exponents, uint32_t (&out)[4]) const {
+        const uint32_t raw[4] = {masked_or<0x000f000fu>(w, exponents), masked_or<0x000f000fu>(w >> 8, exponents), masked_or<0x000f000fu>(w >> 4, exponents),
+                                 masked_or<0x000f000fu>(w >> 12, exponents)};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            __nv_bfloat162 v;
+            memcpy(&v, &raw[i], 4);
+            v = __hadd2(v, low);
+            memcpy(&out[i], &v, 4);
+        }
+    }
+};
+
+// Scales and zero points of a lane's two rows, from a record in shared memory.
+__device__ __forceinline__ void take_record(uint32_t record, int wide, float2 &scale, uint32_t &z0, uint32_t &z8) {
+    uint32_t zeros;
+    if (wide) {
+        asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(scale.x), "=f"(scale.y) : "r"(record) : "memory");
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(zeros) : "r"(record + 8) : "memory");
+    } else {
+        uint32_t both;
+        asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(both), "=r"(zeros) : "r"(record) : "memory");
+        __half2 pair;
+        memcpy(&pair, &both, 4);
+        scale = __half22float2(pair);
+    }
+    z0 = zeros & 255;
+    z8 = zeros >> 8 & 255;
+}
+__device__ __forceinline__ uint4 load_shared(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+
+template <typename H> __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<H, __half>::value)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void store(const W4Params &p, int m, int row, float v) {
+    const float y = v * (p.x_scale ? p.x_scale[m] : 1.f) + (p.bias ? p.bias[row] : 0.f);
+    const long long at = m * p.y_stride + row;
+    if (p.out_dtype == MSNH_B200_F32) static_cast<float *>(p.y)[at] = y;
+    else if (p.out_dtype == MSNH_B200_F16) static_cast<__half *>(p.y)[at] = __float2half_rn(y);
+    else static_cast<__nv_bfloat16 *>(p.y)[at] = __float2bfloat16_rn(y);
+}
+
+// A block stays for its share of the tiles, kTiles at a time for each of its sets of `split` warps; the warps of a set share the tiles' k,
+// and so may the blocks of a cluster. What both kernels need of that.
+template <int kTiles> struct Share {
+    int lane, warp, ranks, rank, sets, turn, from, to, mine;     // turn: tiles of one; this block's, and this warp's first one
+    int begin, first, count;                                     // units of k: the block's first, the warp's first, how many
+    int block_units;
+    __device__ __forceinline__ Share(const W4Params &p, int cluster_blocks, int cluster_rank) {
+        lane = threadIdx.x % 32;
+        warp = threadIdx.x / 32;
+        ranks = cluster_blocks;
+        rank = cluster_rank;
+        sets = kWarps / p.split;
+        turn = kTiles * sets;
+        const int place = blockIdx.x / ranks, places = gridDim.x / ranks;
+        from = static_cast<int>(static_cast<long long>(p.tiles) * place / places);
+        to = static_cast<int>(static_cast<long long>(p.tiles) * (place + 1) / places);
+        mine = from + warp / p.split * kTiles;
+        begin = min(rank * p.split * p.share, p.units);
+        block_units = min(begin + p.split * p.share, p.units) - begin;
+        first = min(begin + warp % p.split * p.share, p.units);
+        count = warp < kWarps ? min(first + p.share, p.units) - first : 0;
+    }
+};
+
+// A warp's units of every turn's tiles, one turn after the other, through a ring with cp.async. Of a tile that is not the block's nothing is
+// copied, and what its sums are made of is never stored.
+template <int kTiles, int kAhead> struct Units {
+    const uint8_t *codes;
+    long long unit_bytes, tile_bytes, next_turn;
+    uint32_t ring, ring_end, fill, slot;
+    int pitch, copy_tile, to, turn, copied, count, lane;
+    bool copies_record;
+    __device__ __forceinline__ Units(const W4Params &p, const Share<kTiles> &s, uint32_t rings) {
+        lane = s.lane;
+        pitch = static_cast<int>(p.unit_bytes);
+        unit_bytes = p.unit_bytes;
+        tile_bytes = p.units * p.unit_bytes;
+        next_turn = s.turn * tile_bytes - s.count * p.unit_bytes;
+        codes = p.packed + s.mine * tile_bytes + s.first * p.unit_bytes + lane * 16;
+        copy_tile = s.mine;
+        to = s.to;
+        turn = s.turn;
+        count = s.count;
+        copied = 0;
+        ring = fill = slot = rings + s.warp * kAhead * kTiles * pitch;
+        ring_end = ring + kAhead * kTiles * pitch;
+        copies_record = lane * 16 < pitch - kCodeBytes;
+        if (count && s.warp < kWarps)
+#pragma unroll 1
+            for (int u = 0; u < kAhead - 1; ++u) copy();
+    }
+    __device__ __forceinline__ void copy() {
+#pragma unroll
+        for (int r = 0; r < kTiles; ++r)
+            if (copy_tile + r < to) {
+                const uint8_t *at = codes + r * tile_bytes;
+                const uint32_t into = fill + r * pitch + lane * 16;
+                copy16(into, at);
+                copy16(into + 512, at + 512);
+                if (copies_record) copy16(into + 1024, at + 1024);
+            }
+        copy_commit();
+        codes += unit_bytes;
+        if (++copied == count) {
+            copied = 0;
+            copy_tile += turn;
+            codes += next_turn;
+        }
+        fill += kTiles * pitch;
+        if (fill == ring_end) fill = ring;
+    }
+    __device__ __forceinline__ void wait() {                     // for the unit at `slot`; the one behind it may be overwritten then
+        copy_wait<kAhead - 2>();
+        __syncwarp();                                            // (records are other lanes' copies)
+        copy();
+    }
+    __device__ __forceinline__ void next() {
+        slot += kTiles * pitch;
+        if (slot == ring_end) slot = ring;
+    }
+};
+
+// The way of a turn's sums [warp][column][row] from the warps that multiply to those that add up: `full` counts the former's arrivals,
+// `empty` the latter's. Neither waits for its own kind, so the copies run on meanwhile. The waits have a limit, after which the host learns
+// of it and the block ends.
+struct Handover { uint64_t full, empty; };
+__device__ __forceinline__ uint32_t shared_address(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void barrier_init(uint64_t *b, int count) { asm volatile("mbarrier.init.shared.b64 [%0], %1;" ::"r"(shared_address(b)), "r"(count) : "memory"); }
+__device__ __forceinline__ void barrier_arrive(uint64_t *b) { asm volatile("mbarrier.arrive.shared.b64 _, [%0];" ::"r"(shared_address(b)) : "memory"); }
+__device__ __forceinline__ bool barrier_wait(uint64_t *b, int parity, int *error) {
+    for (int i = 0; i < 1 << 20; ++i) {
+        uint32_t done;
+        asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }" : "=r"(done) : "r"(shared_address(b)), "r"(parity) : "memory");
+        if (done) return true;
+    }
+    report_error(error, 4);
+    return false;
+}
+
+// The outputs of a turn, in a fixed order: four threads an output, each every fourth of the warps that share a tile's k. sums: [warp][row of
+// the activations][row of the tiles]. `threads`: a multiple of 32.
+template <int kRows, typename Put>
+__device__ __forceinline__ void add_up(const W4Params &p, int sets, int columns, const float *sums, int thread, int threads, Put put) {
+    const int per_set = kRows * p.rows, each = kRows * columns;
+    for (int i = thread; i < sets * per_set * 4; i += threads) {                // (a multiple of 64)
+        const int o = i / 4, set = o / per_set, in_set = o - set * per_set;
+        const float *from = sums + set * p.split * each + in_set;
+        float v = 0.f;
+#pragma unroll
+        for (int j = 0; j < kWarps / 4; ++j) {
+            const int w = j * 4 + i % 4;
+            if (w < p.split) v += from[w * each];
+        }
+        v += __shfl_xor_sync(~0u, v, 1);
+        v += __shfl_xor_sync(~0u, v, 2);
+        if (i % 4 == 0) put(o, set * (kRows / kTileRows) + in_set % kRows / kTileRows, in_set % kTileRows, in_set / kRows, v);
+    }
+}
+
+// What a kernel does with a block's turns: multiply(tile) leaves a warp's sums in registers, leave(to) puts them down.
+template <int kTiles, int kCount, typename Cluster, typename Multiply, typename Leave>
+__device__ __forceinline__ void turns(const W4Params &p, const Share<kTiles> &s, Cluster &cluster, float *sums, Handover &hand, Multiply multiply, Leave leave) {
+    constexpr int kRows = kTiles * kTileRows;
+    const auto put = [&](int tile, int place, int row, int m, float v) {
+        if (tile + place < s.to && (tile + place) * kTileRows + row < p.n) store(p, m, (tile + place) * kTileRows + row, v);
+    };
+    if (s.ranks > 1) {
+        float *const outputs = sums + kWarps * kRows * kCount;
+        for (int tile = s.from; tile < s.to; tile += s.turn) {
+            if (s.warp < kWarps) {
+                multiply();
+                leave(sums + s.warp * kRows * kCount);
+            }
+            __syncthreads();
+            add_up<kRows>(p, s.sets, kCount, sums, threadIdx.x, kThreads, [&](int o, int, int, int, float v) { outputs[o] = v; });
+            cluster.sync();
+            for (int o = s.rank * kThreads + threadIdx.x; o < s.sets * kRows * p.rows; o += s.ranks * kThreads) {
+                float v = 0.f;
+                for (int q = 0; q < s.ranks; ++q) v += *cluster.map_shared_rank(&outputs[o], q);
+                const int set = o / (kRows * p.rows), m = o % (kRows * p.rows) / kRows, row = o % kRows;
+                put(tile, set * kTiles + row / kTileRows, row % kTileRows, m, v);
+            }
+            cluster.sync();                                      // (no block goes on while another reads its sums)
+        }
+        return;
+    }
+    int parity = 0;
+    if (s.warp < kWarps) {
+        for (int tile = s.from; tile < s.to; tile += s.turn, parity ^= 1) {
+            multiply();
+            if (tile != s.from && !barrier_wait(&hand.empty, parity ^ 1, p.error)) return;
+            leave(sums + s.warp * kRows * kCount);
+            __syncwarp();
+            if (s.lane == 0) barrier_arrive(&hand.full);
+        }
+    } else {
+        for (int tile = s.from; tile < s.to; tile += s.turn, parity ^= 1) {
+            if (!barrier_wait(&hand.full, parity, p.error)) return;
+            add_up<kRows>(p, s.sets, kCount, sums, threadIdx.x - kWarps * 32, kSummers * 32, [&](int, int place, int row, int m, float v) { put(tile, place, row, m, v); });
+            __syncwarp();
+            if (s.lane == 0) barrier_arrive(&hand.empty);
+        }
+    }
+}
+// Floats of one buffer of sums: the warps', and a block's outputs where a cluster adds them up (all its warps share one set's k then).
+template <int kRows, int kCount> constexpr int kSumsOf = (kWarps + 1) * kRows * kCount;
+
+// One or two rows: products of whole numbers. An activation is fixed-point relative to the largest of its row and span, four signed 8-bit
+// digits (30 bits and the sign), and each digit of each row is a column of m16n8k32: one row leaves seven of the eight columns of a product
+// empty anyway. Codes are 8-bit operands after two masks and a shift for 8 of them, where 16-bit ones take nine instructions, and the
+// instructions are what bounds this beside the memory. Sums of a span are exact in 32 bits:
+//   sum (code - zero) X = sum code X - zero sum X,  |sum code X| <= 128 * 15 * 128,
+// accumulated on 1.5 * 2^23's bits, so that the result is a float without a conversion. Scales of weights and activations are applied to
+// that in fp32. An infinity or NaN makes its row's results NaN.
+constexpr int kDigits = 4, kIntegerRows = 2, kTopBit = 29;       // |X| < 2^(kTopBit + 1)
+constexpr uint32_t kIntegerBase = 0x4b400000u;                   // 12582912
+
+__device__ __forceinline__ void mma_integer(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// four values of a row from `at` on, zeros beyond k
+__device__ __forceinline__ void load_four(const W4Params &p, int m, int at, float (&v)[4]) {
+    const long long first = m * p.x_stride + at;
+    const bool whole = p.vectors && at + 4 <= p.k;
+    if (p.dtype == MSNH_B200_F32) {
+        const float *x = static_cast<const float *>(p.x) + first;
+        if (whole) {
+            const float4 t = __ldg(reinterpret_cast<const float4 *>(x));
+            v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = at + i < p.k ? x[i] : 0.f;
+        }
+    } else if (p.dtype == MSNH_B200_E4M3) {
+        const uint8_t *x = static_cast<const uint8_t *>(p.x) + first;
+        uint32_t raw = 0;
+        if (whole) {
+            raw = __ldg(reinterpret_cast<const uint32_t *>(x));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) raw |= at + i < p.k ? static_cast<uint32_t>(x[i]) << (8 * i) : 0u;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            __nv_fp8_e4m3 e;
+            e.__x = static_cast<uint8_t>(raw >> (8 * i));
+            v[i] = static_cast<float>(e);
+        }
+    } else {
+        const uint16_t *x = static_cast<const uint16_t *>(p.x) + first;
+        uint2 raw = make_uint2(0, 0);
+        if (whole) {
+            raw = __ldg(reinterpret_cast<const uint2 *>(x));
+        } else {
+            if (at < p.k) raw.x = x[0];
+            if (at + 1 < p.k) raw.x |= static_cast<uint32_t>(x[1]) << 16;
+            if (at + 2 < p.k) raw.y = x[2];
+            if (at + 3 < p.k) raw.y |= static_cast<uint32_t>(x[3]) << 16;
+        }
+        if (p.dtype == MSNH_B200_F16) {
+            __half2 h[2];
+            memcpy(h, &raw, 8);
+            const float2 a = __half22float2(h[0]), b = __half22float2(h[1]);
+            v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+        } else {
+            v[0] = __uint_as_float(raw.x << 16); v[1] = __uint_as_float(raw.x & 0xffff0000u);
+            v[2] = __uint_as_float(raw.y << 16); v[3] = __uint_as_float(raw.y & 0xffff0000u);
+        }
+    }
+}
+
+// The digits of 128 values of a row, by a warp, a lane four of them. digits: [half unit][row][digit][4 x 16 bytes] in the order the lanes
+// of the product read them; meta: [span][row][pair of digits] their sums and, twice, the activations' scale (16 bytes).
+// `unit` counts from where the two begin, `at` is the first value's place in the row.
+__device__ __forceinline__ void make_digits(const W4Params &p, int unit, int m, int at, int lane, uint8_t *digits, uint8_t *meta) {
+    const int lanes = 32 / p.spans;
+    float v[4];
+    load_four(p, m, at + lane * 4, v);
+    float top = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+    bool finite = true;                                          // (a maximum drops NaN)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) finite &= fabsf(v[t]) <= 3.4028235e38f;
+    for (int o = 1; o < lanes; o *= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+    const unsigned mask = lanes == 32 ? ~0u : (1u << lanes) - 1;
+    finite = (__ballot_sync(~0u, finite) >> (lane / lanes * lanes) & mask) == mask;
+    const int exponent = max(-90, static_cast<int>(__float_as_uint(top) >> 23) - 127);
+    const float up = __uint_as_float(static_cast<uint32_t>(127 + kTopBit - exponent) << 23);
+    const uint32_t unit_of = finite ? static_cast<uint32_t>(127 + exponent - kTopBit) << 23 : 0x7fffffffu;
+    int x[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) x[t] = finite ? __float2int_rn(v[t] * up) : 0;
+    const int in_half = lane * 4 % 64;
+    uint8_t *const to = digits + (static_cast<size_t>(unit * 2 + lane / 16) * p.rows + m) * (kDigits * 64) + in_half % 32 / 8 * 16 + in_half / 32 * 8 + in_half % 8;
+#pragma unroll
+    for (int pair = 0; pair < kDigits / 2; ++pair) {
+        int sums = 0;                                            // of two digits, 16 bits each: at most 128 * 128
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+            uint32_t bytes = 0;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int digit = static_cast<int8_t>(x[t]);     // what is left is a multiple of 256 then
+                bytes |= static_cast<uint32_t>(digit & 255) << (8 * t);
+                x[t] = (x[t] - digit) >> 8;
+                sums += digit << (16 * d);
+            }
+            *reinterpret_cast<uint32_t *>(to + (pair * 2 + d) * 64) = bytes;
+        }
+        for (int o = 1; o < lanes; o *= 2) sums += __shfl_xor_sync(~0u, sums, o);
+        const int first = static_cast<int16_t>(sums);
+        if (lane % lanes == 0)
+            *reinterpret_cast<uint4 *>(meta + ((static_cast<size_t>(unit * p.spans + lane / lanes) * p.rows + m) * (kDigits / 2) + pair) * 16) =
+                make_uint4(static_cast<uint32_t>(first), static_cast<uint32_t>((sums - first) >> 16), unit_of, unit_of);
+    }
+}
+
+// All digits into the workspace, a warp 128 values of a row.
+__global__ void w4_digits_kernel(const __grid_constant__ W4Params p) {
+    pdl_launch_dependents();
+    const int i = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+    if (i < p.units * p.rows) make_digits(p, i / p.rows, i % p.rows, i / p.rows * kUnitK, threadIdx.x % 32, p.digits_made, p.meta_made);
+}
+
+// Shared memory: sums, rings, digits, meta.
+template <int kTiles, int kAhead>
+__global__ void __launch_bounds__(kThreads, 1) w4_integer_kernel(const __grid_constant__ W4Params p) {
+    constexpr int kRows = kTiles * kTileRows;
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ Handover hand;
+    if (threadIdx.x == 0) {
+        barrier_init(&hand.full, kWarps);
+        barrier_init(&hand.empty, kSummers);
+    }
+    auto cluster = cooperative_groups::this_cluster();
+    const Share<kTiles> s(p, cluster.num_blocks(), cluster.block_rank());
+    const uint32_t smem_at = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
+    Units<kTiles, kAhead> units(p, s, smem_at + p.ring_at);
+    const int lane = s.lane, half_digits = p.rows * kDigits * 64, span_meta = p.rows * kDigits * 8;
+    if (p.digits_made) {
+        const uint8_t *digits = p.digits_made + static_cast<size_t>(s.begin) * 2 * half_digits, *meta = p.meta_made + static_cast<size_t>(s.begin) * p.spans * span_meta;
+        pdl_wait();
+        for (int i = threadIdx.x * 16; i < s.block_units * 2 * half_digits; i += kThreads * 16) copy16(smem_at + p.x_at + i, digits + i);
+        for (int i = threadIdx.x * 16; i < s.block_units * p.spans * span_meta; i += kThreads * 16) copy16(smem_at + p.meta_at + i, meta + i);
+        copy_commit();
+        copy_wait<0>();
+    } else {
+        for (int i = s.warp; i < s.block_units * p.rows; i += kWarps + kSummers)
+            make_digits(p, i / p.rows, i % p.rows, (s.begin + i / p.rows) * kUnitK, lane, smem + p.x_at, smem + p.meta_at);
+    }
+    __syncthreads();
+    // (columns beyond the rows' digits are the last one's again; their sums go nowhere)
+    const uint32_t x_at = smem_at + p.x_at + 2 * (s.first - s.begin) * half_digits + min(lane / 4, p.rows * kDigits - 1) * 64 + lane % 4 * 16;
+    const uint32_t meta_at = smem_at + p.meta_at + (s.first - s.begin) * p.spans * span_meta + min(lane % 4, p.rows * kDigits / 2 - 1) * 16;
+    const int record = p.wide ? 16 : 8, span = 4 / p.spans;      // span: in steps of 32 values
+
+    float acc[kTiles][4];
+    const auto multiply = [&] {
+        int part[kTiles][4];
+#pragma unroll
+        for (int r = 0; r < kTiles; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                acc[r][i] = 0.f;
+                part[r][i] = kIntegerBase;
+            }
+        uint32_t x_now = x_at, meta_now = meta_at;
+#pragma unroll 1
+        for (int u = 0; u < s.count; ++u) {
+            units.wait();
+            uint4 now[2][kTiles], x[2];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                for (int r = 0; r < kTiles; ++r) now[half][r] = load_shared(units.slot + r * units.pitch + half * 512 + lane * 16);
+                x[half] = load_shared(x_now);
+                x_now += half_digits;
+            }
+#pragma unroll
+            for (int step = 0; step < 4; ++step) {
+                const int half = step / 2;
+#pragma unroll
+                for (int r = 0; r < kTiles; ++r) {
+                    const uint32_t w0 = step % 2 ? now[half][r].z : now[half][r].x, w8 = step % 2 ? now[half][r].w : now[half][r].y;
+                    const uint32_t a[4] = {w0 & 0x0f0f0f0fu, w8 & 0x0f0f0f0fu, w0 >> 4 & 0x0f0f0f0fu, w8 >> 4 & 0x0f0f0f0fu};
+                    mma_integer(part[r], a, step % 2 ? x[half].z : x[half].x, step % 2 ? x[half].w : x[half].y);
+                }
+                if (step == 3 || (step == 1 && span <= 2) || span == 1) {
+                    const uint4 meta = load_shared(meta_now);
+                    const float unit_of = __uint_as_float(meta.z);
+                    meta_now += span_meta;
+#pragma unroll
+                    for (int r = 0; r < kTiles; ++r) {
+                        float2 scale;
+                        uint32_t z0, z8;
+                        take_record(units.slot + r * units.pitch + kCodeBytes + (step / span * 8 + lane / 4) * record, p.wide, scale, z0, z8);
+                        const float factor[2] = {scale.x * unit_of, scale.y * unit_of};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int sum = part[r][i] - static_cast<int>(i < 2 ? z0 : z8) * static_cast<int>(i % 2 ? meta.y : meta.x);
+                            acc[r][i] = fmaf(factor[i / 2], __int_as_float(sum) - 12582912.f, acc[r][i]);
+                            part[r][i] = kIntegerBase;
+                        }
+                    }
+                }
+            }
+            units.next();
+        }
+    };
+    // lanes 4 i and 4 i + 2 have digits 0 and 1 of the two rows, their neighbours 2 and 3
+    const auto leave = [&](float *to) {
+#pragma unroll
+        for (int r = 0; r < kTiles; ++r)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float v = fmaf(acc[r][2 * i + 1], 256.f, acc[r][2 * i]);
+                v = fmaf(__shfl_down_sync(~0u, v, 1), 65536.f, v);
+                if (lane % 2 == 0) to[lane % 4 / 2 * kRows + r * kTileRows + lane / 4 + i * 8] = v;
+            }
+    };
+    turns<kTiles, kIntegerRows>(p, s, cluster, reinterpret_cast<float *>(smem), hand, multiply, leave);
+    copy_wait<0>();
+}
+
+// More rows: rows of the weights are the 16 rows of m16n8k16, activations its columns. Operands of the codes less zero point are made in
+// registers (exact); a span's products are summed on the tensor cores and its scale is applied to that sum in fp32.
+// kStaged: the activations are laid out as operands in shared memory once, in the order the lanes read them; otherwise they are read from
+// memory (the caches) for every tile.
+template <typename X, int kColumns, int kTiles, int kAhead, bool kStaged>
+__global__ void __launch_bounds__(kThreads, 1) w4_linear_kernel(const __grid_constant__ W4Params p) {
+    using H = typename Operand<X>::Type;
+    constexpr int kParts = Operand<X>::kParts, kRows = kTiles * kTileRows;
+    extern __shared__ __align__(16) uint8_t smem[];              // sums, rings, activations [part][step of 32 values][row][4 x 16 bytes]
+    __shared__ Handover hand;
+    if (threadIdx.x == 0) {
+        barrier_init(&hand.full, kWarps);
+        barrier_init(&hand.empty, kSummers);
+    }
+    auto cluster = cooperative_groups::this_cluster();
+    const Share<kTiles> s(p, cluster.num_blocks(), cluster.block_rank());
+    const uint32_t smem_at = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
+    Units<kTiles, kAhead> units(p, s, smem_at + p.ring_at);
+    const int lane = s.lane, part_pitch = 4 * s.block_units * p.rows * 64;
+    if (kStaged) {
+        for (int i = threadIdx.x; i < part_pitch / 16; i += kThreads) {
+            const int t = i % 4, m = i / 4 % p.rows, at = (s.begin * 4 + i / 4 / p.rows) * 32 + t * 8;
+            const X *row = static_cast<const X *>(p.x) + m * p.x_stride + at;
+            uint32_t b[kParts][4];
+            if (p.vectors && at + 8 <= p.k) load_x<X, true>(row, 8, b);
+            else load_x<X, false>(row, p.k - at, b);
+#pragma unroll
+            for (int part = 0; part < kParts; ++part)
+                *reinterpret_cast<uint4 *>(smem + p.x_at + part * part_pitch + i * 16) = make_uint4(b[part][0], b[part][1], b[part][2], b[part][3]);
+        }
+    }
+    __syncthreads();
+    // (a column beyond the rows is the last row again; its sums are not stored)
+    const int record = p.wide ? 16 : 8, span = 4 / p.spans;      // span: in steps of 32 values
+    const uint32_t staged_at = smem_at + p.x_at + (4 * (s.first - s.begin) * p.rows * 4 + lane % 4) * 16;
+    float acc[kTiles][kColumns][4];
+    const auto multiply = [&] {
+        float part[kTiles][kColumns][4] = {};
+#pragma unroll
+        for (int r = 0; r < kTiles; ++r)
+#pragma unroll
+            for (int c = 0; c < kColumns; ++c) acc[r][c][0] = acc[r][c][1] = acc[r][c][2] = acc[r][c][3] = 0.f;
+        uint32_t x_now = staged_at;
+        int k_now = s.first * kUnitK + lane % 4 * 8;
+        float2 scale[kTiles];
+        Zero<H> zero[kTiles][2];
+#pragma unroll 1
+        for (int u = 0; u < s.count; ++u) {
+            units.wait();
+#pragma unroll
+            for (int step = 0; step < 4; ++step) {
+                uint32_t a[kTiles][2][4];
+#pragma unroll
+                for (int r = 0; r < kTiles; ++r) {
+                    const uint32_t at = units.slot + r * units.pitch;
+                    if (step == 0 || (step == 2 && span <= 2) || span == 1) {
+                        uint32_t z0, z8;
+                        take_record(at + kCodeBytes + (step / span * 8 + lane / 4) * record, p.wide, scale[r], z0, z8);
+                        zero[r][0].set(z0);
+                        zero[r][1].set(z8);
+                    }
+                    uint2 now;
+                    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(now.x), "=r"(now.y) : "r"(at + step / 2 * 512 + lane * 16 + step % 2 * 8) : "memory");
+                    uint32_t low[4], high[4];
+                    zero[r][0].operand(now.x, p.exponents, low);
+                    zero[r][1].operand(now.y, p.exponents, high);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) { a[r][i][0] = low[2 * i]; a[r][i][1] = high[2 * i]; a[r][i][2] = low[2 * i + 1]; a[r][i][3] = high[2 * i + 1]; }
+                }
+#pragma unroll
+                for (int c = 0; c < kColumns; ++c) {
+                    const int m = min(c * 8 + lane / 4, p.rows - 1);
+                    uint32_t b[kParts][4];
+                    if (kStaged) {
+#pragma unroll
+                        for (int i = 0; i < kParts; ++i) {
+                            const uint4 v = load_shared(x_now + m * 64 + i * part_pitch);
+                            memcpy(b[i], &v, 16);
+                        }
+                    } else {
+                        const X *row = static_cast<const X *>(p.x) + m * p.x_stride + k_now;
+                        if (p.vectors && k_now + 8 <= p.k) load_x<X, true>(row, 8, b);
+                        else load_x<X, false>(row, p.k - k_now, b);
+                    }
+#pragma unroll
+                    for (int i = 0; i < kParts; ++i)
+#pragma unroll
+                        for (int r = 0; r < kTiles; ++r) {
+                            mma<H>(part[r][c], a[r][0], b[i][0], b[i][1]);
+                            mma<H>(part[r][c], a[r][1], b[i][2], b[i][3]);
+                        }
+                }
+                x_now += p.rows * 64;
+                k_now += 32;
+                if (step == 3 || (step == 1 && span <= 2) || span == 1)
+#pragma unroll
+                    for (int r = 0; r < kTiles; ++r)
+#pragma unroll
+                        for (int c = 0; c < kColumns; ++c)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                acc[r][c][i] = fmaf(i < 2 ? scale[r].x : scale[r].y, part[r][c][i], acc[r][c][i]);
+                                part[r][c][i] = 0.f;
+                            }
+            }
+            units.next();
+        }
+    };
+    const auto leave = [&](float *to) {
+#pragma unroll
+        for (int r = 0; r < kTiles; ++r)
+#pragma unroll
+            for (int c = 0; c < kColumns; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) to[(c * 8 + lane % 4 * 2 + i % 2) * kRows + r * kTileRows + lane / 4 + i / 2 * 8] = acc[r][c][i];
+    };
+    turns<kTiles, kColumns * 8>(p, s, cluster, reinterpret_cast<float *>(smem), hand, multiply, leave);
+    copy_wait<0>();
+}
+
+constexpr size_t kSmemMost = 224 * 1024;                         // of shared memory for a block
+
+template <typename Kernel>
+cudaError_t launch(const MsnhB200Ctx *ctx, Kernel kernel, std::atomic<uint64_t> &done, const W4Params &p, int blocks, int ranks, size_t smem, bool dependent, void *stream) {
+    // the attribute is a kernel's and a device's: set by the first call there
+    const uint64_t bit = 1ull << (ctx->device & 63);
+    if (!(done.load(std::memory_order_acquire) & bit)) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemMost));
+        if (e != cudaSuccess) return e;
+        done.fetch_or(bit, std::memory_order_release);
+    }
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(blocks * ranks);
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = smem;
+    config.stream = static_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ranks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = attr;
+    config.numAttrs = dependent ? 2 : 1;
+    return cudaLaunchKernelEx(&config, kernel, p);
+}
+
+// How many warps of a block share a tile's k: what takes the fewest units one after the other in the busiest warp (tiles at a time x units
+// of each), the more the better at the same count. Where that leaves SMs without a block, a cluster shares it further, down to two units
+// of k a warp; and where that is what makes room for the activations (x_bytes: of those of some units). Returns whether there is room.
+template <typename Bytes>
+bool share_out(const MsnhB200Ctx *ctx, W4Params &p, int tiles, Bytes x_bytes, int &ranks, int &blocks) {
+    const auto per_turn = [&](int split) { return kWarps / split * tiles; };
+    const auto up = [](int a, int b) { return (a + b - 1) / b; };
+    const auto cost = [&](int split) {
+        const int most = up(p.tiles, std::min(up(p.tiles, per_turn(split)), ctx->sm_count));
+        return static_cast<long long>(up(most, per_turn(split))) * up(p.units, split);
+    };
+    p.split = 1;
+    for (int split = 2; split <= kWarps && split <= p.units; split *= 2)
+        if (cost(split) <= cost(p.split)) p.split = split;
+    const int turns = up(p.tiles, per_turn(p.split));
+    const auto units = [&] { return std::min(p.units, p.split * up(p.units, p.split * ranks)); };
+    ranks = 1;
+    while (ranks < 8 && turns * ranks * 2 <= ctx->sm_count && p.split * ranks * 4 <= p.units) ranks *= 2;
+    const int wanted = ranks;
+    while (ranks < 8 && p.x_at + x_bytes(units()) > kSmemMost && p.split * ranks * 2 <= p.units) ranks *= 2;
+    const bool room = p.x_at + x_bytes(units()) <= kSmemMost;
+    if (!room) ranks = wanted;
+    p.share = up(p.units, p.split * ranks);
+    p.block_units = units();
+    blocks = std::min(turns, ctx->sm_count / ranks);
+    return room;
+}
+
+// Digits are made by every block for itself, or, where that is over kOwnDigits turns of its warps (1 us each), by a launch before it.
+constexpr int kOwnDigits = 2;
+size_t digit_bytes(int rows, int units) { return static_cast<size_t>(units) * 2 * rows * kDigits * 64; }
+size_t meta_bytes(int rows, int units, int spans) { return static_cast<size_t>(units) * spans * rows * kDigits * 8; }
+bool digits_apart(int rows, int units) { return rows <= kIntegerRows && rows * units > kOwnDigits * (kWarps + kSummers); }
+
+template <int kTiles, int kAhead>
+bool launch_integer(const MsnhB200Ctx *ctx, W4Params p, void *stream, cudaError_t &e) {
+    p.ring_at = kSumsOf<kTiles * kTileRows, kIntegerRows> * 4;
+    p.x_at = p.ring_at + kWarps * kAhead * kTiles * static_cast<int>(p.unit_bytes);
+    const auto bytes = [&](int units) { return digit_bytes(p.rows, units) + meta_bytes(p.rows, units, p.spans); };
+    int ranks, blocks;
+    if (!share_out(ctx, p, kTiles, bytes, ranks, blocks)) return false;
+    p.meta_at = p.x_at + static_cast<int>(digit_bytes(p.rows, p.block_units));
+    if (p.digits_made) {
+        p.meta_made = p.digits_made + digit_bytes(p.rows, p.units);
+        e = launch_token_kernel(w4_digits_kernel, dim3((p.units * p.rows + 3) / 4), 128, 0, stream, false, p);
+        if (e != cudaSuccess) return true;
+    }
+    static std::atomic<uint64_t> done{0};
+    e = launch(ctx, w4_integer_kernel<kTiles, kAhead>, done, p, blocks, ranks, p.x_at + bytes(p.block_units), p.digits_made && ctx->pdl, stream);
+    return true;
+}
+
+template <typename X, int kColumns, int kTiles, int kAhead>
+cudaError_t launch(const MsnhB200Ctx *ctx, W4Params p, void *stream) {
+    p.ring_at = kSumsOf<kTiles * kTileRows, kColumns * 8> * 4;
+    p.x_at = p.ring_at + kWarps * kAhead * kTiles * static_cast<int>(p.unit_bytes);
+    p.exponents = Zero<typename Operand<X>::Type>::kExponents;
+    const auto bytes = [&](int units) { return static_cast<size_t>(Operand<X>::kParts) * 4 * units * p.rows * 64; };
+    int ranks, blocks;
+    const bool staged = share_out(ctx, p, kTiles, bytes, ranks, blocks);
+    static std::atomic<uint64_t> done[2];
+    return staged ? launch(ctx, w4_linear_kernel<X, kColumns, kTiles, kAhead, true>, done[0], p, blocks, ranks, p.x_at + bytes(p.block_units), false, stream)
+                  : launch(ctx, w4_linear_kernel<X, kColumns, kTiles, kAhead, false>, done[1], p, blocks, ranks, p.x_at, false, stream);
+}
+
+template <typename X>
+cudaError_t launch(const MsnhB200Ctx *ctx, const W4Params &p, void *stream) {
+    if (p.rows <= kIntegerRows) {
+        // two tiles at a time where every SM has several
+        const bool two = p.unit_bytes <= 1152 && p.tiles >= 8 * ctx->sm_count;
+        cudaError_t e = cudaSuccess;
+        if (two ? launch_integer<2, 3>(ctx, p, stream, e) : launch_integer<1, 5>(ctx, p, stream, e)) return e;
+    }
+    if (p.rows <= 8) return launch<X, 1, 1, 5>(ctx, p, stream);
+    if (p.rows <= 16) return launch<X, 2, 1, 4>(ctx, p, stream);
+    if (p.rows <= 32) return launch<X, 4, 1, 4>(ctx, p, stream);
+    return launch<X, 8, 1, 3>(ctx, p, stream);
+}
+
+size_t workspace_of(const W4Layout &l, const MsnhB200W4Linear &a) {
+    if (a.rows < 1 || !digits_apart(a.rows, l.units)) return 0;
+    return digit_bytes(a.rows, l.units) + meta_bytes(a.rows, l.units, l.spans);
 }
 
 int check_weights(MsnhB200Ctx *ctx, const MsnhB200W4 *w, const char *what) {
@@ -117,11 +882,11 @@ int check_weights(MsnhB200Ctx *ctx, const MsnhB200W4 *w, const char *what) {
 }
 
 template <typename S, typename Out>
-cudaError_t launch_pack_scales(const W4Layout &l, const void *scales, const uint8_t *zeros, uint8_t *packed, void *stream) {
-    const long long count = static_cast<long long>(l.tiles) * l.groups * kTileRows;
+cudaError_t launch_pack_records(const W4Layout &l, const void *scales, const uint8_t *zeros, uint8_t *packed, void *stream) {
+    const long long count = static_cast<long long>(l.tiles) * l.units * l.spans * 8;
     const unsigned grid = static_cast<unsigned>(std::min<long long>((count + 255) / 256, 148 * 16));
-    return launch_token_kernel(w4_pack_scales_kernel<S, Out>, dim3(grid), 256, 0, stream, false, static_cast<const S *>(scales), zeros, l.n, l.groups, count,
-                               reinterpret_cast<Out *>(packed + l.scales_at), packed + l.zeros_at);
+    return launch_token_kernel(w4_pack_records_kernel<S, Out>, dim3(grid), 256, 0, stream, false, static_cast<const S *>(scales), zeros, l.n, l.k, l.units,
+                               l.spans, l.group, l.groups, l.unit_bytes, count, packed);
 }
 
 }  // namespace
@@ -150,19 +915,19 @@ int msnh_b200_w4_pack(MsnhB200Ctx *ctx, const MsnhB200W4 *w, const uint8_t *code
     CUDA_TRY(ctx, scope.status);
     const W4Layout l(*w);
     uint8_t *out = static_cast<uint8_t *>(packed);
-    const long long words = static_cast<long long>(l.tiles) * l.blocks * (kBlockBytes / 4);
+    const long long words = static_cast<long long>(l.tiles) * l.units * (kCodeBytes / 4);
     const unsigned grid = static_cast<unsigned>(std::min<long long>((words + 255) / 256, 148 * 32));
-    CUDA_TRY(ctx, launch_token_kernel(w4_pack_codes_kernel, dim3(grid), 256, 0, stream, false, codes, codes_stride, l.n, l.k, l.blocks, words, reinterpret_cast<uint32_t *>(out)));
-    CUDA_TRY(ctx, w->scale_dtype == MSNH_B200_F16  ? (launch_pack_scales<__half, __half>(l, scales, zeros, out, stream))
-                : w->scale_dtype == MSNH_B200_BF16 ? (launch_pack_scales<__nv_bfloat16, float>(l, scales, zeros, out, stream))
-                                                   : (launch_pack_scales<float, float>(l, scales, zeros, out, stream)));
+    CUDA_TRY(ctx, launch_token_kernel(w4_pack_codes_kernel, dim3(grid), 256, 0, stream, false, codes, codes_stride, l.n, l.k, l.units, l.unit_bytes, words, out));
+    CUDA_TRY(ctx, w->scale_dtype == MSNH_B200_F16  ? (launch_pack_records<__half, __half>(l, scales, zeros, out, stream))
+                : w->scale_dtype == MSNH_B200_BF16 ? (launch_pack_records<__nv_bfloat16, float>(l, scales, zeros, out, stream))
+                                                   : (launch_pack_records<float, float>(l, scales, zeros, out, stream)));
     return MSNH_B200_OK;
 } catch (...) { return caught(ctx); }
 
 int msnh_b200_w4_linear_workspace(MsnhB200Ctx *ctx, const MsnhB200W4 *w, const MsnhB200W4Linear *a, size_t *bytes) try {
     if (!ctx || !w || !a || !bytes) return MSNH_B200_ERR_ARG;
     if (const int rc = check_weights(ctx, w, "w4_linear_workspace")) return rc;
-    *bytes = 0;
+    *bytes = workspace_of(W4Layout(*w), *a);
     return MSNH_B200_OK;
 } catch (...) { return caught(ctx); }
 
@@ -179,12 +944,19 @@ int msnh_b200_w4_linear(MsnhB200Ctx *ctx, const MsnhB200W4 *w, const MsnhB200W4L
     DeviceScope scope(ctx->device);
     CUDA_TRY(ctx, scope.status);
     const W4Layout l(*w);
-    const W4Params p = {static_cast<const uint8_t *>(w->packed), a->x, a->y, a->x_scale, a->bias, a->x_stride, a->y_stride, l.scales_at, l.zeros_at,
-                        l.n, l.k, l.group, l.blocks, l.groups, a->rows, static_cast<int>(l.scale_size), w->has_zeros};
-    const cudaError_t e = a->dtype == MSNH_B200_F32  ? launch<float>(p, a->out_dtype, stream)
-                        : a->dtype == MSNH_B200_F16  ? launch<__half>(p, a->out_dtype, stream)
-                        : a->dtype == MSNH_B200_BF16 ? launch<__nv_bfloat16>(p, a->out_dtype, stream)
-                                                     : launch<__nv_fp8_e4m3>(p, a->out_dtype, stream);
+    const size_t wanted = workspace_of(l, *a);
+    if (wanted && (!a->workspace || a->workspace_bytes < wanted || !aligned16(a->workspace)))
+        return fail(ctx, MSNH_B200_ERR_ARG, "w4_linear: %zu bytes of workspace, 16-byte aligned, are wanted", wanted);
+    // eight values of x at a time where every row allows it
+    const size_t vector = 8 * dtype_size(a->dtype), piece = std::min<size_t>(vector, 16);
+    const int vectors = reinterpret_cast<uintptr_t>(a->x) % piece == 0 && (a->rows == 1 || a->x_stride * dtype_size(a->dtype) % piece == 0);
+    const W4Params p = {static_cast<const uint8_t *>(w->packed), a->x, a->y, a->x_scale, a->bias, a->x_stride, a->y_stride, static_cast<long long>(l.unit_bytes),
+                        l.n, l.k, l.tiles, l.units, a->rows, a->dtype, l.wide, l.spans, vectors, a->out_dtype, 0, 0, 0, 0, 0, 0, wanted ? static_cast<uint8_t *>(a->workspace) : nullptr, nullptr, ctx->dev_err_flag, 0};
+    if (const int rc = check_device_flag(ctx, ctx->err_flag)) return rc;        // (a call before this one)
+    const cudaError_t e = a->dtype == MSNH_B200_F32  ? launch<float>(ctx, p, stream)
+                        : a->dtype == MSNH_B200_F16  ? launch<__half>(ctx, p, stream)
+                        : a->dtype == MSNH_B200_BF16 ? launch<__nv_bfloat16>(ctx, p, stream)
+                                                     : launch<__nv_fp8_e4m3>(ctx, p, stream);
     CUDA_TRY(ctx, e);
     return MSNH_B200_OK;
 } catch (...) { return caught(ctx); }
