@@ -38,6 +38,159 @@ __device__ __forceinline__ void block_sum_max(float &sum, float &top) {
 // largest |t|. (1 / top is infinite below 2^-127; the division is exact there, too.)
 __device__ __forceinline__ float code_of(float t, float top, float inverse) { return top > 1e-30f ? t * inverse : t / top * 448.f; }
 
+__device__ __forceinline__ void copy16(uint32_t to, const void *from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
+
+// Rows that a block (or a warp, kWarp) keeps in registers: one pass over memory, whose bytes bound it. A thread has kVecs vectors of 16 bytes
+// of a row. With kStages it stays for every gridDim-th row and has the next kStages - 1 rows' vectors copied into shared memory meanwhile
+// (its own, so it waits for nothing but its own copies); in registers they would cost half of the threads that keep the memory busy.
+// 8-bit codes are h * w * (448 / max|h w|): the norm's factor cancels, so one reduction gives both the sum of squares and what the codes
+// need.
+template <typename T, typename W, bool k8, int kVecs, bool kWarp, int kStages>
+__global__ void __launch_bounds__(kWarp ? 128 : kStages ? 512 : 1024) rms_norm_vectors_kernel(const __grid_constant__ RmsNormParams p) {
+    constexpr int kVec = Vec16<T>::kVec, kParts = kVec * sizeof(W) / 16;
+    extern __shared__ __align__(16) uint4 rows_ahead[];          // [kStages][kVecs][x, residual][thread]
+    __shared__ float part[2][2][32];
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = kWarp ? 1 : blockDim.x / 32;
+    const int thread = kWarp ? lane : threadIdx.x, threads = kWarp ? 32 : blockDim.x, vectors = p.cols / kVec;
+    const long long step = kWarp ? static_cast<long long>(gridDim.x) * (blockDim.x / 32) : gridDim.x;
+    long long row = kWarp ? blockIdx.x * static_cast<long long>(blockDim.x / 32) + warp : blockIdx.x;
+    const auto x_of = [&](long long at) { return reinterpret_cast<const uint4 *>(static_cast<const T *>(p.x) + at * p.x_stride); };
+    const auto residual_of = [&](long long at) { return reinterpret_cast<const uint4 *>(static_cast<const T *>(p.residual) + at * p.residual_stride); };
+    const auto weights_of = [&](int v, float (&c)[kVec]) {
+        uint4 raw[kParts];
+#pragma unroll
+        for (int j = 0; j < kParts; ++j) raw[j] = __ldg(static_cast<const uint4 *>(p.weight) + v * kParts + j);
+        const W *values = reinterpret_cast<const W *>(raw);
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) c[j] = to_float(values[j]);
+    };
+    const uint32_t mine = static_cast<uint32_t>(__cvta_generic_to_shared(rows_ahead + threadIdx.x)), pitch = blockDim.x * 16;
+    long long ahead = row;
+    int filled = 0, stage = 0;
+    const auto copy_next = [&] {
+        if (ahead < p.rows) {
+            const uint4 *x = x_of(ahead), *residual = residual_of(ahead);
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) {
+                const int v = thread + i * threads;
+                const uint32_t to = mine + (filled * kVecs + i) * 2 * pitch;
+                if (v < vectors) {
+                    copy16(to, x + v);
+                    if (p.residual) copy16(to + pitch, residual + v);
+                }
+            }
+        }
+        copy_commit();
+        ahead += step;
+        filled = filled == kStages - 1 ? 0 : filled + 1;
+    };
+#pragma unroll 1
+    for (int i = 0; i < kStages - 1; ++i) copy_next();
+    for (int turn = 0; row < p.rows; row += step, turn ^= 1) {
+        if constexpr (kStages > 0) {
+            copy_next();
+            copy_wait<kStages - 1>();
+        }
+        float h[kVecs][kVec], sum = 0.f, top = 0.f;
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+            const int v = thread + i * threads;
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) h[i][j] = 0.f;
+            if (v >= vectors) continue;
+            uint4 x, r = make_uint4(0, 0, 0, 0);
+            if constexpr (kStages > 0) {
+                x = rows_ahead[((stage * kVecs + i) * 2) * blockDim.x + threadIdx.x];
+                if (p.residual) r = rows_ahead[((stage * kVecs + i) * 2 + 1) * blockDim.x + threadIdx.x];
+            } else {
+                x = x_of(row)[v];
+                if (p.residual) r = residual_of(row)[v];
+            }
+            float a[kVec], b[kVec];
+            Vec16<T>::unpack(x, a);
+            Vec16<T>::unpack(r, b);
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) {
+                h[i][j] = a[j] + b[j];
+                sum += h[i][j] * h[i][j];
+            }
+            if (p.residual_out) reinterpret_cast<uint4 *>(static_cast<T *>(p.residual_out) + row * p.residual_out_stride)[v] = Vec16<T>::pack(h[i]);
+            if constexpr (k8) {                                  // (h times weight is all that is needed from here on)
+                weights_of(v, b);
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) {
+                    h[i][j] *= b[j];
+                    top = fmaxf(top, fabsf(h[i][j]));
+                }
+            }
+        }
+        stage = stage == kStages - 1 ? 0 : stage + 1;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            sum += __shfl_xor_sync(~0u, sum, o);
+            if (k8) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+        }
+        if (!kWarp && warps > 1) {
+            // (two sets of places: the next row's are written while this one's may still be read)
+            if (lane == 0) { part[turn][0][warp] = sum; part[turn][1][warp] = top; }
+            __syncthreads();
+            sum = lane < warps ? part[turn][0][lane] : 0.f;
+            top = lane < warps ? part[turn][1][lane] : 0.f;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) {
+                sum += __shfl_xor_sync(~0u, sum, o);
+                if (k8) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+            }
+        }
+        const float factor = rsqrtf(sum / p.cols + p.eps);
+        if constexpr (k8) {
+            const float scale = top * factor / 448.f;
+            if (thread == 0) p.y_scale[row] = scale;
+            // (448 / top is infinite below 2^-119: both are taken times 2^64 there. No codes for a row without a scale.)
+            if (!(top > 1e-30f)) {
+                top *= 18446744073709551616.f;
+#pragma unroll
+                for (int i = 0; i < kVecs; ++i)
+#pragma unroll
+                    for (int j = 0; j < kVec; ++j) h[i][j] *= 18446744073709551616.f;
+            }
+            const float inverse = 448.f / top;
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) {
+                const int v = thread + i * threads;
+                if (v >= vectors) continue;
+                uint32_t codes[kVec / 4] = {};
+                if (scale > 0.f)
+#pragma unroll
+                    for (int j = 0; j < kVec / 4; ++j) {
+                        float c[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) c[k] = h[i][4 * j + k] * inverse;
+                        codes[j] = to_e4m3x2(c[0], c[1]) | static_cast<uint32_t>(to_e4m3x2(c[2], c[3])) << 16;
+                    }
+                uint32_t *to = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(p.y) + row * p.y_stride + v * kVec);
+                if constexpr (kVec == 8) *reinterpret_cast<uint2 *>(to) = make_uint2(codes[0], codes[1]);
+                else *to = codes[0];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) {
+                const int v = thread + i * threads;
+                if (v >= vectors) continue;
+                float c[kVec];
+                weights_of(v, c);
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) c[j] = h[i][j] * factor * c[j];
+                reinterpret_cast<uint4 *>(static_cast<T *>(p.y) + row * p.y_stride)[v] = Vec16<T>::pack(c);
+            }
+        }
+    }
+}
+
 // A block a row, two passes over it: the sum of squares and (8 bits) the largest |h * w|, then the outputs. Any row length,
 // alignment and stride.
 template <typename T, typename W, bool k8>
@@ -70,17 +223,57 @@ __global__ void rms_norm_rows_kernel(RmsNormParams p) {
     }
 }
 
-template <typename T, typename W>
-cudaError_t launch(const RmsNormParams &p, bool out8, void *stream) {
+template <typename T, typename W, bool k8, int kVecs, bool kWarp, int kStages>
+cudaError_t launch_vectors(const MsnhB200Ctx *ctx, const RmsNormParams &p, int vectors, void *stream) {
+    const auto kernel = rms_norm_vectors_kernel<T, W, k8, kVecs, kWarp, kStages>;
+    const int threads = kWarp ? 128 : (vectors + kVecs * 32 - 1) / (kVecs * 32) * 32, rows = kWarp ? 4 : 1;
+    const size_t smem = static_cast<size_t>(threads) * kVecs * 32 * kStages;
+    if (smem > 48 * 1024) {
+        // the attribute is a kernel's and a device's: set by the first call there
+        static std::atomic<uint64_t> done{0};
+        const uint64_t bit = 1ull << (ctx->device & 63);
+        if (!(done.load(std::memory_order_acquire) & bit)) {
+            const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 512 * kVecs * 32 * kStages);
+            if (e != cudaSuccess) return e;
+            done.fetch_or(bit, std::memory_order_release);
+        }
+    }
+    const long long all = (p.rows + rows - 1) / rows, blocks = kStages ? std::min<long long>(all, ctx->sm_count * static_cast<long long>(std::min<size_t>(1024 / threads, kStages ? (208 * 1024) / smem : 1))) : all;
+    return launch_token_kernel(kernel, dim3(static_cast<unsigned>(blocks)), threads, smem, stream, false, p);
+}
+
+// Many rows: a warp a row where that suffices (no barrier), or up to 512 threads that stay. Few rows: a vector a thread, so that a row's
+// bytes are all asked for at once.
+template <typename T, typename W, bool k8>
+cudaError_t launch(const MsnhB200Ctx *ctx, const RmsNormParams &p, bool aligned, void *stream) {
+    const int vectors = p.cols / Vec16<T>::kVec;
+    if (aligned && vectors <= 4096) {
+        if (p.rows >= 4 * ctx->sm_count && vectors <= 2048)
+            return vectors <= 32     ? launch_vectors<T, W, k8, 1, true, 3>(ctx, p, vectors, stream)
+                   : vectors <= 64   ? launch_vectors<T, W, k8, 2, true, 3>(ctx, p, vectors, stream)
+                   : vectors <= 128  ? launch_vectors<T, W, k8, 4, true, 3>(ctx, p, vectors, stream)
+                   : vectors <= 1024 ? launch_vectors<T, W, k8, 2, false, 3>(ctx, p, vectors, stream) : launch_vectors<T, W, k8, 4, false, 2>(ctx, p, vectors, stream);
+        return vectors <= 1024   ? launch_vectors<T, W, k8, 1, false, 0>(ctx, p, vectors, stream)
+               : vectors <= 2048 ? launch_vectors<T, W, k8, 2, false, 0>(ctx, p, vectors, stream) : launch_vectors<T, W, k8, 4, false, 0>(ctx, p, vectors, stream);
+    }
     const int threads = p.cols <= 256 ? 64 : p.cols <= 2048 ? 256 : 1024;
-    const dim3 grid(static_cast<unsigned>(p.rows));
-    return out8 ? launch_token_kernel(rms_norm_rows_kernel<T, W, true>, grid, threads, 0, stream, false, p)
-                : launch_token_kernel(rms_norm_rows_kernel<T, W, false>, grid, threads, 0, stream, false, p);
+    return launch_token_kernel(rms_norm_rows_kernel<T, W, k8>, dim3(static_cast<unsigned>(p.rows)), threads, 0, stream, false, p);
+}
+
+template <typename T, typename W>
+cudaError_t launch(const MsnhB200Ctx *ctx, const RmsNormParams &p, bool out8, void *stream) {
+    // whole vectors of 16 bytes (of codes: as many values) everywhere
+    constexpr int kVec = Vec16<T>::kVec;
+    const auto fits = [](const void *at, long long stride, size_t size, size_t bytes) { return reinterpret_cast<uintptr_t>(at) % bytes == 0 && stride * size % bytes == 0; };
+    const bool aligned = p.cols % kVec == 0 && fits(p.x, p.x_stride, sizeof(T), 16) && fits(p.residual, p.residual ? p.residual_stride : 0, sizeof(T), 16) &&
+                         fits(p.residual_out, p.residual_out ? p.residual_out_stride : 0, sizeof(T), 16) && aligned16(p.weight) &&
+                         fits(p.y, p.y_stride, out8 ? 1 : sizeof(T), out8 ? kVec : 16);
+    return out8 ? launch<T, W, true>(ctx, p, aligned, stream) : launch<T, W, false>(ctx, p, aligned, stream);
 }
 
 template <typename T>
-cudaError_t launch(const RmsNormParams &p, int weight_dtype, bool out8, void *stream) {
-    return weight_dtype == MSNH_B200_F32 ? launch<T, float>(p, out8, stream) : launch<T, T>(p, out8, stream);
+cudaError_t launch(const MsnhB200Ctx *ctx, const RmsNormParams &p, int weight_dtype, bool out8, void *stream) {
+    return weight_dtype == MSNH_B200_F32 ? launch<T, float>(ctx, p, out8, stream) : launch<T, T>(ctx, p, out8, stream);
 }
 
 }  // namespace
@@ -106,9 +299,9 @@ extern "C" int msnh_b200_rms_norm(MsnhB200Ctx *ctx, const MsnhB200RmsNorm *a, vo
     CUDA_TRY(ctx, scope.status);
     const RmsNormParams p = {a->x, a->residual, a->weight, a->residual_out, a->y, a->y_scale, a->rows, a->x_stride, a->residual_stride,
                              a->residual_out_stride, a->y_stride, a->cols, a->eps};
-    const cudaError_t e = a->dtype == MSNH_B200_F32 ? launch<float, float>(p, out8, stream)
-                        : a->dtype == MSNH_B200_F16 ? launch<__half>(p, a->weight_dtype, out8, stream)
-                                                    : launch<__nv_bfloat16>(p, a->weight_dtype, out8, stream);
+    const cudaError_t e = a->dtype == MSNH_B200_F32 ? launch<float, float>(ctx, p, out8, stream)
+                        : a->dtype == MSNH_B200_F16 ? launch<__half>(ctx, p, a->weight_dtype, out8, stream)
+                                                    : launch<__nv_bfloat16>(ctx, p, a->weight_dtype, out8, stream);
     CUDA_TRY(ctx, e);
     return MSNH_B200_OK;
 } catch (...) { return caught(ctx); }
