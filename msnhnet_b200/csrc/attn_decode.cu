@@ -12,7 +12,6 @@
 // A warp copies its tiles through a ring of its own with cp.async (rows of 16-byte pieces, gathered page by page), running on into the
 // tiles of its next pair while it works on this one's, and keeps running maximum, sum and values of the query heads in registers. Warps
 // wait for nobody. 16-bit caches: m16n8k16. fp32 caches: CUDA cores (tf32 would lose 13 bits of the products).
-#include "common.cuh"
 #include "kv_cache.h"
 #include "token_types.cuh"
 
@@ -480,7 +479,7 @@ __global__ void __launch_bounds__(Heads::kWarps * 32, Heads::kBlocks) attn_decod
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ Side<Heads> side;
     constexpr int kWarps = Heads::kWarps, kThreads = kWarps * 32, kStages = Heads::kStages;
-    pdl_launch_dependents();
+    pdl_enter();
     const int pairs = p.c.heads * p.chunks, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     long long line = 0;
     for (int base = 0; base < p.rows; base += kThreads) {
@@ -629,7 +628,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_co
     constexpr int kWarps = kJoinThreads / 32;
     __shared__ float4 values[kWarps][64];
     __shared__ float2 state[kWarps];
-    pdl_wait();
+    pdl_enter();
     const int row = blockIdx.x, head = blockIdx.y, kv = head / p.each, chunk = head % p.each / p.chunk, in_chunk = head % p.each % p.chunk;
     const int pairs = p.c.heads * p.chunks, dim = p.c.dim;
     const long long before = p.prefix[row], after = p.prefix[row + 1], line = p.prefix[p.rows], length = quotient(after - before, pairs);
@@ -714,37 +713,37 @@ AttnPlan plan_of(const MsnhB200Ctx *ctx, const MsnhB200KvCache &c, const MsnhB20
 }
 
 template <typename Heads>
-cudaError_t launch(int device, const AttnParams &p, int blocks, void *stream) {
+cudaError_t launch(const MsnhB200Ctx *ctx, const AttnParams &p, int blocks, void *stream) {
     // the attribute is a kernel's and a device's: set by the first call there
     static std::atomic<uint64_t> done{0};
-    const uint64_t bit = 1ull << (device & 63);
+    const uint64_t bit = 1ull << (ctx->device & 63);
     if (!(done.load(std::memory_order_acquire) & bit)) {
         const cudaError_t e = cudaFuncSetAttribute(attn_decode_kernel<Heads>, cudaFuncAttributeMaxDynamicSharedMemorySize, Heads::kWarps * Ring<typename Heads::Type, Heads::kDim, Heads::kStages>::kBytes);
         if (e != cudaSuccess) return e;
         done.fetch_or(bit, std::memory_order_release);
     }
-    return launch_token_kernel(attn_decode_kernel<Heads>, dim3(blocks), Heads::kWarps * 32, Heads::kWarps * Ring<typename Heads::Type, Heads::kDim, Heads::kStages>::kBytes, stream, false, p);
+    return launch_token_kernel(attn_decode_kernel<Heads>, dim3(blocks), Heads::kWarps * 32, Heads::kWarps * Ring<typename Heads::Type, Heads::kDim, Heads::kStages>::kBytes, stream, ctx->pdl, p);
 }
 
 // Ring depths and blocks of an SM: as far as the shared memory goes.
 template <typename T>
-cudaError_t launch16(int device, const AttnParams &p, int blocks, void *stream) {
+cudaError_t launch16(const MsnhB200Ctx *ctx, const AttnParams &p, int blocks, void *stream) {
     const bool few = p.chunk <= 8;
-    if (p.c.dim <= 32) return few ? launch<TensorHeads<T, 32, 1, 8, 2>>(device, p, blocks, stream) : launch<TensorHeads<T, 32, 2, 8, 2>>(device, p, blocks, stream);
-    if (p.c.dim <= 64) return few ? launch<TensorHeads<T, 64, 1, 5, 2>>(device, p, blocks, stream) : launch<TensorHeads<T, 64, 2, 5, 2>>(device, p, blocks, stream);
-    if (p.c.dim <= 96) return few ? launch<TensorHeads<T, 96, 1, 4, 2>>(device, p, blocks, stream) : launch<TensorHeads<T, 96, 2, 4, 2>>(device, p, blocks, stream);
-    if (p.c.dim <= 128) return few ? launch<TensorHeads<T, 128, 1, 3, 2>>(device, p, blocks, stream) : launch<TensorHeads<T, 128, 2, 3, 2>>(device, p, blocks, stream);
-    if (p.c.dim <= 192) return few ? launch<TensorHeads<T, 192, 1, 4, 1>>(device, p, blocks, stream) : launch<TensorHeads<T, 192, 2, 4, 1>>(device, p, blocks, stream);
-    return few ? launch<TensorHeads<T, 256, 1, 3, 1>>(device, p, blocks, stream) : launch<TensorHeads<T, 256, 2, 3, 1>>(device, p, blocks, stream);
+    if (p.c.dim <= 32) return few ? launch<TensorHeads<T, 32, 1, 8, 2>>(ctx, p, blocks, stream) : launch<TensorHeads<T, 32, 2, 8, 2>>(ctx, p, blocks, stream);
+    if (p.c.dim <= 64) return few ? launch<TensorHeads<T, 64, 1, 5, 2>>(ctx, p, blocks, stream) : launch<TensorHeads<T, 64, 2, 5, 2>>(ctx, p, blocks, stream);
+    if (p.c.dim <= 96) return few ? launch<TensorHeads<T, 96, 1, 4, 2>>(ctx, p, blocks, stream) : launch<TensorHeads<T, 96, 2, 4, 2>>(ctx, p, blocks, stream);
+    if (p.c.dim <= 128) return few ? launch<TensorHeads<T, 128, 1, 3, 2>>(ctx, p, blocks, stream) : launch<TensorHeads<T, 128, 2, 3, 2>>(ctx, p, blocks, stream);
+    if (p.c.dim <= 192) return few ? launch<TensorHeads<T, 192, 1, 4, 1>>(ctx, p, blocks, stream) : launch<TensorHeads<T, 192, 2, 4, 1>>(ctx, p, blocks, stream);
+    return few ? launch<TensorHeads<T, 256, 1, 3, 1>>(ctx, p, blocks, stream) : launch<TensorHeads<T, 256, 2, 3, 1>>(ctx, p, blocks, stream);
 }
 template <int kHeads>
-cudaError_t launch32(int device, const AttnParams &p, int blocks, void *stream) {
-    if (p.c.dim <= 32) return launch<PlainHeads<32, kHeads, 8, 4>>(device, p, blocks, stream);
-    if (p.c.dim <= 64) return launch<PlainHeads<64, kHeads, 5, 4>>(device, p, blocks, stream);
-    if (p.c.dim <= 96) return launch<PlainHeads<96, kHeads, 4, 4>>(device, p, blocks, stream);
-    if (p.c.dim <= 128) return launch<PlainHeads<128, kHeads, 3, 4>>(device, p, blocks, stream);
-    if (p.c.dim <= 192) return launch<PlainHeads<192, kHeads, 3, 2>>(device, p, blocks, stream);
-    return launch<PlainHeads<256, kHeads, 3, 2>>(device, p, blocks, stream);
+cudaError_t launch32(const MsnhB200Ctx *ctx, const AttnParams &p, int blocks, void *stream) {
+    if (p.c.dim <= 32) return launch<PlainHeads<32, kHeads, 8, 4>>(ctx, p, blocks, stream);
+    if (p.c.dim <= 64) return launch<PlainHeads<64, kHeads, 5, 4>>(ctx, p, blocks, stream);
+    if (p.c.dim <= 96) return launch<PlainHeads<96, kHeads, 4, 4>>(ctx, p, blocks, stream);
+    if (p.c.dim <= 128) return launch<PlainHeads<128, kHeads, 3, 4>>(ctx, p, blocks, stream);
+    if (p.c.dim <= 192) return launch<PlainHeads<192, kHeads, 3, 2>>(ctx, p, blocks, stream);
+    return launch<PlainHeads<256, kHeads, 3, 2>>(ctx, p, blocks, stream);
 }
 
 // Many pairs have few parts each, and their blocks should all be there at once; few pairs have many.
@@ -800,10 +799,10 @@ int msnh_b200_attn_decode(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, const Msnh
         p.rows = std::min(l.rows, a->rows - row);
         cudaError_t e;
         if (c->dtype == MSNH_B200_F32)
-            e = l.chunk == 1 ? launch32<1>(ctx->device, p, l.blocks, stream) : l.chunk <= 4 ? launch32<4>(ctx->device, p, l.blocks, stream)
-                                                                                           : launch32<8>(ctx->device, p, l.blocks, stream);
+            e = l.chunk == 1 ? launch32<1>(ctx, p, l.blocks, stream) : l.chunk <= 4 ? launch32<4>(ctx, p, l.blocks, stream)
+                                                                                           : launch32<8>(ctx, p, l.blocks, stream);
         else
-            e = c->dtype == MSNH_B200_F16 ? launch16<__half>(ctx->device, p, l.blocks, stream) : launch16<__nv_bfloat16>(ctx->device, p, l.blocks, stream);
+            e = c->dtype == MSNH_B200_F16 ? launch16<__half>(ctx, p, l.blocks, stream) : launch16<__nv_bfloat16>(ctx, p, l.blocks, stream);
         CUDA_TRY(ctx, e);
         if (l.whole) continue;
         e = c->dtype == MSNH_B200_F32 ? launch_join<float>(ctx, p, l.workers, stream) : c->dtype == MSNH_B200_F16 ? launch_join<__half>(ctx, p, l.workers, stream)

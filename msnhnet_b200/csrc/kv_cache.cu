@@ -2,9 +2,9 @@
 //
 // Append, fork and compact are two launches: one block decides (which pages, in what order: the lowest free ones first, by a scan
 // over the page counts, so the result does not depend on timing) and writes its decisions into the workspace, then a grid moves the
-// rows. The second launch may be scheduled while the first runs.
-#include "common.cuh"
+// rows. Every launch may be scheduled while the one before it runs, and waits for it (pdl_enter).
 #include "kv_cache.h"
+#include "token_types.cuh"
 
 namespace msnh {
 namespace {
@@ -34,15 +34,37 @@ __device__ __forceinline__ int block_scan(int value, int *total) {
     return before + sum - value;
 }
 
+// Page counts of kEach pages from `first` on (1, a count that is none's business, beyond the last).
+constexpr int kEach = 8;
+__device__ __forceinline__ void load_refs(const KvParams &c, int first, int (&refs)[kEach]) {
+    if (first + kEach <= c.n_pages && reinterpret_cast<uintptr_t>(c.refs) % 16 == 0) {
+#pragma unroll
+        for (int i = 0; i < kEach / 4; ++i) {
+            const int4 v = reinterpret_cast<const int4 *>(c.refs + first)[i];
+            refs[4 * i] = v.x; refs[4 * i + 1] = v.y; refs[4 * i + 2] = v.z; refs[4 * i + 3] = v.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) refs[i] = first + i < c.n_pages ? c.refs[first + i] : 1;
+    }
+}
+
 // The `need` lowest free pages, in order, into list; returns how many there are of them (at most need). For the whole block.
 __device__ int lowest_free(const KvParams &c, int need, int *list) {
     int found = 0;
-    for (int base = 0; base < c.n_pages && found < need; base += kDecide) {
-        const int page = base + threadIdx.x;
-        const bool is_free = page < c.n_pages && c.refs[page] == 0;
-        int total;
-        const int rank = found + block_scan(is_free, &total);
-        if (is_free && rank < need) list[rank] = page;
+    for (long long base = 0; base < c.n_pages && found < need; base += kDecide * kEach) {
+        const int first = static_cast<int>(min(base + threadIdx.x * kEach, static_cast<long long>(c.n_pages)));
+        int refs[kEach], mine = 0;
+        load_refs(c, first, refs);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) mine += refs[i] == 0;
+        int total, rank = found + block_scan(mine, &total);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            if (refs[i] == 0) {
+                if (rank < need) list[rank] = first + i;
+                ++rank;
+            }
         found += total;
     }
     __syncthreads();
@@ -53,7 +75,7 @@ __device__ int lowest_free(const KvParams &c, int need, int *list) {
 struct AppendWork { int first, need, had, start; };              // first of its pages in the list; start: the length before, -1: refused
 
 __global__ void kv_append_decide_kernel(KvParams c, const int *seqs, const int *starts, int n, int n_tokens, AppendWork *work, int *list) {
-    pdl_launch_dependents();
+    pdl_enter();
     int all = 0;
     for (int base = 0; base < n; base += kDecide) {
         const int i = base + threadIdx.x;
@@ -99,7 +121,7 @@ __global__ void kv_append_decide_kernel(KvParams c, const int *seqs, const int *
 template <typename Unit>
 __global__ void kv_append_write_kernel(KvParams c, const int *seqs, const int *starts, int n, int n_tokens, const AppendWork *work, const Unit *k_new,
                                        const Unit *v_new, long long token_stride, long long head_stride, int units) {
-    pdl_wait();
+    pdl_enter();
     const int per_token = c.heads * units;
     const long long total = static_cast<long long>(n_tokens) * per_token;
     for (long long u = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; u < total; u += static_cast<long long>(gridDim.x) * blockDim.x) {
@@ -126,24 +148,44 @@ __global__ void kv_append_write_kernel(KvParams c, const int *seqs, const int *s
     }
 }
 
-// The first `rows` tokens of page src to page dst, keys and values, by threads `first`, first + step, ...
+// The first `rows` tokens of page src to page dst, keys and values, by threads `first`, first + step, ... Four units a turn, so that their
+// reads are under way together.
 template <typename Unit>
 __device__ __forceinline__ void copy_rows(const KvParams &c, int src, int dst, int rows, int units, int first, int step) {
     const Unit *k = reinterpret_cast<const Unit *>(c.k) + src * c.k_page, *v = reinterpret_cast<const Unit *>(c.v) + src * c.v_page;
     Unit *k_to = reinterpret_cast<Unit *>(c.k) + dst * c.k_page, *v_to = reinterpret_cast<Unit *>(c.v) + dst * c.v_page;
     const int per_token = c.heads * units, total = rows * per_token;
-    for (int u = first; u < total; u += step) {
-        const int place = u / per_token, head = u % per_token / units, unit = u % units;
-        const long long at_k = place * c.k_token + head * c.k_head + unit, at_v = place * c.v_token + head * c.v_head + unit;
-        k_to[at_k] = k[at_k];
-        v_to[at_v] = v[at_v];
+    const bool flat = c.k_token == per_token && c.v_token == per_token && c.k_head == units && c.v_head == units;     // tokens one behind the other
+    for (int base = first; base < total; base += 4 * step) {
+        long long at_k[4], at_v[4];
+        Unit a[4], b[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int u = base + i * step;
+            if (u >= total) break;
+            if (flat) {
+                at_k[i] = at_v[i] = u;
+            } else {
+                const int place = u / per_token, head = u % per_token / units, unit = u % units;
+                at_k[i] = place * c.k_token + head * c.k_head + unit;
+                at_v[i] = place * c.v_token + head * c.v_head + unit;
+            }
+            a[i] = k[at_k[i]];
+            b[i] = v[at_v[i]];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (base + i * step >= total) break;
+            k_to[at_k[i]] = a[i];
+            v_to[at_v[i]] = b[i];
+        }
     }
 }
 
 struct ForkWork { int from, to, rows, full; };                   // the copied page and its rows (to < 0: none); full < 0: refused
 
 __global__ void kv_fork_decide_kernel(KvParams c, const int *src, const int *dst, int n, ForkWork *work, int *list) {
-    pdl_launch_dependents();
+    pdl_enter();
     int all = 0;
     for (int base = 0; base < n; base += kDecide) {
         const int i = base + threadIdx.x;
@@ -189,7 +231,7 @@ __global__ void kv_fork_decide_kernel(KvParams c, const int *src, const int *dst
 
 template <typename Unit>
 __global__ void kv_fork_copy_kernel(KvParams c, const int *src, const int *dst, const ForkWork *work, int units) {
-    pdl_wait();
+    pdl_enter();
     const ForkWork w = work[blockIdx.x];
     if (w.full < 0) return;
     const long long a = src[blockIdx.x] * c.table_stride, b = dst[blockIdx.x] * c.table_stride;
@@ -204,6 +246,7 @@ __global__ void kv_fork_copy_kernel(KvParams c, const int *src, const int *dst, 
 
 __global__ void kv_free_kernel(KvParams c, const int *seqs) {
     __shared__ int length;
+    pdl_enter();
     const int s = seqs[blockIdx.x];
     if (s < 0 || s >= c.n_seqs) {
         if (threadIdx.x == 0) atomicAdd(c.refused, 1);
@@ -220,27 +263,43 @@ __global__ void kv_free_kernel(KvParams c, const int *seqs) {
 
 // work: [0] the number of moves, then n_pages each: where a page's contents go, the moves' destinations, their sources
 __global__ void kv_compact_decide_kernel(KvParams c, int *refs_out, int *work) {
-    pdl_launch_dependents();
+    pdl_enter();
     int *where = work + 1, *to = where + c.n_pages, *from = to + c.n_pages;
     int live = 0;
-    for (int page = threadIdx.x; page < c.n_pages; page += kDecide) live += c.refs[page] != 0;
+    for (long long base = 0; base < c.n_pages; base += kDecide * kEach) {
+        const int first = static_cast<int>(min(base + threadIdx.x * kEach, static_cast<long long>(c.n_pages)));
+        int refs[kEach];
+        load_refs(c, first, refs);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) live += refs[i] != 0 && first + i < c.n_pages;
+    }
     int n_live;
     block_scan(live, &n_live);
     int holes = 0, movers = 0;
-    for (int base = 0; base < c.n_pages; base += kDecide) {
-        const int page = base + threadIdx.x;
-        const int count = page < c.n_pages ? c.refs[page] : 0;
-        const bool hole = page < n_live && count == 0, mover = page >= n_live && page < c.n_pages && count != 0;
+    for (long long base = 0; base < c.n_pages; base += kDecide * kEach) {
+        const int first = static_cast<int>(min(base + threadIdx.x * kEach, static_cast<long long>(c.n_pages)));
+        int refs[kEach], mine = 0;                               // holes in the low half, movers in the high one (at most 8192 of each)
+        load_refs(c, first, refs);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int page = first + i;
+            if (page < n_live) mine += refs[i] == 0;
+            else if (page < c.n_pages) mine += (refs[i] != 0) << 16;
+        }
         int total;
-        const int rank = block_scan(static_cast<int>(hole) + (static_cast<int>(mover) << 16), &total);   // (at most kDecide of each)
-        if (hole) to[holes + (rank & 0xffff)] = page;
-        if (mover) from[movers + (rank >> 16)] = page;
+        const int rank = block_scan(mine, &total);
+        int hole = holes + (rank & 0xffff), mover = movers + (rank >> 16);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int page = first + i;
+            if (page >= c.n_pages) break;
+            if (page < n_live && refs[i] == 0) to[hole++] = page;
+            if (page >= n_live && refs[i] != 0) from[mover++] = page;
+            where[page] = page;
+            if (refs_out != c.refs) refs_out[page] = refs[i];
+        }
         holes += total & 0xffff;
         movers += total >> 16;
-        if (page < c.n_pages) {
-            where[page] = page;
-            if (refs_out != c.refs) refs_out[page] = count;
-        }
     }
     __syncthreads();
     for (int i = threadIdx.x; i < movers; i += kDecide) {
@@ -253,7 +312,7 @@ __global__ void kv_compact_decide_kernel(KvParams c, int *refs_out, int *work) {
 
 template <typename Unit>
 __global__ void kv_compact_move_kernel(KvParams c, const int *work, int *table_out, int units) {
-    pdl_wait();
+    pdl_enter();
     const int moves = work[0];
     const int *where = work + 1, *to = where + c.n_pages, *from = to + c.n_pages;
     const long long entries = static_cast<long long>(c.n_seqs) * c.max_pages;
@@ -268,6 +327,7 @@ __global__ void kv_compact_move_kernel(KvParams c, const int *work, int *table_o
 
 template <typename Unit>
 __global__ void kv_copy_pages_kernel(KvParams c, const int *src, const int *dst, int n, int units) {
+    pdl_enter();
     for (int i = blockIdx.x; i < n; i += gridDim.x) {
         const int a = src[i], b = dst[i];
         if (a < 0 || a >= c.n_pages || b < 0 || b >= c.n_pages || a == b) {
@@ -331,7 +391,7 @@ int msnh_b200_kv_append(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, const int32_
     AppendWork *work = static_cast<AppendWork *>(workspace);
     int *list = reinterpret_cast<int *>(work + n);
     const KvParams p = kv_params(*c);
-    CUDA_TRY(ctx, launch_token_kernel(kv_append_decide_kernel, dim3(1), kDecide, 0, stream, false, p, seqs, starts, n, n_tokens, work, list));
+    CUDA_TRY(ctx, launch_token_kernel(kv_append_decide_kernel, dim3(1), kDecide, 0, stream, ctx->pdl, p, seqs, starts, n, n_tokens, work, list));
     if (n_tokens == 0) return MSNH_B200_OK;
     const size_t size = dtype_size(c->dtype);
     const bool wide = kv_rows_multiple_of(*c, 16) && aligned16(k_new) && aligned16(v_new) && new_token_stride * size % 16 == 0 && new_head_stride * size % 16 == 0;
@@ -341,7 +401,7 @@ int msnh_b200_kv_append(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, const int32_
     const dim3 grid(blocks_for(ctx, static_cast<long long>(n_tokens) * c->n_kv_heads * units, 256));
     const auto write = [&](auto unit) {
         using Unit = decltype(unit);
-        return launch_token_kernel(kv_append_write_kernel<Unit>, grid, 256, 0, stream, true, q, seqs, starts, n, n_tokens, work, static_cast<const Unit *>(k_new),
+        return launch_token_kernel(kv_append_write_kernel<Unit>, grid, 256, 0, stream, ctx->pdl, q, seqs, starts, n, n_tokens, work, static_cast<const Unit *>(k_new),
                                    static_cast<const Unit *>(v_new), new_token_stride / per, new_head_stride / per, units);
     };
     CUDA_TRY(ctx, wide ? write(uint4()) : size == 4 ? write(uint32_t()) : write(uint16_t()));
@@ -361,13 +421,13 @@ int msnh_b200_kv_fork(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, const int32_t 
     ForkWork *work = static_cast<ForkWork *>(workspace);
     int *list = reinterpret_cast<int *>(work + n);
     const KvParams p = kv_params(*c);
-    CUDA_TRY(ctx, launch_token_kernel(kv_fork_decide_kernel, dim3(1), kDecide, 0, stream, false, p, src, dst, n, work, list));
+    CUDA_TRY(ctx, launch_token_kernel(kv_fork_decide_kernel, dim3(1), kDecide, 0, stream, ctx->pdl, p, src, dst, n, work, list));
     const size_t size = dtype_size(c->dtype);
     const bool wide = kv_rows_multiple_of(*c, 16);
     int units;
     const KvParams q = in_units(p, size, wide ? 16 : size, &units);
     const dim3 grid(n, std::max(1, std::min(8, 2 * ctx->sm_count / n)));
-    const auto copy = [&](auto unit) { return launch_token_kernel(kv_fork_copy_kernel<decltype(unit)>, grid, 256, 0, stream, true, q, src, dst, work, units); };
+    const auto copy = [&](auto unit) { return launch_token_kernel(kv_fork_copy_kernel<decltype(unit)>, grid, 256, 0, stream, ctx->pdl, q, src, dst, work, units); };
     CUDA_TRY(ctx, wide ? copy(uint4()) : size == 4 ? copy(uint32_t()) : copy(uint16_t()));
     return MSNH_B200_OK;
 } catch (...) { return caught(ctx); }
@@ -380,7 +440,7 @@ int msnh_b200_kv_free(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, const int32_t 
     if (!seqs) return fail(ctx, MSNH_B200_ERR_ARG, "kv_free: null seqs");
     DeviceScope scope(ctx->device);
     CUDA_TRY(ctx, scope.status);
-    CUDA_TRY(ctx, launch_token_kernel(kv_free_kernel, dim3(n), 128, 0, stream, false, kv_params(*c), seqs));
+    CUDA_TRY(ctx, launch_token_kernel(kv_free_kernel, dim3(n), 128, 0, stream, ctx->pdl, kv_params(*c), seqs));
     return MSNH_B200_OK;
 } catch (...) { return caught(ctx); }
 
@@ -394,13 +454,13 @@ int msnh_b200_kv_compact(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, int32_t *ta
     CUDA_TRY(ctx, scope.status);
     int *work = static_cast<int *>(workspace);
     const KvParams p = kv_params(*c);
-    CUDA_TRY(ctx, launch_token_kernel(kv_compact_decide_kernel, dim3(1), kDecide, 0, stream, false, p, refs_out, work));
+    CUDA_TRY(ctx, launch_token_kernel(kv_compact_decide_kernel, dim3(1), kDecide, 0, stream, ctx->pdl, p, refs_out, work));
     const size_t size = dtype_size(c->dtype);
     const bool wide = kv_rows_multiple_of(*c, 16);
     int units;
     const KvParams q = in_units(p, size, wide ? 16 : size, &units);
     const dim3 grid(blocks_for(ctx, std::max<long long>(c->n_pages, static_cast<long long>(c->n_seqs) * c->max_pages / 256), 1));
-    const auto move = [&](auto unit) { return launch_token_kernel(kv_compact_move_kernel<decltype(unit)>, grid, 256, 0, stream, true, q, work, table_out, units); };
+    const auto move = [&](auto unit) { return launch_token_kernel(kv_compact_move_kernel<decltype(unit)>, grid, 256, 0, stream, ctx->pdl, q, work, table_out, units); };
     CUDA_TRY(ctx, wide ? move(uint4()) : size == 4 ? move(uint32_t()) : move(uint16_t()));
     return MSNH_B200_OK;
 } catch (...) { return caught(ctx); }
@@ -418,7 +478,7 @@ int msnh_b200_kv_copy_pages(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, const in
     int units;
     const KvParams q = in_units(kv_params(*c), size, wide ? 16 : size, &units);
     const dim3 grid(blocks_for(ctx, n, 1));
-    const auto copy = [&](auto unit) { return launch_token_kernel(kv_copy_pages_kernel<decltype(unit)>, grid, 256, 0, stream, false, q, src, dst, n, units); };
+    const auto copy = [&](auto unit) { return launch_token_kernel(kv_copy_pages_kernel<decltype(unit)>, grid, 256, 0, stream, ctx->pdl, q, src, dst, n, units); };
     CUDA_TRY(ctx, wide ? copy(uint4()) : size == 4 ? copy(uint32_t()) : copy(uint16_t()));
     return MSNH_B200_OK;
 } catch (...) { return caught(ctx); }

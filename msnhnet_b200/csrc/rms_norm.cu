@@ -68,6 +68,7 @@ __global__ void __launch_bounds__(kWarp ? 128 : kStages ? 512 : 1024) rms_norm_v
 #pragma unroll
         for (int j = 0; j < kVec; ++j) c[j] = to_float(values[j]);
     };
+    pdl_enter();
     const uint32_t mine = static_cast<uint32_t>(__cvta_generic_to_shared(rows_ahead + threadIdx.x)), pitch = blockDim.x * 16;
     long long ahead = row;
     int filled = 0, stage = 0;
@@ -195,6 +196,7 @@ __global__ void __launch_bounds__(kWarp ? 128 : kStages ? 512 : 1024) rms_norm_v
 // alignment and stride.
 template <typename T, typename W, bool k8>
 __global__ void rms_norm_rows_kernel(RmsNormParams p) {
+    pdl_enter();
     const long long row = blockIdx.x;
     const T *x = static_cast<const T *>(p.x) + row * p.x_stride;
     const T *residual = p.residual ? static_cast<const T *>(p.residual) + row * p.residual_stride : nullptr;
@@ -239,7 +241,7 @@ cudaError_t launch_vectors(const MsnhB200Ctx *ctx, const RmsNormParams &p, int v
         }
     }
     const long long all = (p.rows + rows - 1) / rows, blocks = kStages ? std::min<long long>(all, ctx->sm_count * static_cast<long long>(std::min<size_t>(1024 / threads, kStages ? (208 * 1024) / smem : 1))) : all;
-    return launch_token_kernel(kernel, dim3(static_cast<unsigned>(blocks)), threads, smem, stream, false, p);
+    return launch_token_kernel(kernel, dim3(static_cast<unsigned>(blocks)), threads, smem, stream, ctx->pdl, p);
 }
 
 // Many rows: a warp a row where that suffices (no barrier), or up to 512 threads that stay. Few rows: a vector a thread, so that a row's
@@ -257,7 +259,7 @@ cudaError_t launch(const MsnhB200Ctx *ctx, const RmsNormParams &p, bool aligned,
                : vectors <= 2048 ? launch_vectors<T, W, k8, 2, false, 0>(ctx, p, vectors, stream) : launch_vectors<T, W, k8, 4, false, 0>(ctx, p, vectors, stream);
     }
     const int threads = p.cols <= 256 ? 64 : p.cols <= 2048 ? 256 : 1024;
-    return launch_token_kernel(rms_norm_rows_kernel<T, W, k8>, dim3(static_cast<unsigned>(p.rows)), threads, 0, stream, false, p);
+    return launch_token_kernel(rms_norm_rows_kernel<T, W, k8>, dim3(static_cast<unsigned>(p.rows)), threads, 0, stream, ctx->pdl, p);
 }
 
 template <typename T, typename W>

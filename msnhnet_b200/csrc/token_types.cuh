@@ -4,8 +4,16 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <stdint.h>
+#include "common.cuh"
 
 namespace msnh {
+
+// First thing in a kernel that is launched while the one before it may still run: waits until that one has ended and its writes are
+// visible, then lets the next launch be scheduled. In this order the next one may take it that everything before this kernel has ended.
+__device__ __forceinline__ void pdl_enter() {
+    pdl_wait();
+    pdl_launch_dependents();
+}
 
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }

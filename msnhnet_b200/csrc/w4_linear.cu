@@ -1,6 +1,5 @@
 // Products with 4-bit weights (msnh_b200_w4_pack, msnh_b200_w4_linear).
 #include <cooperative_groups.h>
-#include "common.cuh"
 #include "token_ops.h"
 #include "token_types.cuh"
 
@@ -538,7 +537,7 @@ __device__ __forceinline__ void make_digits(const W4Params &p, int unit, int m, 
 
 // All digits into the workspace, a warp 128 values of a row.
 __global__ void w4_digits_kernel(const __grid_constant__ W4Params p) {
-    pdl_launch_dependents();
+    pdl_enter();
     const int i = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
     if (i < p.units * p.rows) make_digits(p, i / p.rows, i % p.rows, i / p.rows * kUnitK, threadIdx.x % 32, p.digits_made, p.meta_made);
 }
@@ -556,11 +555,12 @@ __global__ void __launch_bounds__(kThreads, 1) w4_integer_kernel(const __grid_co
     auto cluster = cooperative_groups::this_cluster();
     const Share<kTiles> s(p, cluster.num_blocks(), cluster.block_rank());
     const uint32_t smem_at = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
+    if (!p.digits_made) pdl_enter();                             // (when the launch that makes them has begun, everything before it has ended)
     Units<kTiles, kAhead> units(p, s, smem_at + p.ring_at);
     const int lane = s.lane, half_digits = p.rows * kDigits * 64, span_meta = p.rows * kDigits * 8;
     if (p.digits_made) {
         const uint8_t *digits = p.digits_made + static_cast<size_t>(s.begin) * 2 * half_digits, *meta = p.meta_made + static_cast<size_t>(s.begin) * p.spans * span_meta;
-        pdl_wait();
+        pdl_enter();
         for (int i = threadIdx.x * 16; i < s.block_units * 2 * half_digits; i += kThreads * 16) copy16(smem_at + p.x_at + i, digits + i);
         for (int i = threadIdx.x * 16; i < s.block_units * p.spans * span_meta; i += kThreads * 16) copy16(smem_at + p.meta_at + i, meta + i);
         copy_commit();
@@ -660,6 +660,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_linear_kernel(const __grid_con
     auto cluster = cooperative_groups::this_cluster();
     const Share<kTiles> s(p, cluster.num_blocks(), cluster.block_rank());
     const uint32_t smem_at = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
+    pdl_enter();
     Units<kTiles, kAhead> units(p, s, smem_at + p.ring_at);
     const int lane = s.lane, part_pitch = 4 * s.block_units * p.rows * 64;
     if (kStaged) {
@@ -834,11 +835,11 @@ bool launch_integer(const MsnhB200Ctx *ctx, W4Params p, void *stream, cudaError_
     p.meta_at = p.x_at + static_cast<int>(digit_bytes(p.rows, p.block_units));
     if (p.digits_made) {
         p.meta_made = p.digits_made + digit_bytes(p.rows, p.units);
-        e = launch_token_kernel(w4_digits_kernel, dim3((p.units * p.rows + 3) / 4), 128, 0, stream, false, p);
+        e = launch_token_kernel(w4_digits_kernel, dim3((p.units * p.rows + 3) / 4), 128, 0, stream, ctx->pdl, p);
         if (e != cudaSuccess) return true;
     }
     static std::atomic<uint64_t> done{0};
-    e = launch(ctx, w4_integer_kernel<kTiles, kAhead>, done, p, blocks, ranks, p.x_at + bytes(p.block_units), p.digits_made && ctx->pdl, stream);
+    e = launch(ctx, w4_integer_kernel<kTiles, kAhead>, done, p, blocks, ranks, p.x_at + bytes(p.block_units), ctx->pdl, stream);
     return true;
 }
 
@@ -851,8 +852,8 @@ cudaError_t launch(const MsnhB200Ctx *ctx, W4Params p, void *stream) {
     int ranks, blocks;
     const bool staged = share_out(ctx, p, kTiles, bytes, ranks, blocks);
     static std::atomic<uint64_t> done[2];
-    return staged ? launch(ctx, w4_linear_kernel<X, kColumns, kTiles, kAhead, true>, done[0], p, blocks, ranks, p.x_at + bytes(p.block_units), false, stream)
-                  : launch(ctx, w4_linear_kernel<X, kColumns, kTiles, kAhead, false>, done[1], p, blocks, ranks, p.x_at, false, stream);
+    return staged ? launch(ctx, w4_linear_kernel<X, kColumns, kTiles, kAhead, true>, done[0], p, blocks, ranks, p.x_at + bytes(p.block_units), ctx->pdl, stream)
+                  : launch(ctx, w4_linear_kernel<X, kColumns, kTiles, kAhead, false>, done[1], p, blocks, ranks, p.x_at, ctx->pdl, stream);
 }
 
 template <typename X>
