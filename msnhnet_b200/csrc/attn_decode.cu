@@ -20,7 +20,7 @@ namespace {
 
 constexpr int kTile = 16;                    // tokens of a tile
 constexpr int kMaxRows = 256;                // rows of a launch: what they see is kept in shared memory
-constexpr int kStart = 3, kLeast = 4;        // tiles that a pair's start counts for; tiles of a share, where there are as many
+constexpr int kStart = 3, kLeast = 2;        // tiles that a pair's start counts for; tiles of a share, where there are as many
 constexpr int kWholeTiles = 8;               // sequences of at most so many tiles are not cut
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 

@@ -148,13 +148,13 @@ __global__ void kv_append_write_kernel(KvParams c, const int *seqs, const int *s
     }
 }
 
-// The first `rows` tokens of page src to page dst, keys and values, by threads `first`, first + step, ... Four units a turn, so that their
-// reads are under way together.
+// Of the first `rows` tokens of page src the units from `first` on, `step` apart, below `total`, keys and values, to page dst. Four units a
+// turn, so that their reads are under way together.
 template <typename Unit>
-__device__ __forceinline__ void copy_rows(const KvParams &c, int src, int dst, int rows, int units, int first, int step) {
+__device__ __forceinline__ void copy_units(const KvParams &c, int src, int dst, int units, int first, int step, int total) {
     const Unit *k = reinterpret_cast<const Unit *>(c.k) + src * c.k_page, *v = reinterpret_cast<const Unit *>(c.v) + src * c.v_page;
     Unit *k_to = reinterpret_cast<Unit *>(c.k) + dst * c.k_page, *v_to = reinterpret_cast<Unit *>(c.v) + dst * c.v_page;
-    const int per_token = c.heads * units, total = rows * per_token;
+    const int per_token = c.heads * units;
     const bool flat = c.k_token == per_token && c.v_token == per_token && c.k_head == units && c.v_head == units;     // tokens one behind the other
     for (int base = first; base < total; base += 4 * step) {
         long long at_k[4], at_v[4];
@@ -181,6 +181,8 @@ __device__ __forceinline__ void copy_rows(const KvParams &c, int src, int dst, i
         }
     }
 }
+
+constexpr int kPiece = 1024;           // units of a page that a block of 256 threads moves at a time
 
 struct ForkWork { int from, to, rows, full; };                   // the copied page and its rows (to < 0: none); full < 0: refused
 
@@ -241,7 +243,7 @@ __global__ void kv_fork_copy_kernel(KvParams c, const int *src, const int *dst, 
         c.table[b + j] = page;
         if (page >= 0 && page < c.n_pages) atomicAdd(&c.refs[page], 1);
     }
-    if (w.to >= 0) copy_rows<Unit>(c, w.from, w.to, w.rows, units, first, step);
+    if (w.to >= 0) copy_units<Unit>(c, w.from, w.to, units, first, step, w.rows * c.heads * units);
 }
 
 __global__ void kv_free_kernel(KvParams c, const int *seqs) {
@@ -322,7 +324,12 @@ __global__ void kv_compact_move_kernel(KvParams c, const int *work, int *table_o
         const bool held = j * c.page_size < c.lengths[s] && page >= 0 && page < c.n_pages;
         table_out[s * c.table_stride + j] = held ? where[page] : page;
     }
-    for (int i = blockIdx.x; i < moves; i += gridDim.x) copy_rows<Unit>(c, from[i], to[i], c.page_size, units, threadIdx.x, blockDim.x);
+    // pieces of pages, so that the blocks end together
+    const int total = c.page_size * c.heads * units, pieces = (total + kPiece - 1) / kPiece;
+    for (long long i = blockIdx.x; i < static_cast<long long>(moves) * pieces; i += gridDim.x) {
+        const int move = static_cast<int>(i / pieces), first = static_cast<int>(i - static_cast<long long>(move) * pieces) * kPiece;
+        copy_units<Unit>(c, from[move], to[move], units, first + threadIdx.x, blockDim.x, min(total, first + kPiece));
+    }
 }
 
 template <typename Unit>
@@ -334,7 +341,7 @@ __global__ void kv_copy_pages_kernel(KvParams c, const int *src, const int *dst,
             if (a != b && threadIdx.x == 0) atomicAdd(c.refused, 1);
             continue;
         }
-        copy_rows<Unit>(c, a, b, c.page_size, units, threadIdx.x, blockDim.x);
+        copy_units<Unit>(c, a, b, units, threadIdx.x, blockDim.x, c.page_size * c.heads * units);
     }
 }
 

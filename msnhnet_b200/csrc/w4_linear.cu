@@ -119,52 +119,57 @@ __device__ __forceinline__ void interleave(uint32_t (&v)[4]) {
     }
 }
 
-// Eight values of a row, `left` of which are there (all and aligned: kFast), as operands: two k-steps of two registers a part, values 0 and 2,
-// 1 and 3, 4 and 6, 5 and 7.
-template <typename X, bool kFast> __device__ __forceinline__ void load_x(const X *row, int left, uint32_t (&out)[Operand<X>::kParts][4]) {
-    if constexpr (std::is_same<X, float>::value) {
-        float v[8];
-        if (kFast) {
-            const float4 a = __ldg(reinterpret_cast<const float4 *>(row)), b = __ldg(reinterpret_cast<const float4 *>(row) + 1);
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        } else {
+// Eight values of a row: read whole (aligned, all there), or the first `left` of them and zeros; then as operands, two k-steps of two
+// registers a part, values 0 and 2, 1 and 3, 4 and 6, 5 and 7.
+template <typename X> struct Raw {
+    uint4 v;
+    __device__ __forceinline__ void load(const X *row) { v = __ldg(reinterpret_cast<const uint4 *>(row)); }
+    __device__ __forceinline__ void load(const X *row, int left) {
+        X one[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = i < left ? row[i] : 0.f;
-        }
+        for (int i = 0; i < 8; ++i) one[i] = i < left ? row[i] : from_float<X>(0.f);
+        memcpy(&v, one, 16);
+    }
+    __device__ __forceinline__ void operands(uint32_t (&out)[1][4]) const {
+        out[0][0] = v.x; out[0][1] = v.y; out[0][2] = v.z; out[0][3] = v.w;
+        interleave(out[0]);
+    }
+};
+template <> struct Raw<float> {
+    float v[8];
+    __device__ __forceinline__ void load(const float *row) {
+        const float4 a = __ldg(reinterpret_cast<const float4 *>(row)), b = __ldg(reinterpret_cast<const float4 *>(row) + 1);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    }
+    __device__ __forceinline__ void load(const float *row, int left) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < left ? row[i] : 0.f;
+    }
+    __device__ __forceinline__ void operands(uint32_t (&out)[3][4]) const {
 #pragma unroll
         for (int i = 0; i < 4; ++i) split2(v[i / 2 * 4 + i % 2], v[i / 2 * 4 + i % 2 + 2], out[0][i], out[1][i], out[2][i]);
-    } else if constexpr (std::is_same<X, __nv_fp8_e4m3>::value) {
-        uint16_t raw[4];
-        if (kFast) {
-            const uint2 a = __ldg(reinterpret_cast<const uint2 *>(row));
-            memcpy(raw, &a, 8);
-        } else {
-            const uint8_t *bytes = reinterpret_cast<const uint8_t *>(row);
+    }
+};
+template <> struct Raw<__nv_fp8_e4m3> {
+    uint2 v;
+    __device__ __forceinline__ void load(const __nv_fp8_e4m3 *row) { v = __ldg(reinterpret_cast<const uint2 *>(row)); }
+    __device__ __forceinline__ void load(const __nv_fp8_e4m3 *row, int left) {
+        uint8_t bytes[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                raw[i] = 2 * i < left ? bytes[2 * i] : 0;
-                if (2 * i + 1 < left) raw[i] |= static_cast<uint16_t>(bytes[2 * i + 1] << 8);
-            }
-        }
+        for (int i = 0; i < 8; ++i) bytes[i] = i < left ? reinterpret_cast<const uint8_t *>(row)[i] : 0;
+        memcpy(&v, bytes, 8);
+    }
+    __device__ __forceinline__ void operands(uint32_t (&out)[1][4]) const {
+        uint16_t pairs[4];
+        memcpy(pairs, &v, 8);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(raw[i], __NV_E4M3);
+            const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(pairs[i], __NV_E4M3);
             memcpy(&out[0][i], &h, 4);
         }
         interleave(out[0]);
-    } else {
-        if (kFast) {
-            const uint4 a = __ldg(reinterpret_cast<const uint4 *>(row));
-            out[0][0] = a.x; out[0][1] = a.y; out[0][2] = a.z; out[0][3] = a.w;
-        } else {
-            X v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = i < left ? row[i] : from_float<X>(0.f);
-            memcpy(out[0], v, 16);
-        }
-        interleave(out[0]);
     }
-}
+};
 
 // (w & mask) | exponents in one instruction, which takes one constant at most: the exponents come in a register
 template <uint32_t kMask> __device__ __forceinline__ uint32_t masked_or(uint32_t w, uint32_t exponents) {
@@ -664,15 +669,30 @@ __global__ void __launch_bounds__(kThreads, 1) w4_linear_kernel(const __grid_con
     Units<kTiles, kAhead> units(p, s, smem_at + p.ring_at);
     const int lane = s.lane, part_pitch = 4 * s.block_units * p.rows * 64;
     if (kStaged) {
-        for (int i = threadIdx.x; i < part_pitch / 16; i += kThreads) {
-            const int t = i % 4, m = i / 4 % p.rows, at = (s.begin * 4 + i / 4 / p.rows) * 32 + t * 8;
-            const X *row = static_cast<const X *>(p.x) + m * p.x_stride + at;
-            uint32_t b[kParts][4];
-            if (p.vectors && at + 8 <= p.k) load_x<X, true>(row, 8, b);
-            else load_x<X, false>(row, p.k - at, b);
+        // four places of a thread at a time, so that their reads are under way together
+        constexpr int kBatch = 4;
+        for (int base = threadIdx.x; base < part_pitch / 16; base += kBatch * kThreads) {
+            Raw<X> raw[kBatch];
+            const X *rows[kBatch];
+            int left[kBatch];
 #pragma unroll
-            for (int part = 0; part < kParts; ++part)
-                *reinterpret_cast<uint4 *>(smem + p.x_at + part * part_pitch + i * 16) = make_uint4(b[part][0], b[part][1], b[part][2], b[part][3]);
+            for (int j = 0; j < kBatch; ++j) {
+                const int i = base + j * kThreads, m = i / 4 % p.rows, at = (s.begin * 4 + i / 4 / p.rows) * 32 + i % 4 * 8;
+                rows[j] = static_cast<const X *>(p.x) + m * p.x_stride + at;
+                left[j] = i < part_pitch / 16 ? p.k - at : -1;
+                if (p.vectors && left[j] >= 8) raw[j].load(rows[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) {
+                const int i = base + j * kThreads;
+                if (i >= part_pitch / 16) break;
+                if (!(p.vectors && left[j] >= 8)) raw[j].load(rows[j], left[j]);
+                uint32_t b[kParts][4];
+                raw[j].operands(b);
+#pragma unroll
+                for (int part = 0; part < kParts; ++part)
+                    *reinterpret_cast<uint4 *>(smem + p.x_at + part * part_pitch + i * 16) = make_uint4(b[part][0], b[part][1], b[part][2], b[part][3]);
+            }
         }
     }
     __syncthreads();
@@ -725,8 +745,10 @@ __global__ void __launch_bounds__(kThreads, 1) w4_linear_kernel(const __grid_con
                         }
                     } else {
                         const X *row = static_cast<const X *>(p.x) + m * p.x_stride + k_now;
-                        if (p.vectors && k_now + 8 <= p.k) load_x<X, true>(row, 8, b);
-                        else load_x<X, false>(row, p.k - k_now, b);
+                        Raw<X> raw;
+                        if (p.vectors && k_now + 8 <= p.k) raw.load(row);
+                        else raw.load(row, p.k - k_now);
+                        raw.operands(b);
                     }
 #pragma unroll
                     for (int i = 0; i < kParts; ++i)
