@@ -192,6 +192,51 @@ __global__ void __launch_bounds__(kWarp ? 128 : kStages ? 512 : 1024) rms_norm_v
     }
 }
 
+// Rows of any alignment in registers: values thread, thread + threads, ... (kEach of them), a value at a time. One pass over memory, but four
+// to eight times the instructions of the vectors.
+template <typename T, typename W, bool k8, int kEach>
+__global__ void __launch_bounds__(1024) rms_norm_values_kernel(const __grid_constant__ RmsNormParams p) {
+    pdl_enter();
+    const long long row = blockIdx.x;
+    const T *x = static_cast<const T *>(p.x) + row * p.x_stride;
+    const T *residual = p.residual ? static_cast<const T *>(p.residual) + row * p.residual_stride : nullptr;
+    T *residual_out = p.residual_out ? static_cast<T *>(p.residual_out) + row * p.residual_out_stride : nullptr;
+    const W *weight = static_cast<const W *>(p.weight);
+    float h[kEach], sum = 0.f, top = 0.f;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+        const int i = threadIdx.x + j * blockDim.x;
+        h[j] = i < p.cols ? to_float(x[i]) : 0.f;
+        if (residual && i < p.cols) h[j] += to_float(residual[i]);
+    }
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+        const int i = threadIdx.x + j * blockDim.x;
+        sum += h[j] * h[j];
+        if (residual_out && i < p.cols) residual_out[i] = from_float<T>(h[j]);
+        if (k8) {                                                // (h times weight is all that is needed from here on)
+            h[j] *= i < p.cols ? to_float(weight[i]) : 0.f;
+            top = fmaxf(top, fabsf(h[j]));
+        }
+    }
+    block_sum_max(sum, top);
+    const float r = rsqrtf(sum / p.cols + p.eps), scale = top * r / 448.f;
+    if (k8 && threadIdx.x == 0) p.y_scale[row] = scale;
+    // (448 / top is infinite below 2^-119: both are taken times 2^64 there. No codes for a row without a scale.)
+    float lift = 1.f;
+    if (!(top > 1e-30f)) lift = 18446744073709551616.f;
+    const bool codes = scale > 0.f;
+    const float inverse = 448.f / (top * lift);
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+        const int i = threadIdx.x + j * blockDim.x;
+        if (i < p.cols) {
+            if (k8) static_cast<uint8_t *>(p.y)[row * p.y_stride + i] = codes ? static_cast<uint8_t>(to_e4m3x2(h[j] * lift * inverse, 0.f)) : 0;
+            else static_cast<T *>(p.y)[row * p.y_stride + i] = from_float<T>(h[j] * r * to_float(weight[i]));
+        }
+    }
+}
+
 // A block a row, two passes over it: the sum of squares and (8 bits) the largest |h * w|, then the outputs. Any row length,
 // alignment and stride.
 template <typename T, typename W, bool k8>
@@ -258,7 +303,11 @@ cudaError_t launch(const MsnhB200Ctx *ctx, const RmsNormParams &p, bool aligned,
         return vectors <= 1024   ? launch_vectors<T, W, k8, 1, false, 0>(ctx, p, vectors, stream)
                : vectors <= 2048 ? launch_vectors<T, W, k8, 2, false, 0>(ctx, p, vectors, stream) : launch_vectors<T, W, k8, 4, false, 0>(ctx, p, vectors, stream);
     }
-    const int threads = p.cols <= 256 ? 64 : p.cols <= 2048 ? 256 : 1024;
+    const dim3 rows(static_cast<unsigned>(p.rows));
+    const auto threads_of = [&](int each) { return (p.cols + each * 32 - 1) / (each * 32) * 32; };
+    if (p.cols <= 4096) return launch_token_kernel(rms_norm_values_kernel<T, W, k8, 8>, rows, threads_of(8), 0, stream, ctx->pdl, p);
+    if (p.cols <= 16384) return launch_token_kernel(rms_norm_values_kernel<T, W, k8, 16>, rows, threads_of(16), 0, stream, ctx->pdl, p);
+    const int threads = 1024;
     return launch_token_kernel(rms_norm_rows_kernel<T, W, k8>, dim3(static_cast<unsigned>(p.rows)), threads, 0, stream, ctx->pdl, p);
 }
 

@@ -75,7 +75,7 @@ struct W4Params {
     int dtype, wide, spans, vectors, out_dtype;
     int split, share, block_units;           // warps that share a tile's k in a block; units of k of each, of the block at most
     int ring_at, x_at, meta_at;              // of the rings and the activations, in shared memory
-    uint8_t *digits_made, *meta_made;        // in the workspace, or null
+    uint8_t *digits_made, *meta_made;        // digits (or 16-bit operands) and what belongs to them in the workspace, or null
     int *error;                              // where the host learns of a wait that ran out
     uint32_t exponents;                      // of the operands' type (a parameter, so that the compiler takes it for a variable)
 };
@@ -408,6 +408,15 @@ __device__ __forceinline__ void turns(const W4Params &p, const Share<kTiles> &s,
         }
         return;
     }
+    if (s.to - s.from <= s.turn) {                               // (one turn: all can add up)
+        if (s.warp < kWarps && s.from < s.to) {
+            multiply();
+            leave(sums + s.warp * kRows * kCount);
+        }
+        __syncthreads();
+        if (s.from < s.to) add_up<kRows>(p, s.sets, kCount, sums, threadIdx.x, kThreads, [&](int, int place, int row, int m, float v) { put(s.from, place, row, m, v); });
+        return;
+    }
     int parity = 0;
     if (s.warp < kWarps) {
         for (int tile = s.from; tile < s.to; tile += s.turn, parity ^= 1) {
@@ -648,10 +657,32 @@ __global__ void __launch_bounds__(kThreads, 1) w4_integer_kernel(const __grid_co
     copy_wait<0>();
 }
 
+// The activations at place i of the 16-bit operands, [step of 32 values][row][4 x 16 bytes], from unit `begin` on.
+template <typename X> __device__ __forceinline__ void load_raw(const W4Params &p, int begin, int i, Raw<X> &raw) {
+    const int m = i / 4 % p.rows, at = (begin * 4 + i / 4 / p.rows) * 32 + i % 4 * 8;
+    const X *row = static_cast<const X *>(p.x) + m * p.x_stride + at;
+    if (p.vectors && at + 8 <= p.k) raw.load(row);
+    else raw.load(row, p.k - at);
+}
+
+// All of them into the workspace, [part] first.
+template <typename X> __global__ void w4_operands_kernel(const __grid_constant__ W4Params p) {
+    pdl_enter();
+    const int i = blockIdx.x * blockDim.x + threadIdx.x, all = p.units * p.rows * 16;
+    if (i >= all) return;
+    Raw<X> raw;
+    load_raw<X>(p, 0, i, raw);
+    uint32_t b[Operand<X>::kParts][4];
+    raw.operands(b);
+#pragma unroll
+    for (int part = 0; part < Operand<X>::kParts; ++part)
+        reinterpret_cast<uint4 *>(p.digits_made)[static_cast<size_t>(part) * all + i] = make_uint4(b[part][0], b[part][1], b[part][2], b[part][3]);
+}
+
 // More rows: rows of the weights are the 16 rows of m16n8k16, activations its columns. Operands of the codes less zero point are made in
 // registers (exact); a span's products are summed on the tensor cores and its scale is applied to that sum in fp32.
-// kStaged: the activations are laid out as operands in shared memory once, in the order the lanes read them; otherwise they are read from
-// memory (the caches) for every tile.
+// The activations, as operands in the order the lanes read them, are made by a launch before this one, or by every block where there are
+// few. kStaged: they are in shared memory; otherwise they are read from the workspace (the caches) for every tile.
 template <typename X, int kColumns, int kTiles, int kAhead, bool kStaged>
 __global__ void __launch_bounds__(kThreads, 1) w4_linear_kernel(const __grid_constant__ W4Params p) {
     using H = typename Operand<X>::Type;
@@ -665,35 +696,41 @@ __global__ void __launch_bounds__(kThreads, 1) w4_linear_kernel(const __grid_con
     auto cluster = cooperative_groups::this_cluster();
     const Share<kTiles> s(p, cluster.num_blocks(), cluster.block_rank());
     const uint32_t smem_at = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
-    pdl_enter();
+    if (!p.digits_made) pdl_enter();                             // (when the launch that makes them has begun, everything before it has ended)
     Units<kTiles, kAhead> units(p, s, smem_at + p.ring_at);
     const int lane = s.lane, part_pitch = 4 * s.block_units * p.rows * 64;
     if (kStaged) {
-        // four places of a thread at a time, so that their reads are under way together
-        constexpr int kBatch = 4;
-        for (int base = threadIdx.x; base < part_pitch / 16; base += kBatch * kThreads) {
-            Raw<X> raw[kBatch];
-            const X *rows[kBatch];
-            int left[kBatch];
+        if (p.digits_made) {
+            pdl_enter();
 #pragma unroll
-            for (int j = 0; j < kBatch; ++j) {
-                const int i = base + j * kThreads, m = i / 4 % p.rows, at = (s.begin * 4 + i / 4 / p.rows) * 32 + i % 4 * 8;
-                rows[j] = static_cast<const X *>(p.x) + m * p.x_stride + at;
-                left[j] = i < part_pitch / 16 ? p.k - at : -1;
-                if (p.vectors && left[j] >= 8) raw[j].load(rows[j]);
+            for (int part = 0; part < kParts; ++part) {
+                const uint8_t *from = p.digits_made + (static_cast<size_t>(part) * p.units + s.begin) * p.rows * 256;
+                for (int i = threadIdx.x * 16; i < part_pitch; i += kThreads * 16) copy16(smem_at + p.x_at + part * part_pitch + i, from + i);
             }
+            copy_commit();
+            copy_wait<0>();
+        } else {
+            // (four places of a thread at a time, so that their reads are under way together)
+            constexpr int kBatch = 4;
+            for (int base = threadIdx.x; base < part_pitch / 16; base += kBatch * kThreads) {
+                Raw<X> raw[kBatch];
 #pragma unroll
-            for (int j = 0; j < kBatch; ++j) {
-                const int i = base + j * kThreads;
-                if (i >= part_pitch / 16) break;
-                if (!(p.vectors && left[j] >= 8)) raw[j].load(rows[j], left[j]);
-                uint32_t b[kParts][4];
-                raw[j].operands(b);
+                for (int j = 0; j < kBatch; ++j)
+                    if (base + j * kThreads < part_pitch / 16) load_raw<X>(p, s.begin, base + j * kThreads, raw[j]);
 #pragma unroll
-                for (int part = 0; part < kParts; ++part)
-                    *reinterpret_cast<uint4 *>(smem + p.x_at + part * part_pitch + i * 16) = make_uint4(b[part][0], b[part][1], b[part][2], b[part][3]);
+                for (int j = 0; j < kBatch; ++j) {
+                    const int i = base + j * kThreads;
+                    if (i >= part_pitch / 16) break;
+                    uint32_t b[kParts][4];
+                    raw[j].operands(b);
+#pragma unroll
+                    for (int part = 0; part < kParts; ++part)
+                        *reinterpret_cast<uint4 *>(smem + p.x_at + part * part_pitch + i * 16) = make_uint4(b[part][0], b[part][1], b[part][2], b[part][3]);
+                }
             }
         }
+    } else {
+        pdl_enter();
     }
     __syncthreads();
     // (a column beyond the rows is the last row again; its sums are not stored)
@@ -707,7 +744,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_linear_kernel(const __grid_con
 #pragma unroll
             for (int c = 0; c < kColumns; ++c) acc[r][c][0] = acc[r][c][1] = acc[r][c][2] = acc[r][c][3] = 0.f;
         uint32_t x_now = staged_at;
-        int k_now = s.first * kUnitK + lane % 4 * 8;
+        int step_now = s.first * 4;
         float2 scale[kTiles];
         Zero<H> zero[kTiles][2];
 #pragma unroll 1
@@ -744,11 +781,12 @@ __global__ void __launch_bounds__(kThreads, 1) w4_linear_kernel(const __grid_con
                             memcpy(b[i], &v, 16);
                         }
                     } else {
-                        const X *row = static_cast<const X *>(p.x) + m * p.x_stride + k_now;
-                        Raw<X> raw;
-                        if (p.vectors && k_now + 8 <= p.k) raw.load(row);
-                        else raw.load(row, p.k - k_now);
-                        raw.operands(b);
+                        const uint4 *from = reinterpret_cast<const uint4 *>(p.digits_made) + (static_cast<size_t>(step_now) * p.rows + m) * 4 + lane % 4;
+#pragma unroll
+                        for (int i = 0; i < kParts; ++i) {
+                            const uint4 v = __ldg(from + static_cast<size_t>(i) * p.units * p.rows * 16);
+                            memcpy(b[i], &v, 16);
+                        }
                     }
 #pragma unroll
                     for (int i = 0; i < kParts; ++i)
@@ -759,7 +797,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_linear_kernel(const __grid_con
                         }
                 }
                 x_now += p.rows * 64;
-                k_now += 32;
+                ++step_now;
                 if (step == 3 || (step == 1 && span <= 2) || span == 1)
 #pragma unroll
                     for (int r = 0; r < kTiles; ++r)
@@ -846,6 +884,11 @@ constexpr int kOwnDigits = 2;
 size_t digit_bytes(int rows, int units) { return static_cast<size_t>(units) * 2 * rows * kDigits * 64; }
 size_t meta_bytes(int rows, int units, int spans) { return static_cast<size_t>(units) * spans * rows * kDigits * 8; }
 bool digits_apart(int rows, int units) { return rows <= kIntegerRows && rows * units > kOwnDigits * (kWarps + kSummers); }
+// 16-bit operands are made by every block where they are at most kOwnOperands bytes, which find room beside the sums and rings of every
+// kernel (86 KB at least); a launch before it makes more than that, and blocks without room for them read them from the workspace.
+constexpr size_t kOwnOperands = 80 * 1024;
+size_t operand_bytes(int rows, int dtype, int units) { return static_cast<size_t>(dtype == MSNH_B200_F32 ? 3 : 1) * units * rows * 256; }
+bool operands_apart(int rows, int dtype, int units) { return operand_bytes(rows, dtype, units) > kOwnOperands; }
 
 template <int kTiles, int kAhead>
 bool launch_integer(const MsnhB200Ctx *ctx, W4Params p, void *stream, cudaError_t &e) {
@@ -873,6 +916,12 @@ cudaError_t launch(const MsnhB200Ctx *ctx, W4Params p, void *stream) {
     const auto bytes = [&](int units) { return static_cast<size_t>(Operand<X>::kParts) * 4 * units * p.rows * 64; };
     int ranks, blocks;
     const bool staged = share_out(ctx, p, kTiles, bytes, ranks, blocks);
+    if (!operands_apart(p.rows, p.dtype, p.units)) p.digits_made = nullptr;
+    if (!staged && !p.digits_made) return cudaErrorInvalidConfiguration;         // (there is nothing to read them from)
+    if (p.digits_made) {
+        const cudaError_t e = launch_token_kernel(w4_operands_kernel<X>, dim3((p.units * p.rows * 16 + 127) / 128), 128, 0, stream, ctx->pdl, p);
+        if (e != cudaSuccess) return e;
+    }
     static std::atomic<uint64_t> done[2];
     return staged ? launch(ctx, w4_linear_kernel<X, kColumns, kTiles, kAhead, true>, done[0], p, blocks, ranks, p.x_at + bytes(p.block_units), ctx->pdl, stream)
                   : launch(ctx, w4_linear_kernel<X, kColumns, kTiles, kAhead, false>, done[1], p, blocks, ranks, p.x_at, ctx->pdl, stream);
@@ -884,7 +933,9 @@ cudaError_t launch(const MsnhB200Ctx *ctx, const W4Params &p, void *stream) {
         // two tiles at a time where every SM has several
         const bool two = p.unit_bytes <= 1152 && p.tiles >= 8 * ctx->sm_count;
         cudaError_t e = cudaSuccess;
-        if (two ? launch_integer<2, 3>(ctx, p, stream, e) : launch_integer<1, 5>(ctx, p, stream, e)) return e;
+        W4Params digits = p;
+        if (!digits_apart(p.rows, p.units)) digits.digits_made = nullptr;
+        if (two ? launch_integer<2, 3>(ctx, digits, stream, e) : launch_integer<1, 5>(ctx, digits, stream, e)) return e;
     }
     if (p.rows <= 8) return launch<X, 1, 1, 5>(ctx, p, stream);
     if (p.rows <= 16) return launch<X, 2, 1, 4>(ctx, p, stream);
@@ -893,8 +944,9 @@ cudaError_t launch(const MsnhB200Ctx *ctx, const W4Params &p, void *stream) {
 }
 
 size_t workspace_of(const W4Layout &l, const MsnhB200W4Linear &a) {
-    if (a.rows < 1 || !digits_apart(a.rows, l.units)) return 0;
-    return digit_bytes(a.rows, l.units) + meta_bytes(a.rows, l.units, l.spans);
+    if (a.rows < 1) return 0;
+    const size_t digits = digits_apart(a.rows, l.units) ? digit_bytes(a.rows, l.units) + meta_bytes(a.rows, l.units, l.spans) : 0;
+    return std::max(digits, operands_apart(a.rows, a.dtype, l.units) ? operand_bytes(a.rows, a.dtype, l.units) : 0);
 }
 
 int check_weights(MsnhB200Ctx *ctx, const MsnhB200W4 *w, const char *what) {
