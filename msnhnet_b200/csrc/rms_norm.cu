@@ -202,12 +202,18 @@ __global__ void __launch_bounds__(1024) rms_norm_values_kernel(const __grid_cons
     const T *residual = p.residual ? static_cast<const T *>(p.residual) + row * p.residual_stride : nullptr;
     T *residual_out = p.residual_out ? static_cast<T *>(p.residual_out) + row * p.residual_out_stride : nullptr;
     const W *weight = static_cast<const W *>(p.weight);
+    // (a place beyond the row reads its last value again: all reads are under way before the first is looked at)
+    T a[kEach], b[kEach];
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) a[j] = x[min(static_cast<int>(threadIdx.x + j * blockDim.x), p.cols - 1)];
+    if (residual)
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) b[j] = residual[min(static_cast<int>(threadIdx.x + j * blockDim.x), p.cols - 1)];
     float h[kEach], sum = 0.f, top = 0.f;
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
-        const int i = threadIdx.x + j * blockDim.x;
-        h[j] = i < p.cols ? to_float(x[i]) : 0.f;
-        if (residual && i < p.cols) h[j] += to_float(residual[i]);
+        h[j] = to_float(a[j]) + (residual ? to_float(b[j]) : 0.f);
+        if (static_cast<int>(threadIdx.x + j * blockDim.x) >= p.cols) h[j] = 0.f;
     }
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
@@ -305,7 +311,7 @@ cudaError_t launch(const MsnhB200Ctx *ctx, const RmsNormParams &p, bool aligned,
     }
     const dim3 rows(static_cast<unsigned>(p.rows));
     const auto threads_of = [&](int each) { return (p.cols + each * 32 - 1) / (each * 32) * 32; };
-    if (p.cols <= 4096) return launch_token_kernel(rms_norm_values_kernel<T, W, k8, 8>, rows, threads_of(8), 0, stream, ctx->pdl, p);
+    if (p.cols <= 8192) return launch_token_kernel(rms_norm_values_kernel<T, W, k8, 8>, rows, threads_of(8), 0, stream, ctx->pdl, p);
     if (p.cols <= 16384) return launch_token_kernel(rms_norm_values_kernel<T, W, k8, 16>, rows, threads_of(16), 0, stream, ctx->pdl, p);
     const int threads = 1024;
     return launch_token_kernel(rms_norm_rows_kernel<T, W, k8>, dim3(static_cast<unsigned>(p.rows)), threads, 0, stream, ctx->pdl, p);
