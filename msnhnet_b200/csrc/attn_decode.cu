@@ -35,7 +35,7 @@ struct AttnParams {
     int first_row;                                       // of this launch
     int whole;
     float scale;
-    long long *prefix;                                   // workspace: the line's tiles before each row (rows + 1), then the parts
+    int *prefix;                                         // workspace: the line's tiles before each row (rows + 1), then the parts
     float2 *part_ml;                                     // [slot][chunk] maximum and sum
     float *part;                                         // [slot][chunk][dim]
 };
@@ -50,14 +50,10 @@ __device__ __forceinline__ Row row_of(const AttnParams &p, int row) {
 }
 __device__ __forceinline__ int tiles_of(const Row &r) { return r.last > r.first ? (r.last - 1) / kTile - r.first / kTile + 1 : 0; }
 
-// (the quotients here are of small numbers most of the time, and a 64-bit division takes a hundred instructions)
-__device__ __forceinline__ long long quotient(long long a, long long b) {
-    return ((a | b) >> 32) == 0 ? static_cast<long long>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
-}
-
-// The share of a warp, in tiles of the line.
-__device__ __forceinline__ long long share_of(long long line, int workers) {
-    return max(quotient(line + workers - 1, workers), static_cast<long long>(kStart + kLeast));
+// The share of a warp, in tiles of the line. (A launch's line has less than 2^30 tiles: code for longer ones is a microsecond of reading
+// instructions alone.)
+__device__ __forceinline__ int share_of(int line, int workers) {
+    return max((line + workers - 1) / workers, kStart + kLeast);
 }
 
 // 16 bytes to shared memory, of which the first `bytes` are copied (16 or none) and the others are 0
@@ -427,9 +423,9 @@ template <int kDim_, int kHeads_, int kStages_, int kWarps_> struct PlainHeads {
 
 // What a block keeps beside its rings.
 template <typename Heads> struct Side {
-    long long prefix[kMaxRows + 1];                              // the line's tiles before each row
+    int prefix[kMaxRows + 1];                                    // the line's tiles before each row
     int seq[kMaxRows], first[kMaxRows], last[kMaxRows];
-    long long warp_sum[Heads::kWarps];
+    int warp_sum[Heads::kWarps];
     __align__(16) float scratch[Heads::kWarps][Heads::kScratch];
     int masks[Heads::kWarps][Heads::kStages];
 };
@@ -438,16 +434,16 @@ template <typename Heads> struct Side {
 template <typename Heads> struct Walk {
     const AttnParams &p;
     const Side<Heads> &side;
-    long long left;                                              // of the share
+    int left;                                                    // of the share
     int row, pair, pairs, at, length;                            // where it stands: row (of the launch), pair, tile of the line within it
     int worker;
 
-    __device__ __forceinline__ int length_of(int r) const { return static_cast<int>(quotient(side.prefix[r + 1] - side.prefix[r], pairs)); }
+    __device__ __forceinline__ int length_of(int r) const { return p.whole ? 1 : (side.last[r] - 1) / kTile - side.first[r] / kTile + 1 + kStart; }
     // tiles [begin, end) of the row's tiles; slot of the workspace or -1
-    struct Piece { int row, pair, begin, end; long long slot; };
+    struct Piece { int row, pair, begin, end, slot; };
     __device__ __forceinline__ bool next(Piece &piece) {
         while (left > 0) {
-            const int to = static_cast<int>(min(static_cast<long long>(length), at + left));
+            const int to = min(length, at + left);
             piece.row = row;
             piece.pair = pair;
             if (p.whole) {
@@ -457,7 +453,7 @@ template <typename Heads> struct Walk {
             } else {
                 piece.begin = max(0, at - kStart);
                 piece.end = to - kStart;
-                piece.slot = piece.begin == 0 && to == length ? -1 : 2LL * worker + (piece.begin == 0);
+                piece.slot = piece.begin == 0 && to == length ? -1 : 2 * worker + (piece.begin == 0);
             }
             left -= to - at;
             at = 0;
@@ -481,7 +477,7 @@ __global__ void __launch_bounds__(Heads::kWarps * 32, Heads::kBlocks) attn_decod
     constexpr int kWarps = Heads::kWarps, kThreads = kWarps * 32, kStages = Heads::kStages;
     pdl_enter();
     const int pairs = p.c.heads * p.chunks, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    long long line = 0;
+    int line = 0;
     for (int base = 0; base < p.rows; base += kThreads) {
         const int i = base + threadIdx.x;
         Row r = {0, 0, 0};
@@ -492,16 +488,16 @@ __global__ void __launch_bounds__(Heads::kWarps * 32, Heads::kBlocks) attn_decod
             side.last[i] = r.last;
         }
         const int tiles = tiles_of(r);
-        const long long mine = tiles == 0 ? 0 : static_cast<long long>(p.whole ? 1 : tiles + kStart) * pairs;
-        long long sum = mine;
+        const int mine = tiles == 0 ? 0 : (p.whole ? 1 : tiles + kStart) * pairs;
+        int sum = mine;
 #pragma unroll
         for (int o = 1; o < 32; o *= 2) {
-            const long long below = __shfl_up_sync(~0u, sum, o);
+            const int below = __shfl_up_sync(~0u, sum, o);
             if (lane >= o) sum += below;
         }
         if (lane == 31) side.warp_sum[warp] = sum;
         __syncthreads();
-        long long before = line;
+        int before = line;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
             if (w < warp) before += side.warp_sum[w];
@@ -523,7 +519,7 @@ __global__ void __launch_bounds__(Heads::kWarps * 32, Heads::kBlocks) attn_decod
         }
     // the share; neighbours in the line are in different blocks, so that a short line is spread over the SMs
     const int workers = gridDim.x * kWarps, worker = warp * gridDim.x + blockIdx.x;
-    const long long share = p.whole ? quotient(line + workers - 1, workers) : share_of(line, workers), unit = worker * share;
+    const int share = p.whole ? (line + workers - 1) / workers : share_of(line, workers), unit = worker * share;
     if (unit >= line) return;
     int low = 0;                                                 // the last row that begins at or before the share
     for (int step = kMaxRows / 32; step; step = step == kMaxRows / 32 ? 1 : 0) {
@@ -533,9 +529,8 @@ __global__ void __launch_bounds__(Heads::kWarps * 32, Heads::kBlocks) attn_decod
     }
     Walk<Heads> ahead = {p, side, min(share, line - unit), low, 0, pairs, 0, 0, worker};
     ahead.length = ahead.length_of(low);
-    const long long in_row = unit - side.prefix[low];
-    ahead.pair = static_cast<int>(quotient(in_row, ahead.length));
-    ahead.at = static_cast<int>(in_row - static_cast<long long>(ahead.pair) * ahead.length);
+    ahead.pair = (unit - side.prefix[low]) / ahead.length;
+    ahead.at = unit - side.prefix[low] - ahead.pair * ahead.length;
     Walk<Heads> walk = ahead;
 
     // the copies' side: the piece they are at, its next tile, and a lane's page of one of the next 32 tiles
@@ -602,7 +597,7 @@ __global__ void __launch_bounds__(Heads::kWarps * 32, Heads::kBlocks) attn_decod
             --left;
         }
         if (piece.slot >= 0) {
-            const long long at = piece.slot * p.chunk;
+            const long long at = static_cast<long long>(piece.slot) * p.chunk;
             h.finish(heads, p.c.dim, lane,
                      [&](int i, float top, float sum, bool writes) { if (writes) p.part_ml[at + i] = make_float2(top, sum); return 1.f; },
                      [&](int i, int d, float v) { p.part[(at + i) * p.c.dim + d] = v; });
@@ -619,9 +614,9 @@ __global__ void __launch_bounds__(Heads::kWarps * 32, Heads::kBlocks) attn_decod
     }
 }
 
-constexpr int kJoinFew = 128, kJoinMany = 512;                // threads of a joining block
+constexpr int kJoinFew = 128, kJoinMany = 1024;                // threads of a joining block
 
-// A block a (row, query head): the parts of a pair that was cut, in the order of the tokens. Each warp has every fourth or sixteenth part,
+// A block a (row, query head): the parts of a pair that was cut, in the order of the tokens. Each warp has every fourth or 32nd part,
 // a lane four columns of up to two blocks of 128.
 template <typename T, int kJoinThreads>
 __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_constant__ AttnParams p, int workers) {
@@ -631,17 +626,17 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_co
     pdl_enter();
     const int row = blockIdx.x, head = blockIdx.y, kv = head / p.each, chunk = head % p.each / p.chunk, in_chunk = head % p.each % p.chunk;
     const int pairs = p.c.heads * p.chunks, dim = p.c.dim;
-    const long long before = p.prefix[row], after = p.prefix[row + 1], line = p.prefix[p.rows], length = quotient(after - before, pairs);
+    const int before = p.prefix[row], after = p.prefix[row + 1], line = p.prefix[p.rows], length = (after - before) / pairs;
     if (length == 0) return;
-    const long long share = share_of(line, workers), unit = before + (kv * p.chunks + chunk) * length;
-    const long long first = quotient(unit + kStart, share), last = quotient(unit + length - 1, share);
+    const int share = share_of(line, workers), unit = before + (kv * p.chunks + chunk) * length;
+    const int first = (unit + kStart) / share, last = (unit + length - 1) / share;
     if (first == last) return;                                   // (finished by its warp)
-    const int parts = static_cast<int>(last - first) + 1, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const int parts = last - first + 1, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     float top = -INFINITY, sum = 0.f;
     float4 acc[2] = {};
 #pragma unroll 4
     for (int i = warp; i < parts; i += kWarps) {
-        const long long at = (2 * (first + i) + (i == 0)) * p.chunk + in_chunk;
+        const long long at = static_cast<long long>(2 * (first + i) + (i == 0)) * p.chunk + in_chunk;
         const float2 one = p.part_ml[at];
         const float *from = p.part + at * dim;
         float4 v[2];
@@ -696,16 +691,19 @@ AttnPlan plan_of(const MsnhB200Ctx *ctx, const MsnhB200KvCache &c, const MsnhB20
     l.each = a.n_heads / c.n_kv_heads;
     l.chunk = std::min(l.each, c.dtype == MSNH_B200_F32 ? 8 : 16);
     l.chunks = (l.each + l.chunk - 1) / l.chunk;
-    l.rows = std::min(a.rows, kMaxRows);
     const BlockShape shape = block_shape(c.dtype, c.head_dim);
-    const long long pairs = static_cast<long long>(l.rows) * c.n_kv_heads * l.chunks, blocks = static_cast<long long>(ctx->sm_count) * shape.of_sm;
+    const long long blocks = static_cast<long long>(ctx->sm_count) * shape.of_sm;
     const long long most_tokens = static_cast<long long>(c.max_pages) * c.page_size, seen = a.window > 0 ? std::min<long long>(most_tokens, a.window) : most_tokens;
     const long long tiles = (seen + kTile - 1) / kTile + (a.window > 0);        // (a window may start inside a tile)
     l.whole = tiles <= kWholeTiles;
+    const long long row_tiles = (tiles + kStart) * c.n_kv_heads * l.chunks;
+    l.rows = static_cast<int>(std::min<long long>(std::min(a.rows, kMaxRows), ((1LL << 30) - 1) / row_tiles));
+    if (l.rows == 0) return l;                                   // (a row alone is too long)
+    const long long pairs = static_cast<long long>(l.rows) * c.n_kv_heads * l.chunks;
     l.blocks = static_cast<int>(std::min(l.whole ? pairs : pairs * tiles, blocks));
     l.workers = l.blocks * shape.warps;
     if (!l.whole) {
-        l.ml_at = (static_cast<size_t>(l.rows + 1) * 8 + 15) / 16 * 16;
+        l.ml_at = (static_cast<size_t>(l.rows + 1) * 4 + 15) / 16 * 16;
         l.part_at = (l.ml_at + static_cast<size_t>(l.workers) * 2 * l.chunk * sizeof(float2) + 15) / 16 * 16;
         l.bytes = l.part_at + static_cast<size_t>(l.workers) * 2 * l.chunk * c.head_dim * 4;
     }
@@ -761,6 +759,7 @@ int check_attn(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, const MsnhB200AttnDec
     if (c->head_dim > 256 || c->head_dim * dtype_size(c->dtype) % 16) return fail(ctx, MSNH_B200_ERR_UNSUPPORTED, "%s: heads of %d values (a multiple of 16 bytes and at most 256 values are wanted)", what, c->head_dim);
     if (!kv_rows_multiple_of(*c, 16)) return fail(ctx, MSNH_B200_ERR_UNSUPPORTED, "%s: the cache's rows are not 16-byte aligned", what);
     if (!a->seqs && a->rows > c->n_seqs) return fail(ctx, MSNH_B200_ERR_ARG, "%s: %d rows of %d sequences", what, a->rows, c->n_seqs);
+    if (a->rows && plan_of(ctx, *c, *a).rows == 0) return fail(ctx, MSNH_B200_ERR_UNSUPPORTED, "%s: a row of 2^34 and more tokens times heads", what);
     return MSNH_B200_OK;
 }
 
@@ -793,7 +792,7 @@ int msnh_b200_attn_decode(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, const Msnh
     uint8_t *work = static_cast<uint8_t *>(a->workspace);
     AttnParams p = {kv_params(*c), static_cast<const uint8_t *>(a->q), static_cast<uint8_t *>(a->out), a->lse, a->seqs, a->q_row_stride, a->q_head_stride,
                     a->out_row_stride, a->out_head_stride, 0, a->n_heads, l.each, l.chunk, l.chunks, a->window, 0, l.whole, a->scale,
-                    reinterpret_cast<long long *>(work), reinterpret_cast<float2 *>(work + l.ml_at), reinterpret_cast<float *>(work + l.part_at)};
+                    reinterpret_cast<int *>(work), reinterpret_cast<float2 *>(work + l.ml_at), reinterpret_cast<float *>(work + l.part_at)};
     for (int row = 0; row < a->rows; row += l.rows) {
         p.first_row = row;
         p.rows = std::min(l.rows, a->rows - row);
