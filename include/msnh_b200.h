@@ -351,7 +351,7 @@ typedef struct MsnhB200RmsNorm {
 } MsnhB200RmsNorm;
 int  msnh_b200_rms_norm(MsnhB200Ctx *ctx, const MsnhB200RmsNorm *args, void *stream);
 
-/* Products with 4-bit weights. A weight row n of k values is stored as codes 0..15 with a scale and a zero point for every
+/* Products with 4-bit weights. A weight row n (below 2^30) of k (up to 2^27) values is stored as codes 0..15 with a scale and a zero point for every
  * `group` values (a multiple of 32; the last group may be shorter): w = (code - zero) * scale, zero = 8 without `zeros`.
  * w4_pack lays codes, scales and zeros out as the kernels read them, once, into `packed` (w4_pack_bytes of them, 16-byte
  * aligned):

@@ -281,7 +281,7 @@ cudaError_t launch_vectors(const MsnhB200Ctx *ctx, const RmsNormParams &p, int v
     const auto kernel = rms_norm_vectors_kernel<T, W, k8, kVecs, kWarp, kStages>;
     const int threads = kWarp ? 128 : (vectors + kVecs * 32 - 1) / (kVecs * 32) * 32, rows = kWarp ? 4 : 1;
     const size_t smem = static_cast<size_t>(threads) * kVecs * 32 * kStages;
-    if (smem > 48 * 1024) {
+    if (smem > 47 * 1024) {                                      // (the kernel's own 256 bytes count to the 48 KB that need no attribute)
         // the attribute is a kernel's and a device's: set by the first call there
         static std::atomic<uint64_t> done{0};
         const uint64_t bit = 1ull << (ctx->device & 63);

@@ -949,8 +949,11 @@ size_t workspace_of(const W4Layout &l, const MsnhB200W4Linear &a) {
     return std::max(digits, operands_apart(a.rows, a.dtype, l.units) ? operand_bytes(a.rows, a.dtype, l.units) : 0);
 }
 
+constexpr int kMostOutputs = 1 << 30, kMostValues = 1 << 27;
 int check_weights(MsnhB200Ctx *ctx, const MsnhB200W4 *w, const char *what) {
-    if (w->n < 1 || w->k < 1 || w->n > (1 << 30) || w->k > (1 << 30)) return fail(ctx, MSNH_B200_ERR_ARG, "%s: %d x %d weights", what, w->n, w->k);
+    if (w->n < 1 || w->k < 1) return fail(ctx, MSNH_B200_ERR_ARG, "%s: %d x %d weights", what, w->n, w->k);
+    // (64 rows times 16 pieces of k / 128 units are counted in 32 bits)
+    if (w->n > kMostOutputs || w->k > kMostValues) return fail(ctx, MSNH_B200_ERR_UNSUPPORTED, "%s: %d x %d weights (at most 2^30 x 2^27 are taken)", what, w->n, w->k);
     if (w->group < 32 || w->group % 32) return fail(ctx, MSNH_B200_ERR_UNSUPPORTED, "%s: groups of %d values (a multiple of 32 is wanted)", what, w->group);
     if (!is_float_type(w->scale_dtype)) return fail(ctx, MSNH_B200_ERR_UNSUPPORTED, "%s: scales of type %d", what, w->scale_dtype);
     return MSNH_B200_OK;

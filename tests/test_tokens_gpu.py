@@ -77,6 +77,20 @@ def test_norm_matches_the_formula(ops, dtype, rows, cols):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("cols", [1, 64, 250, 256, 512, 520, 1024, 2048, 2056, 5120, 8200, 12288, 16384])
+def test_norm_of_many_rows(ops, dtype, cols):
+    # more rows than the blocks that the device holds at once take together
+    rows = 1300 if cols > 1024 else 5000
+    x, r, w = randn(rows, cols, seed=15, dtype=dtype), randn(rows, cols, seed=16, dtype=dtype), randn(cols, seed=17, dtype=dtype)
+    y, h = ops.rms_norm(x, w, residual=r)
+    _, want = norm_ref(x, r, w, 1e-6)
+    check_norm(y, want, cols, dtype)
+    assert torch.equal(h, (x.float() + r.float()).to(dtype))
+    codes, scale = ops.rms_norm(x, w, residual=None, out_dtype=E4M3)
+    check_codes(codes, scale, norm_ref(x, None, w, 1e-6)[1], cols)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("extra,front", [(8, 0), (3, 0), (0, 1), (8, 8)])
 def test_norm_takes_strides_and_alignments(ops, dtype, extra, front):
     rows, cols = 5, 1024
@@ -196,6 +210,27 @@ def test_w4_matches_the_formula(ops, dtype, rows, k, n, group, zeros, bias):
     check_w4(y, x, w, x_scale, b, k)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16, E4M3])
+@pytest.mark.parametrize("rows,k,n,group,zeros", [(1, 130, 18960, 32, True), (2, 256, 19001, 128, False), (1, 900, 40000, 64, True), (3, 200, 19001, 32, True),
+                                                  (24, 140, 20000, 64, False), (64, 256, 18944, 128, True)])
+def test_w4_of_many_outputs(ops, dtype, rows, k, n, group, zeros):
+    codes, scales, z, w = w4_data(n, k, group, zeros)
+    x, x_scale = w4_x(rows, k, dtype, 32)
+    check_w4(ops.w4_linear(x, ops.w4_pack(codes, scales, z, k=k, group=group), x_scale=x_scale), x, w, x_scale, None, k)
+
+
+@pytest.mark.parametrize("rows,k", [(1, 20000), (2, 33000), (3, 20000), (16, 12000), (64, 9000)])
+def test_w4_of_long_rows(ops, rows, k):
+    # operands that no block has room for, and units that many blocks share
+    codes, scales, z, w = w4_data(100, k, 128, True)
+    weights = ops.w4_pack(codes, scales, z, k=k, group=128)
+    for dtype in (F32, F16, E4M3):
+        x, x_scale = w4_x(rows, k, dtype, 33)
+        y = ops.w4_linear(x, weights, x_scale=x_scale, out_dtype=F32)
+        check_w4(y, x, w, x_scale, None, k)
+        assert torch.equal(y, ops.w4_linear(x, weights, x_scale=x_scale, out_dtype=F32))
+
+
 @pytest.mark.parametrize("scale_dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("out_dtype", [F32, F16, BF16])
 def test_w4_scale_and_output_types(ops, scale_dtype, out_dtype):
@@ -277,6 +312,11 @@ def test_w4_refuses(ops):
         ops.w4_linear(x, weights, bias=torch.zeros(16, device="cuda", dtype=F16))
     with pytest.raises(_ffi.KernelError, match="overlap"):
         ops.w4_linear(x.expand(2, 64), weights, out=torch.empty(1, 16, device="cuda", dtype=F16).expand(2, 16))
+    import ctypes
+    size = ctypes.c_size_t()
+    for n, k, want in ((0, 64, 1), (16, 2 ** 27 + 1, 2), (2 ** 30 + 1, 64, 2), (16, 2 ** 27, 0)):
+        shape = _ffi.W4(None, n, k, 32, _ffi.F16, 0)
+        assert ops.lib.msnh_b200_w4_pack_bytes(ops.h, shape, ctypes.byref(size)) == want
     a = _ffi.W4Linear(x.data_ptr(), None, None, None, 1, _ffi.F16, _ffi.F16, 64, 16, None, 0)
     assert ops.lib.msnh_b200_w4_linear(ops.h, weights.ref, a, None) == 1
     a.y, a.dtype = x.data_ptr(), 9
@@ -411,6 +451,23 @@ def test_attention_of_large_scores(ops, dtype):
     assert bool(torch.isnan(out[2]).all())
 
 
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("longest", [60, 700])
+def test_attention_of_many_rows(ops, dtype, longest):
+    # more rows than one launch takes, in any order, some twice and some of no sequence
+    lengths = [(i * 37) % longest for i in range(90)]
+    cache, keys, values = make_cache(lengths, 16, 2, 32, dtype, 82)
+    pick = [(i * 53) % 95 - 2 for i in range(600)]
+    q = randn(600, 4, 32, seed=83, dtype=dtype)
+    out, lse = ops.attn_decode(q, cache, seqs=ints(*pick), return_lse=True)
+    none = torch.zeros(0, 2, 32, device="cuda", dtype=dtype)
+    seen = [keys[s] if 0 <= s < 90 else none for s in pick], [values[s] if 0 <= s < 90 else none for s in pick]
+    check_attn(out, lse, q, *seen, 32 ** -0.5)
+    for part in (slice(0, 256), slice(300, 301)):                     # as much of it as one launch takes, and one row alone
+        some, some_lse = ops.attn_decode(q[part], cache, seqs=ints(*pick[part]), return_lse=True)
+        check_attn(some, some_lse, q[part], seen[0][part], seen[1][part], 32 ** -0.5)
+
+
 def test_attention_beyond_32_bits(ops):
     # the last pages of a cache of more than 2^32 bytes a side (and 2^31 values)
     from msnhnet_b200 import tokens
@@ -454,6 +511,14 @@ def test_attention_refuses(ops):
     wide, _, _ = make_cache([20], 16, 1, 264, F16, 57)
     with pytest.raises(_ffi.KernelError, match="256"):
         ops.attn_decode(randn(1, 2, 264, seed=58, dtype=F16), wide)
+    args = _ffi.AttnDecode(q.data_ptr(), q.data_ptr(), None, None, 2, 4, 256, 64, 256, 64, 0.125, 0, None, 0)
+    cache.args.max_pages = cache.args.table_stride = 64               # (long enough to be cut, so a workspace is wanted)
+    assert ops.lib.msnh_b200_attn_decode(ops.h, cache.ref, args, None) == 1 and "workspace" in ops.ctx.error()
+    cache.args.max_pages = cache.args.table_stride = 2 ** 27 - 1
+    cache.args.n_kv_heads = args.n_heads = 16
+    assert ops.lib.msnh_b200_attn_decode(ops.h, cache.ref, args, None) == 2 and "2^34" in ops.ctx.error()
+    cache.args.max_pages = cache.args.table_stride = cache.max_pages
+    cache.args.n_kv_heads = 2
     from msnhnet_b200 import tokens
     with pytest.raises(ValueError):
         tokens.PagedCache(cache.k_pages, cache.v_pages[:1], cache.page_table, cache.lengths, cache.refs)
