@@ -263,10 +263,18 @@ __global__ void kv_free_kernel(KvParams c, const int *seqs) {
     }
 }
 
-// work: [0] the number of moves, then n_pages each: where a page's contents go, the moves' destinations, their sources
+// A compaction's decisions: [0] the number of moves, then n_pages each (up to 8, so that 16-byte stores fit): where a page's contents go,
+// the moves' destinations, their sources.
+struct CompactWork {
+    int *moves, *where, *to, *from;
+    __host__ __device__ static long long pitch(int n_pages) { return (n_pages + 7LL) / 8 * 8; }
+    __host__ __device__ static size_t bytes(int n_pages) { return (4 + 3 * static_cast<size_t>(pitch(n_pages))) * 4; }
+    __device__ CompactWork(int *work, int n_pages) : moves(work), where(work + 4), to(where + pitch(n_pages)), from(to + pitch(n_pages)) {}
+};
+
 __global__ void kv_compact_decide_kernel(KvParams c, int *refs_out, int *work) {
     pdl_enter();
-    int *where = work + 1, *to = where + c.n_pages, *from = to + c.n_pages;
+    const CompactWork w(work, c.n_pages);
     int live = 0;
     for (long long base = 0; base < c.n_pages; base += kDecide * kEach) {
         const int first = static_cast<int>(min(base + threadIdx.x * kEach, static_cast<long long>(c.n_pages)));
@@ -295,40 +303,43 @@ __global__ void kv_compact_decide_kernel(KvParams c, int *refs_out, int *work) {
         for (int i = 0; i < kEach; ++i) {
             const int page = first + i;
             if (page >= c.n_pages) break;
-            if (page < n_live && refs[i] == 0) to[hole++] = page;
-            if (page >= n_live && refs[i] != 0) from[mover++] = page;
-            where[page] = page;
+            if (page < n_live && refs[i] == 0) w.to[hole++] = page;
+            if (page >= n_live && refs[i] != 0) w.from[mover++] = page;
             if (refs_out != c.refs) refs_out[page] = refs[i];
         }
+        if (first < c.n_pages)
+#pragma unroll
+            for (int i = 0; i < kEach; i += 4) *reinterpret_cast<int4 *>(w.where + first + i) = make_int4(first + i, first + i + 1, first + i + 2, first + i + 3);
         holes += total & 0xffff;
         movers += total >> 16;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < movers; i += kDecide) {
-        where[from[i]] = to[i];
-        refs_out[to[i]] = c.refs[from[i]];
-        refs_out[from[i]] = 0;
-    }
-    if (threadIdx.x == 0) work[0] = movers;
+    for (int i = threadIdx.x; i < movers; i += kDecide) w.where[w.from[i]] = w.to[i];
+    if (threadIdx.x == 0) *w.moves = movers;
 }
 
 template <typename Unit>
-__global__ void kv_compact_move_kernel(KvParams c, const int *work, int *table_out, int units) {
+__global__ void kv_compact_move_kernel(KvParams c, int *work, int *table_out, int *refs_out, int units) {
     pdl_enter();
-    const int moves = work[0];
-    const int *where = work + 1, *to = where + c.n_pages, *from = to + c.n_pages;
+    const CompactWork w(work, c.n_pages);
+    const int moves = *w.moves;
     const long long entries = static_cast<long long>(c.n_seqs) * c.max_pages;
     for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < entries; i += static_cast<long long>(gridDim.x) * blockDim.x) {
         const long long s = i / c.max_pages, j = i % c.max_pages;
         const int page = c.table[s * c.table_stride + j];
         const bool held = j * c.page_size < c.lengths[s] && page >= 0 && page < c.n_pages;
-        table_out[s * c.table_stride + j] = held ? where[page] : page;
+        table_out[s * c.table_stride + j] = held ? w.where[page] : page;
     }
     // pieces of pages, so that the blocks end together
     const int total = c.page_size * c.heads * units, pieces = (total + kPiece - 1) / kPiece;
     for (long long i = blockIdx.x; i < static_cast<long long>(moves) * pieces; i += gridDim.x) {
         const int move = static_cast<int>(i / pieces), first = static_cast<int>(i - static_cast<long long>(move) * pieces) * kPiece;
-        copy_units<Unit>(c, from[move], to[move], units, first + threadIdx.x, blockDim.x, min(total, first + kPiece));
+        const int from = w.from[move], to = w.to[move];
+        if (first == 0 && threadIdx.x == 0) {
+            refs_out[to] = c.refs[from];
+            refs_out[from] = 0;
+        }
+        copy_units<Unit>(c, from, to, units, first + threadIdx.x, blockDim.x, min(total, first + kPiece));
     }
 }
 
@@ -354,7 +365,7 @@ KvParams in_units(KvParams p, size_t size, size_t bytes, int *units) {
 }
 
 size_t workspace_bytes_of(const MsnhB200KvCache &c, int n) {
-    return std::max(static_cast<size_t>(n) * sizeof(AppendWork) + static_cast<size_t>(c.n_pages) * 4, (static_cast<size_t>(c.n_pages) * 3 + 1) * 4);
+    return std::max(static_cast<size_t>(n) * sizeof(AppendWork) + static_cast<size_t>(c.n_pages) * 4, CompactWork::bytes(c.n_pages));
 }
 
 int check_workspace(MsnhB200Ctx *ctx, const MsnhB200KvCache &c, int n, const void *workspace, size_t bytes, const char *what) {
@@ -467,7 +478,7 @@ int msnh_b200_kv_compact(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, int32_t *ta
     int units;
     const KvParams q = in_units(p, size, wide ? 16 : size, &units);
     const dim3 grid(blocks_for(ctx, std::max<long long>(c->n_pages, static_cast<long long>(c->n_seqs) * c->max_pages / 256), 1));
-    const auto move = [&](auto unit) { return launch_token_kernel(kv_compact_move_kernel<decltype(unit)>, grid, 256, 0, stream, ctx->pdl, q, work, table_out, units); };
+    const auto move = [&](auto unit) { return launch_token_kernel(kv_compact_move_kernel<decltype(unit)>, grid, 256, 0, stream, ctx->pdl, q, work, table_out, refs_out, units); };
     CUDA_TRY(ctx, wide ? move(uint4()) : size == 4 ? move(uint32_t()) : move(uint16_t()));
     return MSNH_B200_OK;
 } catch (...) { return caught(ctx); }

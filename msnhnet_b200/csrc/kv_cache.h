@@ -31,8 +31,9 @@ inline int check_cache(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, bool upkeep, 
     if (!is_float_type(c->dtype)) return fail(ctx, MSNH_B200_ERR_UNSUPPORTED, "%s: a cache of type %d", what, c->dtype);
     if (c->n_pages < 1 || c->page_size < 1 || c->n_kv_heads < 1 || c->head_dim < 1 || c->n_seqs < 1 || c->max_pages < 1)
         return fail(ctx, MSNH_B200_ERR_ARG, "%s: the cache's sizes must be positive", what);
-    if (static_cast<int64_t>(c->max_pages) * c->page_size > 0x7fffffff || static_cast<int64_t>(c->page_size) * c->n_kv_heads * c->head_dim > 0x7fffffff)
-        return fail(ctx, MSNH_B200_ERR_UNSUPPORTED, "%s: 2^31 tokens of a sequence, or values of a page, and more", what);
+    if (static_cast<int64_t>(c->max_pages) * c->page_size > 0x7fffffff || static_cast<int64_t>(c->page_size) * c->n_kv_heads * c->head_dim >= 1 << 30)
+        return fail(ctx, MSNH_B200_ERR_UNSUPPORTED, "%s: 2^31 tokens of a sequence or 2^30 values of a page, and more", what);
+    if (c->n_pages > 1 << 30) return fail(ctx, MSNH_B200_ERR_UNSUPPORTED, "%s: %d pages (at most 2^30 are taken)", what, c->n_pages);
     if (!c->k_pages || !c->v_pages || !c->page_table || !c->lengths) return fail(ctx, MSNH_B200_ERR_ARG, "%s: null pages, table or lengths", what);
     if (upkeep && (!c->refs || !c->refused)) return fail(ctx, MSNH_B200_ERR_ARG, "%s: null refs or refused", what);
     if (c->table_stride < c->max_pages) return fail(ctx, MSNH_B200_ERR_ARG, "%s: rows of the page table overlap", what);
