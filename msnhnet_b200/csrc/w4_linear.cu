@@ -853,7 +853,8 @@ cudaError_t launch(const MsnhB200Ctx *ctx, Kernel kernel, std::atomic<uint64_t> 
 
 // How many warps of a block share a tile's k: what takes the fewest units one after the other in the busiest warp (tiles at a time x units
 // of each), the more the better at the same count. Where that leaves SMs without a block, a cluster shares it further, down to two units
-// of k a warp; and where that is what makes room for the activations (x_bytes: of those of some units). Returns whether there is room.
+// of k a warp; and where that is what makes room for the activations (x_bytes: of those of some units). (A cluster has room for the outputs of one
+// set of warps.) Returns whether there is room.
 template <typename Bytes>
 bool share_out(const MsnhB200Ctx *ctx, W4Params &p, int tiles, Bytes x_bytes, int &ranks, int &blocks) {
     const auto per_turn = [&](int split) { return kWarps / split * tiles; };
@@ -868,9 +869,9 @@ bool share_out(const MsnhB200Ctx *ctx, W4Params &p, int tiles, Bytes x_bytes, in
     const int turns = up(p.tiles, per_turn(p.split));
     const auto units = [&] { return std::min(p.units, p.split * up(p.units, p.split * ranks)); };
     ranks = 1;
-    while (ranks < 8 && turns * ranks * 2 <= ctx->sm_count && p.split * ranks * 4 <= p.units) ranks *= 2;
+    while (p.split == kWarps && ranks < 8 && turns * ranks * 2 <= ctx->sm_count && p.split * ranks * 4 <= p.units) ranks *= 2;
     const int wanted = ranks;
-    while (ranks < 8 && p.x_at + x_bytes(units()) > kSmemMost && p.split * ranks * 2 <= p.units) ranks *= 2;
+    while (p.split == kWarps && ranks < 8 && p.x_at + x_bytes(units()) > kSmemMost && p.split * ranks * 2 <= p.units) ranks *= 2;
     const bool room = p.x_at + x_bytes(units()) <= kSmemMost;
     if (!room) ranks = wanted;
     p.share = up(p.units, p.split * ranks);

@@ -219,6 +219,15 @@ def test_w4_of_many_outputs(ops, dtype, rows, k, n, group, zeros):
     check_w4(ops.w4_linear(x, ops.w4_pack(codes, scales, z, k=k, group=group), x_scale=x_scale), x, w, x_scale, None, k)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, E4M3])
+@pytest.mark.parametrize("rows,k,n", [(1, 5000, 3200), (7, 7100, 3200), (13, 5000, 3200), (20, 5000, 3200), (30, 5000, 4700), (64, 1000, 3200), (48, 4096, 2048)])
+def test_w4_of_a_few_turns(ops, dtype, rows, k, n):
+    # tiles and units in numbers that the warps of a block share in two or more sets
+    codes, scales, z, w = w4_data(n, k, 128, True)
+    x, x_scale = w4_x(rows, k, dtype, 34)
+    check_w4(ops.w4_linear(x, ops.w4_pack(codes, scales, z, k=k, group=128), x_scale=x_scale), x, w, x_scale, None, k)
+
+
 @pytest.mark.parametrize("rows,k", [(1, 20000), (2, 33000), (3, 20000), (16, 12000), (64, 9000)])
 def test_w4_of_long_rows(ops, rows, k):
     # operands that no block has room for, and units that many blocks share
