@@ -678,6 +678,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_co
 // How a call is cut up: query heads of a pair, warps, slots of the workspace.
 struct AttnPlan {
     int each, chunk, chunks, rows, blocks, workers, whole;       // rows: of a launch
+    long long tiles;                                             // of a row at most
     size_t ml_at, part_at, bytes;
 };
 
@@ -695,6 +696,7 @@ AttnPlan plan_of(const MsnhB200Ctx *ctx, const MsnhB200KvCache &c, const MsnhB20
     const long long blocks = static_cast<long long>(ctx->sm_count) * shape.of_sm;
     const long long most_tokens = static_cast<long long>(c.max_pages) * c.page_size, seen = a.window > 0 ? std::min<long long>(most_tokens, a.window) : most_tokens;
     const long long tiles = (seen + kTile - 1) / kTile + (a.window > 0);        // (a window may start inside a tile)
+    l.tiles = tiles;
     l.whole = tiles <= kWholeTiles;
     const long long row_tiles = (tiles + kStart) * c.n_kv_heads * l.chunks;
     l.rows = static_cast<int>(std::min<long long>(std::min(a.rows, kMaxRows), ((1LL << 30) - 1) / row_tiles));
@@ -744,12 +746,17 @@ cudaError_t launch32(const MsnhB200Ctx *ctx, const AttnParams &p, int blocks, vo
     return launch<PlainHeads<256, kHeads, 3, 2>>(ctx, p, blocks, stream);
 }
 
-// Many pairs have few parts each, and their blocks should all be there at once; few pairs have many.
+// A pair has at most as many parts as there are shares of its tiles, or as it has warps to itself. Parts that few warps take turns at cost
+// more than starting 32 warps does from kManyParts on: with 74 and 148 parts a pair 80 against 72 us (2 rows of 60000 fp16 tokens) and 47
+// against 35 (one of 30000), with 51 as much either way (one of 4000: 15.5 and 14.7), with 9 and 7 the other way round (16 rows of 4000:
+// 43 against 59; one of 500: 10.9 against 13.5).
+constexpr int kManyParts = 32;
 template <typename T>
-cudaError_t launch_join(const MsnhB200Ctx *ctx, const AttnParams &p, int workers, void *stream) {
+cudaError_t launch_join(const MsnhB200Ctx *ctx, const AttnParams &p, int workers, long long tiles, void *stream) {
     const dim3 grid(p.rows, p.n_heads);
-    return static_cast<long long>(p.rows) * p.c.heads * p.chunks * 8 >= workers ? launch_token_kernel(attn_join_kernel<T, kJoinFew>, grid, kJoinFew, 0, stream, ctx->pdl, p, workers)
-                                                                                : launch_token_kernel(attn_join_kernel<T, kJoinMany>, grid, kJoinMany, 0, stream, ctx->pdl, p, workers);
+    const long long parts = std::min<long long>(workers / (static_cast<long long>(p.rows) * p.c.heads * p.chunks), (tiles + kStart) / (kStart + kLeast));
+    return parts < kManyParts ? launch_token_kernel(attn_join_kernel<T, kJoinFew>, grid, kJoinFew, 0, stream, ctx->pdl, p, workers)
+                              : launch_token_kernel(attn_join_kernel<T, kJoinMany>, grid, kJoinMany, 0, stream, ctx->pdl, p, workers);
 }
 
 int check_attn(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, const MsnhB200AttnDecode *a, const char *what) {
@@ -804,8 +811,8 @@ int msnh_b200_attn_decode(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, const Msnh
             e = c->dtype == MSNH_B200_F16 ? launch16<__half>(ctx, p, l.blocks, stream) : launch16<__nv_bfloat16>(ctx, p, l.blocks, stream);
         CUDA_TRY(ctx, e);
         if (l.whole) continue;
-        e = c->dtype == MSNH_B200_F32 ? launch_join<float>(ctx, p, l.workers, stream) : c->dtype == MSNH_B200_F16 ? launch_join<__half>(ctx, p, l.workers, stream)
-                                                                                                                 : launch_join<__nv_bfloat16>(ctx, p, l.workers, stream);
+        e = c->dtype == MSNH_B200_F32 ? launch_join<float>(ctx, p, l.workers, l.tiles, stream) : c->dtype == MSNH_B200_F16 ? launch_join<__half>(ctx, p, l.workers, l.tiles, stream)
+                                                                                                                 : launch_join<__nv_bfloat16>(ctx, p, l.workers, l.tiles, stream);
         CUDA_TRY(ctx, e);
     }
     return MSNH_B200_OK;
