@@ -295,24 +295,33 @@ cudaError_t launch_vectors(const MsnhB200Ctx *ctx, const RmsNormParams &p, int v
     return launch_token_kernel(kernel, dim3(static_cast<unsigned>(blocks)), threads, smem, stream, ctx->pdl, p);
 }
 
-// Many rows: a warp a row where that suffices (no barrier), or up to 512 threads that stay. Few rows: a vector a thread, so that a row's
-// bytes are all asked for at once.
+// A block a row, a vector a thread as far as that goes, so that a row's bytes are all asked for at once, except for many rows (600 of them
+// take as long either way):
+// - rows of up to 64 vectors: a warp a row, which needs no barrier (4100 fp16 rows of 256 and 512 values: 3.0 and 4.2 us against 4.7 and
+//   4.8; at 128 vectors it loses, 8.3 against 7.4);
+// - long rows to 8 bits, which leave a block more to compute than to write: blocks that stay and copy ahead (4100 bf16 rows of 5120 and
+//   8192 values: 28.3 and 42.9 us, 5.1 TB/s, against 31.5 and 51.9; at 2048 values 14.5 against 13.2, and rows of x's own type lose at all
+//   lengths: 4100 fp32 rows of 5120 values 58 against 52 us, 4.9 TB/s).
 template <typename T, typename W, bool k8>
 cudaError_t launch(const MsnhB200Ctx *ctx, const RmsNormParams &p, bool aligned, void *stream) {
     const int vectors = p.cols / Vec16<T>::kVec;
     if (aligned && vectors <= 4096) {
-        if (p.rows >= 4 * ctx->sm_count && vectors <= 2048)
-            return vectors <= 32     ? launch_vectors<T, W, k8, 1, true, 3>(ctx, p, vectors, stream)
-                   : vectors <= 64   ? launch_vectors<T, W, k8, 2, true, 3>(ctx, p, vectors, stream)
-                   : vectors <= 128  ? launch_vectors<T, W, k8, 4, true, 3>(ctx, p, vectors, stream)
-                   : vectors <= 1024 ? launch_vectors<T, W, k8, 2, false, 3>(ctx, p, vectors, stream) : launch_vectors<T, W, k8, 4, false, 2>(ctx, p, vectors, stream);
+        if (p.rows >= 4 * ctx->sm_count) {
+            if (vectors <= 32) return launch_vectors<T, W, k8, 1, true, 3>(ctx, p, vectors, stream);
+            if (vectors <= 64) return launch_vectors<T, W, k8, 2, true, 3>(ctx, p, vectors, stream);
+            if constexpr (k8) {
+                if (vectors > 512 && vectors <= 1024) return launch_vectors<T, W, k8, 2, false, 3>(ctx, p, vectors, stream);
+                if (vectors > 1024 && vectors <= 2048) return launch_vectors<T, W, k8, 4, false, 2>(ctx, p, vectors, stream);
+            }
+        }
         return vectors <= 1024   ? launch_vectors<T, W, k8, 1, false, 0>(ctx, p, vectors, stream)
                : vectors <= 2048 ? launch_vectors<T, W, k8, 2, false, 0>(ctx, p, vectors, stream) : launch_vectors<T, W, k8, 4, false, 0>(ctx, p, vectors, stream);
     }
+    // (eight values a thread: 600 fp16 rows of 1001 and 6879 values 3.5 and 15.1 us, in two passes 5.7 and 16.8; sixteen would have 12001
+    // values in 39.0 us, two passes have them in 36.5)
     const dim3 rows(static_cast<unsigned>(p.rows));
     const auto threads_of = [&](int each) { return (p.cols + each * 32 - 1) / (each * 32) * 32; };
     if (p.cols <= 8192) return launch_token_kernel(rms_norm_values_kernel<T, W, k8, 8>, rows, threads_of(8), 0, stream, ctx->pdl, p);
-    if (p.cols <= 16384) return launch_token_kernel(rms_norm_values_kernel<T, W, k8, 16>, rows, threads_of(16), 0, stream, ctx->pdl, p);
     const int threads = 1024;
     return launch_token_kernel(rms_norm_rows_kernel<T, W, k8>, dim3(static_cast<unsigned>(p.rows)), threads, 0, stream, ctx->pdl, p);
 }

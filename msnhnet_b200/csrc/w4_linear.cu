@@ -928,15 +928,16 @@ cudaError_t launch(const MsnhB200Ctx *ctx, W4Params p, void *stream) {
                   : launch(ctx, w4_linear_kernel<X, kColumns, kTiles, kAhead, false>, done[1], p, blocks, ranks, p.x_at, ctx->pdl, stream);
 }
 
+// Whole numbers for one and two rows of many tiles, two tiles at a time: one fp16, bf16 and fp32 row times 8192 x 28672 take 30.3, 32.2 and
+// 32.2 us (3.9 TB/s), with 16-bit operands 34.1, 41.3 and 56.3; times 4096 x 12288 11.8, 12.5 and 12.3 against 12.1, 13.5 and 17.3. With
+// fewer tiles their preparation is the longer one: times 4096 x 4096 7.5 us against 6.2, 6.5 and 7.9.
 template <typename X>
 cudaError_t launch(const MsnhB200Ctx *ctx, const W4Params &p, void *stream) {
-    if (p.rows <= kIntegerRows) {
-        // two tiles at a time where every SM has several
-        const bool two = p.unit_bytes <= 1152 && p.tiles >= 8 * ctx->sm_count;
+    if (p.rows <= kIntegerRows && p.tiles >= 4 * ctx->sm_count) {
         cudaError_t e = cudaSuccess;
         W4Params digits = p;
         if (!digits_apart(p.rows, p.units)) digits.digits_made = nullptr;
-        if (two ? launch_integer<2, 3>(ctx, digits, stream, e) : launch_integer<1, 5>(ctx, digits, stream, e)) return e;
+        if (launch_integer<2, 3>(ctx, digits, stream, e)) return e;
     }
     if (p.rows <= 8) return launch<X, 1, 1, 5>(ctx, p, stream);
     if (p.rows <= 16) return launch<X, 2, 1, 4>(ctx, p, stream);
