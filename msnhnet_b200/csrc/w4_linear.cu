@@ -81,6 +81,7 @@ struct W4Params {
 };
 
 constexpr int kWarps = 16, kSummers = 4, kThreads = (kWarps + kSummers) * 32;      // warps that multiply, and that add up
+constexpr int kMostRanks = 8;                // blocks of a cluster
 
 __device__ __forceinline__ void copy16(uint32_t to, const void *from) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
@@ -399,8 +400,13 @@ __device__ __forceinline__ void turns(const W4Params &p, const Share<kTiles> &s,
             add_up<kRows>(p, s.sets, kCount, sums, threadIdx.x, kThreads, [&](int o, int, int, int, float v) { outputs[o] = v; });
             cluster.sync();
             for (int o = s.rank * kThreads + threadIdx.x; o < s.sets * kRows * p.rows; o += s.ranks * kThreads) {
-                float v = 0.f;
-                for (int q = 0; q < s.ranks; ++q) v += *cluster.map_shared_rank(&outputs[o], q);
+                float v = 0.f, others[kMostRanks];               // (all reads are under way before the first is added)
+#pragma unroll
+                for (int q = 0; q < kMostRanks; ++q)
+                    if (q < s.ranks) others[q] = *cluster.map_shared_rank(&outputs[o], q);
+#pragma unroll
+                for (int q = 0; q < kMostRanks; ++q)
+                    if (q < s.ranks) v += others[q];
                 const int set = o / (kRows * p.rows), m = o % (kRows * p.rows) / kRows, row = o % kRows;
                 put(tile, set * kTiles + row / kTileRows, row % kTileRows, m, v);
             }
@@ -438,7 +444,7 @@ __device__ __forceinline__ void turns(const W4Params &p, const Share<kTiles> &s,
 // Floats of one buffer of sums: the warps', and a block's outputs where a cluster adds them up (all its warps share one set's k then).
 template <int kRows, int kCount> constexpr int kSumsOf = (kWarps + 1) * kRows * kCount;
 
-// One or two rows: products of whole numbers. An activation is fixed-point relative to the largest of its row and span, four signed 8-bit
+// One or two rows (w4_integer_kernel): products of whole numbers. An activation is fixed-point relative to the largest of its row and span, four signed 8-bit
 // digits (30 bits and the sign), and each digit of each row is a column of m16n8k32: one row leaves seven of the eight columns of a product
 // empty anyway. Codes are 8-bit operands after two masks and a shift for 8 of them, where 16-bit ones take nine instructions, and the
 // instructions are what bounds this beside the memory. Sums of a span are exact in 32 bits:
@@ -824,10 +830,139 @@ __global__ void __launch_bounds__(kThreads, 1) w4_linear_kernel(const __grid_con
     copy_wait<0>();
 }
 
+// Still more rows, whose activations no block has room for and every tile would read again from the caches: a warp has a tile to itself, and
+// the block's warps go through k together, each unit's activations copied once for all of them, a ring ahead like the weights. Where that
+// leaves SMs without a block, the blocks of a cluster share k.
+// 64 fp16 rows times 8192 x 8192 take 43.5 us (197 TFLOP/s) where reading them from the caches for every tile took 100; times 4096 x 4096
+// 25.6 (40 before). Of the 2.2 us of a unit the products are 1.1 and the reads of the activations' operands from shared memory another 1.1:
+// tcgen05 would need the weights as operands in shared memory, scaled before they are summed or unloaded for every group.
+template <typename X, int kColumns, int kAhead>
+__global__ void __launch_bounds__(kWarps * 32, 1) w4_rows_kernel(const __grid_constant__ W4Params p) {
+    using H = typename Operand<X>::Type;
+    constexpr int kParts = Operand<X>::kParts, kCount = kColumns * 8, kThreads = kWarps * 32;
+    extern __shared__ __align__(16) uint8_t smem[];              // the weights' rings, the activations' [stage][part][step of 32 values][row][4 x 16 bytes]
+    auto cluster = cooperative_groups::this_cluster();
+    const Share<1> s(p, cluster.num_blocks(), cluster.block_rank());
+    const uint32_t smem_at = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
+    Units<1, kAhead> units(p, s, smem_at + p.ring_at);
+    const int lane = s.lane, part_bytes = p.rows * 256, stage_bytes = kParts * part_bytes;
+    const int all = (s.to - s.from + s.turn - 1) / s.turn * s.block_units;      // units of all turns
+    int issued = 0, next = 0, fill = 0, stage = 0;
+    const auto copy_x = [&] {
+        if (issued < all) {
+#pragma unroll
+            for (int part = 0; part < kParts; ++part) {
+                const uint8_t *from = p.digits_made + (static_cast<size_t>(part) * p.units + s.begin + next) * part_bytes;
+                const uint32_t to = smem_at + p.x_at + fill * stage_bytes + part * part_bytes;
+                for (int i = threadIdx.x * 16; i < part_bytes; i += kThreads * 16) copy16(to + i, from + i);
+            }
+        }
+        ++issued;
+        next = next + 1 == s.block_units ? 0 : next + 1;
+        fill = fill == kAhead - 1 ? 0 : fill + 1;
+    };
+    pdl_enter();
+#pragma unroll 1
+    for (int i = 0; i < kAhead - 1; ++i) copy_x();
+    copy_commit();
+    copy_wait<0>();                                              // (from here on a group a unit)
+    const int record = p.wide ? 16 : 8, span = 4 / p.spans;      // span: in steps of 32 values
+    float acc[kColumns][4];
+    for (int tile = s.mine, first = s.from; first < s.to; first += s.turn, tile += s.turn) {
+        float part[kColumns][4] = {};
+        float2 scale;
+        Zero<H> zero[2];
+#pragma unroll
+        for (int c = 0; c < kColumns; ++c) acc[c][0] = acc[c][1] = acc[c][2] = acc[c][3] = 0.f;
+#pragma unroll 1
+        for (int u = 0; u < s.block_units; ++u) {
+            copy_wait<kAhead - 2>();
+            __syncthreads();                                     // (everybody's copies; the stage that is filled next has been read)
+            copy_x();
+            units.copy();
+            if (tile < s.to) {
+                uint32_t x_now = smem_at + p.x_at + stage * stage_bytes + lane % 4 * 16;
+#pragma unroll
+                for (int step = 0; step < 4; ++step) {
+                    if (step == 0 || (step == 2 && span <= 2) || span == 1) {
+                        uint32_t z0, z8;
+                        take_record(units.slot + kCodeBytes + (step / span * 8 + lane / 4) * record, p.wide, scale, z0, z8);
+                        zero[0].set(z0);
+                        zero[1].set(z8);
+                    }
+                    uint2 now;
+                    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(now.x), "=r"(now.y) : "r"(units.slot + step / 2 * 512 + lane * 16 + step % 2 * 8) : "memory");
+                    uint32_t low[4], high[4], a[2][4];
+                    zero[0].operand(now.x, p.exponents, low);
+                    zero[1].operand(now.y, p.exponents, high);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) { a[i][0] = low[2 * i]; a[i][1] = high[2 * i]; a[i][2] = low[2 * i + 1]; a[i][3] = high[2 * i + 1]; }
+#pragma unroll
+                    for (int c = 0; c < kColumns; ++c) {
+                        const int m = min(c * 8 + lane / 4, p.rows - 1);        // (a column beyond the rows is the last row again)
+#pragma unroll
+                        for (int i = 0; i < kParts; ++i) {
+                            const uint4 b = load_shared(x_now + m * 64 + i * part_bytes);
+                            mma<H>(part[c], a[0], b.x, b.y);
+                            mma<H>(part[c], a[1], b.z, b.w);
+                        }
+                    }
+                    x_now += p.rows * 64;
+                    if (step == 3 || (step == 1 && span <= 2) || span == 1)
+#pragma unroll
+                        for (int c = 0; c < kColumns; ++c)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                acc[c][i] = fmaf(i < 2 ? scale.x : scale.y, part[c][i], acc[c][i]);
+                                part[c][i] = 0.f;
+                            }
+                }
+            }
+            units.next();
+            stage = stage == kAhead - 1 ? 0 : stage + 1;
+        }
+        if (s.ranks == 1 && tile < s.to)
+#pragma unroll
+            for (int c = 0; c < kColumns; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int m = c * 8 + lane % 4 * 2 + i % 2, row = tile * kTileRows + lane / 4 + i / 2 * 8;
+                    if (m < p.rows && row < p.n) store(p, m, row, acc[c][i]);
+                }
+    }
+    copy_wait<0>();
+    if (s.ranks == 1) return;
+    // (one turn then: the sums take the rings' place, [warp][column][row])
+    __syncthreads();
+    float *const sums = reinterpret_cast<float *>(smem);
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sums[(s.warp * kCount + c * 8 + lane % 4 * 2 + i % 2) * kTileRows + lane / 4 + i / 2 * 8] = acc[c][i];
+    cluster.sync();
+    for (int o = s.rank * kThreads + threadIdx.x; o < kWarps * p.rows * (kTileRows / 4); o += s.ranks * kThreads) {
+        const int set = o / (p.rows * (kTileRows / 4)), m = o / (kTileRows / 4) % p.rows, quarter = o % (kTileRows / 4);
+        if (s.from + set >= s.to) continue;
+        float4 v[kMostRanks];                                    // (all reads are under way before the first is added)
+#pragma unroll
+        for (int q = 0; q < kMostRanks; ++q)
+            if (q < s.ranks) v[q] = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(&sums[(set * kCount + m) * kTileRows + quarter * 4], q));
+#pragma unroll
+        for (int q = 1; q < kMostRanks; ++q)
+            if (q < s.ranks) { v[0].x += v[q].x; v[0].y += v[q].y; v[0].z += v[q].z; v[0].w += v[q].w; }
+        const int row = (s.from + set) * kTileRows + quarter * 4;
+        if (row < p.n) store(p, m, row, v[0].x);
+        if (row + 1 < p.n) store(p, m, row + 1, v[0].y);
+        if (row + 2 < p.n) store(p, m, row + 2, v[0].z);
+        if (row + 3 < p.n) store(p, m, row + 3, v[0].w);
+    }
+    cluster.sync();                                              // (no block ends while another reads its sums)
+}
+
 constexpr size_t kSmemMost = 224 * 1024;                         // of shared memory for a block
 
 template <typename Kernel>
-cudaError_t launch(const MsnhB200Ctx *ctx, Kernel kernel, std::atomic<uint64_t> &done, const W4Params &p, int blocks, int ranks, size_t smem, bool dependent, void *stream) {
+cudaError_t launch(const MsnhB200Ctx *ctx, Kernel kernel, std::atomic<uint64_t> &done, const W4Params &p, int blocks, int ranks, int threads, size_t smem, bool dependent, void *stream) {
     // the attribute is a kernel's and a device's: set by the first call there
     const uint64_t bit = 1ull << (ctx->device & 63);
     if (!(done.load(std::memory_order_acquire) & bit)) {
@@ -837,7 +972,7 @@ cudaError_t launch(const MsnhB200Ctx *ctx, Kernel kernel, std::atomic<uint64_t> 
     }
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(blocks * ranks);
-    config.blockDim = dim3(kThreads);
+    config.blockDim = dim3(threads);
     config.dynamicSmemBytes = smem;
     config.stream = static_cast<cudaStream_t>(stream);
     cudaLaunchAttribute attr[2];
@@ -849,6 +984,34 @@ cudaError_t launch(const MsnhB200Ctx *ctx, Kernel kernel, std::atomic<uint64_t> 
     config.attrs = attr;
     config.numAttrs = dependent ? 2 : 1;
     return cudaLaunchKernelEx(&config, kernel, p);
+}
+
+// Clusters of `ranks` blocks, a block an SM, that the device holds at the same time: fewer than SMs / ranks, since a cluster lies in one
+// part of the device (74, 33 and 15 of 2, 4 and 8 blocks; one cluster more runs after all the others). Asked for once.
+int clusters_at_once(const MsnhB200Ctx *ctx, int ranks) {
+    static std::atomic<int> known[64][4];
+    if (ranks == 1) return ctx->sm_count;
+    std::atomic<int> &place = known[ctx->device & 63][ranks == 2 ? 1 : ranks == 4 ? 2 : 3];
+    int n = place.load(std::memory_order_relaxed);
+    if (n) return n;
+    const auto kernel = w4_linear_kernel<__half, 1, 1, 5, true>;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(ranks);
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = kSmemMost;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ranks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    config.attrs = attr;
+    config.numAttrs = 1;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemMost)) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, kernel, &config) != cudaSuccess || n < 1) {
+        cudaGetLastError();                                      // (a cluster less than would fit costs time only)
+        n = std::max(1, ctx->sm_count / ranks * 3 / 4);
+    }
+    place.store(n, std::memory_order_relaxed);
+    return n;
 }
 
 // How many warps of a block share a tile's k: what takes the fewest units one after the other in the busiest warp (tiles at a time x units
@@ -869,14 +1032,14 @@ bool share_out(const MsnhB200Ctx *ctx, W4Params &p, int tiles, Bytes x_bytes, in
     const int turns = up(p.tiles, per_turn(p.split));
     const auto units = [&] { return std::min(p.units, p.split * up(p.units, p.split * ranks)); };
     ranks = 1;
-    while (p.split == kWarps && ranks < 8 && turns * ranks * 2 <= ctx->sm_count && p.split * ranks * 4 <= p.units) ranks *= 2;
+    while (p.split == kWarps && ranks < kMostRanks && turns <= clusters_at_once(ctx, ranks * 2) && p.split * ranks * 4 <= p.units) ranks *= 2;
     const int wanted = ranks;
-    while (p.split == kWarps && ranks < 8 && p.x_at + x_bytes(units()) > kSmemMost && p.split * ranks * 2 <= p.units) ranks *= 2;
+    while (p.split == kWarps && ranks < kMostRanks && p.x_at + x_bytes(units()) > kSmemMost && p.split * ranks * 2 <= p.units) ranks *= 2;
     const bool room = p.x_at + x_bytes(units()) <= kSmemMost;
     if (!room) ranks = wanted;
     p.share = up(p.units, p.split * ranks);
     p.block_units = units();
-    blocks = std::min(turns, ctx->sm_count / ranks);
+    blocks = std::min(turns, clusters_at_once(ctx, ranks));
     return room;
 }
 
@@ -905,7 +1068,7 @@ bool launch_integer(const MsnhB200Ctx *ctx, W4Params p, void *stream, cudaError_
         if (e != cudaSuccess) return true;
     }
     static std::atomic<uint64_t> done{0};
-    e = launch(ctx, w4_integer_kernel<kTiles, kAhead>, done, p, blocks, ranks, p.x_at + bytes(p.block_units), ctx->pdl, stream);
+    e = launch(ctx, w4_integer_kernel<kTiles, kAhead>, done, p, blocks, ranks, kThreads, p.x_at + bytes(p.block_units), ctx->pdl, stream);
     return true;
 }
 
@@ -924,13 +1087,33 @@ cudaError_t launch(const MsnhB200Ctx *ctx, W4Params p, void *stream) {
         if (e != cudaSuccess) return e;
     }
     static std::atomic<uint64_t> done[2];
-    return staged ? launch(ctx, w4_linear_kernel<X, kColumns, kTiles, kAhead, true>, done[0], p, blocks, ranks, p.x_at + bytes(p.block_units), ctx->pdl, stream)
-                  : launch(ctx, w4_linear_kernel<X, kColumns, kTiles, kAhead, false>, done[1], p, blocks, ranks, p.x_at, ctx->pdl, stream);
+    return staged ? launch(ctx, w4_linear_kernel<X, kColumns, kTiles, kAhead, true>, done[0], p, blocks, ranks, kThreads, p.x_at + bytes(p.block_units), ctx->pdl, stream)
+                  : launch(ctx, w4_linear_kernel<X, kColumns, kTiles, kAhead, false>, done[1], p, blocks, ranks, kThreads, p.x_at, ctx->pdl, stream);
+}
+
+template <typename X, int kColumns, int kAhead>
+cudaError_t launch_rows(const MsnhB200Ctx *ctx, W4Params p, void *stream) {
+    const int turns = (p.tiles + kWarps - 1) / kWarps;
+    int ranks = 1;
+    while (ranks < kMostRanks && turns <= clusters_at_once(ctx, ranks * 2) && ranks * 2 <= p.units) ranks *= 2;
+    p.split = 1;
+    p.share = (p.units + ranks - 1) / ranks;
+    p.block_units = p.share;
+    p.ring_at = 0;
+    p.x_at = kWarps * kAhead * static_cast<int>(p.unit_bytes);
+    p.exponents = Zero<typename Operand<X>::Type>::kExponents;
+    const cudaError_t e = launch_token_kernel(w4_operands_kernel<X>, dim3((p.units * p.rows * 16 + 127) / 128), 128, 0, stream, ctx->pdl, p);
+    if (e != cudaSuccess) return e;
+    const size_t rings = p.x_at + static_cast<size_t>(kAhead) * Operand<X>::kParts * p.rows * 256, sums = static_cast<size_t>(kWarps) * kTileRows * kColumns * 8 * 4;
+    static std::atomic<uint64_t> done{0};
+    return launch(ctx, w4_rows_kernel<X, kColumns, kAhead>, done, p, std::min(turns, clusters_at_once(ctx, ranks)), ranks, kWarps * 32, std::max(rings, ranks > 1 ? sums : 0), ctx->pdl, stream);
 }
 
 // Whole numbers for one and two rows of many tiles, two tiles at a time: one fp16, bf16 and fp32 row times 8192 x 28672 take 30.3, 32.2 and
 // 32.2 us (3.9 TB/s), with 16-bit operands 34.1, 41.3 and 56.3; times 4096 x 12288 11.8, 12.5 and 12.3 against 12.1, 13.5 and 17.3. With
 // fewer tiles their preparation is the longer one: times 4096 x 4096 7.5 us against 6.2, 6.5 and 7.9.
+// Nine to sixteen rows keep their activations in shared memory where tiles are few, so that all warps of a block can share k (nine fp16 rows
+// times 4096 x 4096 10.1 us against 14.1; sixteen times 4096 x 12288 and 8192 x 28672 29.8 and 105 us against 22.7 and 68).
 template <typename X>
 cudaError_t launch(const MsnhB200Ctx *ctx, const W4Params &p, void *stream) {
     if (p.rows <= kIntegerRows && p.tiles >= 4 * ctx->sm_count) {
@@ -940,15 +1123,16 @@ cudaError_t launch(const MsnhB200Ctx *ctx, const W4Params &p, void *stream) {
         if (launch_integer<2, 3>(ctx, digits, stream, e)) return e;
     }
     if (p.rows <= 8) return launch<X, 1, 1, 5>(ctx, p, stream);
-    if (p.rows <= 16) return launch<X, 2, 1, 4>(ctx, p, stream);
-    if (p.rows <= 32) return launch<X, 4, 1, 4>(ctx, p, stream);
-    return launch<X, 8, 1, 3>(ctx, p, stream);
+    if (p.rows <= 16) return p.tiles >= 4 * ctx->sm_count ? launch_rows<X, 2, 4>(ctx, p, stream) : launch<X, 2, 1, 4>(ctx, p, stream);
+    if (p.rows <= 32) return launch_rows<X, 4, 4>(ctx, p, stream);
+    if (p.rows <= 48) return launch_rows<X, 6, 3>(ctx, p, stream);
+    return launch_rows<X, 8, 3>(ctx, p, stream);
 }
 
 size_t workspace_of(const W4Layout &l, const MsnhB200W4Linear &a) {
     if (a.rows < 1) return 0;
     const size_t digits = digits_apart(a.rows, l.units) ? digit_bytes(a.rows, l.units) + meta_bytes(a.rows, l.units, l.spans) : 0;
-    return std::max(digits, operands_apart(a.rows, a.dtype, l.units) ? operand_bytes(a.rows, a.dtype, l.units) : 0);
+    return std::max(digits, a.rows > 8 || operands_apart(a.rows, a.dtype, l.units) ? operand_bytes(a.rows, a.dtype, l.units) : 0);
 }
 
 constexpr int kMostOutputs = 1 << 30, kMostValues = 1 << 27;

@@ -228,6 +228,33 @@ def test_w4_of_a_few_turns(ops, dtype, rows, k, n):
     check_w4(ops.w4_linear(x, ops.w4_pack(codes, scales, z, k=k, group=128), x_scale=x_scale), x, w, x_scale, None, k)
 
 
+@pytest.mark.parametrize("rows", [1, 2])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_w4_values_of_all_sizes_times_many_outputs(ops, rows, dtype):
+    k, n = 256, 9500
+    codes, scales, z, w = w4_data(n, k, 64, True)
+    weights = ops.w4_pack(codes, scales, z, k=k, group=64)
+    x = randn(rows, k, seed=35) * torch.exp2(torch.randint(-12, 12, (rows, k), generator=gen(36), device="cuda").float())
+    check_w4(ops.w4_linear(x.to(dtype), weights, out_dtype=F32), x.to(dtype), w, None, None, k)
+    for at in (0, 1, 63, 64, 130, 255):                               # each weight by itself
+        x = torch.zeros(rows, k, device="cuda", dtype=dtype)
+        x[rows - 1, at] = 1
+        y = ops.w4_linear(x, weights, out_dtype=F32)
+        assert torch.equal(y[rows - 1].double(), w[:, at].float().double()) and bool((y[:rows - 1] == 0).all())
+    x = randn(rows, k, seed=37, dtype=dtype)
+    x[0, 200] = float("nan")
+    y = ops.w4_linear(x, weights, out_dtype=F32)
+    assert bool(torch.isnan(y[0]).all())
+    check_w4(y[1:], x[1:], w, None, None, k)
+
+
+@pytest.mark.parametrize("rows,k,n,dtype", [(1, 20000, 9600, F32), (2, 33000, 9500, F16), (2, 5000, 12000, E4M3)])
+def test_w4_of_long_rows_times_many_outputs(ops, rows, k, n, dtype):
+    codes, scales, z, w = w4_data(n, k, 128, True)
+    x, x_scale = w4_x(rows, k, dtype, 38)
+    check_w4(ops.w4_linear(x, ops.w4_pack(codes, scales, z, k=k, group=128), x_scale=x_scale, out_dtype=F32), x, w, x_scale, None, k)
+
+
 @pytest.mark.parametrize("rows,k", [(1, 20000), (2, 33000), (3, 20000), (16, 12000), (64, 9000)])
 def test_w4_of_long_rows(ops, rows, k):
     # operands that no block has room for, and units that many blocks share
