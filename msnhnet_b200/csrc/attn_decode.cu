@@ -12,6 +12,11 @@
 // A warp copies its tiles through a ring of its own with cp.async (rows of 16-byte pieces, gathered page by page), running on into the
 // tiles of its next pair while it works on this one's, and keeps running maximum, sum and values of the query heads in registers. Warps
 // wait for nobody. 16-bit caches: m16n8k16. fp32 caches: CUDA cores (tf32 would lose 13 bits of the products).
+//
+// Measured, both launches: two sequences of up to 131072 fp16 tokens with 8 key heads of 128 (538 MB) 105 us, 5.1 TB/s; 48 of up to 8192
+// bf16 tokens (197 MB) 46 us, 4.3 TB/s, of which the launches, the first tiles and the join are 12; nine of up to 1500 fp32 tokens 14.4 us.
+// Blocks in equal parts of a sequence instead of shares by warp had 115, 140 and 35 us; two to eight times as many blocks, taken up as SMs
+// come free, 114 to 144 us for the first: a warp's start costs 3.5 us.
 #include "kv_cache.h"
 #include "token_types.cuh"
 
@@ -20,8 +25,12 @@ namespace {
 
 constexpr int kTile = 16;                    // tokens of a tile
 constexpr int kMaxRows = 256;                // rows of a launch: what they see is kept in shared memory
-constexpr int kStart = 3, kLeast = 2;        // tiles that a pair's start counts for; tiles of a share, where there are as many
-constexpr int kWholeTiles = 8;               // sequences of at most so many tiles are not cut
+// Tiles that a pair's start counts for, and tiles of a share, where there are as many. (16 rows of 500 fp16 tokens with kStart 1, 3, 6: 29.4,
+// 29.7 and 32.4 us; 48 sequences of up to 8192 bf16 tokens with 0 and 3: 64 and 50.6.)
+constexpr int kStart = 3, kLeast = 2;
+// Sequences of at most so many tiles are not cut, which saves the join (one of 37 and 120 fp16 tokens: 6.6 and 10.3 us, cut 12.0 and 13.1);
+// with 32 tiles to a warp one of 500 tokens takes 28.0 us, cut 10.9.
+constexpr int kWholeTiles = 8;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct AttnParams {
