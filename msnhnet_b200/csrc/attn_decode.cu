@@ -13,7 +13,7 @@
 // tiles of its next pair while it works on this one's, and keeps running maximum, sum and values of the query heads in registers. Warps
 // wait for nobody. 16-bit caches: m16n8k16. fp32 caches: CUDA cores (tf32 would lose 13 bits of the products).
 //
-// Measured, both launches: two sequences of up to 131072 fp16 tokens with 8 key heads of 128 (538 MB) 105 us, 5.1 TB/s; 48 of up to 8192
+// Measured, both launches: two sequences of up to 131072 fp16 tokens with 8 key heads of 128 (538 MB) 105 to 110 us, 4.9 to 5.1 TB/s; 48 of up to 8192
 // bf16 tokens (197 MB) 46 us, 4.3 TB/s, of which the launches, the first tiles and the join are 12; nine of up to 1500 fp32 tokens 14.4 us.
 // Blocks in equal parts of a sequence instead of shares by warp had 115, 140 and 35 us; two to eight times as many blocks, taken up as SMs
 // come free, 114 to 144 us for the first: a warp's start costs 3.5 us.
