@@ -54,7 +54,6 @@ struct Args {
     PyObject *const *args;
     MsnhB200Ctx *ctx;
     c10::Device device;
-    cudaStream_t stream;
 
     Args(PyObject *const *a, Py_ssize_t n, Py_ssize_t wanted) : args(a), device(c10::kCUDA, 0) {
         if (n != wanted) wrong("wrong number of arguments");
@@ -63,8 +62,8 @@ struct Args {
         if (PyErr_Occurred()) throw Refused();
         if (!ctx) wrong("the operators' context is closed");
         device = c10::Device(c10::kCUDA, static_cast<c10::DeviceIndex>(index));
-        stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
     }
+    cudaStream_t stream() const { return c10::cuda::getCurrentCUDAStream(device.index()).stream(); }
     const at::Tensor &tensor(int i, const char *name) const {
         if (!THPVariable_Check(args[i])) wrong(std::string(name) + ": a tensor is wanted");
         const at::Tensor &t = THPVariable_Unpack(args[i]);
@@ -154,7 +153,7 @@ PyObject *rms_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
                                       scale.defined() ? static_cast<float *>(scale.mutable_data_ptr()) : nullptr, rows, static_cast<int32_t>(cols), type_of(type),
                                       type_of(weight.scalar_type()), type_of(out_type), x.stride(0), residual ? residual->stride(0) : 0,
                                       kept.defined() ? kept.stride(0) : 0, y.stride(0), static_cast<float>(a.number(4))};
-        check(a.ctx, msnh_b200_rms_norm(a.ctx, &call, a.stream));
+        check(a.ctx, msnh_b200_rms_norm(a.ctx, &call, a.stream()));
         if (!scale.defined() && !kept.defined()) return wrap(y);
         if (!scale.defined()) return Py_BuildValue("(NN)", wrap(y), wrap(kept));
         if (!kept.defined()) return Py_BuildValue("(NN)", wrap(y), wrap(scale));
@@ -190,7 +189,7 @@ PyObject *w4_linear(PyObject *, PyObject *const *args, Py_ssize_t n) {
             scratch = a.empty({static_cast<int64_t>(call.workspace_bytes)}, at::kByte);
             call.workspace = scratch.mutable_data_ptr();
         }
-        check(a.ctx, msnh_b200_w4_linear(a.ctx, weights, &call, a.stream));
+        check(a.ctx, msnh_b200_w4_linear(a.ctx, weights, &call, a.stream()));
         return wrap(y);
     });
 }
@@ -225,7 +224,7 @@ PyObject *attn_decode(PyObject *, PyObject *const *args, Py_ssize_t n) {
             scratch = a.empty({static_cast<int64_t>(call.workspace_bytes)}, at::kByte);
             call.workspace = scratch.mutable_data_ptr();
         }
-        check(a.ctx, msnh_b200_attn_decode(a.ctx, cache, &call, a.stream));
+        check(a.ctx, msnh_b200_attn_decode(a.ctx, cache, &call, a.stream()));
         return want_lse ? Py_BuildValue("(NN)", wrap(out), wrap(lse)) : wrap(out);
     });
 }
@@ -256,7 +255,7 @@ PyObject *kv_append(PyObject *, PyObject *const *args, Py_ssize_t n) {
         if (tokens > INT32_MAX) wrong("k, v: too many tokens");
         const at::Tensor scratch = kv_scratch(a, cache, count);
         check(a.ctx, msnh_b200_kv_append(a.ctx, cache, seqs ? ints(*seqs) : nullptr, starts ? ints(*starts) : nullptr, static_cast<int>(count), k.const_data_ptr(),
-                                         v.const_data_ptr(), k.stride(0), k.stride(1), static_cast<int>(tokens), scratch.mutable_data_ptr(), scratch.numel(), a.stream));
+                                         v.const_data_ptr(), k.stride(0), k.stride(1), static_cast<int>(tokens), scratch.mutable_data_ptr(), scratch.numel(), a.stream()));
         Py_RETURN_NONE;
     });
 }
@@ -266,27 +265,29 @@ void pair_of(const at::Tensor &src, const at::Tensor &dst) {
     vector_of(dst, src.numel(), at::kInt, "dst");
 }
 
-// address of the cache's struct, src, dst
+// address of the cache's struct, its k_pages, src, dst
 PyObject *kv_fork(PyObject *, PyObject *const *args, Py_ssize_t n) {
     return guarded([&]() -> PyObject * {
-        const Args a(args, n, 5);
+        const Args a(args, n, 6);
         const MsnhB200KvCache *cache = a.pointer<MsnhB200KvCache>(2);
-        const at::Tensor &src = a.tensor(3, "src"), &dst = a.tensor(4, "dst");
+        a.tensor(3, "the cache");
+        const at::Tensor &src = a.tensor(4, "src"), &dst = a.tensor(5, "dst");
         pair_of(src, dst);
         const at::Tensor scratch = kv_scratch(a, cache, src.numel());
-        check(a.ctx, msnh_b200_kv_fork(a.ctx, cache, ints(src), ints(dst), static_cast<int>(src.numel()), scratch.mutable_data_ptr(), scratch.numel(), a.stream));
+        check(a.ctx, msnh_b200_kv_fork(a.ctx, cache, ints(src), ints(dst), static_cast<int>(src.numel()), scratch.mutable_data_ptr(), scratch.numel(), a.stream()));
         Py_RETURN_NONE;
     });
 }
 
-// address of the cache's struct, seqs
+// address of the cache's struct, its k_pages, seqs
 PyObject *kv_free(PyObject *, PyObject *const *args, Py_ssize_t n) {
     return guarded([&]() -> PyObject * {
-        const Args a(args, n, 4);
-        const at::Tensor &seqs = a.tensor(3, "seqs");
+        const Args a(args, n, 5);
+        a.tensor(3, "the cache");
+        const at::Tensor &seqs = a.tensor(4, "seqs");
         vector_of(seqs, seqs.numel(), at::kInt, "seqs");
         if (seqs.numel() > INT32_MAX) wrong("seqs: too many");
-        check(a.ctx, msnh_b200_kv_free(a.ctx, a.pointer<MsnhB200KvCache>(2), ints(seqs), static_cast<int>(seqs.numel()), a.stream));
+        check(a.ctx, msnh_b200_kv_free(a.ctx, a.pointer<MsnhB200KvCache>(2), ints(seqs), static_cast<int>(seqs.numel()), a.stream()));
         Py_RETURN_NONE;
     });
 }
@@ -302,19 +303,20 @@ PyObject *kv_compact(PyObject *, PyObject *const *args, Py_ssize_t n) {
         vector_of(refs_out, cache->n_pages, at::kInt, "refs_out");
         const at::Tensor scratch = kv_scratch(a, cache, 0);
         check(a.ctx, msnh_b200_kv_compact(a.ctx, cache, static_cast<int32_t *>(table_out.mutable_data_ptr()), static_cast<int32_t *>(refs_out.mutable_data_ptr()),
-                                          scratch.mutable_data_ptr(), scratch.numel(), a.stream));
+                                          scratch.mutable_data_ptr(), scratch.numel(), a.stream()));
         Py_RETURN_NONE;
     });
 }
 
-// address of the cache's struct, src, dst
+// address of the cache's struct, its k_pages, src, dst
 PyObject *kv_copy_pages(PyObject *, PyObject *const *args, Py_ssize_t n) {
     return guarded([&]() -> PyObject * {
-        const Args a(args, n, 5);
-        const at::Tensor &src = a.tensor(3, "src"), &dst = a.tensor(4, "dst");
+        const Args a(args, n, 6);
+        a.tensor(3, "the cache");
+        const at::Tensor &src = a.tensor(4, "src"), &dst = a.tensor(5, "dst");
         pair_of(src, dst);
         if (src.numel() > INT32_MAX) wrong("src: too many pages");
-        check(a.ctx, msnh_b200_kv_copy_pages(a.ctx, a.pointer<MsnhB200KvCache>(2), ints(src), ints(dst), static_cast<int>(src.numel()), a.stream));
+        check(a.ctx, msnh_b200_kv_copy_pages(a.ctx, a.pointer<MsnhB200KvCache>(2), ints(src), ints(dst), static_cast<int>(src.numel()), a.stream()));
         Py_RETURN_NONE;
     });
 }

@@ -140,11 +140,11 @@ class TokenOps:
 
     def kv_fork(self, cache, src, dst):
         """Sequences dst (int32, empty before) become copies of sequences src."""
-        _tokens.kv_fork(self._ctx, self._index, cache.address, src, dst)
+        _tokens.kv_fork(self._ctx, self._index, cache.address, cache.k_pages, src, dst)
 
     def kv_free(self, cache, seqs):
         """Sequences seqs (int32) give their pages back."""
-        _tokens.kv_free(self._ctx, self._index, cache.address, seqs)
+        _tokens.kv_free(self._ctx, self._index, cache.address, cache.k_pages, seqs)
 
     def kv_compact(self, cache, table_out=None, refs_out=None):
         """Moves live pages together: afterwards they are the first ones. table_out, refs_out: where the new table and counts go
@@ -154,4 +154,4 @@ class TokenOps:
 
     def kv_copy_pages(self, cache, src, dst):
         """Contents of pages src (int32) to pages dst."""
-        _tokens.kv_copy_pages(self._ctx, self._index, cache.address, src, dst)
+        _tokens.kv_copy_pages(self._ctx, self._index, cache.address, cache.k_pages, src, dst)

@@ -802,3 +802,15 @@ def test_on_another_stream_and_in_a_graph(ops):
     graph.replay()                                                    # the second replay appends a second token
     torch.cuda.synchronize()
     assert torch.equal(out, again) and kept.lengths.tolist() == [n + 2 for n in lengths]
+
+
+def test_upkeep_refuses_a_cache_of_another_device(ops):
+    # (a tensor of the CPU stands for one of another GPU)
+    cache, _, _ = make_cache([5, 0, 3], 4, 1, 8, F16, 94)
+    before = cache.lengths.tolist(), cache.refs.tolist()
+    cache.k_pages = cache.k_pages.cpu()
+    for call in (lambda: ops.kv_fork(cache, ints(0), ints(1)), lambda: ops.kv_free(cache, ints(0)), lambda: ops.kv_copy_pages(cache, ints(0), ints(1)),
+                 lambda: ops.kv_append(cache, cache.k_pages[0, :3], cache.k_pages[0, :3])):
+        with pytest.raises(ValueError, match="cpu"):
+            call()
+    assert (cache.lengths.tolist(), cache.refs.tolist()) == before
