@@ -18,10 +18,17 @@ E4M3 = torch.float8_e4m3fn
 
 class Reader:
     """A decoder of `layers` layers: width features, heads query heads over kv_heads key heads of head_dim, ffn hidden values, vocab tokens.
-    At most n_seqs sequences of max_tokens (features and tokens) each."""
+    At most n_seqs sequences of max_tokens (features and tokens) each, MAX_ROWS of them in a call. What cannot fit raises ValueError
+    before anything is launched."""
+
+    MAX_ROWS = 64                            # of w4_linear
 
     def __init__(self, ops, channels=512, width=512, layers=2, heads=8, kv_heads=2, head_dim=64, ffn=1024, vocab=1000, n_seqs=8, max_tokens=256, page=16, seed=1):
         self.ops, self.width, self.heads, self.kv_heads, self.head_dim, self.layers = ops, width, heads, kv_heads, head_dim, layers
+        self.vocab, self.n_seqs, self.max_tokens = vocab, n_seqs, max_tokens
+        # Tokens of each sequence, at most: the sequences' numbers lie on the GPU, so a step counts for all of them. Where a count reaches
+        # max_tokens the lengths are looked up.
+        self.most = [0] * n_seqs
         g = torch.Generator(device=ops.device).manual_seed(seed)
 
         def normal(*shape):
@@ -72,18 +79,49 @@ class Reader:
         y, scale, _ = ops.rms_norm(delta, self.last_norm, residual=h, residual_out=h, out_dtype=E4M3)
         return ops.w4_linear(y, self.head, x_scale=scale, out_dtype=torch.float32)
 
+    def _take(self, n, seqs, named=None):
+        """Counts n tokens more for sequences `named` (seqs on the GPU without it); ValueError where one of them has no place for them."""
+        known = range(self.n_seqs) if named is None else named
+        if max((self.most[i] for i in known), default=0) + n > self.max_tokens:
+            self.most = self.caches[0].lengths.tolist()              # (waits for the GPU)
+            if named is None:
+                known = [i for i in seqs.tolist() if 0 <= i < self.n_seqs]
+            full = [i for i in known if self.most[i] + n > self.max_tokens]
+            if full:
+                raise ValueError(f"sequences {full}: {n} more tokens would pass {self.max_tokens}")
+        for i in known:
+            self.most[i] += n
+
     def look(self, features, seq):
         """features [cells, channels] (at most 64 cells) become the first tokens of the empty sequence `seq`; logits of every cell."""
         n = features.shape[0]
+        if not 0 <= seq < self.n_seqs or not 0 < n <= self.MAX_ROWS:
+            raise ValueError(f"{n} cells for sequence {seq}: 1 to {self.MAX_ROWS} cells, {self.n_seqs} sequences")
+        self._take(n, None, [seq])
         x = self.ops.w4_linear(features.half(), self.project) + self.position[:n]
         one = torch.tensor([seq], dtype=torch.int32, device=x.device)
         starts = torch.tensor([0, n], dtype=torch.int32, device=x.device)
         return self._decode(x, one.expand(n).contiguous(), lambda cache, k, v: self.ops.kv_append(cache, k, v, seqs=one, starts=starts))
 
     def step(self, ids, seqs):
-        """One token (ids: int64 [n]) behind each of the sequences seqs (int32 [n]); the logits of what follows."""
-        x = self.embedding[ids] + self.position[self.caches[0].lengths[seqs.long()].long()]
-        return self._decode(x, seqs, lambda cache, k, v: self.ops.kv_append(cache, k, v, seqs=seqs))
+        """One token (ids: int64 [n], at most 64) behind each of the sequences seqs (int32 [n]); the logits of what follows. A row whose
+        token or sequence is none leaves every sequence as it was; its logits are NaN."""
+        return self._step(ids, seqs)
+
+    def _step(self, ids, seqs, named=None):
+        if len(ids) != len(seqs) or len(ids) > self.MAX_ROWS:
+            raise ValueError(f"{len(ids)} tokens for {len(seqs)} sequences: as many, and at most {self.MAX_ROWS}")
+        self._take(1, seqs, named)
+        if named is not None:                                        # (all of them known to be in range)
+            return self._decode(self.embedding[ids] + self.position[self.caches[0].lengths[seqs.long()].long()], seqs,
+                                lambda cache, k, v: self.ops.kv_append(cache, k, v, seqs=seqs))
+        # (indexes are kept in range: one that is not would end the process's use of the GPU)
+        seq, token = seqs.clamp(0, self.n_seqs - 1), ids.clamp(0, self.vocab - 1)
+        there = (seq == seqs) & (token == ids)
+        at = self.caches[0].lengths.index_select(0, seq).clamp_(0, self.max_tokens - 1)
+        seqs = torch.where(there, seqs, -1)
+        logits = self._decode(self.embedding.index_select(0, token) + self.position.index_select(0, at), seqs, lambda cache, k, v: self.ops.kv_append(cache, k, v, seqs=seqs))
+        return torch.where(there[:, None], logits, float("nan"))
 
     def fork(self, src, dst):
         for cache in self.caches:
@@ -98,14 +136,23 @@ class Reader:
             self.ops.kv_compact(cache)
 
     def read(self, features, n_tokens):
-        """The likeliest tokens, one after the other, for each of a list of feature maps [cells, channels]: int64 [maps, n_tokens]."""
+        """The likeliest tokens, one after the other, for each of a list of feature maps [cells, channels]: int64 [maps, n_tokens]. Takes
+        sequences 0, 1, ... and forgets them again."""
+        if not 0 < len(features) <= min(self.n_seqs, self.MAX_ROWS) or n_tokens < 1:
+            raise ValueError(f"{n_tokens} tokens for {len(features)} maps: at least one of each, {min(self.n_seqs, self.MAX_ROWS)} maps at most")
+        for f in features:
+            if not 0 < f.shape[0] <= self.MAX_ROWS or f.shape[0] + n_tokens - 1 > self.max_tokens:
+                raise ValueError(f"{f.shape[0]} cells and {n_tokens} tokens: at most {self.MAX_ROWS} cells, {self.max_tokens} of both")
+        named = list(range(len(features)))
         seqs = torch.arange(len(features), dtype=torch.int32, device=self.position.device)
         ids = torch.stack([self.look(f, i)[-1].argmax() for i, f in enumerate(features)])
         said = [ids]
         for _ in range(n_tokens - 1):
-            ids = self.step(ids, seqs).argmax(-1)
+            ids = self._step(ids, seqs, named).argmax(-1)
             said.append(ids)
         self.forget(seqs)
+        for i in named:
+            self.most[i] = 0
         return torch.stack(said, 1)
 
 
@@ -130,7 +177,7 @@ def main():
     net = Net(text, synth.make_blob(text, synth.load_factors("resnet18")), fp16=True, batch=a.images, flags=_ffi.PLAN_KEEP_ALL)
     features = features_of(net, synth.make_images(a.images, 3, 224, 224))
     net.close()
-    reader = Reader(tokens.TokenOps(), n_seqs=a.images)
+    reader = Reader(tokens.TokenOps(), n_seqs=a.images, max_tokens=max(256, features.shape[1] + a.tokens))
     reader.read(list(features), 2)
     torch.cuda.synchronize()
     began = time.perf_counter()

@@ -117,3 +117,36 @@ def test_reader_behind_a_net(ops):
     reader = Reader(ops, n_seqs=2)
     said = reader.read(list(features), 5)
     assert said.shape == (2, 5) and np.array_equal(said.cpu().numpy(), reader.read(list(features), 5).cpu().numpy())
+
+
+def test_reader_fills_a_sequence_and_refuses_more(ops):
+    from msnhnet_b200.reader import Reader
+    reader = Reader(ops, n_seqs=2, max_tokens=52)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    first, second = (torch.randn(n, 512, generator=g, device="cuda") for n in (49, 10))
+    reader.look(first, 0)
+    reader.look(second, 1)
+    for token in (4, 5, 6):
+        reader.step(torch.tensor([token], device="cuda"), ints(0))
+    with pytest.raises(ValueError, match="52"):
+        reader.step(torch.tensor([7], device="cuda"), ints(0))
+    assert reader.caches[0].lengths.tolist() == [52, 10]
+    assert bool(torch.isfinite(reader.step(torch.tensor([7], device="cuda"), ints(1))).all())
+    assert reader.caches[1].lengths.tolist() == [52, 11]
+    reader.forget(ints(0, 1))
+    said = reader.read([first, second], 4)
+    assert torch.equal(said, reader.read([first, second], 4))
+    with pytest.raises(ValueError):
+        reader.read([first, second], 5)
+
+
+def test_reader_leaves_out_rows_of_no_sequence_and_no_token(ops):
+    from msnhnet_b200.reader import Reader
+    reader = Reader(ops, n_seqs=3)
+    features = torch.randn(20, 512, generator=torch.Generator(device="cuda").manual_seed(6), device="cuda")
+    for seq in range(3):
+        reader.look(features, seq)
+    logits = reader.step(torch.tensor([5, 1000, 5, -1, 5], device="cuda"), ints(0, 1, 3, 2, -1))
+    assert torch.isnan(logits).all(-1).tolist() == [False, True, True, True, True] and bool(torch.isfinite(logits[0]).all())
+    assert [c.lengths.tolist() for c in reader.caches] == [[21, 20, 20]] * 2
+    assert [c.refused() for c in reader.caches] == [4, 4]
