@@ -10,6 +10,7 @@
 #include <torch/csrc/DynamicTypes.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 
 #include <cmath>
@@ -67,6 +68,7 @@ struct Args {
     const at::Tensor &tensor(int i, const char *name) const {
         if (!THPVariable_Check(args[i])) wrong(std::string(name) + ": a tensor is wanted");
         const at::Tensor &t = THPVariable_Unpack(args[i]);
+        if (t.requires_grad() && c10::GradMode::is_enabled()) wrong(std::string(name) + ": requires a gradient, and these operators have none (torch.no_grad() takes it as it is)");
         if (t.device() != device) wrong(std::string(name) + ": a tensor on " + t.device().str() + " in a call of " + device.str());
         return t;
     }

@@ -9,7 +9,8 @@
     out = ops.attn_decode(q, cache)
 
 Calls enqueue on torch's current stream of the tensors' device and do not wait; nothing here computes anything. Wrong types, shapes or
-devices raise ValueError before the call, what the library refuses raises _ffi.KernelError. The checks and the C call are native
+devices raise ValueError before the call, and so does a tensor that requires a gradient where torch records gradients: the operators have
+none, and their results would be cut off unnoticed. What the library refuses raises _ffi.KernelError. The checks and the C call are native
 (host/tokens_torch.cpp): in Python they took longer than the kernels of one token.
 """
 import ctypes as C
@@ -23,6 +24,11 @@ from . import _tokens  # noqa: E402  (needs torch's and the kernel library's sym
 
 _DTYPE = {torch.float32: _ffi.F32, torch.float16: _ffi.F16, torch.bfloat16: _ffi.BF16, torch.float8_e4m3fn: _ffi.E4M3}
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _no_gradient(*tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError("a tensor requires a gradient, and these operators have none (torch.no_grad() takes it as it is)")
 
 
 class W4Weights:
@@ -54,6 +60,7 @@ class PagedCache:
                 raise ValueError("page_table, lengths and refs are int32")
         if not lengths.is_contiguous() or not refs.is_contiguous():
             raise ValueError("lengths and refs are contiguous")
+        _no_gradient(k_pages, v_pages)
         self.device = k_pages.device
         if not k_pages.is_cuda or any(t.device != self.device for t in (v_pages, page_table, lengths, refs)):
             raise ValueError("the cache's tensors are on one GPU")
@@ -108,6 +115,7 @@ class TokenOps:
         for t in (codes, scales, zeros):
             if t is not None and t.device != self.device:
                 raise ValueError(f"a tensor on {t.device} in a call of {self.device}")
+        _no_gradient(scales)
         w = W4Weights(None, n, k, group, scales.dtype, zeros is not None)
         size = C.c_size_t()
         self.ctx.check(self.lib.msnh_b200_w4_pack_bytes(self.h, w.ref, C.byref(size)))

@@ -50,3 +50,19 @@ def test_tensors_of_another_device_are_refused(ops, cache):
         ops.kv_compact(cache)
     with pytest.raises(ValueError, match="a tensor on cpu"):
         ops.w4_pack(torch.zeros(4, 16, dtype=torch.uint8), torch.ones(4, 1, dtype=torch.float16), k=32, group=32)
+
+
+def test_tensors_that_require_a_gradient_are_refused(ops, cache):
+    x, w = torch.zeros(2, 8), torch.ones(8, requires_grad=True)
+    grad = {"match": "gradient"}
+    with pytest.raises(ValueError, **grad):
+        ops.rms_norm(x.requires_grad_(), torch.ones(8))
+    with pytest.raises(ValueError, **grad):
+        ops.attn_decode(torch.zeros(2, 1, 8, requires_grad=True), cache)
+    cache.k_pages.requires_grad_()
+    with pytest.raises(ValueError, **grad):
+        ops.kv_free(cache, ints(0))
+    with pytest.raises(ValueError, **grad):
+        tokens.PagedCache(cache.k_pages, cache.v_pages, cache.page_table, cache.lengths, cache.refs)
+    with torch.no_grad(), pytest.raises(ValueError, match="cpu"):    # (the next thing that is wrong)
+        ops.rms_norm(x, w)

@@ -814,3 +814,20 @@ def test_upkeep_refuses_a_cache_of_another_device(ops):
         with pytest.raises(ValueError, match="cpu"):
             call()
     assert (cache.lengths.tolist(), cache.refs.tolist()) == before
+
+
+def test_inputs_that_require_a_gradient(ops):
+    x, r, w = randn(3, 64, seed=95), randn(3, 64, seed=96), randn(64, seed=97)
+    codes, scales, z, _ = w4_data(32, 64, 32, True)
+    weights = ops.w4_pack(codes, scales, z, k=64, group=32)
+    cache, _, _ = make_cache([5, 9, 2], 4, 2, 16, F32, 98)
+    q = randn(3, 4, 16, seed=99)
+    calls = [(lambda a: ops.rms_norm(a, w), x), (lambda a: ops.rms_norm(x, a), w), (lambda a: ops.rms_norm(x, w, residual=a)[0], r), (lambda a: ops.w4_linear(a, weights), x),
+             (lambda a: ops.w4_linear(x, weights, bias=a), randn(32, seed=100)), (lambda a: ops.attn_decode(a, cache), q),
+             (lambda a: ops.w4_pack(codes, a, z, k=64, group=32).packed, scales)]
+    for call, t in calls:
+        want, t = call(t), t.detach().clone().requires_grad_()
+        with pytest.raises(ValueError, match="gradient"):
+            call(t)
+        with torch.no_grad():
+            assert torch.equal(call(t), want)
