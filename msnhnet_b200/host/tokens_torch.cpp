@@ -72,6 +72,19 @@ struct Args {
         if (t.device() != device) wrong(std::string(name) + ": a tensor on " + t.device().str() + " in a call of " + device.str());
         return t;
     }
+    // The call writes into t: torch learns of it as of its own writes in place, so what was saved of t for a backward pass counts as lost.
+    static void writes(const at::Tensor &t) {
+        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    }
+    // The tensors of a cache, which a call of its upkeep writes.
+    void writes_cache(int i) const {
+        if (!PyTuple_Check(args[i])) wrong("the cache: a tuple of tensors is wanted");
+        for (Py_ssize_t k = 0; k < PyTuple_GET_SIZE(args[i]); ++k) {
+            PyObject *one = PyTuple_GET_ITEM(args[i], k);
+            if (!THPVariable_Check(one)) wrong("the cache: a tuple of tensors is wanted");
+            writes(THPVariable_Unpack(one));
+        }
+    }
     const at::Tensor *maybe(int i, const char *name) const { return args[i] == Py_None ? nullptr : &tensor(i, name); }
     at::ScalarType dtype(int i, at::ScalarType otherwise) const {
         if (args[i] == Py_None) return otherwise;
@@ -156,6 +169,8 @@ PyObject *rms_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
                                       type_of(weight.scalar_type()), type_of(out_type), x.stride(0), residual ? residual->stride(0) : 0,
                                       kept.defined() ? kept.stride(0) : 0, y.stride(0), static_cast<float>(a.number(4))};
         check(a.ctx, msnh_b200_rms_norm(a.ctx, &call, a.stream()));
+        if (out) a.writes(*out);
+        if (residual_out) a.writes(*residual_out);
         if (!scale.defined() && !kept.defined()) return wrap(y);
         if (!scale.defined()) return Py_BuildValue("(NN)", wrap(y), wrap(kept));
         if (!kept.defined()) return Py_BuildValue("(NN)", wrap(y), wrap(scale));
@@ -192,6 +207,7 @@ PyObject *w4_linear(PyObject *, PyObject *const *args, Py_ssize_t n) {
             call.workspace = scratch.mutable_data_ptr();
         }
         check(a.ctx, msnh_b200_w4_linear(a.ctx, weights, &call, a.stream()));
+        if (out) a.writes(*out);
         return wrap(y);
     });
 }
@@ -227,6 +243,7 @@ PyObject *attn_decode(PyObject *, PyObject *const *args, Py_ssize_t n) {
             call.workspace = scratch.mutable_data_ptr();
         }
         check(a.ctx, msnh_b200_attn_decode(a.ctx, cache, &call, a.stream()));
+        if (given) a.writes(*given);
         return want_lse ? Py_BuildValue("(NN)", wrap(out), wrap(lse)) : wrap(out);
     });
 }
@@ -239,17 +256,17 @@ at::Tensor kv_scratch(const Args &a, const MsnhB200KvCache *cache, int64_t n) {
 }
 const int32_t *ints(const at::Tensor &t) { return static_cast<const int32_t *>(t.const_data_ptr()); }
 
-// address of the cache's struct, its k_pages, k, v, seqs or None, starts or None
+// address of the cache's struct, its k_pages, all its tensors, k, v, seqs or None, starts or None
 PyObject *kv_append(PyObject *, PyObject *const *args, Py_ssize_t n) {
     return guarded([&]() -> PyObject * {
-        const Args a(args, n, 8);
+        const Args a(args, n, 9);
         const MsnhB200KvCache *cache = a.pointer<MsnhB200KvCache>(2);
-        const at::Tensor &pages = a.tensor(3, "the cache"), &k = a.tensor(4, "k"), &v = a.tensor(5, "v");
+        const at::Tensor &pages = a.tensor(3, "the cache"), &k = a.tensor(5, "k"), &v = a.tensor(6, "v");
         if (k.dim() != 3 || v.sizes() != k.sizes() || k.size(1) != cache->n_kv_heads || k.size(2) != cache->head_dim || k.scalar_type() != pages.scalar_type() ||
             v.scalar_type() != k.scalar_type())
             wrong("k, v: [tokens, " + std::to_string(cache->n_kv_heads) + ", " + std::to_string(cache->head_dim) + "] of the cache's type " + c10::toString(pages.scalar_type()));
         if (v.strides() != k.strides() || (k.stride(2) != 1 && k.size(2) > 1)) wrong("k, v: the same strides, the values of a head side by side");
-        const at::Tensor *seqs = a.maybe(6, "seqs"), *starts = a.maybe(7, "starts");
+        const at::Tensor *seqs = a.maybe(7, "seqs"), *starts = a.maybe(8, "starts");
         const int64_t tokens = k.size(0), count = !starts ? tokens : starts->dim() == 1 && starts->size(0) ? starts->size(0) - 1 : -1;
         if (starts) vector_of(*starts, count + 1, at::kInt, "starts");
         if (count < 0) wrong("starts: one more than sequences");
@@ -258,6 +275,7 @@ PyObject *kv_append(PyObject *, PyObject *const *args, Py_ssize_t n) {
         const at::Tensor scratch = kv_scratch(a, cache, count);
         check(a.ctx, msnh_b200_kv_append(a.ctx, cache, seqs ? ints(*seqs) : nullptr, starts ? ints(*starts) : nullptr, static_cast<int>(count), k.const_data_ptr(),
                                          v.const_data_ptr(), k.stride(0), k.stride(1), static_cast<int>(tokens), scratch.mutable_data_ptr(), scratch.numel(), a.stream()));
+        a.writes_cache(4);
         Py_RETURN_NONE;
     });
 }
@@ -267,58 +285,64 @@ void pair_of(const at::Tensor &src, const at::Tensor &dst) {
     vector_of(dst, src.numel(), at::kInt, "dst");
 }
 
-// address of the cache's struct, its k_pages, src, dst
+// address of the cache's struct, its k_pages, all its tensors, src, dst
 PyObject *kv_fork(PyObject *, PyObject *const *args, Py_ssize_t n) {
     return guarded([&]() -> PyObject * {
-        const Args a(args, n, 6);
+        const Args a(args, n, 7);
         const MsnhB200KvCache *cache = a.pointer<MsnhB200KvCache>(2);
         a.tensor(3, "the cache");
-        const at::Tensor &src = a.tensor(4, "src"), &dst = a.tensor(5, "dst");
+        const at::Tensor &src = a.tensor(5, "src"), &dst = a.tensor(6, "dst");
         pair_of(src, dst);
         const at::Tensor scratch = kv_scratch(a, cache, src.numel());
         check(a.ctx, msnh_b200_kv_fork(a.ctx, cache, ints(src), ints(dst), static_cast<int>(src.numel()), scratch.mutable_data_ptr(), scratch.numel(), a.stream()));
+        a.writes_cache(4);
         Py_RETURN_NONE;
     });
 }
 
-// address of the cache's struct, its k_pages, seqs
+// address of the cache's struct, its k_pages, all its tensors, seqs
 PyObject *kv_free(PyObject *, PyObject *const *args, Py_ssize_t n) {
     return guarded([&]() -> PyObject * {
-        const Args a(args, n, 5);
+        const Args a(args, n, 6);
         a.tensor(3, "the cache");
-        const at::Tensor &seqs = a.tensor(4, "seqs");
+        const at::Tensor &seqs = a.tensor(5, "seqs");
         vector_of(seqs, seqs.numel(), at::kInt, "seqs");
         if (seqs.numel() > INT32_MAX) wrong("seqs: too many");
         check(a.ctx, msnh_b200_kv_free(a.ctx, a.pointer<MsnhB200KvCache>(2), ints(seqs), static_cast<int>(seqs.numel()), a.stream()));
+        a.writes_cache(4);
         Py_RETURN_NONE;
     });
 }
 
-// address of the cache's struct, its page table, table_out, refs_out
+// address of the cache's struct, its page table, all its tensors, table_out, refs_out
 PyObject *kv_compact(PyObject *, PyObject *const *args, Py_ssize_t n) {
     return guarded([&]() -> PyObject * {
-        const Args a(args, n, 6);
+        const Args a(args, n, 7);
         const MsnhB200KvCache *cache = a.pointer<MsnhB200KvCache>(2);
-        const at::Tensor &table = a.tensor(3, "the cache"), &table_out = a.tensor(4, "table_out"), &refs_out = a.tensor(5, "refs_out");
+        const at::Tensor &table = a.tensor(3, "the cache"), &table_out = a.tensor(5, "table_out"), &refs_out = a.tensor(6, "refs_out");
         if (table_out.sizes() != table.sizes() || table_out.strides() != table.strides() || table_out.scalar_type() != at::kInt)
             wrong("table_out: int32, the page table's shape and strides");
         vector_of(refs_out, cache->n_pages, at::kInt, "refs_out");
         const at::Tensor scratch = kv_scratch(a, cache, 0);
         check(a.ctx, msnh_b200_kv_compact(a.ctx, cache, static_cast<int32_t *>(table_out.mutable_data_ptr()), static_cast<int32_t *>(refs_out.mutable_data_ptr()),
                                           scratch.mutable_data_ptr(), scratch.numel(), a.stream()));
+        a.writes_cache(4);
+        a.writes(table_out);
+        a.writes(refs_out);
         Py_RETURN_NONE;
     });
 }
 
-// address of the cache's struct, its k_pages, src, dst
+// address of the cache's struct, its k_pages, all its tensors, src, dst
 PyObject *kv_copy_pages(PyObject *, PyObject *const *args, Py_ssize_t n) {
     return guarded([&]() -> PyObject * {
-        const Args a(args, n, 6);
+        const Args a(args, n, 7);
         a.tensor(3, "the cache");
-        const at::Tensor &src = a.tensor(4, "src"), &dst = a.tensor(5, "dst");
+        const at::Tensor &src = a.tensor(5, "src"), &dst = a.tensor(6, "dst");
         pair_of(src, dst);
         if (src.numel() > INT32_MAX) wrong("src: too many pages");
         check(a.ctx, msnh_b200_kv_copy_pages(a.ctx, a.pointer<MsnhB200KvCache>(2), ints(src), ints(dst), static_cast<int>(src.numel()), a.stream()));
+        a.writes_cache(4);
         Py_RETURN_NONE;
     });
 }

@@ -66,6 +66,7 @@ class PagedCache:
             raise ValueError("the cache's tensors are on one GPU")
         self.k_pages, self.v_pages, self.page_table, self.lengths, self.refs = k_pages, v_pages, page_table, lengths, refs
         self.refused_count = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self.tensors = k_pages, v_pages, page_table, lengths, refs, self.refused_count
         self.dtype = k_pages.dtype
         self.n_pages, self.page_size, self.n_kv_heads, self.head_dim = k_pages.shape
         self.n_seqs, self.max_pages = page_table.shape
@@ -144,22 +145,22 @@ class TokenOps:
     def kv_append(self, cache, k, v, seqs=None, starts=None):
         """Tokens behind their sequences' own: k, v [tokens, n_kv_heads, head_dim]; one token for each of seqs (int32; without it for
         sequences 0, 1, ...), or rows starts[i] to starts[i + 1] (int32, one more than sequences) for sequence seqs[i]."""
-        _tokens.kv_append(self._ctx, self._index, cache.address, cache.k_pages, k, v, seqs, starts)
+        _tokens.kv_append(self._ctx, self._index, cache.address, cache.k_pages, cache.tensors, k, v, seqs, starts)
 
     def kv_fork(self, cache, src, dst):
         """Sequences dst (int32, empty before) become copies of sequences src."""
-        _tokens.kv_fork(self._ctx, self._index, cache.address, cache.k_pages, src, dst)
+        _tokens.kv_fork(self._ctx, self._index, cache.address, cache.k_pages, cache.tensors, src, dst)
 
     def kv_free(self, cache, seqs):
         """Sequences seqs (int32) give their pages back."""
-        _tokens.kv_free(self._ctx, self._index, cache.address, cache.k_pages, seqs)
+        _tokens.kv_free(self._ctx, self._index, cache.address, cache.k_pages, cache.tensors, seqs)
 
     def kv_compact(self, cache, table_out=None, refs_out=None):
         """Moves live pages together: afterwards they are the first ones. table_out, refs_out: where the new table and counts go
         (the cache's own without them)."""
-        _tokens.kv_compact(self._ctx, self._index, cache.address, cache.page_table, cache.page_table if table_out is None else table_out,
+        _tokens.kv_compact(self._ctx, self._index, cache.address, cache.page_table, cache.tensors, cache.page_table if table_out is None else table_out,
                            cache.refs if refs_out is None else refs_out)
 
     def kv_copy_pages(self, cache, src, dst):
         """Contents of pages src (int32) to pages dst."""
-        _tokens.kv_copy_pages(self._ctx, self._index, cache.address, cache.k_pages, src, dst)
+        _tokens.kv_copy_pages(self._ctx, self._index, cache.address, cache.k_pages, cache.tensors, src, dst)

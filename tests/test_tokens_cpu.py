@@ -22,6 +22,7 @@ def cache():
     c = tokens.PagedCache.__new__(tokens.PagedCache)
     c.k_pages, c.v_pages = torch.zeros(4, 2, 1, 8), torch.zeros(4, 2, 1, 8)
     c.page_table, c.lengths, c.refs = (torch.zeros(*shape, dtype=torch.int32) for shape in ((2, 3), (2,), (4,)))
+    c.tensors = c.k_pages, c.v_pages, c.page_table, c.lengths, c.refs
     c.args = _ffi.KvCache(c.k_pages.data_ptr(), c.v_pages.data_ptr(), 16, 8, 8, 16, 8, 8, c.page_table.data_ptr(), c.lengths.data_ptr(), c.refs.data_ptr(), None, 3, 4, 2, 1, 8,
                           2, 3, _ffi.F32)
     c.address = ctypes.addressof(c.args)

@@ -831,3 +831,31 @@ def test_inputs_that_require_a_gradient(ops):
             call(t)
         with torch.no_grad():
             assert torch.equal(call(t), want)
+
+
+def test_writes_are_known_to_torch(ops):
+    # what is written in place no longer counts as what was saved for a backward pass
+    x, r, w, out = randn(3, 64, seed=101), randn(3, 64, seed=102), randn(64, seed=103), randn(3, 64, seed=104)
+    codes, scales, z, _ = w4_data(64, 64, 32, True)
+    weights = ops.w4_pack(codes, scales, z, k=64, group=32)
+    cache, _, _ = make_cache([5, 9, 2, 0], 4, 2, 16, F32, 105)
+    q, kv, o = randn(4, 4, 16, seed=106), randn(1, 2, 16, seed=107), randn(4, 4, 16, seed=108)
+    table, refs = torch.zeros_like(cache.page_table), torch.zeros_like(cache.refs)
+    calls = [(lambda: ops.rms_norm(x, w, residual=r, residual_out=r, out=out), [out, r], [x, w]), (lambda: ops.w4_linear(x, weights, out=out), [out], [x]),
+             (lambda: ops.attn_decode(q, cache, out=o), [o], [q, cache.k_pages, cache.lengths]),
+             (lambda: ops.kv_append(cache, kv, kv, seqs=ints(2)), [cache.k_pages, cache.v_pages, cache.lengths, cache.refs, cache.page_table], [kv]),
+             (lambda: ops.kv_fork(cache, ints(0), ints(3)), [cache.k_pages, cache.v_pages, cache.lengths, cache.refs, cache.page_table], []),
+             (lambda: ops.kv_free(cache, ints(0)), [cache.lengths, cache.refs], []), (lambda: ops.kv_copy_pages(cache, ints(0), ints(1)), [cache.k_pages, cache.v_pages], []),
+             (lambda: ops.kv_compact(cache, table_out=table, refs_out=refs), [cache.k_pages, cache.v_pages, table, refs], [])]
+    for call, written, read in calls:
+        before = [t._version for t in written], [t._version for t in read]
+        call()
+        assert all(t._version > v for t, v in zip(written, before[0])) and [t._version for t in read] == before[1]
+    with torch.no_grad():
+        a = torch.ones(3, 64, device="cuda", requires_grad=True)
+    y = a * out
+    ops.rms_norm(x, w, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with torch.inference_mode():                                      # tensors without such a count
+        ops.rms_norm(x, w, out=torch.empty_like(x))
