@@ -18,25 +18,33 @@ struct RmsNormParams {
     float eps;
 };
 
-// Sum and maximum over a block; every thread gets both. A NaN among the squares makes the sum NaN, so the maximum may drop it.
+// The largest of top, |a| and |b|, or NaN where one is: of the products with the weights, which the sum of squares knows nothing of.
+__device__ __forceinline__ float max_or_nan(float top, float a, float b) {
+    float y;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(top), "f"(a), "f"(b));
+    return y;
+}
+// The same over a warp, of values that are not negative: their bits have the numbers' order, infinity and NaN above all of them.
+__device__ __forceinline__ float warp_max_or_nan(float top) { return __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(top))); }
+
+// Sum and maximum over a block; every thread gets both.
 __device__ __forceinline__ void block_sum_max(float &sum, float &top) {
     __shared__ float part[2][32];
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        sum += __shfl_xor_sync(~0u, sum, o);
-        top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-    }
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+    top = warp_max_or_nan(top);
     const int warps = blockDim.x / 32, lane = threadIdx.x % 32;
     if (lane == 0) { part[0][threadIdx.x / 32] = sum; part[1][threadIdx.x / 32] = top; }
     __syncthreads();
     sum = lane < warps ? part[0][lane] : 0.f;
     top = lane < warps ? part[1][lane] : 0.f;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        sum += __shfl_xor_sync(~0u, sum, o);
-        top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-    }
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+    top = warp_max_or_nan(top);
 }
+
+// The scale of a row's 8-bit codes; NaN, which leaves the codes 0, where a product with a weight is not finite.
+__device__ __forceinline__ float scale_of(float top, float factor) { return top <= 3.4028235e38f ? top * factor / 448.f : __uint_as_float(0x7fffffffu); }
 
 // value / scale without the scale's own rounding: t * 448 / top, where t is the value before its row's common factor and top the
 // largest |t|. (1 / top is infinite below 2^-127; the division is exact there, too.)
@@ -127,18 +135,15 @@ __global__ void __launch_bounds__(kWarp ? 128 : kStages ? 512 : 1024) rms_norm_v
             if constexpr (k8) {                                  // (h times weight is all that is needed from here on)
                 weights_of(v, b);
 #pragma unroll
-                for (int j = 0; j < kVec; ++j) {
-                    h[i][j] *= b[j];
-                    top = fmaxf(top, fabsf(h[i][j]));
-                }
+                for (int j = 0; j < kVec; ++j) h[i][j] *= b[j];
+#pragma unroll
+                for (int j = 0; j < kVec; j += 2) top = max_or_nan(top, h[i][j], h[i][j + 1]);
             }
         }
         stage = stage == kStages - 1 ? 0 : stage + 1;
 #pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            sum += __shfl_xor_sync(~0u, sum, o);
-            if (k8) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-        }
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+        if (k8) top = warp_max_or_nan(top);
         if (!kWarp && warps > 1) {
             // (two sets of places: the next row's are written while this one's may still be read)
             if (lane == 0) { part[turn][0][warp] = sum; part[turn][1][warp] = top; }
@@ -146,14 +151,12 @@ __global__ void __launch_bounds__(kWarp ? 128 : kStages ? 512 : 1024) rms_norm_v
             sum = lane < warps ? part[turn][0][lane] : 0.f;
             top = lane < warps ? part[turn][1][lane] : 0.f;
 #pragma unroll
-            for (int o = 16; o; o >>= 1) {
-                sum += __shfl_xor_sync(~0u, sum, o);
-                if (k8) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-            }
+            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+            if (k8) top = warp_max_or_nan(top);
         }
         const float factor = rsqrtf(sum / p.cols + p.eps);
         if constexpr (k8) {
-            const float scale = top * factor / 448.f;
+            const float scale = scale_of(top, factor);
             if (thread == 0) p.y_scale[row] = scale;
             // (448 / top is infinite below 2^-119: both are taken times 2^64 there. No codes for a row without a scale.)
             if (!(top > 1e-30f)) {
@@ -226,11 +229,11 @@ __global__ void __launch_bounds__(1024) rms_norm_values_kernel(const __grid_cons
         if (residual_out && i < p.cols) residual_out[i] = from_float<T>(h[j]);
         if (k8) {                                                // (h times weight is all that is needed from here on)
             h[j] *= i < p.cols ? to_float(weight[i]) : 0.f;
-            top = fmaxf(top, fabsf(h[j]));
+            if (j % 2) top = max_or_nan(top, h[j - 1], h[j]);
         }
     }
     block_sum_max(sum, top);
-    const float r = rsqrtf(sum / p.cols + p.eps), scale = top * r / 448.f;
+    const float r = rsqrtf(sum / p.cols + p.eps), scale = scale_of(top, r);
     if (k8 && threadIdx.x == 0) p.y_scale[row] = scale;
     // (448 / top is infinite below 2^-119: both are taken times 2^64 there. No codes for a row without a scale.)
     float lift = 1.f;
@@ -261,11 +264,11 @@ __global__ void rms_norm_rows_kernel(RmsNormParams p) {
     for (int i = threadIdx.x; i < p.cols; i += blockDim.x) {
         const float h = to_float(x[i]) + (residual ? to_float(residual[i]) : 0.f);
         sum += h * h;
-        if (k8) top = fmaxf(top, fabsf(h * to_float(weight[i])));
+        if (k8) top = max_or_nan(top, h * to_float(weight[i]), 0.f);
     }
     block_sum_max(sum, top);
     const float r = rsqrtf(sum / p.cols + p.eps);
-    const float scale = top * r / 448.f, inverse = 448.f / top;
+    const float scale = scale_of(top, r), inverse = 448.f / top;
     if (k8 && threadIdx.x == 0) p.y_scale[row] = scale;
     for (int i = threadIdx.x; i < p.cols; i += blockDim.x) {
         const float h = to_float(x[i]) + (residual ? to_float(residual[i]) : 0.f);

@@ -859,3 +859,15 @@ def test_writes_are_known_to_torch(ops):
         y.sum().backward()
     with torch.inference_mode():                                      # tensors without such a count
         ops.rms_norm(x, w, out=torch.empty_like(x))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows,cols", [(3, 96), (700, 256), (3, 1024), (700, 5120), (700, 12288), (3, 4097), (3, 40000)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_norm_to_8_bits_with_a_weight_that_is_no_number(ops, dtype, rows, cols, bad):
+    # every row's y is not finite then; a value of 0 times an infinite weight is NaN, too
+    x, w = randn(rows, cols, seed=109, dtype=dtype), randn(cols, seed=110, dtype=dtype)
+    x[1, cols // 2] = 0
+    w[cols // 2] = bad
+    codes, scale = ops.rms_norm(x, w, out_dtype=E4M3)
+    assert bool(torch.isnan(scale).all()) and bool((codes.float() == 0).all())
