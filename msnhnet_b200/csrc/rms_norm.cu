@@ -27,12 +27,12 @@ __device__ __forceinline__ float max_or_nan(float top, float a, float b) {
 // The same over a warp, of values that are not negative: their bits have the numbers' order, infinity and NaN above all of them.
 __device__ __forceinline__ float warp_max_or_nan(float top) { return __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(top))); }
 
-// Sum and maximum over a block; every thread gets both.
-__device__ __forceinline__ void block_sum_max(float &sum, float &top) {
+// Sum and, for 8 bits, maximum over a block; every thread gets both.
+template <bool k8> __device__ __forceinline__ void block_sum_max(float &sum, float &top) {
     __shared__ float part[2][32];
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-    top = warp_max_or_nan(top);
+    if (k8) top = warp_max_or_nan(top);
     const int warps = blockDim.x / 32, lane = threadIdx.x % 32;
     if (lane == 0) { part[0][threadIdx.x / 32] = sum; part[1][threadIdx.x / 32] = top; }
     __syncthreads();
@@ -40,11 +40,14 @@ __device__ __forceinline__ void block_sum_max(float &sum, float &top) {
     top = lane < warps ? part[1][lane] : 0.f;
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-    top = warp_max_or_nan(top);
+    if (k8) top = warp_max_or_nan(top);
 }
 
-// The scale of a row's 8-bit codes; NaN, which leaves the codes 0, where a product with a weight is not finite.
-__device__ __forceinline__ float scale_of(float top, float factor) { return top <= 3.4028235e38f ? top * factor / 448.f : __uint_as_float(0x7fffffffu); }
+// The scale of a row's 8-bit codes; NaN, which leaves the codes 0, where a product with a weight is not finite; 0 for zeros, whose factor
+// is infinite without an eps.
+__device__ __forceinline__ float scale_of(float top, float factor) {
+    return top == 0.f ? 0.f : top <= 3.4028235e38f ? top * factor / 448.f : __uint_as_float(0x7fffffffu);
+}
 
 // value / scale without the scale's own rounding: t * 448 / top, where t is the value before its row's common factor and top the
 // largest |t|. (1 / top is infinite below 2^-127; the division is exact there, too.)
@@ -232,7 +235,7 @@ __global__ void __launch_bounds__(1024) rms_norm_values_kernel(const __grid_cons
             if (j % 2) top = max_or_nan(top, h[j - 1], h[j]);
         }
     }
-    block_sum_max(sum, top);
+    block_sum_max<k8>(sum, top);
     const float r = rsqrtf(sum / p.cols + p.eps), scale = scale_of(top, r);
     if (k8 && threadIdx.x == 0) p.y_scale[row] = scale;
     // (448 / top is infinite below 2^-119: both are taken times 2^64 there. No codes for a row without a scale.)
@@ -266,7 +269,7 @@ __global__ void rms_norm_rows_kernel(RmsNormParams p) {
         sum += h * h;
         if (k8) top = max_or_nan(top, h * to_float(weight[i]), 0.f);
     }
-    block_sum_max(sum, top);
+    block_sum_max<k8>(sum, top);
     const float r = rsqrtf(sum / p.cols + p.eps);
     const float scale = scale_of(top, r), inverse = 448.f / top;
     if (k8 && threadIdx.x == 0) p.y_scale[row] = scale;

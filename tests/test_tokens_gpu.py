@@ -871,3 +871,13 @@ def test_norm_to_8_bits_with_a_weight_that_is_no_number(ops, dtype, rows, cols, 
     w[cols // 2] = bad
     codes, scale = ops.rms_norm(x, w, out_dtype=E4M3)
     assert bool(torch.isnan(scale).all()) and bool((codes.float() == 0).all())
+
+
+@pytest.mark.parametrize("rows,cols", [(3, 96), (700, 256), (700, 5120), (700, 12288), (3, 4097), (3, 40000)])
+def test_norm_to_8_bits_of_zeros_without_an_eps(ops, rows, cols):
+    x, w = randn(rows, cols, seed=111, dtype=BF16), randn(cols, seed=112, dtype=BF16)
+    x[1] = 0
+    codes, scale = ops.rms_norm(x, w, eps=0.0, out_dtype=E4M3)
+    assert float(scale[1]) == 0 and bool((codes[1].float() == 0).all())
+    others = [i for i in range(rows) if i != 1]
+    check_codes(codes[others], scale[others], norm_ref(x[others], None, w, 0.0)[1], cols)
