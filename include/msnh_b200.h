@@ -335,7 +335,9 @@ const char *msnh_b200_static_last_error(void);
 /* y = h * rsqrt(mean(h^2) + eps) * weight, h = x + residual (x alone without a residual), over rows of `cols` values.
  * h is held in fp32; residual_out (may be NULL; may be x's or the residual's memory) receives it rounded to `dtype`.
  * out_dtype = dtype, or MSNH_B200_E4M3: y_scale[row] = max|y| / 448 and y holds y / y_scale to the nearest (ties to even);
- * a row of zeros has scale 0 and codes 0, a row whose y is not finite scale NaN and codes 0. y may be x's, the residual's or
+ * a row of zeros has scale 0 and codes 0, a row whose y is not finite scale NaN and codes 0. h * weight and the sum of h^2 are fp32,
+ * too: where the sum passes its range (values from about 1e19 on) a row's y is 0 (and NaN at infinities) in `dtype`, and in 8 bits a
+ * row where either is not finite has scale NaN and codes 0. y may be x's, the residual's or
  * residual_out's memory only where types and strides agree (y then overwrites what lay there). */
 typedef struct MsnhB200RmsNorm {
     const void *x, *residual, *weight;

@@ -43,10 +43,10 @@ template <bool k8> __device__ __forceinline__ void block_sum_max(float &sum, flo
     if (k8) top = warp_max_or_nan(top);
 }
 
-// The scale of a row's 8-bit codes; NaN, which leaves the codes 0, where a product with a weight is not finite; 0 for zeros, whose factor
-// is infinite without an eps.
+// The scale of a row's 8-bit codes; NaN, which leaves the codes 0, where a product with a weight is not finite or the sum of squares is not
+// (the factor is 0 then); 0 for zeros, whose factor is infinite without an eps.
 __device__ __forceinline__ float scale_of(float top, float factor) {
-    return top == 0.f ? 0.f : top <= 3.4028235e38f ? top * factor / 448.f : __uint_as_float(0x7fffffffu);
+    return top == 0.f ? 0.f : top <= 3.4028235e38f && factor > 0.f ? top * factor / 448.f : __uint_as_float(0x7fffffffu);
 }
 
 // value / scale without the scale's own rounding: t * 448 / top, where t is the value before its row's common factor and top the

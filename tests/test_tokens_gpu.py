@@ -881,3 +881,17 @@ def test_norm_to_8_bits_of_zeros_without_an_eps(ops, rows, cols):
     assert float(scale[1]) == 0 and bool((codes[1].float() == 0).all())
     others = [i for i in range(rows) if i != 1]
     check_codes(codes[others], scale[others], norm_ref(x[others], None, w, 0.0)[1], cols)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,cols", [(5, 96), (700, 64), (700, 512), (5, 1024), (700, 5120), (700, 12288), (5, 16384), (5, 4097), (5, 40000)])
+def test_norm_to_8_bits_of_rows_whose_squares_overflow(ops, dtype, rows, cols):
+    # no zeros in the place of values that are none: the scale says so
+    x, w = randn(rows, cols, seed=113), randn(cols, seed=115, dtype=dtype)
+    x[0] *= 1e30
+    x[2, cols // 2] = 1e25
+    x = x.to(dtype)
+    codes, scale = ops.rms_norm(x, w, out_dtype=E4M3)
+    assert torch.isnan(scale).tolist() == [i in (0, 2) for i in range(rows)] and bool((codes[[0, 2]].float() == 0).all())
+    others = [i for i in range(rows) if i not in (0, 2)]
+    check_codes(codes[others], scale[others], norm_ref(x[others], None, w, 1e-6)[1], cols)
