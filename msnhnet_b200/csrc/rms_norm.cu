@@ -254,17 +254,18 @@ __global__ void __launch_bounds__(1024) rms_norm_values_kernel(const __grid_cons
 }
 
 // A block a row, two passes over it: the sum of squares and (8 bits) the largest |h * w|, then the outputs. Any row length,
-// alignment and stride.
+// alignment and stride. (Places are unsigned: one behind a row of up to 2^31 - 1 values may pass 2^31.)
 template <typename T, typename W, bool k8>
 __global__ void rms_norm_rows_kernel(RmsNormParams p) {
     pdl_enter();
     const long long row = blockIdx.x;
+    const uint32_t cols = p.cols;
     const T *x = static_cast<const T *>(p.x) + row * p.x_stride;
     const T *residual = p.residual ? static_cast<const T *>(p.residual) + row * p.residual_stride : nullptr;
     T *residual_out = p.residual_out ? static_cast<T *>(p.residual_out) + row * p.residual_out_stride : nullptr;
     const W *weight = static_cast<const W *>(p.weight);
     float sum = 0.f, top = 0.f;
-    for (int i = threadIdx.x; i < p.cols; i += blockDim.x) {
+    for (uint32_t i = threadIdx.x; i < cols; i += blockDim.x) {
         const float h = to_float(x[i]) + (residual ? to_float(residual[i]) : 0.f);
         sum += h * h;
         if (k8) top = max_or_nan(top, h * to_float(weight[i]), 0.f);
@@ -273,7 +274,7 @@ __global__ void rms_norm_rows_kernel(RmsNormParams p) {
     const float r = rsqrtf(sum / p.cols + p.eps);
     const float scale = scale_of(top, r), inverse = 448.f / top;
     if (k8 && threadIdx.x == 0) p.y_scale[row] = scale;
-    for (int i = threadIdx.x; i < p.cols; i += blockDim.x) {
+    for (uint32_t i = threadIdx.x; i < cols; i += blockDim.x) {
         const float h = to_float(x[i]) + (residual ? to_float(residual[i]) : 0.f);
         const float w = to_float(weight[i]);
         if (residual_out) residual_out[i] = from_float<T>(h);

@@ -895,3 +895,11 @@ def test_norm_to_8_bits_of_rows_whose_squares_overflow(ops, dtype, rows, cols):
     assert torch.isnan(scale).tolist() == [i in (0, 2) for i in range(rows)] and bool((codes[[0, 2]].float() == 0).all())
     others = [i for i in range(rows) if i not in (0, 2)]
     check_codes(codes[others], scale[others], norm_ref(x[others], None, w, 1e-6)[1], cols)
+
+
+def test_norm_of_the_longest_row(ops):
+    # (a thread's next place behind the row's end passes 2^31)
+    cols = 2 ** 31 - 1
+    x, y = torch.ones(1, cols, device="cuda", dtype=F16), torch.zeros(1, cols, device="cuda", dtype=F16)
+    ops.rms_norm(x, x[0], eps=0.0, out=y)
+    assert bool((y == 1).all())
