@@ -389,11 +389,15 @@ __device__ __forceinline__ void add_up(const W4Params &p, int sets, int columns,
 }
 
 // What a kernel does with a block's turns: multiply(tile) leaves a warp's sums in registers, leave(to) puts them down.
-template <int kTiles, int kCount, typename Cluster, typename Multiply, typename Leave>
-__device__ __forceinline__ void turns(const W4Params &p, const Share<kTiles> &s, Cluster &cluster, float *sums, Handover &hand, Multiply multiply, Leave leave) {
+// seen(m, v) is told of every output.
+template <int kTiles, int kCount, typename Cluster, typename Multiply, typename Leave, typename Seen>
+__device__ __forceinline__ void turns(const W4Params &p, const Share<kTiles> &s, Cluster &cluster, float *sums, Handover &hand, Multiply multiply, Leave leave, Seen seen) {
     constexpr int kRows = kTiles * kTileRows;
     const auto put = [&](int tile, int place, int row, int m, float v) {
-        if (tile + place < s.to && (tile + place) * kTileRows + row < p.n) store(p, m, (tile + place) * kTileRows + row, v);
+        if (tile + place < s.to && (tile + place) * kTileRows + row < p.n) {
+            seen(m, v);
+            store(p, m, (tile + place) * kTileRows + row, v);
+        }
     };
     if (s.ranks > 1) {
         float *const outputs = sums + kWarps * kRows * kCount;
@@ -456,7 +460,7 @@ template <int kRows, int kCount> constexpr int kSumsOf = (kWarps + 1) * kRows * 
 // instructions are what bounds this beside the memory. Sums of a span are exact in 32 bits:
 //   sum (code - zero) X = sum code X - zero sum X,  |sum code X| <= 128 * 15 * 128,
 // accumulated on 1.5 * 2^23's bits, so that the result is a float without a conversion. Scales of weights and activations are applied to
-// that in fp32. An infinity or NaN makes its row's results NaN.
+// that in fp32. An infinity or NaN makes its row's results NaN; a block that meets one computes its part of the row again (plain_row).
 constexpr int kDigits = 4, kIntegerRows = 2, kTopBit = 29;       // |X| < 2^(kTopBit + 1)
 constexpr uint32_t kIntegerBase = 0x4b400000u;                   // 12582912
 
@@ -561,6 +565,32 @@ __device__ __forceinline__ void make_digits(const W4Params &p, int unit, int m, 
     }
 }
 
+// Row m of the outputs of the block's tiles from the formula, value by value: for activations that have no digits. A warp an output; a lane
+// eight values at a time, those of one word of the codes.
+template <int kTiles> __device__ __noinline__ void plain_row(const W4Params &p, const Share<kTiles> &s, int m) {
+    const int at = s.lane % 16, half = at / 8, quarter = at / 2 % 4, step = at % 2, in_unit = half * 64 + step * 32 + quarter * 8, record = p.wide ? 16 : 8;
+    for (int i = s.from * kTileRows + s.warp; i < min(s.to * kTileRows, p.n); i += kWarps + kSummers) {
+        const int row = i % kTileRows, pair = row % 8, high = row / 8;
+        const uint8_t *tile = p.packed + static_cast<long long>(i / kTileRows) * p.units * p.unit_bytes;
+        float sum = 0.f;
+        for (int u = s.lane / 16; u < p.units; u += 2) {
+            const uint8_t *unit = tile + u * p.unit_bytes, *span = unit + kCodeBytes + (in_unit / (kUnitK / p.spans) * 8 + pair) * record;
+            const uint32_t word = *reinterpret_cast<const uint32_t *>(unit + half * 512 + (pair * 4 + quarter) * 16 + (2 * step + high) * 4);
+            const float scale = p.wide ? reinterpret_cast<const float *>(span)[high] : __half2float(reinterpret_cast<const __half *>(span)[high]);
+            const int zero = span[(p.wide ? 8 : 4) + high];
+            float x[8];
+            load_four(p, m, u * kUnitK + in_unit, *reinterpret_cast<float (*)[4]>(x));
+            load_four(p, m, u * kUnitK + in_unit + 4, *reinterpret_cast<float (*)[4]>(x + 4));
+#pragma unroll
+            for (int v = 0; v < 8; ++v)
+                if (u * kUnitK + in_unit + v < p.k) sum = fmaf(x[v], static_cast<float>(static_cast<int>(word >> (v % 4 * 8 + v / 4 * 4) & 15) - zero) * scale, sum);
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+        if (s.lane == 0) store(p, m, i, sum);
+    }
+}
+
 // All digits into the workspace, a warp 128 values of a row.
 __global__ void w4_digits_kernel(const __grid_constant__ W4Params p) {
     pdl_enter();
@@ -574,9 +604,11 @@ __global__ void __launch_bounds__(kThreads, 1) w4_integer_kernel(const __grid_co
     constexpr int kRows = kTiles * kTileRows;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ Handover hand;
+    __shared__ int again[kIntegerRows];                          // rows that have no digits
     if (threadIdx.x == 0) {
         barrier_init(&hand.full, kWarps);
         barrier_init(&hand.empty, kSummers);
+        again[0] = again[1] = 0;
     }
     auto cluster = cooperative_groups::this_cluster();
     const Share<kTiles> s(p, cluster.num_blocks(), cluster.block_rank());
@@ -665,8 +697,12 @@ __global__ void __launch_bounds__(kThreads, 1) w4_integer_kernel(const __grid_co
                 if (lane % 2 == 0) to[lane % 4 / 2 * kRows + r * kTileRows + lane / 4 + i * 8] = v;
             }
     };
-    turns<kTiles, kIntegerRows>(p, s, cluster, reinterpret_cast<float *>(smem), hand, multiply, leave);
+    turns<kTiles, kIntegerRows>(p, s, cluster, reinterpret_cast<float *>(smem), hand, multiply, leave, [&](int m, float v) { if (!(fabsf(v) <= 3.4028235e38f)) again[m] = 1; });
     copy_wait<0>();
+    __syncthreads();
+#pragma unroll 1
+    for (int m = 0; m < p.rows; ++m)
+        if (again[m]) plain_row<kTiles>(p, s, m);
 }
 
 // The activations at place i of the 16-bit operands, [step of 32 values][row][4 x 16 bytes], from unit `begin` on.
@@ -832,7 +868,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_linear_kernel(const __grid_con
 #pragma unroll
                 for (int i = 0; i < 4; ++i) to[(c * 8 + lane % 4 * 2 + i % 2) * kRows + r * kTileRows + lane / 4 + i / 2 * 8] = acc[r][c][i];
     };
-    turns<kTiles, kColumns * 8>(p, s, cluster, reinterpret_cast<float *>(smem), hand, multiply, leave);
+    turns<kTiles, kColumns * 8>(p, s, cluster, reinterpret_cast<float *>(smem), hand, multiply, leave, [](int, float) {});
     copy_wait<0>();
 }
 

@@ -903,3 +903,30 @@ def test_norm_of_the_longest_row(ops):
     x, y = torch.ones(1, cols, device="cuda", dtype=F16), torch.zeros(1, cols, device="cuda", dtype=F16)
     ops.rms_norm(x, x[0], eps=0.0, out=y)
     assert bool((y == 1).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rows,k,n", [(1, 200, 48), (2, 200, 9500), (1, 200, 19001), (5, 200, 48), (2, 5000, 9500), (13, 200, 9500), (40, 200, 48)])
+@pytest.mark.parametrize("scale_dtype,group", [(F16, 64), (BF16, 32)])
+def test_w4_infinities_are_infinities(ops, dtype, rows, k, n, scale_dtype, group):
+    # in every kernel as in the formula: the infinity's sign times the weight's, NaN for a weight of 0 or infinities of both signs
+    codes, scales, z, w = w4_data(n, k, group, True, scale_dtype)
+    weights = ops.w4_pack(codes, scales, z, k=k, group=group)
+    x = randn(rows, k, seed=117, dtype=dtype)
+    last = rows - 1
+    x[last, 3], x[last, k - 7] = float("inf"), float("-inf")
+    y = ops.w4_linear(x, weights, out_dtype=F32)
+    a, b = w[:, 3].sign(), -w[:, k - 7].sign()
+    none = (a == 0) | (b == 0) | (a != b)
+    assert torch.equal(torch.isnan(y[last]), none) and bool(none.any()) and bool((~none).any())
+    assert torch.equal(y[last][~none].double(), a[~none] * math.inf)
+    check_w4(y[:last], x[:last], w, None, None, k)
+    x[last, k - 7] = 1
+    x[last, 5] = float("inf")
+    x[last, 6] = float("inf")
+    y = ops.w4_linear(x, weights, out_dtype=F32)
+    signs = w[:, [3, 5, 6]].sign()
+    whole = (signs[:, 0] != 0) & (signs == signs[:, :1]).all(1)
+    assert torch.equal(torch.isnan(y[last]), ~whole) and torch.equal(y[last][whole].double(), signs[whole, 0] * math.inf)
+    x[last, 9] = float("nan")
+    assert bool(torch.isnan(ops.w4_linear(x, weights, out_dtype=F32)[last]).all())
