@@ -371,7 +371,7 @@ int  msnh_b200_w4_pack(MsnhB200Ctx *ctx, const MsnhB200W4 *weights, const uint8_
 /* y[row][n] = x_scale[row] * sum_k x[row][k] w[n][k] + bias[n], summed in fp32 and rounded once. At most
  * MSNH_B200_W4_MAX_ROWS rows (a product of more rows is not bound by its weights). One and two rows times many outputs are
  * multiplied in whole numbers: a value of x is taken to 2^-29 of the largest power of two in its row and span of 32, 64 or 128
- * values (a row with an infinity or NaN is not: it follows the formula, as everywhere). */
+ * values, or of 2^-90 where that is more. (A row with an infinity or NaN, or with results below 2^-100, is multiplied value by value.) */
 #define MSNH_B200_W4_MAX_ROWS 64
 typedef struct MsnhB200W4Linear {
     const void *x;

@@ -460,9 +460,12 @@ template <int kRows, int kCount> constexpr int kSumsOf = (kWarps + 1) * kRows * 
 // instructions are what bounds this beside the memory. Sums of a span are exact in 32 bits:
 //   sum (code - zero) X = sum code X - zero sum X,  |sum code X| <= 128 * 15 * 128,
 // accumulated on 1.5 * 2^23's bits, so that the result is a float without a conversion. Scales of weights and activations are applied to
-// that in fp32. An infinity or NaN makes its row's results NaN; a block that meets one computes its part of the row again (plain_row).
-constexpr int kDigits = 4, kIntegerRows = 2, kTopBit = 29;       // |X| < 2^(kTopBit + 1)
+// that in fp32. An infinity or NaN makes its row's results NaN, and values below 2^-119 have no digits; a block that
+// meets either in its outputs computes its part of the row again (plain_row).
+constexpr int kDigits = 4, kIntegerRows = 2, kTopBit = 29, kLeast = -90;         // |X| < 2^(kTopBit + 1); least exponent of a span
 constexpr uint32_t kIntegerBase = 0x4b400000u;                   // 12582912
+// Whether an output tells that its row's activations have digits: it is finite and, unless it is 0, well above the least unit.
+__device__ __forceinline__ bool has_digits(float v) { return v == 0.f || (fabsf(v) >= 7.8886090522101181e-31f && fabsf(v) <= 3.4028235e38f); }       // 2^-100
 
 __device__ __forceinline__ void mma_integer(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -534,12 +537,17 @@ __device__ __forceinline__ void make_digits(const W4Params &p, int unit, int m, 
     for (int o = 1; o < lanes; o *= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
     const unsigned mask = lanes == 32 ? ~0u : (1u << lanes) - 1;
     finite = (__ballot_sync(~0u, finite) >> (lane / lanes * lanes) & mask) == mask;
-    const int exponent = max(-90, static_cast<int>(__float_as_uint(top) >> 23) - 127);
+    // (No unit is below 2^(kLeast - kTopBit), so that it and its products with scales are normal numbers. Values that are less than such a
+    // unit become one of them: not 0, or nothing would show that they are there.)
+    const int exponent = max(kLeast, static_cast<int>(__float_as_uint(top) >> 23) - 127);
     const float up = __uint_as_float(static_cast<uint32_t>(127 + kTopBit - exponent) << 23);
     const uint32_t unit_of = finite ? static_cast<uint32_t>(127 + exponent - kTopBit) << 23 : 0x7fffffffu;
     int x[4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) x[t] = finite ? __float2int_rn(v[t] * up) : 0;
+    for (int t = 0; t < 4; ++t) {
+        x[t] = finite ? __float2int_rn(v[t] * up) : 0;
+        if (exponent == kLeast && x[t] == 0 && v[t] != 0.f) x[t] = v[t] > 0.f ? 1 : -1;
+    }
     const int in_half = lane * 4 % 64;
     uint8_t *const to = digits + (static_cast<size_t>(unit * 2 + lane / 16) * p.rows + m) * (kDigits * 64) + in_half % 32 / 8 * 16 + in_half / 32 * 8 + in_half % 8;
 #pragma unroll
@@ -697,7 +705,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_integer_kernel(const __grid_co
                 if (lane % 2 == 0) to[lane % 4 / 2 * kRows + r * kTileRows + lane / 4 + i * 8] = v;
             }
     };
-    turns<kTiles, kIntegerRows>(p, s, cluster, reinterpret_cast<float *>(smem), hand, multiply, leave, [&](int m, float v) { if (!(fabsf(v) <= 3.4028235e38f)) again[m] = 1; });
+    turns<kTiles, kIntegerRows>(p, s, cluster, reinterpret_cast<float *>(smem), hand, multiply, leave, [&](int m, float v) { if (!has_digits(v)) again[m] = 1; });
     copy_wait<0>();
     __syncthreads();
 #pragma unroll 1

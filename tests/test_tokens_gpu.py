@@ -930,3 +930,20 @@ def test_w4_infinities_are_infinities(ops, dtype, rows, k, n, scale_dtype, group
     assert torch.equal(torch.isnan(y[last]), ~whole) and torch.equal(y[last][whole].double(), signs[whole, 0] * math.inf)
     x[last, 9] = float("nan")
     assert bool(torch.isnan(ops.w4_linear(x, weights, out_dtype=F32)[last]).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [48, 9500])
+@pytest.mark.parametrize("rows", [1, 2, 5])
+@pytest.mark.parametrize("power", [-115, -100, -92, -60, 60, 100])
+def test_w4_of_small_and_large_activations(ops, dtype, n, rows, power):
+    # the same relative error, whatever the activations' exponent and the number of outputs
+    k = 256
+    codes, scales, z, w = w4_data(n, k, 64, True)
+    weights = ops.w4_pack(codes, scales, z, k=k, group=64)
+    x = (randn(rows, k, seed=116) * 2.0 ** power).to(dtype)
+    check_w4(ops.w4_linear(x, weights, out_dtype=F32), x, w, None, None, k)
+    x[:, :64] = 0                                                     # beside spans of zeros, and in one span of ordinary ones
+    x[:, 64:128] = randn(rows, 64, seed=118, dtype=dtype)
+    check_w4(ops.w4_linear(x, weights, out_dtype=F32), x, w, None, None, k)
+    assert bool((ops.w4_linear(torch.zeros_like(x), weights, out_dtype=F32) == 0).all())
