@@ -186,9 +186,11 @@ template <uint32_t kMask> __device__ __forceinline__ uint32_t masked_or(uint32_t
 }
 // The 16-bit operands of a word of codes, less their row's zero point: values 0 and 2, 1 and 3, 4 and 6, 5 and 7. fp16: a half-byte below
 // the exponent of 1024 is 1024 + code, one four bits higher 1024 + 16 code; bf16 has seven bits behind its leading one, so every half-byte
-// is moved to the lowest place: 128 + code. All exact.
+// is moved to the lowest place: 128 + code. All exact. Operands are 1 / kUnit of the codes: bf16 and fp32 activations go up to 2^128, and the
+// sum of a span, up to 15 * 128 of them, must not be infinite where its scale would bring it back.
 template <typename H> struct Zero;
 template <> struct Zero<__half> {
+    static constexpr float kUnit = 1.f;
     static constexpr uint32_t kExponents = 0x64006400u;
     __half2 low, high;
     __device__ __forceinline__ void set(uint32_t z) {
@@ -211,10 +213,11 @@ template <> struct Zero<__half> {
     }
 };
 template <> struct Zero<__nv_bfloat16> {
-    static constexpr uint32_t kExponents = 0x43004300u;
+    static constexpr float kUnit = 2048.f;
+    static constexpr uint32_t kExponents = 0x3d803d80u;
     __nv_bfloat162 low;
     __device__ __forceinline__ void set(uint32_t z) {
-        const uint32_t a = (0xc300u + z) * 0x10001u;                                           // -(128 + zero)
+        const uint32_t a = (0xbd80u + z) * 0x10001u;                                           // -(128 + zero) / kUnit
         memcpy(&low, &a, 4);
     }
     __device__ __forceinline__ void operand(uint32_t w, uint32_t exponents, uint32_t (&out)[4]) const {
@@ -874,7 +877,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_linear_kernel(const __grid_con
 #pragma unroll
             for (int c = 0; c < kColumns; ++c)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) to[(c * 8 + lane % 4 * 2 + i % 2) * kRows + r * kTileRows + lane / 4 + i / 2 * 8] = acc[r][c][i];
+                for (int i = 0; i < 4; ++i) to[(c * 8 + lane % 4 * 2 + i % 2) * kRows + r * kTileRows + lane / 4 + i / 2 * 8] = acc[r][c][i] * Zero<H>::kUnit;
     };
     turns<kTiles, kColumns * 8>(p, s, cluster, reinterpret_cast<float *>(smem), hand, multiply, leave, [](int, float) {});
     copy_wait<0>();
@@ -977,7 +980,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) w4_rows_kernel(const __grid_co
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int m = c * 8 + lane % 4 * 2 + i % 2, row = tile * kTileRows + lane / 4 + i / 2 * 8;
-                    if (m < p.rows && row < p.n) store(p, m, row, acc[c][i]);
+                    if (m < p.rows && row < p.n) store(p, m, row, acc[c][i] * Zero<H>::kUnit);
                 }
     }
     copy_wait<0>();
@@ -988,7 +991,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) w4_rows_kernel(const __grid_co
 #pragma unroll
     for (int c = 0; c < kColumns; ++c)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sums[(s.warp * kCount + c * 8 + lane % 4 * 2 + i % 2) * kTileRows + lane / 4 + i / 2 * 8] = acc[c][i];
+        for (int i = 0; i < 4; ++i) sums[(s.warp * kCount + c * 8 + lane % 4 * 2 + i % 2) * kTileRows + lane / 4 + i / 2 * 8] = acc[c][i] * Zero<H>::kUnit;
     cluster.sync();
     for (int o = s.rank * kThreads + threadIdx.x; o < kWarps * p.rows * (kTileRows / 4); o += s.ranks * kThreads) {
         const int set = o / (p.rows * (kTileRows / 4)), m = o / (kTileRows / 4) % p.rows, quarter = o % (kTileRows / 4);

@@ -947,3 +947,16 @@ def test_w4_of_small_and_large_activations(ops, dtype, n, rows, power):
     x[:, 64:128] = randn(rows, 64, seed=118, dtype=dtype)
     check_w4(ops.w4_linear(x, weights, out_dtype=F32), x, w, None, None, k)
     assert bool((ops.w4_linear(torch.zeros_like(x), weights, out_dtype=F32) == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,k,n", [(1, 256, 48), (1, 256, 9500), (2, 256, 9500), (5, 256, 48), (9, 256, 48), (13, 256, 9500), (20, 256, 100), (40, 256, 48), (64, 1000, 48)])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_w4_of_activations_near_the_largest(ops, dtype, rows, k, n, group):
+    # products with codes pass the largest number, results do not
+    codes, scales, z, w = w4_data(n, k, group, True)
+    x = randn(rows, k, seed=119)
+    x[:, 3:83:10] = (1 + torch.rand(rows, 8, generator=gen(120), device="cuda")) * 2.0 ** 124 * torch.tensor([1, -1, 1, 1, -1, 1, -1, -1], device="cuda")
+    x = x.to(dtype)
+    assert float((x.double().abs() @ w.abs().T).max()) < 3e38 and float(x.double().abs().max()) * 15 > 3.5e38
+    check_w4(ops.w4_linear(x, ops.w4_pack(codes, scales, z, k=k, group=group), out_dtype=F32), x, w, None, None, k)
