@@ -109,9 +109,12 @@ template <typename H> __device__ __forceinline__ uint32_t pack2(float a, float b
 }
 // the three bf16 parts of two fp32 values
 __device__ __forceinline__ void split2(float a, float b, uint32_t &high, uint32_t &middle, uint32_t &low) {
-    high = pack2<__nv_bfloat16>(a, b);
+    // (the largest fp32 values would be rounded to an infinity: their first part is the largest bf16 value)
+    constexpr float kMost = 3.3895313892515355e38f;
+    const bool fa = fabsf(a) <= 3.4028235e38f, fb = fabsf(b) <= 3.4028235e38f;
+    high = pack2<__nv_bfloat16>(fa ? fminf(fmaxf(a, -kMost), kMost) : a, fb ? fminf(fmaxf(b, -kMost), kMost) : b);
     // (what is left of an infinity or NaN is 0: the first part carries it)
-    const float ra = fabsf(a) <= 3.3e38f ? a - __uint_as_float(high << 16) : 0.f, rb = fabsf(b) <= 3.3e38f ? b - __uint_as_float(high & 0xffff0000u) : 0.f;
+    const float ra = fa ? a - __uint_as_float(high << 16) : 0.f, rb = fb ? b - __uint_as_float(high & 0xffff0000u) : 0.f;
     middle = pack2<__nv_bfloat16>(ra, rb);
     low = pack2<__nv_bfloat16>(ra - __uint_as_float(middle << 16), rb - __uint_as_float(middle & 0xffff0000u));
 }

@@ -960,3 +960,13 @@ def test_w4_of_activations_near_the_largest(ops, dtype, rows, k, n, group):
     x = x.to(dtype)
     assert float((x.double().abs() @ w.abs().T).max()) < 3e38 and float(x.double().abs().max()) * 15 > 3.5e38
     check_w4(ops.w4_linear(x, ops.w4_pack(codes, scales, z, k=k, group=group), out_dtype=F32), x, w, None, None, k)
+
+
+@pytest.mark.parametrize("rows,n", [(1, 48), (3, 9500), (6, 48), (20, 48)])
+@pytest.mark.parametrize("value", [3.4028234663852886e38, -3.4e38, 3.39e38, 3.389e38, -3.31e38])
+def test_w4_of_the_largest_activations(ops, rows, n, value):
+    # fp32 values above the largest bf16 one, and just below it, are exact sums of their parts, too
+    codes, scales, z, w = w4_data(n, 160, 32, True)
+    x = randn(rows, 160, seed=121)
+    x[rows - 1, 50] = value
+    check_w4(ops.w4_linear(x, ops.w4_pack(codes, scales, z, k=160, group=32)), x, w, None, None, 160)
