@@ -166,6 +166,9 @@ int  msnh_b200_ctx_create(int device, MsnhB200Ctx **ctx);
 int  msnh_b200_ctx_destroy(MsnhB200Ctx *ctx);
 /* Text of the last failure on this context (valid until the next call on it). Never NULL. */
 const char *msnh_b200_last_error(MsnhB200Ctx *ctx);
+/* For tests of failure handling: leaves `code` where kernels of the context report a bounded wait that ran out. Done by the host; no
+ * kernel is involved. */
+int  msnh_b200_ctx_set_error(MsnhB200Ctx *ctx, int code);
 /* Pinned host memory for inputs/outputs of plan_run (plain malloc'ed buffers work too, slower). */
 int  msnh_b200_host_alloc(MsnhB200Ctx *ctx, size_t bytes, void **ptr);
 int  msnh_b200_host_free(MsnhB200Ctx *ctx, void *ptr);
@@ -385,6 +388,8 @@ typedef struct MsnhB200W4Linear {
     void   *workspace;                 /* w4_linear_workspace bytes, 16-byte aligned; NULL if 0     */
     size_t  workspace_bytes;
 } MsnhB200W4Linear;
+/* Waits inside the kernels are bounded. Should one run out, that call's outputs are not complete, and the next w4_linear of the context
+ * (or the next run of a plan) returns MSNH_B200_ERR_DEVICE_TIMEOUT instead of its own work. */
 int  msnh_b200_w4_linear_workspace(MsnhB200Ctx *ctx, const MsnhB200W4 *weights, const MsnhB200W4Linear *args, size_t *bytes);
 int  msnh_b200_w4_linear(MsnhB200Ctx *ctx, const MsnhB200W4 *weights, const MsnhB200W4Linear *args, void *stream);
 

@@ -27,7 +27,7 @@ struct TView {
 
 // Device error flag codes written by kernels whose bounded waits ran out.
 enum { DEV_ERR_NONE = 0, DEV_ERR_WAIT_FULL = 1, DEV_ERR_WAIT_EMPTY = 2, DEV_ERR_WAIT_ACC_FULL = 3,
-       DEV_ERR_WAIT_ACC_EMPTY = 4, DEV_ERR_TMEM_ALLOC = 5 };
+       DEV_ERR_WAIT_ACC_EMPTY = 4, DEV_ERR_TMEM_ALLOC = 5, DEV_ERR_WAIT_SUMS = 6 };       // (6: 4-bit products)
 
 
 // ---- tensor-core convolution (conv_umma.cuh) --------------------------------------------------------------------------

@@ -70,6 +70,7 @@ int check_device_flag(MsnhB200Ctx *ctx, volatile int *flag) {
     const int code = *flag;
     if (code != 0) {
         *flag = 0;
+        if (code == DEV_ERR_WAIT_SUMS) return fail(ctx, MSNH_B200_ERR_DEVICE_TIMEOUT, "a bounded wait inside an earlier 4-bit product ran out (code %d): its outputs are not complete", code);
         return fail(ctx, MSNH_B200_ERR_DEVICE_TIMEOUT, "a bounded wait inside the conv kernel ran out (code %d)", code);
     }
     return MSNH_B200_OK;
@@ -276,6 +277,12 @@ int msnh_b200_ctx_destroy(MsnhB200Ctx *ctx) {
     if (ctx->err_flag) cudaFreeHost(const_cast<int *>(ctx->err_flag));
     if (ctx->stream) cudaStreamDestroy(ctx->stream);
     delete ctx;
+    return MSNH_B200_OK;
+}
+
+int msnh_b200_ctx_set_error(MsnhB200Ctx *ctx, int code) {
+    if (!ctx || !ctx->err_flag) return MSNH_B200_ERR_ARG;
+    *ctx->err_flag = code;
     return MSNH_B200_OK;
 }
 

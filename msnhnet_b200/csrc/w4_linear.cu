@@ -358,19 +358,23 @@ template <int kTiles, int kAhead> struct Units {
 };
 
 // The way of a turn's sums [warp][column][row] from the warps that multiply to those that add up: `full` counts the former's arrivals,
-// `empty` the latter's. Neither waits for its own kind, so the copies run on meanwhile. The waits have a limit, after which the host learns
-// of it and the block ends.
+// `empty` the latter's. Neither waits for its own kind, so the copies run on meanwhile. The waits have a limit (0.8 s, where the longest
+// turn, of k = 2^27, takes 50 ms), after which the host learns of it and the block ends.
+constexpr long long kWaitCycles = 1500000000LL;
 struct Handover { uint64_t full, empty; };
 __device__ __forceinline__ uint32_t shared_address(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void barrier_init(uint64_t *b, int count) { asm volatile("mbarrier.init.shared.b64 [%0], %1;" ::"r"(shared_address(b)), "r"(count) : "memory"); }
 __device__ __forceinline__ void barrier_arrive(uint64_t *b) { asm volatile("mbarrier.arrive.shared.b64 _, [%0];" ::"r"(shared_address(b)) : "memory"); }
 __device__ __forceinline__ bool barrier_wait(uint64_t *b, int parity, int *error) {
-    for (int i = 0; i < 1 << 20; ++i) {
+    const auto there = [&] {
         uint32_t done;
         asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }" : "=r"(done) : "r"(shared_address(b)), "r"(parity) : "memory");
-        if (done) return true;
-    }
-    report_error(error, 4);
+        return done != 0;
+    };
+    if (there()) return true;
+    for (const long long began = clock64(); clock64() - began <= kWaitCycles;)
+        if (there()) return true;
+    report_error(error, DEV_ERR_WAIT_SUMS);
     return false;
 }
 

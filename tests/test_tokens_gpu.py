@@ -970,3 +970,18 @@ def test_w4_of_the_largest_activations(ops, rows, n, value):
     x = randn(rows, 160, seed=121)
     x[rows - 1, 50] = value
     check_w4(ops.w4_linear(x, ops.w4_pack(codes, scales, z, k=160, group=32)), x, w, None, None, 160)
+
+
+@pytest.mark.parametrize("rows,n", [(1, 48), (2, 9500), (7, 48), (40, 48)])
+def test_w4_reports_a_wait_that_ran_out(rows, n):
+    # the code is left by the host (no kernel waits in vain); the next call says what it was, and the one after it works
+    from msnhnet_b200 import tokens
+    ops = tokens.TokenOps(0)
+    codes, scales, z, w = w4_data(n, 160, 32, True)
+    weights, x = ops.w4_pack(codes, scales, z, k=160, group=32), randn(rows, 160, seed=122)
+    ops.ctx.check(ops.lib.msnh_b200_ctx_set_error(ops.h, 6))
+    with pytest.raises(_ffi.KernelError, match="status 5: a bounded wait inside an earlier 4-bit product"):
+        ops.w4_linear(x, weights)
+    check_w4(ops.w4_linear(x, weights), x, w, None, None, 160)
+    ops.close()
+    assert _ffi.kernel_lib().msnh_b200_ctx_set_error(None, 6) == 1
