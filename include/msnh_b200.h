@@ -432,7 +432,8 @@ int  msnh_b200_attn_decode(MsnhB200Ctx *ctx, const MsnhB200KvCache *cache, const
 
 /* Upkeep of the cache; sequence numbers and counts lie on the device. A sequence is named at most once in a call (fork: as
  * dst; it may be src of several, but not src and dst). `workspace`: kv_workspace bytes, 16-byte aligned.
- *   append : tokens behind each sequence's own: starts (n + 1 offsets into k_new / v_new's rows) or NULL = one token each;
+ *   append : tokens behind each sequence's own: starts (n + 1 offsets into k_new / v_new's rows, in order; all sequences of the call
+ *            are refused where one is below the one before) or NULL = one token each;
  *            the pages that opens are the lowest free ones, in the order of the call
  *   fork   : dst (empty before) becomes a copy of src: full pages are shared, the tokens of a last page that is not full are
  *            copied to the lowest free page

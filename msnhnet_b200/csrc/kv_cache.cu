@@ -82,12 +82,14 @@ struct AppendWork { int first, need, had, start; };              // first of its
 __global__ void kv_append_decide_kernel(KvParams c, const int *seqs, const int *starts, int n, int n_tokens, AppendWork *work, int *list) {
     pdl_enter();
     int all = 0;
+    bool down = false;                                           // starts that are not in order: then no token's sequence is certain
     for (int base = 0; base < n; base += kDecide) {
         const int i = base + threadIdx.x;
         AppendWork w = {0, 0, 0, -1};
         if (i < n) {
             const int s = seqs ? seqs[i] : i;
             const long long from = starts ? starts[i] : i, to = starts ? starts[i + 1] : i + 1;
+            down |= to < from;
             if (s >= 0 && s < c.n_seqs && from >= 0 && to >= from && to <= n_tokens) {
                 const long long len = max(c.lengths[s], 0), had = (len + c.page_size - 1) / c.page_size;
                 const long long want = (len + to - from + c.page_size - 1) / c.page_size;
@@ -100,9 +102,10 @@ __global__ void kv_append_decide_kernel(KvParams c, const int *seqs, const int *
         all += total;
     }
     const int found = lowest_free(c, all, list);
+    if (starts) down = __syncthreads_or(down);
     for (int i = threadIdx.x; i < n; i += kDecide) {
         AppendWork w = work[i];
-        if (w.start >= 0 && w.need > 0 && w.first + w.need > found) work[i].start = w.start = -1;
+        if (w.start >= 0 && (down || (w.need > 0 && w.first + w.need > found))) work[i].start = w.start = -1;
         if (w.start < 0) { atomicAdd(c.refused, 1); continue; }
         const int s = seqs ? seqs[i] : i;
         c.lengths[s] = w.start + (starts ? starts[i + 1] - starts[i] : 1);

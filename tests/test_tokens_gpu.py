@@ -985,3 +985,17 @@ def test_w4_reports_a_wait_that_ran_out(rows, n):
     check_w4(ops.w4_linear(x, weights), x, w, None, None, 160)
     ops.close()
     assert _ffi.kernel_lib().msnh_b200_ctx_set_error(None, 6) == 1
+
+
+@pytest.mark.parametrize("starts", [[0, 5, 3, 8], [0, 2, 4, 3], [4, 0, 4, 8], [8, 6, 3, 0]])
+def test_append_refuses_starts_that_are_not_in_order(ops, starts):
+    # which sequence a token is of is not certain then: no sequence grows by tokens that nobody writes
+    cache, _, _ = make_cache([3, 4, 0, 7], 4, 1, 16, F16, 123, spare=9, width=5)
+    m = Model(cache)
+    k = randn(8, 1, 16, seed=124, dtype=F16)
+    ops.kv_append(cache, k, k, seqs=ints(0, 1, 2), starts=ints(*starts))
+    m.refused = 3
+    m.same(cache)
+    ops.kv_append(cache, k, k, seqs=ints(0, 1, 2), starts=ints(1, 3, 3, 8))          # a gap at the front, none for one
+    m.append([0, 1, 2], [2, 0, 5], k[1:], k[1:])
+    m.same(cache)
