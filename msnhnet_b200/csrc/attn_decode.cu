@@ -181,6 +181,13 @@ template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b
     memcpy(&r, v, 4);
     return r;
 }
+// the same, rounded toward 0
+template <typename T> __device__ __forceinline__ uint32_t pack2_down(float a, float b) {
+    uint32_t r;
+    if constexpr (std::is_same<T, __half>::value) asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    else asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
 template <typename T> __device__ __forceinline__ void unpack2(uint32_t r, float &a, float &b) {
     T v[2];
     memcpy(v, &r, 4);
@@ -196,8 +203,10 @@ template <typename T, int kDim_, int kGroups_, int kStages_, int kBlocks_> struc
     using Type = T;
     static constexpr int kDim = kDim_, kStages = kStages_, kGroups = kGroups_, kWarps = 4, kBlocks = kBlocks_;
     // fp16 weights are taken times 2^14, so that a weight of 2^-29 of the largest is still a normal number (sum and values carry the
-    // same factor); what a weight loses when it is rounded to the cache's type goes into a second product
+    // same factor); what a weight loses when it is rounded to the cache's type goes into a second product. Both parts are above 0 where the
+    // weight is (2^-38 of the largest at least), so that an infinite value stays one: times parts of both signs, or 0, it would be NaN.
     static constexpr float kLift = std::is_same<T, __half>::value ? 14.f : 0.f;
+    static constexpr float kLeast = std::is_same<T, __half>::value ? 5.9604644775390625e-8f : 1.17549435e-38f;      // smallest fp16, smallest normal bf16
     static constexpr int kScratch = 4;
 
     float acc[kGroups][kDim / 16][4], top[kGroups][2], sum[kGroups][2], scale;
@@ -265,11 +274,11 @@ template <typename T, int kDim_, int kGroups_, int kStages_, int kBlocks_> struc
             for (int h = 0; h < 2; ++h) sum[n][h] = sum[n][h] * keep[n][h] + (w[h] + w[h + 2]);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {                        // tokens l / 4 (+ 8): two heads of a token to two tokens of a head
-                const uint32_t pair = pack2<T>(w[2 * t], w[2 * t + 1]);
+                const uint32_t pair = pack2_down<T>(w[2 * t], w[2 * t + 1]);
                 float a, b;
                 unpack2<T>(pair, a, b);
                 high[n][t] = transposed(pair);
-                low[n][t] = transposed(pack2<T>(w[2 * t] - a, w[2 * t + 1] - b));
+                low[n][t] = transposed(pack2<T>(a > 0.f ? fmaxf(w[2 * t] - a, kLeast) : w[2 * t] - a, b > 0.f ? fmaxf(w[2 * t + 1] - b, kLeast) : w[2 * t + 1] - b));
             }
         }
         if (__any_sync(~0u, grown)) {

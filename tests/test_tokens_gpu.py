@@ -999,3 +999,31 @@ def test_append_refuses_starts_that_are_not_in_order(ops, starts):
     ops.kv_append(cache, k, k, seqs=ints(0, 1, 2), starts=ints(1, 3, 3, 8))          # a gap at the front, none for one
     m.append([0, 1, 2], [2, 0, 5], k[1:], k[1:])
     m.same(cache)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("lengths,each", [([40, 100, 70], 1), ([40, 100, 70], 4), ([300, 2000, 5000], 8), ([300, 2000, 5000], 20)])
+def test_attention_of_infinite_keys_and_values(ops, dtype, lengths, each):
+    cache, keys, values = make_cache(lengths, 16, 2, 64, dtype, 125, spare=6)
+    q = randn(3, 2 * each, 64, seed=126, dtype=dtype) * 0.3
+    q[:, :, 9] = 0.5
+    inf = float("inf")
+    # sequence 0: a key of -inf, a score of -inf: a token of weight 0; 1: an infinite value each in two columns, and both signs in a third;
+    # 2: a key of +inf, which no softmax survives
+    def put(pages, i, token, head, column, value):
+        pages[int(cache.page_table[i, token // 16]), token % 16, head, column] = value
+    put(cache.k_pages, 0, 17, 0, 9, -inf)
+    for token, column, value in ((33, 3, inf), (99, 40, -inf), (5, 50, inf), (6, 50, -inf)):
+        put(cache.v_pages, 1, token, 1, column, value)
+    put(cache.k_pages, 2, 20, 1, 9, inf)
+    out, lse = ops.attn_decode(q, cache, return_lse=True)
+    absent = [torch.zeros(n, dtype=torch.bool, device="cuda") for n in lengths]
+    absent[0][17] = True
+    check_attn(out[:1, :each], lse[:1, :each], q[:1, :each], [keys[0][:, :1]], [values[0][:, :1]], 0.125, absent=absent)
+    check_attn(out[:2, :each], lse[:2, :each], q[:2, :each], [k[:, :1] for k in keys], [v[:, :1] for v in values], 0.125, absent=absent)
+    check_attn(out[:1, each:], lse[:1, each:], q[:1, each:], [keys[0][:, 1:]], [values[0][:, 1:]], 0.125)
+    spoilt = out[1, each:]
+    assert bool((spoilt[:, 3] == inf).all()) and bool((spoilt[:, 40] == -inf).all()) and bool(torch.isnan(spoilt[:, 50]).all())
+    others = [c for c in range(64) if c not in (3, 40, 50)]
+    check_attn(spoilt[None, :, others], lse[1:2, each:], q[1:2, each:], [keys[1][:, 1:]], [values[1][:, 1:, others]], 0.125)
+    assert bool(torch.isnan(out[2, each:]).all()) and bool(torch.isfinite(out[2, :each]).all())
