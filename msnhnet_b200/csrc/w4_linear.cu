@@ -1171,14 +1171,20 @@ cudaError_t launch_rows(const MsnhB200Ctx *ctx, W4Params p, void *stream) {
     return launch(ctx, w4_rows_kernel<X, kColumns, kAhead>, done, p, std::min(turns, clusters_at_once(ctx, ranks)), ranks, kWarps * 32, std::max(rings, ranks > 1 ? sums : 0), ctx->pdl, stream);
 }
 
-// Whole numbers for one and two rows of many tiles, two tiles at a time: one fp16, bf16 and fp32 row times 8192 x 28672 take 30.3, 32.2 and
-// 32.2 us (3.9 TB/s), with 16-bit operands 34.1, 41.3 and 56.3; times 4096 x 12288 11.8, 12.5 and 12.3 against 12.1, 13.5 and 17.3. With
-// fewer tiles their preparation is the longer one: times 4096 x 4096 7.5 us against 6.2, 6.5 and 7.9.
+// Whole numbers for one and two rows of many tiles, two tiles at a time, where their longer preparation is worth it: from four tiles an SM
+// on, from five for two rows of 16 and 8 bits. us in whole numbers / with 16-bit operands:
+//                    1 row fp16     bf16         fp32         2 rows fp16   bf16         fp32
+//     2048 x 9600    7.5 / 7.8      7.5 / 7.8    7.5 / 9.2    10.0 / 7.9    9.9 / 7.9    9.9 / 9.3
+//     4096 x 9600    11.3 / 10.7    11.3 / 10.9  11.3 / 14.0  11.9 / 10.8   11.9 / 11.0  11.9 / 14.5
+//     4096 x 12288   11.6 / 12.1    11.6 / 12.3  11.7 / 15.9  12.3 / 12.2   12.3 / 12.4  12.2 / 16.4
+//     4096 x 20000   14.5 / 15.9    14.5 / 16.2  14.5 / 21.5  15.7 / 16.0   15.7 / 16.4  15.7 / 21.9
+//     8192 x 28672   28.1 / 34.1    28.3 / 35.0  28.2 / 49.8  28.9 / 34.4   29.0 / 35.2  29.0 / 53.8
+// (times 4096 x 4096 one row took 7.5 us in whole numbers, 6.2 with operands.)
 // Nine to sixteen rows keep their activations in shared memory where tiles are few, so that all warps of a block can share k (nine fp16 rows
 // times 4096 x 4096 10.1 us against 14.1; sixteen times 4096 x 12288 and 8192 x 28672 29.8 and 105 us against 22.7 and 68).
 template <typename X>
 cudaError_t launch(const MsnhB200Ctx *ctx, const W4Params &p, void *stream) {
-    if (p.rows <= kIntegerRows && p.tiles >= 4 * ctx->sm_count) {
+    if (p.rows <= kIntegerRows && p.tiles >= (p.rows == 1 || std::is_same<X, float>::value ? 4 : 5) * ctx->sm_count) {
         cudaError_t e = cudaSuccess;
         W4Params digits = p;
         if (!digits_apart(p.rows, p.units)) digits.digits_made = nullptr;
