@@ -1074,22 +1074,30 @@ int clusters_at_once(const MsnhB200Ctx *ctx, int ranks) {
     return n;
 }
 
-// How many warps of a block share a tile's k: what takes the fewest units one after the other in the busiest warp (tiles at a time x units
-// of each), the more the better at the same count. Where that leaves SMs without a block, a cluster shares it further, down to two units
+// How many warps of a block share a tile's k, `tiles` at a time: what takes the fewest units one after the other in the busiest warp (turns x
+// units of each), the more the better at the same count; and the turns of that block.
+struct Split { int warps, turns; };
+Split split_of(const MsnhB200Ctx *ctx, const W4Params &p, int tiles) {
+    const auto up = [](int a, int b) { return (a + b - 1) / b; };
+    const auto turns = [&](int split) {
+        const int per_turn = kWarps / split * tiles;
+        return up(up(p.tiles, std::min(up(p.tiles, per_turn), ctx->sm_count)), per_turn);
+    };
+    const auto cost = [&](int split) { return static_cast<long long>(turns(split)) * up(p.units, split); };
+    int best = 1;
+    for (int split = 2; split <= kWarps && split <= p.units; split *= 2)
+        if (cost(split) <= cost(best)) best = split;
+    return {best, turns(best)};
+}
+
+// How a launch is cut up: warps as above. Where that leaves SMs without a block, a cluster shares it further, down to two units
 // of k a warp; and where that is what makes room for the activations (x_bytes: of those of some units). (A cluster has room for the outputs of one
 // set of warps.) Returns whether there is room.
 template <typename Bytes>
 bool share_out(const MsnhB200Ctx *ctx, W4Params &p, int tiles, Bytes x_bytes, int &ranks, int &blocks) {
-    const auto per_turn = [&](int split) { return kWarps / split * tiles; };
     const auto up = [](int a, int b) { return (a + b - 1) / b; };
-    const auto cost = [&](int split) {
-        const int most = up(p.tiles, std::min(up(p.tiles, per_turn(split)), ctx->sm_count));
-        return static_cast<long long>(up(most, per_turn(split))) * up(p.units, split);
-    };
-    p.split = 1;
-    for (int split = 2; split <= kWarps && split <= p.units; split *= 2)
-        if (cost(split) <= cost(p.split)) p.split = split;
-    const int turns = up(p.tiles, per_turn(p.split));
+    p.split = split_of(ctx, p, tiles).warps;
+    const int turns = up(p.tiles, kWarps / p.split * tiles);
     const auto units = [&] { return std::min(p.units, p.split * up(p.units, p.split * ranks)); };
     ranks = 1;
     while (p.split == kWarps && ranks < kMostRanks && turns <= clusters_at_once(ctx, ranks * 2) && p.split * ranks * 4 <= p.units) ranks *= 2;
@@ -1104,7 +1112,8 @@ bool share_out(const MsnhB200Ctx *ctx, W4Params &p, int tiles, Bytes x_bytes, in
 }
 
 // Digits are made by every block for itself, or, where that is over kOwnDigits turns of its warps (1 us each), by a launch before it: one and
-// two rows times 8192 x 28672 30.3 and 30.5 us, by every block 33.0 and 38.2; times 2048 x 40000, which is below, 15.6 against 17.2 apart.
+// two rows times 8192 x 28672 28.2 and 29.1 us, by every block 31.3 and 37.0; times 2048 x 40000, which is below, 14.8 and 19.3 against 16.0
+// and 19.1 apart.
 constexpr int kOwnDigits = 2;
 size_t digit_bytes(int rows, int units) { return static_cast<size_t>(units) * 2 * rows * kDigits * 64; }
 size_t meta_bytes(int rows, int units, int spans) { return static_cast<size_t>(units) * spans * rows * kDigits * 8; }
@@ -1171,20 +1180,30 @@ cudaError_t launch_rows(const MsnhB200Ctx *ctx, W4Params p, void *stream) {
     return launch(ctx, w4_rows_kernel<X, kColumns, kAhead>, done, p, std::min(turns, clusters_at_once(ctx, ranks)), ranks, kWarps * 32, std::max(rings, ranks > 1 ? sums : 0), ctx->pdl, stream);
 }
 
-// Whole numbers for one and two rows of many tiles, two tiles at a time, where their longer preparation is worth it: from four tiles an SM
-// on, from five for two rows of 16 and 8 bits. us in whole numbers / with 16-bit operands:
-//                    1 row fp16     bf16         fp32         2 rows fp16   bf16         fp32
-//     2048 x 9600    7.5 / 7.8      7.5 / 7.8    7.5 / 9.2    10.0 / 7.9    9.9 / 7.9    9.9 / 9.3
-//     4096 x 9600    11.3 / 10.7    11.3 / 10.9  11.3 / 14.0  11.9 / 10.8   11.9 / 11.0  11.9 / 14.5
-//     4096 x 12288   11.6 / 12.1    11.6 / 12.3  11.7 / 15.9  12.3 / 12.2   12.3 / 12.4  12.2 / 16.4
-//     4096 x 20000   14.5 / 15.9    14.5 / 16.2  14.5 / 21.5  15.7 / 16.0   15.7 / 16.4  15.7 / 21.9
-//     8192 x 28672   28.1 / 34.1    28.3 / 35.0  28.2 / 49.8  28.9 / 34.4   29.0 / 35.2  29.0 / 53.8
-// (times 4096 x 4096 one row took 7.5 us in whole numbers, 6.2 with operands.)
+// Whole numbers for one and two rows of many tiles, two tiles at a time, where their longer preparation is worth it: for 16- and 8-bit
+// activations one row from 4 tiles an SM and k of 2048 on, two rows from 5 and 4096, and from 4 where a block is through in one turn with
+// them and not without; for fp32 ones, which are three operands otherwise, from 4 tiles on whatever k. us in whole numbers / with 16-bit operands (8-bit and bf16 activations as fp16 within 3 %):
+//                    1 row fp16     fp32           2 rows fp16    fp32
+//     512 x 12288    4.7 / 4.9      4.7 / 5.6      5.3 / 5.8      5.2 / 6.5       (one turn against two)
+//     512 x 40000    9.5 / 8.9      9.5 / 9.9      12.8 / 11.2    12.7 / 12.3     (three against five)
+//     768 x 16000    5.6 / 4.9                     6.1 / 5.2                      (one of either)
+//     1024 x 9600    6.5 / 5.6      6.4 / 6.5      7.8 / 6.2      7.8 / 7.0
+//     1024 x 40000   11.6 / 12.0    11.6 / 14.1    14.5 / 14.3    14.6 / 16.0
+//     2048 x 9600    7.5 / 7.8      7.5 / 9.2      10.0 / 7.9     9.9 / 9.3
+//     2048 x 20000   10.2 / 12.1    10.2 / 14.0    13.3 / 12.2    13.3 / 14.3
+//     2048 x 40000   14.8 / 19.8    14.8 / 22.7    19.3 / 20.1    19.2 / 23.0
+//     4096 x 9600    11.3 / 10.7    11.3 / 14.0    11.9 / 10.8    11.9 / 14.5
+//     4096 x 12288   11.6 / 12.1    11.7 / 15.9    12.3 / 12.2    12.2 / 16.4
+//     4096 x 20000   14.5 / 15.9    14.5 / 21.5    15.7 / 16.0    15.7 / 21.9
+//     8192 x 28672   28.1 / 34.1    28.2 / 49.8    28.9 / 34.4    29.0 / 53.8
+// (times 4096 x 4096 one fp16 row took 7.5 in whole numbers, 6.2 with operands.)
 // Nine to sixteen rows keep their activations in shared memory where tiles are few, so that all warps of a block can share k (nine fp16 rows
 // times 4096 x 4096 10.1 us against 14.1; sixteen times 4096 x 12288 and 8192 x 28672 29.8 and 105 us against 22.7 and 68).
 template <typename X>
 cudaError_t launch(const MsnhB200Ctx *ctx, const W4Params &p, void *stream) {
-    if (p.rows <= kIntegerRows && p.tiles >= (p.rows == 1 || std::is_same<X, float>::value ? 4 : 5) * ctx->sm_count) {
+    if (p.rows <= kIntegerRows && p.tiles >= 4 * ctx->sm_count &&
+        (std::is_same<X, float>::value || (p.tiles >= (3 + p.rows) * ctx->sm_count && p.units >= 16 * p.rows) ||
+         (split_of(ctx, p, 2).turns == 1 && split_of(ctx, p, 1).turns > 1))) {
         cudaError_t e = cudaSuccess;
         W4Params digits = p;
         if (!digits_apart(p.rows, p.units)) digits.digits_made = nullptr;

@@ -906,7 +906,7 @@ def test_norm_of_the_longest_row(ops):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
-@pytest.mark.parametrize("rows,k,n", [(1, 200, 48), (2, 200, 9500), (1, 200, 19001), (5, 200, 48), (2, 5000, 9500), (2, 200, 12001), (2, 5000, 19001), (13, 200, 9500), (40, 200, 48)])
+@pytest.mark.parametrize("rows,k,n", [(1, 200, 48), (2, 200, 9500), (1, 200, 19001), (5, 200, 48), (2, 5000, 9500), (2, 200, 12001), (1, 2100, 9500), (2, 4200, 12001), (2, 5000, 19001), (13, 200, 9500), (40, 200, 48)])
 @pytest.mark.parametrize("scale_dtype,group", [(F16, 64), (BF16, 32)])
 def test_w4_infinities_are_infinities(ops, dtype, rows, k, n, scale_dtype, group):
     # in every kernel as in the formula: the infinity's sign times the weight's, NaN for a weight of 0 or infinities of both signs
@@ -933,12 +933,10 @@ def test_w4_infinities_are_infinities(ops, dtype, rows, k, n, scale_dtype, group
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("n", [48, 9500, 12001])
-@pytest.mark.parametrize("rows", [1, 2, 5])
+@pytest.mark.parametrize("rows,k,n", [(1, 256, 48), (1, 256, 9500), (2, 256, 48), (2, 256, 9500), (5, 256, 48), (5, 256, 9500), (1, 2048, 9500), (2, 4096, 12001)])
 @pytest.mark.parametrize("power", [-115, -100, -92, -60, 60, 100])
-def test_w4_of_small_and_large_activations(ops, dtype, n, rows, power):
+def test_w4_of_small_and_large_activations(ops, dtype, rows, k, n, power):
     # the same relative error, whatever the activations' exponent and the number of outputs
-    k = 256
     codes, scales, z, w = w4_data(n, k, 64, True)
     weights = ops.w4_pack(codes, scales, z, k=k, group=64)
     x = (randn(rows, k, seed=116) * 2.0 ** power).to(dtype)
@@ -950,7 +948,7 @@ def test_w4_of_small_and_large_activations(ops, dtype, n, rows, power):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("rows,k,n", [(1, 256, 48), (1, 256, 9500), (2, 256, 9500), (2, 256, 12001), (5, 256, 48), (9, 256, 48), (13, 256, 9500), (20, 256, 100), (40, 256, 48), (64, 1000, 48)])
+@pytest.mark.parametrize("rows,k,n", [(1, 256, 48), (1, 256, 9500), (2, 256, 9500), (1, 2048, 9500), (2, 4096, 12001), (5, 256, 48), (9, 256, 48), (13, 256, 9500), (20, 256, 100), (40, 256, 48), (64, 1000, 48)])
 @pytest.mark.parametrize("group", [32, 64, 128])
 def test_w4_of_activations_near_the_largest(ops, dtype, rows, k, n, group):
     # products with codes pass the largest number, results do not
@@ -1031,9 +1029,9 @@ def test_attention_of_infinite_keys_and_values(ops, dtype, lengths, each):
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16, E4M3])
 @pytest.mark.parametrize("n", [9457, 9472, 9488, 11825, 11840, 11856, 12288])
-@pytest.mark.parametrize("rows,k", [(1, 2048), (2, 2048), (2, 300)])
+@pytest.mark.parametrize("rows,k", [(1, 2048), (1, 1920), (2, 2048), (2, 300), (2, 3968), (2, 4096)])
 def test_w4_of_as_many_outputs_as_change_the_kernel(ops, dtype, n, rows, k):
-    # four and five 16-row tiles for each of 148 SMs, and one tile more and less
+    # four and five 16-row tiles for each of 148 SMs, and one tile more and less; 15 and 16, 31 and 32 pieces of k
     codes, scales, z, w = w4_data(n, k, 128, True)
     x, x_scale = w4_x(rows, k, dtype, 127)
     check_w4(ops.w4_linear(x, ops.w4_pack(codes, scales, z, k=k, group=128), x_scale=x_scale, out_dtype=F32), x, w, x_scale, None, k)
