@@ -25,11 +25,14 @@ namespace {
 
 constexpr int kTile = 16;                    // tokens of a tile
 constexpr int kMaxRows = 256;                // rows of a launch: what they see is kept in shared memory
-// Tiles that a pair's start counts for, and tiles of a share, where there are as many. (16 rows of 500 fp16 tokens with kStart 1, 3, 6: 29.4,
-// 29.7 and 32.4 us; 48 sequences of up to 8192 bf16 tokens with 0 and 3: 64 and 50.6.)
+// Tiles that a pair's start counts for, and tiles of a share, where there are as many. fp16, 32 heads over 8, with kStart 1, 3 and 6: one row
+// of 500 tokens 9.7, 10.8 and 13.1 us, 16 of them 17.2, 16.5 and 18.0, one of 65536 beside 63 of 100 76.7, 75.2 and 75.7, one of 4000 14.2,
+// 14.8 and 16.1; 16 of 4000 and more tokens are the same within 1 %.
 constexpr int kStart = 3, kLeast = 2;
-// Sequences of at most so many tiles are not cut, which saves the join (one of 37 and 120 fp16 tokens: 6.6 and 10.3 us, cut 12.0 and 13.1);
-// with 32 tiles to a warp one of 500 tokens takes 28.0 us, cut 10.9.
+// Where the table's rows (or the window) hold at most so many tiles no sequence is cut, which saves the join: tables of 128 tokens with one
+// row of 37 or 120 tokens 6.6 and 10.3 us, 64 of 120 14.0 (with kWholeTiles 2: 9.1, 10.1, 17.2). With 32, tables of 512 tokens: one, 16, 64
+// and 128 rows of 500 tokens 28.1, 29.8, 36.7 and 50.6 us, cut 10.8, 16.5, 34.2 and 59.5: many pairs would do without the cuts. Lengths are
+// not known on the host: in tables of 4096 tokens one row of 37, 120 and 500 tokens takes 12.1, 13.2 and 13.7 us.
 constexpr int kWholeTiles = 8;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -764,10 +767,12 @@ cudaError_t launch32(const MsnhB200Ctx *ctx, const AttnParams &p, int blocks, vo
     return launch<PlainHeads<256, kHeads, 3, 2>>(ctx, p, blocks, stream);
 }
 
-// A pair has at most as many parts as there are shares of its tiles, or as it has warps to itself. Parts that few warps take turns at cost
-// more than starting 32 warps does from kManyParts on: with 74 and 148 parts a pair 80 against 72 us (2 rows of 60000 fp16 tokens) and 47
-// against 35 (one of 30000), with 51 as much either way (one of 4000: 15.5 and 14.7), with 9 and 7 the other way round (16 rows of 4000:
-// 43 against 59; one of 500: 10.9 against 13.5).
+// The parts of a pair in a full table: as many as there are shares of its tiles, or as it has warps to itself. Parts that few warps take turns
+// at cost more than starting 32 warps does from kManyParts on: with 74 and 148 parts a pair 101 against 97 us (2 rows of 60000 fp16 tokens)
+// and 47.5 against 34.8 (one of 30000), with 51 as much either way (one of 4000: 15.6 and 14.8), with 9 and 7 the other way round (16 rows
+// of 4000: 56 against 72; one of 500: 10.9 against 13.6). It is an estimate, since the host does not know the lengths. A pair can have more
+// parts: beside 63 rows of 100 tokens one of 65536 has some 147, which few warps join in no more time (75 against 92 us); and fewer: of one
+// row of 37 or 500 tokens in a table of 4096 few warps would be through in 9.4 and 10.9 us instead of 12.1 and 13.7.
 constexpr int kManyParts = 32;
 template <typename T>
 cudaError_t launch_join(const MsnhB200Ctx *ctx, const AttnParams &p, int workers, long long tiles, void *stream) {

@@ -1035,3 +1035,45 @@ def test_w4_of_as_many_outputs_as_change_the_kernel(ops, dtype, n, rows, k):
     codes, scales, z, w = w4_data(n, k, 128, True)
     x, x_scale = w4_x(rows, k, dtype, 127)
     check_w4(ops.w4_linear(x, ops.w4_pack(codes, scales, z, k=k, group=128), x_scale=x_scale, out_dtype=F32), x, w, x_scale, None, k)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16, E4M3])
+@pytest.mark.parametrize("rows,k,n,group", [(9, 515, 9500, 128), (13, 300, 19001, 64), (16, 420, 9500, 32), (12, 2100, 12000, 128)])
+def test_w4_of_nine_to_sixteen_rows_of_many_outputs(ops, dtype, rows, k, n, group):
+    codes, scales, z, w = w4_data(n, k, group, True)
+    x, x_scale = w4_x(rows, k, dtype, 128)
+    b = randn(n, seed=129) * 0.1
+    check_w4(ops.w4_linear(x, ops.w4_pack(codes, scales, z, k=k, group=group), bias=b, x_scale=x_scale), x, w, x_scale, b, k)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("cols", [64, 250, 512, 2048, 2056, 4104, 5120, 8200, 12288, 16384])
+def test_norm_of_many_rows_to_8_bits_with_a_residual(ops, dtype, cols):
+    # blocks that stay and copy rows ahead, x's and the residual's; beside the residual and in its place
+    rows = 1300 if cols > 1024 else 5000
+    x, r, w = randn(rows, cols, seed=130, dtype=dtype), randn(rows, cols, seed=131, dtype=dtype) * 2, randn(cols, seed=132, dtype=dtype)
+    want_h, want = norm_ref(x, r, w, 1e-6)
+    codes, scale, h = ops.rms_norm(x, w, residual=r, out_dtype=E4M3)
+    check_codes(codes, scale, want, cols)
+    assert torch.equal(h, (x.float() + r.float()).to(dtype))
+    r2 = r.clone()
+    again, scale2, _ = ops.rms_norm(x, w, residual=r2, residual_out=r2, out_dtype=E4M3)
+    assert torch.equal(again.view(torch.uint8), codes.view(torch.uint8)) and torch.equal(scale2, scale) and torch.equal(r2, h)
+    x2 = x.clone()
+    again, scale2, _ = ops.rms_norm(x2, w, residual=r, residual_out=x2, out_dtype=E4M3)
+    assert torch.equal(again.view(torch.uint8), codes.view(torch.uint8)) and torch.equal(scale2, scale) and torch.equal(x2, h)
+    x2, r2 = x.clone(), r.clone()
+    y, _ = ops.rms_norm(x, w, residual=r)
+    ops.rms_norm(x2, w, residual=r2, residual_out=r2, out=x2)
+    assert torch.equal(x2, y) and torch.equal(r2, h)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("lengths", [[1], [37], [500], [0, 5, 500, 17], [3000] + [20] * 30])
+@pytest.mark.parametrize("width", [256, 4096])
+def test_attention_in_a_table_with_room(ops, dtype, lengths, width):
+    # whether a pair is cut, and how its parts are joined, is decided by what the table could hold
+    cache, keys, values = make_cache(lengths, 16, 2, 64, dtype, 133, width=width)
+    q = randn(len(lengths), 8, 64, seed=134, dtype=dtype)
+    out, lse = ops.attn_decode(q, cache, return_lse=True)
+    check_attn(out, lse, q, keys, values, 0.125)
