@@ -2,9 +2,8 @@
 //
 // y = x_scale * sum over groups of scale * sum_k x (code - zero), + bias. The packed weights are read once; with few rows their bytes bound
 // it, and right behind them the instructions that make operands of codes, with 64 rows the products. Three kernels, chosen at the end of
-// this file by rows and tiles with what either side measured. One fp16 token times 8192 x 28672 (122 MB): 31 us, 3.9 TB/s; times
-// 4096 x 4096 5.9 us; seven 8-bit rows times 5120 x 13824 19 us (2.05 TB/s); 64 fp16 rows
-// times 8192 x 8192 43.5 us.
+// this file by rows, tiles and k with what either side measured. One fp16 token times 8192 x 28672 (122 MB): 28.4 us, 4.3 TB/s; times
+// 4096 x 4096 5.9 us; seven 8-bit rows times 5120 x 13824 19 us (2.05 TB/s); 64 fp16 rows times 8192 x 8192 43.5 us.
 #include <cooperative_groups.h>
 #include "token_ops.h"
 #include "token_types.cuh"
