@@ -306,13 +306,12 @@ cudaError_t launch_vectors(const MsnhB200Ctx *ctx, const RmsNormParams &p, int v
     return launch_token_kernel(kernel, dim3(static_cast<unsigned>(blocks)), threads, smem, stream, ctx->pdl, p);
 }
 
-// A block a row, a vector a thread as far as that goes, so that a row's bytes are all asked for at once, except for many rows (600 of them
-// take as long either way):
+// A block a row, a vector a thread as far as that goes, so that a row's bytes are all asked for at once, except for many rows:
 // - rows of up to 64 vectors: a warp a row, which needs no barrier (4100 fp16 rows of 256 and 512 values: 3.0 and 4.2 us against 4.7 and
 //   4.8; at 128 vectors it loses, 8.3 against 7.4);
 // - long rows to 8 bits, which leave a block more to compute than to write: blocks that stay and copy ahead (4100 bf16 rows of 5120 and
-//   8192 values: 28.3 and 42.9 us, 5.1 TB/s, against 31.5 and 51.9; at 2048 values 14.5 against 13.2, and rows of x's own type lose at all
-//   lengths: 4100 fp32 rows of 5120 values 58 against 52 us, 4.9 TB/s).
+//   8192 values: 28.5 and 43.4 us, 5.1 TB/s, against 31.0 and 50.9; 600 of them 7.3 and 9.9 against 6.8 and 10.2; at 2048 values 4100 rows
+//   lose, 14.4 against 12.9, and rows of x's own type at all lengths: 4100 fp32 rows of 5120 values 58 against 52 us, 4.9 TB/s).
 template <typename T, typename W, bool k8>
 cudaError_t launch(const MsnhB200Ctx *ctx, const RmsNormParams &p, bool aligned, void *stream) {
     const int vectors = p.cols / Vec16<T>::kVec;
