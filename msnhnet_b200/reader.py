@@ -126,6 +126,7 @@ class Reader:
     def fork(self, src, dst):
         for cache in self.caches:
             self.ops.kv_fork(cache, src, dst)
+        self.most = [max(self.most)] * self.n_seqs                    # (which of them are copies, and of which, is known to the GPU only)
 
     def forget(self, seqs):
         for cache in self.caches:

@@ -64,3 +64,17 @@ def test_step_refuses_too_many_rows():
         r.step(torch.zeros(65, dtype=torch.long), torch.arange(65, dtype=torch.int32))
     with pytest.raises(ValueError, match="sequences"):
         r.step(torch.zeros(2, dtype=torch.long), torch.arange(3, dtype=torch.int32))
+
+
+def test_a_fork_may_be_as_long_as_the_longest():
+    class Forks(NoOps):
+        def kv_fork(self, cache, src, dst):
+            pass
+
+    r = Reader(Forks(), channels=64, width=64, layers=2, heads=2, kv_heads=1, head_dim=32, ffn=64, vocab=10, n_seqs=3, max_tokens=64)
+    r.most = [60, 0, 3]
+    r.fork(torch.tensor([0], dtype=torch.int32), torch.tensor([1], dtype=torch.int32))
+    for cache in r.caches:
+        cache.lengths[:] = torch.tensor([0, 60, 3], dtype=torch.int32)                # (the first one has been forgotten since)
+    with pytest.raises(ValueError, match="more tokens"):
+        r.look(torch.zeros(10, 64), 1)
