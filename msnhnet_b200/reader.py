@@ -106,7 +106,7 @@ class Reader:
     def step(self, ids, seqs):
         """One token (ids: int64 [n], at most 64) behind each of the sequences seqs (int32 [n]); the logits of what follows. A row whose
         token or sequence is none leaves every sequence as it was; its logits are NaN."""
-        return self._step(ids, seqs)
+        return self._step(torch.as_tensor(ids, device=self.position.device), seqs)
 
     def _step(self, ids, seqs, named=None):
         if len(ids) != len(seqs) or len(ids) > self.MAX_ROWS:

@@ -150,3 +150,13 @@ def test_reader_leaves_out_rows_of_no_sequence_and_no_token(ops):
     assert torch.isnan(logits).all(-1).tolist() == [False, True, True, True, True] and bool(torch.isfinite(logits[0]).all())
     assert [c.lengths.tolist() for c in reader.caches] == [[21, 20, 20]] * 2
     assert [c.refused() for c in reader.caches] == [4, 4]
+
+
+def test_reader_takes_tokens_from_the_host(ops):
+    from msnhnet_b200.reader import Reader
+    reader = Reader(ops, n_seqs=3)
+    features = torch.randn(20, 512, generator=torch.Generator(device="cuda").manual_seed(7), device="cuda")
+    for seq in range(3):
+        reader.look(features, seq)
+    want = reader.step(torch.tensor([5], device="cuda"), ints(0))
+    assert torch.equal(reader.step(torch.tensor([5]), ints(1)), want) and torch.equal(reader.step([5], ints(2)), want)
