@@ -1077,3 +1077,19 @@ def test_attention_in_a_table_with_room(ops, dtype, lengths, width):
     q = randn(len(lengths), 8, 64, seed=134, dtype=dtype)
     out, lse = ops.attn_decode(q, cache, return_lse=True)
     check_attn(out, lse, q, keys, values, 0.125)
+
+
+@pytest.mark.parametrize("rows,k,n,dtype,group", [(1, 20000, 9600, F16, 128), (2, 33000, 11900, F16, 128), (2, 20000, 11850, BF16, 32), (1, 2050, 9600, E4M3, 64), (2, 4100, 19001, F16, 32)])
+def test_w4_of_long_rows_in_whole_numbers(ops, rows, k, n, dtype, group):
+    # 16- and 8-bit activations that are multiplied so: digits made apart, by clusters' blocks, by every block
+    codes, scales, z, w = w4_data(n, k, group, True)
+    weights = ops.w4_pack(codes, scales, z, k=k, group=group)
+    x, x_scale = w4_x(rows, k, dtype, 135)
+    y = ops.w4_linear(x, weights, x_scale=x_scale, out_dtype=F32)
+    check_w4(y, x, w, x_scale, None, k)
+    assert torch.equal(y, ops.w4_linear(x, weights, x_scale=x_scale, out_dtype=F32))
+    if dtype != E4M3:
+        x[rows - 1, k // 2] = float("nan")
+        y = ops.w4_linear(x, weights, out_dtype=F32)
+        assert bool(torch.isnan(y[rows - 1]).all())
+        check_w4(y[:rows - 1], x[:rows - 1], w, None, None, k)
