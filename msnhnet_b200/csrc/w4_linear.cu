@@ -469,8 +469,8 @@ template <int kRows, int kCount> constexpr int kSumsOf = (kWarps + 1) * kRows * 
 // instructions are what bounds this beside the memory. Sums of a span are exact in 32 bits:
 //   sum (code - zero) X = sum code X - zero sum X,  |sum code X| <= 128 * 15 * 128,
 // accumulated on 1.5 * 2^23's bits, so that the result is a float without a conversion. Scales of weights and activations are applied to
-// that in fp32. An infinity or NaN makes its row's results NaN, and values below 2^-119 have no digits; a block that
-// meets either in its outputs computes its part of the row again (plain_row).
+// that in fp32. An infinity or NaN makes its row's results NaN, and values below 2^-119 have no digits; a block that meets either in its
+// outputs computes its part of the row again (plain_row).
 constexpr int kDigits = 4, kIntegerRows = 2, kTopBit = 29, kLeast = -90;         // |X| < 2^(kTopBit + 1); least exponent of a span
 constexpr uint32_t kIntegerBase = 0x4b400000u;                   // 12582912
 // Whether an output tells that its row's activations have digits: it is finite and, unless it is 0, well above the least unit.
@@ -1182,7 +1182,8 @@ cudaError_t launch_rows(const MsnhB200Ctx *ctx, W4Params p, void *stream) {
 
 // Whole numbers for one and two rows of many tiles, two tiles at a time, where their longer preparation is worth it: for 16- and 8-bit
 // activations one row from 4 tiles an SM and k of 2048 on, two rows from 5 and 4096, and from 4 where a block is through in one turn with
-// them and not without; for fp32 ones, which are three operands otherwise, from 4 tiles on whatever k. us in whole numbers / with 16-bit operands (8-bit and bf16 activations as fp16 within 3 %):
+// them and not without; for fp32 ones, which are three operands otherwise, from 4 tiles on whatever k. us in whole numbers / with 16-bit
+// operands (8-bit and bf16 activations as fp16 within 3 %):
 //                    1 row fp16     fp32           2 rows fp16    fp32
 //     512 x 12288    4.7 / 4.9      4.7 / 5.6      5.3 / 5.8      5.2 / 6.5       (one turn against two)
 //     512 x 40000    9.5 / 8.9      9.5 / 9.9      12.8 / 11.2    12.7 / 12.3     (three against five)

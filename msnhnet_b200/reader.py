@@ -124,6 +124,7 @@ class Reader:
         return torch.where(there[:, None], logits, float("nan"))
 
     def fork(self, src, dst):
+        """Sequences dst become copies of sequences src. One that is not empty stays as it is, and every cache counts it as refused."""
         for cache in self.caches:
             self.ops.kv_fork(cache, src, dst)
         self.most = [max(self.most)] * self.n_seqs                    # (which of them are copies, and of which, is known to the GPU only)
