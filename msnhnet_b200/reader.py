@@ -92,11 +92,20 @@ class Reader:
         for i in known:
             self.most[i] += n
 
+    def _empty(self, named):
+        """ValueError where one of the sequences has tokens."""
+        if any(self.most[i] for i in named):
+            self.most = self.caches[0].lengths.tolist()              # (waits for the GPU)
+            full = [i for i in named if self.most[i]]
+            if full:
+                raise ValueError(f"sequences {full} are not empty: no more tokens can be their first ones")
+
     def look(self, features, seq):
         """features [cells, channels] (at most 64 cells) become the first tokens of the empty sequence `seq`; logits of every cell."""
         n = features.shape[0]
         if not 0 <= seq < self.n_seqs or not 0 < n <= self.MAX_ROWS:
             raise ValueError(f"{n} cells for sequence {seq}: 1 to {self.MAX_ROWS} cells, {self.n_seqs} sequences")
+        self._empty([seq])
         self._take(n, None, [seq])
         x = self.ops.w4_linear(features.half(), self.project) + self.position[:n]
         one = torch.tensor([seq], dtype=torch.int32, device=x.device)
@@ -139,13 +148,14 @@ class Reader:
 
     def read(self, features, n_tokens):
         """The likeliest tokens, one after the other, for each of a list of feature maps [cells, channels]: int64 [maps, n_tokens]. Takes
-        sequences 0, 1, ... and forgets them again."""
+        sequences 0, 1, ..., which have to be empty, and forgets them again."""
         if not 0 < len(features) <= min(self.n_seqs, self.MAX_ROWS) or n_tokens < 1:
             raise ValueError(f"{n_tokens} tokens for {len(features)} maps: at least one of each, {min(self.n_seqs, self.MAX_ROWS)} maps at most")
         for f in features:
             if not 0 < f.shape[0] <= self.MAX_ROWS or f.shape[0] + n_tokens - 1 > self.max_tokens:
                 raise ValueError(f"{f.shape[0]} cells and {n_tokens} tokens: at most {self.MAX_ROWS} cells, {self.max_tokens} of both")
         named = list(range(len(features)))
+        self._empty(named)
         seqs = torch.arange(len(features), dtype=torch.int32, device=self.position.device)
         ids = torch.stack([self.look(f, i)[-1].argmax() for i, f in enumerate(features)])
         said = [ids]

@@ -78,3 +78,14 @@ def test_a_fork_may_be_as_long_as_the_longest():
         cache.lengths[:] = torch.tensor([0, 60, 3], dtype=torch.int32)                # (the first one has been forgotten since)
     with pytest.raises(ValueError, match="more tokens"):
         r.look(torch.zeros(10, 64), 1)
+
+
+def test_features_are_the_first_tokens():
+    r = reader()
+    r.most, r.caches[0].lengths[1] = [0, 5, 7], 5
+    with pytest.raises(ValueError, match=r"\[1\] are not empty"):
+        r.look(torch.zeros(10, 64), 1)
+    with pytest.raises(ValueError, match=r"\[1\] are not empty"):
+        r.read(maps(10, 10), 3)
+    with pytest.raises(AssertionError, match="reached"):             # (the third one has been forgotten since it was counted)
+        r.look(torch.zeros(10, 64), 2)
