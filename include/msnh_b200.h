@@ -393,6 +393,40 @@ typedef struct MsnhB200W4Linear {
 int  msnh_b200_w4_linear_workspace(MsnhB200Ctx *ctx, const MsnhB200W4 *weights, const MsnhB200W4Linear *args, size_t *bytes);
 int  msnh_b200_w4_linear(MsnhB200Ctx *ctx, const MsnhB200W4 *weights, const MsnhB200W4Linear *args, void *stream);
 
+/* Rotary positions: of each head the first rotary_dim values are turned in planes of two, (i, i + rotary_dim / 2) or, interleaved,
+ * (2i, 2i + 1), i = 0 .. rotary_dim / 2 - 1, and times `magnitude`; the others are copied:
+ *   y_a = magnitude * (x_a cos t - x_b sin t), y_b = magnitude * (x_a sin t + x_b cos t), t = 2 pi * position * turns[i] / 2^64
+ * turns[i] is the plane's frequency in whole turns a position, as a 64-bit fraction (negative: the other way round). Positions may be
+ * negative and as large as their type: angles do not lose precision by them. y may be x with the same strides. */
+typedef struct MsnhB200Rotary {
+    const void *x;                     /* [tokens][heads][dim]: F32, F16, BF16                     */
+    void *y;                           /* same shape and type                                      */
+    const void *positions;             /* [tokens] int32, or int64 where wide_positions             */
+    const int64_t *turns;              /* [rotary_dim / 2] on the device                           */
+    int64_t tokens;
+    int32_t heads, dim, rotary_dim, dtype, interleaved, wide_positions;
+    int64_t x_token_stride, x_head_stride, y_token_stride, y_head_stride;
+    float   magnitude;
+} MsnhB200Rotary;
+int  msnh_b200_rotary(MsnhB200Ctx *ctx, const MsnhB200Rotary *args, void *stream);
+
+/* Scores of tokens from rows of logits, over p = softmax(logits[row]): log p of the token ids[row] (NaN where that is none), the
+ * entropy -sum p log p, and the `top` likeliest tokens, the first one first, the lowest id first among equal ones, with their log p.
+ * Sums are fp32. Logits of -infinity have p = 0. A row that is no distribution (a NaN, +infinity, or nothing above -infinity) has NaN
+ * throughout, and ids of -1. */
+#define MSNH_B200_SCORES_MAX_TOP 32
+typedef struct MsnhB200TokenScores {
+    const void *logits;                /* [rows][cols]: F32, F16, BF16                             */
+    const int64_t *ids;                /* [rows], or NULL where logprob is                         */
+    float *logprob;                    /* [rows] or NULL                                           */
+    float *entropy;                    /* [rows] or NULL                                           */
+    float *top_logprobs;               /* [rows][top], NULL where top is 0                         */
+    int64_t *top_ids;                  /* [rows][top], NULL where top is 0                         */
+    int64_t rows, logits_stride;
+    int32_t cols, dtype, top;          /* top <= cols and MSNH_B200_SCORES_MAX_TOP                  */
+} MsnhB200TokenScores;
+int  msnh_b200_token_scores(MsnhB200Ctx *ctx, const MsnhB200TokenScores *args, void *stream);
+
 /* A cache of keys and values in pages of page_size tokens. Token t of sequence s lies in page page_table[s][t / page_size] at
  * place t % page_size. Sequences may share full pages (refs counts the sequences that hold a page; 0 = free); a page that is not
  * full belongs to one sequence. All of it is the caller's memory; a fresh cache has lengths and refs of 0.

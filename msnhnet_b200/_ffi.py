@@ -108,6 +108,19 @@ class AttnDecode(C.Structure):
                 ("window", C.c_int32), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
+class Rotary(C.Structure):
+    """MsnhB200Rotary"""
+    _fields_ = [("x", C.c_void_p), ("y", C.c_void_p), ("positions", C.c_void_p), ("turns", C.c_void_p), ("tokens", C.c_int64), ("heads", C.c_int32), ("dim", C.c_int32),
+                ("rotary_dim", C.c_int32), ("dtype", C.c_int32), ("interleaved", C.c_int32), ("wide_positions", C.c_int32), ("x_token_stride", C.c_int64),
+                ("x_head_stride", C.c_int64), ("y_token_stride", C.c_int64), ("y_head_stride", C.c_int64), ("magnitude", C.c_float)]
+
+
+class TokenScores(C.Structure):
+    """MsnhB200TokenScores"""
+    _fields_ = [("logits", C.c_void_p), ("ids", C.c_void_p), ("logprob", C.c_void_p), ("entropy", C.c_void_p), ("top_logprobs", C.c_void_p), ("top_ids", C.c_void_p),
+                ("rows", C.c_int64), ("logits_stride", C.c_int64), ("cols", C.c_int32), ("dtype", C.c_int32), ("top", C.c_int32)]
+
+
 _kernel = None
 _host = None
 
@@ -174,6 +187,8 @@ def kernel_lib():
     lib.msnh_b200_kv_free.argtypes = [vp, C.POINTER(KvCache), vp, i32, vp]
     lib.msnh_b200_kv_compact.argtypes = [vp, C.POINTER(KvCache), vp, vp, vp, C.c_size_t, vp]
     lib.msnh_b200_kv_copy_pages.argtypes = [vp, C.POINTER(KvCache), vp, vp, i32, vp]
+    lib.msnh_b200_rotary.argtypes = [vp, C.POINTER(Rotary), vp]
+    lib.msnh_b200_token_scores.argtypes = [vp, C.POINTER(TokenScores), vp]
     _kernel = lib
     return lib
 
@@ -192,6 +207,7 @@ KERNEL_SYMBOLS = [
     "msnh_b200_rms_norm", "msnh_b200_w4_pack_bytes", "msnh_b200_w4_pack", "msnh_b200_w4_linear_workspace", "msnh_b200_w4_linear",
     "msnh_b200_attn_decode_workspace", "msnh_b200_attn_decode", "msnh_b200_kv_workspace", "msnh_b200_kv_append", "msnh_b200_kv_fork",
     "msnh_b200_kv_free", "msnh_b200_kv_compact", "msnh_b200_kv_copy_pages",
+    "msnh_b200_rotary", "msnh_b200_token_scores",
 ]
 
 

@@ -1,0 +1,160 @@
+// Rotary positions (msnh_b200_rotary): of every head of a token the first 2 * half values are turned in planes of two by the token's
+// position times the plane's frequency; the values behind them are kept.
+//
+// The angle is position * frequency without the whole turns. Frequencies are given in turns, as 64-bit fractions, so the product modulo
+// 2^64 is the exact fraction of a turn for any position: what is left of an angle's error is the frequency's own 2^-64 times the position,
+// and the 2^-25 of a turn's half that the fraction is rounded to in fp32.
+//
+// Every value is read and written once, and those bytes bound it. A block has some tokens' planes: it makes their sines and cosines once
+// (into shared memory, while its first values are on their way) and turns all heads by them, two vectors of 16 bytes at a time.
+#include "token_ops.h"
+#include "token_types.cuh"
+
+namespace msnh {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kTable = 1024;             // planes of a block's tokens at most
+constexpr int kAhead = 4;                // vector pairs of a thread on their way together
+
+struct RotaryParams {
+    const uint8_t *x;
+    uint8_t *y;
+    const void *positions;
+    const unsigned long long *turns;
+    long long tokens, x_token, x_head, y_token, y_head;
+    int heads, dim, half, wide_positions, tokens_of_block, heads_of_block;
+    float magnitude;
+};
+
+// V values side by side (V = 1: of tensors without 16-byte alignment)
+template <typename T, int V> __device__ __forceinline__ void copy_values(T *to, const T *from) {
+    if constexpr (V == 1) *to = *from;
+    else *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(from);
+}
+
+// An item is V planes of a head of a token: values i.. and half + i.. of it, or, interleaved, 2 V values side by side.
+template <typename T, int V, bool kInterleaved>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
+    __shared__ __align__(16) float cosine[kTable], sine[kTable];
+    pdl_enter();
+    const long long first_token = static_cast<long long>(blockIdx.x) * p.tokens_of_block;
+    const int tokens = static_cast<int>(min(static_cast<long long>(p.tokens_of_block), p.tokens - first_token));
+    const int first_head = blockIdx.y * p.heads_of_block, heads = min(p.heads_of_block, p.heads - first_head);
+    const T *x = reinterpret_cast<const T *>(p.x) + first_token * p.x_token + first_head * p.x_head;
+    T *y = reinterpret_cast<T *>(p.y) + first_token * p.y_token + first_head * p.y_head;
+    const int per_head = p.half / V, per_token = per_head * heads, items = per_token * tokens;
+    const int apart = kInterleaved ? V : p.half;
+    bool made = false;
+    for (int base = threadIdx.x; !made || base - static_cast<int>(threadIdx.x) < items; base += kThreads * kAhead) {
+        struct alignas(16) { T v[2 * V]; } pair[kAhead];
+        int plane[kAhead];                                       // of the table
+        long long to[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int item = base + u * kThreads;
+            if (item >= items) break;
+            const int token = item / per_token, rest = item - token * per_token, head = rest / per_head, i = (rest - head * per_head) * V;
+            const int at = kInterleaved ? 2 * i : i;
+            const T *from = x + token * p.x_token + head * p.x_head + at;
+            plane[u] = token * p.half + i;
+            to[u] = token * p.y_token + head * p.y_head + at;
+            copy_values<T, V>(pair[u].v, from);
+            copy_values<T, V>(pair[u].v + V, from + apart);
+        }
+        if (!made) {
+            for (int i = threadIdx.x; i < tokens * p.half; i += kThreads) {
+                const long long token = first_token + i / p.half;
+                const long long position = p.wide_positions ? static_cast<const long long *>(p.positions)[token] : static_cast<const int *>(p.positions)[token];
+                const unsigned long long turned = static_cast<unsigned long long>(position) * p.turns[i % p.half];
+                float s, c;
+                // (the upper half as a signed number: from -1/2 to 1/2 of a turn, in units of 2^-32)
+                sincospif(static_cast<float>(static_cast<int>(turned >> 32)) * 4.656612873077393e-10f, &s, &c);
+                cosine[i] = c * p.magnitude;
+                sine[i] = s * p.magnitude;
+            }
+            __syncthreads();
+            made = true;
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            if (base + u * kThreads >= items) break;
+            float c[V], s[V];
+            if constexpr (V == 1) {
+                c[0] = cosine[plane[u]];
+                s[0] = sine[plane[u]];
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; j += 4) {
+                    *reinterpret_cast<float4 *>(c + j) = *reinterpret_cast<const float4 *>(cosine + plane[u] + j);
+                    *reinterpret_cast<float4 *>(s + j) = *reinterpret_cast<const float4 *>(sine + plane[u] + j);
+                }
+            }
+            T *v = pair[u].v;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                T &first = kInterleaved ? v[2 * j] : v[j], &second = kInterleaved ? v[2 * j + 1] : v[V + j];
+                const float a = to_float(first), b = to_float(second);
+                first = from_float<T>(fmaf(a, c[j], -b * s[j]));
+                second = from_float<T>(fmaf(a, s[j], b * c[j]));
+            }
+            copy_values<T, V>(y + to[u], v);
+            copy_values<T, V>(y + to[u] + apart, v + V);
+        }
+    }
+    // what is not turned
+    const int kept = (p.dim - 2 * p.half) / V;
+    if (kept == 0 || (p.x == p.y && p.x_token == p.y_token && p.x_head == p.y_head)) return;
+    const int kept_of_token = kept * heads;
+    for (int item = threadIdx.x; item < kept_of_token * tokens; item += kThreads) {
+        const int token = item / kept_of_token, rest = item - token * kept_of_token, head = rest / kept, i = 2 * p.half + (rest - head * kept) * V;
+        copy_values<T, V>(y + token * p.y_token + head * p.y_head + i, x + token * p.x_token + head * p.x_head + i);
+    }
+}
+
+template <typename T>
+cudaError_t launch(const MsnhB200Ctx *ctx, const MsnhB200Rotary &a, const RotaryParams &p, dim3 grid, void *stream) {
+    constexpr int V = 16 / sizeof(T);
+    bool wide = p.half % V == 0 && p.dim % V == 0 && aligned16(a.x) && aligned16(a.y);
+    for (const long long stride : {p.x_token, p.x_head, p.y_token, p.y_head}) wide = wide && stride % V == 0;
+    if (wide) return a.interleaved ? launch_token_kernel(rotary_kernel<T, V, true>, grid, kThreads, 0, stream, ctx->pdl, p)
+                                   : launch_token_kernel(rotary_kernel<T, V, false>, grid, kThreads, 0, stream, ctx->pdl, p);
+    return a.interleaved ? launch_token_kernel(rotary_kernel<T, 1, true>, grid, kThreads, 0, stream, ctx->pdl, p)
+                         : launch_token_kernel(rotary_kernel<T, 1, false>, grid, kThreads, 0, stream, ctx->pdl, p);
+}
+
+}  // namespace
+}  // namespace msnh
+
+using namespace msnh;
+
+extern "C" int msnh_b200_rotary(MsnhB200Ctx *ctx, const MsnhB200Rotary *a, void *stream) try {
+    if (!ctx || !a) return MSNH_B200_ERR_ARG;
+    if (!is_float_type(a->dtype)) return fail(ctx, MSNH_B200_ERR_UNSUPPORTED, "rotary: values of type %d", a->dtype);
+    if (a->tokens < 0 || a->heads < 0 || a->dim < 1 || a->rotary_dim < 2 || a->rotary_dim % 2 || a->rotary_dim > a->dim)
+        return fail(ctx, MSNH_B200_ERR_ARG, "rotary: %d values in planes of two of heads of %d", a->rotary_dim, a->dim);
+    if (a->rotary_dim > 2 * kTable || static_cast<long long>(a->heads) * a->dim >= 1 << 27)
+        return fail(ctx, MSNH_B200_ERR_UNSUPPORTED, "rotary: more than %d turned values of a head, or 2^27 values of a token", 2 * kTable);
+    if (a->tokens == 0 || a->heads == 0) return MSNH_B200_OK;
+    if (!a->x || !a->y || !a->positions || !a->turns) return fail(ctx, MSNH_B200_ERR_ARG, "rotary: null x, y, positions or turns");
+    if (a->x_token_stride < 0 || a->x_head_stride < 0 || (a->tokens > 1 && a->y_token_stride < a->dim) || (a->heads > 1 && a->y_head_stride < a->dim))
+        return fail(ctx, MSNH_B200_ERR_ARG, "rotary: a stride of x is negative, or rows of y overlap");
+    DeviceScope scope(ctx->device);
+    CUDA_TRY(ctx, scope.status);
+    RotaryParams p = {static_cast<const uint8_t *>(a->x), static_cast<uint8_t *>(a->y), a->positions, reinterpret_cast<const unsigned long long *>(a->turns), a->tokens,
+                      a->x_token_stride, a->x_head_stride, a->y_token_stride, a->y_head_stride, a->heads, a->dim, a->rotary_dim / 2, a->wide_positions, 1, a->heads,
+                      a->magnitude};
+    // A block's tokens: as many as there are threads for their planes, up to eight, where that leaves every SM some blocks. Few tokens: their heads in
+    // parts, as long as a part has an item for each thread.
+    const long long most = std::max(1, std::min(8, kThreads / p.half));
+    p.tokens_of_block = static_cast<int>(std::max<long long>(1, std::min<long long>(most, a->tokens / (4LL * ctx->sm_count))));
+    const long long blocks = (a->tokens + p.tokens_of_block - 1) / p.tokens_of_block;
+    if (blocks > 0x7fffffff) return fail(ctx, MSNH_B200_ERR_UNSUPPORTED, "rotary: 2^31 tokens and more");
+    const long long vectors = static_cast<long long>(p.heads) * p.half * dtype_size(a->dtype) / 16;
+    const long long parts = std::max<long long>(1, std::min<long long>({vectors / kThreads, ctx->sm_count / blocks, a->heads}));
+    p.heads_of_block = static_cast<int>((a->heads + parts - 1) / parts);
+    const dim3 grid(static_cast<unsigned>(blocks), (a->heads + p.heads_of_block - 1) / p.heads_of_block);
+    CUDA_TRY(ctx, a->dtype == MSNH_B200_F32 ? launch<float>(ctx, *a, p, grid, stream) : a->dtype == MSNH_B200_F16 ? launch<__half>(ctx, *a, p, grid, stream)
+                                                                                                                 : launch<__nv_bfloat16>(ctx, *a, p, grid, stream));
+    return MSNH_B200_OK;
+} catch (...) { return caught(ctx); }

@@ -1,0 +1,323 @@
+// Scores of tokens from rows of logits: log probability of a given one, entropy, the likeliest ones (msnh_b200_token_scores).
+//
+// p = e^(z - m) / s, s = sum e^(z - m), m the running maximum: log p = z - m - log s, entropy = log s + sum e^(z - m) (m - z) / s, in
+// which nothing cancels. One pass: every logit is read once, and those bytes bound it where there are many rows.
+//
+// Each thread keeps its maximum, both sums and the 16-byte chunk in which its maximum lay first. The `top` best logits of a row are
+// among the chunks of the `top` threads whose maxima are the best ones: only those threads' chunks are looked at again, a warp for each
+// thread. What orders logits is a 64-bit key, the number's bits in the numbers' order above the lowest index first, so all keys differ
+// and ties cost nothing. Sorted lists of 32 keys lie across a warp's lanes; two of them are joined by five steps of a bitonic merge.
+//
+// A row is one block's or, where there are fewer rows than SMs, one cluster's: its blocks hand their sums and lists to the first one
+// through distributed shared memory, so that there is one launch and no workspace.
+#include <cooperative_groups.h>
+#include "token_ops.h"
+#include "token_types.cuh"
+
+namespace msnh {
+namespace {
+
+namespace cg = cooperative_groups;
+using Key = unsigned long long;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kFar = 1000.f;           // distances are bounded by it where they are factors, so that 0 times infinity does not come up: e^-1000 is 0
+
+struct ScoreParams {
+    const uint8_t *logits;
+    const long long *ids;
+    float *logprob, *entropy, *top_logprobs;
+    long long *top_ids;
+    long long rows, stride;
+    int cols, top;
+};
+
+// Bits of a float in the numbers' order (-0 counts as 0); above 0 for every number and infinity.
+__device__ __forceinline__ uint32_t ordered(float v) {
+    const uint32_t bits = __float_as_uint(v + 0.f);
+    return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+}
+__device__ __forceinline__ float unordered(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
+__device__ __forceinline__ Key key_of(float v, uint32_t index) { return static_cast<Key>(ordered(v)) << 32 | static_cast<uint32_t>(~index); }
+__device__ __forceinline__ uint32_t index_of(Key key) { return ~static_cast<uint32_t>(key); }
+
+__device__ __forceinline__ float pow2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
+// Sums of some logits: the largest, sum e^(z - top), sum e^(z - top) (top - z).
+struct Sums {
+    float top, sum, more;
+    // to a maximum that is not smaller
+    __device__ __forceinline__ void lift(float best) {
+        if (best == top) return;
+        const float d = best - top, f = pow2(d * -kLog2e);
+        more = f * fmaf(sum, fminf(d, kFar), more);              // (NaN where the distance is)
+        sum *= f;
+        top = best;
+    }
+    // (a sum that is NaN stays one, and so does a maximum of infinity)
+    __device__ __forceinline__ void join(Sums o) {
+        const float best = fmaxf(top, o.top);
+        lift(best);
+        o.lift(best);
+        sum += o.sum;
+        more += o.more;
+    }
+    __device__ __forceinline__ void join_warp() {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) join(Sums{__shfl_xor_sync(~0u, top, o), __shfl_xor_sync(~0u, sum, o), __shfl_xor_sync(~0u, more, o)});
+    }
+};
+
+// Across a warp's lanes: the larger keys of a pair at distance `o` to the lower lanes.
+__device__ __forceinline__ Key exchange(Key mine, int o, bool larger) {
+    const Key other = __shfl_xor_sync(~0u, mine, o);
+    return (mine > other) == larger ? mine : other;
+}
+// 32 keys, lane 0 the largest
+__device__ __forceinline__ Key sort_warp(Key key, int lane) {
+#pragma unroll
+    for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+        for (int o = size / 2; o; o /= 2) key = exchange(key, o, ((lane & o) == 0) == ((lane & size) == 0 || size == 32));
+    return key;
+}
+// The 32 largest of two sorted lists (the other one's key of lane 31 - l is given to lane l), sorted.
+__device__ __forceinline__ Key merge_warp(Key key, Key other_reversed, int lane) {
+    key = key > other_reversed ? key : other_reversed;
+#pragma unroll
+    for (int o = 16; o; o /= 2) key = exchange(key, o, (lane & o) == 0);
+    return key;
+}
+// The lists of a block's warps joined in warp 0; list[] has 32 keys of every warp. Begins and ends with a barrier.
+template <int kWarps> __device__ __forceinline__ Key merge_block(Key key, Key (*list)[32], int warp, int lane) {
+    list[warp][lane] = key;
+    __syncthreads();
+#pragma unroll
+    for (int n = kWarps / 2; n; n /= 2) {
+        if (warp < n) {
+            key = merge_warp(key, list[warp + n][31 - lane], lane);
+            list[warp][lane] = key;
+        }
+        __syncthreads();
+    }
+    return key;
+}
+
+// A row's 16-byte chunks: chunk c has logits c * kVec - shift and on, so that whole chunks are aligned.
+template <typename T> struct Row {
+    static constexpr int kVec = 16 / sizeof(T);
+    const T *at;
+    int cols, shift, chunks;
+    __device__ __forceinline__ Row(const T *from, int cols_) : at(from), cols(cols_) {
+        shift = static_cast<int>(reinterpret_cast<uintptr_t>(from) % 16 / sizeof(T));
+        chunks = static_cast<int>((static_cast<long long>(cols) + shift + kVec - 1) / kVec);
+    }
+    __device__ __forceinline__ int first_of(int chunk) const { return chunk * kVec - shift; }
+    // whether all of the chunk's values are the row's
+    __device__ __forceinline__ bool whole(int chunk) const { return (chunk > 0 || shift == 0) && first_of(chunk) <= cols - kVec; }
+    __device__ __forceinline__ uint4 load_whole(int chunk) const { return *reinterpret_cast<const uint4 *>(at + first_of(chunk)); }
+    // places that are not the row's hold `none`
+    __device__ __forceinline__ void load(int chunk, float (&v)[kVec], float none) const {
+        if (whole(chunk)) {
+            Vec16<T>::unpack(load_whole(chunk), v);
+        } else {
+            const int first = first_of(chunk);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) v[i] = first + i >= 0 && first + i < cols ? to_float(at[first + i]) : none;
+        }
+    }
+};
+
+template <int kWarps> struct ScoreShared {
+    Key list[kWarps][32];
+    Key keys[32];                        // the block's best: of threads, then of logits
+    Sums sums[kWarps], all;
+};
+
+template <typename T, int kThreads, int kCluster>
+__global__ void __launch_bounds__(kThreads) token_scores_kernel(const __grid_constant__ ScoreParams p) {
+    constexpr int kVec = 16 / sizeof(T), kWarps = kThreads / 32, kAhead = 4;
+    __shared__ ScoreShared<kWarps> shared;
+    pdl_enter();
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, part = kCluster > 1 ? blockIdx.x % kCluster : 0;
+    for (long long r = blockIdx.x / kCluster; r < p.rows; r += gridDim.x / kCluster) {
+        const Row<T> row(reinterpret_cast<const T *>(p.logits) + r * p.stride, p.cols);
+        const int per_part = (row.chunks + kCluster - 1) / kCluster, begin = min(part * per_part, row.chunks), end = min(begin + per_part, row.chunks);
+        Sums mine = {-INFINITY, 0.f, 0.f};
+        int best = begin + threadIdx.x;                          // the first chunk that has the maximum
+        const auto take = [&](const float (&v)[kVec], int chunk) {
+            float top = v[0];
+#pragma unroll
+            for (int i = 1; i < kVec; ++i) top = max_or_nan(top, v[i]);
+            if (!(top <= mine.top)) {
+                mine.lift(top);
+                best = chunk;
+            }
+            if (mine.top == -INFINITY) return;                   // (nothing but -infinity so far)
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) {
+                const float d = fminf(mine.top - v[i], kFar), e = pow2(d * -kLog2e);
+                mine.sum += e;
+                mine.more = fmaf(e, d, mine.more);
+            }
+        };
+        for (int c = begin + threadIdx.x; c < end; c += kThreads * kAhead) {
+            if (row.whole(c) && c + kThreads * (kAhead - 1) < end && row.whole(c + kThreads * (kAhead - 1))) {
+                uint4 raw[kAhead];
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) raw[u] = row.load_whole(c + u * kThreads);
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    float v[kVec];
+                    Vec16<T>::unpack(raw[u], v);
+                    take(v, c + u * kThreads);
+                }
+            } else {
+#pragma unroll 1
+                for (int u = 0; u < kAhead && c + u * kThreads < end; ++u) {
+                    float v[kVec];
+                    row.load(c + u * kThreads, v, -INFINITY);
+                    take(v, c + u * kThreads);
+                }
+            }
+        }
+        const float thread_top = mine.top;
+        mine.join_warp();
+        if (lane == 0) shared.sums[warp] = mine;
+        if (p.top > 0) {
+            // the threads with the best maxima (no chunk: below all), then the best logits of their chunks
+            Key key = begin + static_cast<int>(threadIdx.x) < end ? key_of(thread_top, best) : 0;
+            key = merge_block<kWarps>(sort_warp(key, lane), shared.list, warp, lane);
+            if (warp == 0) shared.keys[lane] = key;
+            __syncthreads();
+            Key found = 0;
+            const Key least = shared.keys[p.top - 1];
+            for (int j = warp; j < p.top && shared.keys[j]; j += kWarps) {
+                const int first = begin + (static_cast<int>(index_of(shared.keys[j])) - begin) % kThreads;
+                for (int base = first; base < end; base += kThreads * 32) {
+                    const int c = base + lane * kThreads;
+                    float v[kVec];
+                    if (c < end) row.load(c, v, __uint_as_float(0x7fffffffu));
+#pragma unroll
+                    for (int i = 0; i < kVec; ++i) {
+                        // (what is not of the row is NaN here, and so not above the threshold; neither is a NaN of the row, whose ids are -1 anyway)
+                        Key candidate = c < end && v[i] == v[i] && key_of(v[i], c) >= least ? key_of(v[i], row.first_of(c) + i) : 0;
+                        const Key last = __shfl_sync(~0u, found, p.top - 1);
+                        unsigned who = __ballot_sync(~0u, candidate > last);
+                        while (who) {
+                            const Key next = __shfl_sync(~0u, candidate, __ffs(who) - 1);
+                            who &= who - 1;
+                            const int place = __popc(__ballot_sync(~0u, found > next));
+                            const Key above = __shfl_up_sync(~0u, found, 1);
+                            found = lane < place ? found : lane == place ? next : above;
+                        }
+                    }
+                }
+            }
+            __syncthreads();                                     // (the list and the keys have been read)
+            found = merge_block<kWarps>(found, shared.list, warp, lane);
+            if (warp == 0) shared.keys[lane] = found;
+        }
+        __syncthreads();
+        if (warp == 0) {
+            Sums all = lane < kWarps ? shared.sums[lane] : Sums{-INFINITY, 0.f, 0.f};
+            all.join_warp();
+            if (lane == 0) shared.all = all;
+        }
+        if constexpr (kCluster > 1) cg::this_cluster().sync();
+        if (part == 0 && warp == 0) {
+            __syncwarp();
+            Sums all = shared.all;
+            Key key = p.top > 0 ? shared.keys[lane] : 0;
+            if constexpr (kCluster > 1) {
+#pragma unroll 1
+                for (int o = 1; o < kCluster; ++o) {
+                    const ScoreShared<kWarps> *other = cg::this_cluster().map_shared_rank(&shared, o);
+                    all.join(other->all);
+                    if (p.top > 0) key = merge_warp(key, other->keys[31 - lane], lane);
+                }
+            }
+            const float nan = __uint_as_float(0x7fffffffu);
+            // (a maximum of +infinity has sums of 0 or NaN)
+            const bool good = all.top > -INFINITY && all.top < INFINITY && all.sum >= 1.f;
+            const float log_sum = good ? logf(all.sum) : nan;
+            if (lane == 0) {
+                if (p.entropy) p.entropy[r] = good ? log_sum + all.more / all.sum : nan;
+                if (p.logprob) {
+                    const long long id = p.ids[r];
+                    p.logprob[r] = good && id >= 0 && id < p.cols ? to_float(row.at[id]) - all.top - log_sum : nan;
+                }
+            }
+            if (lane < p.top) {
+                p.top_ids[r * p.top + lane] = good ? static_cast<long long>(index_of(key)) : -1;
+                p.top_logprobs[r * p.top + lane] = good ? unordered(static_cast<uint32_t>(key >> 32)) - all.top - log_sum : nan;
+            }
+        }
+        if constexpr (kCluster > 1) cg::this_cluster().sync();
+        else __syncthreads();                                    // (shared memory is the next row's)
+    }
+}
+
+template <typename T, int kThreads, int kCluster>
+cudaError_t launch(const MsnhB200Ctx *ctx, const ScoreParams &p, void *stream) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(static_cast<unsigned>(std::min<long long>(p.rows, 1 << 24)) * kCluster);
+    config.blockDim = kThreads;
+    config.stream = static_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute attr[2];
+    if (kCluster > 1) {
+        attr[config.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[config.numAttrs].val.clusterDim.x = kCluster;
+        attr[config.numAttrs].val.clusterDim.y = attr[config.numAttrs].val.clusterDim.z = 1;
+        ++config.numAttrs;
+    }
+    if (ctx->pdl) {
+        attr[config.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[config.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+        ++config.numAttrs;
+    }
+    config.attrs = attr;
+    return cudaLaunchKernelEx(&config, token_scores_kernel<T, kThreads, kCluster>, p);
+}
+
+// Blocks of a row: as many as leave every SM two, each with 4096 logits at least. Short rows: 128 threads.
+template <typename T>
+cudaError_t launch_by_size(const MsnhB200Ctx *ctx, const ScoreParams &p, void *stream) {
+    if (p.cols <= 4096) return launch<T, 128, 1>(ctx, p, stream);
+    const long long parts = std::min<long long>(2LL * ctx->sm_count / p.rows, p.cols / 4096);
+    if (parts >= 8) return launch<T, 512, 8>(ctx, p, stream);
+    if (parts >= 4) return launch<T, 512, 4>(ctx, p, stream);
+    if (parts >= 2) return launch<T, 512, 2>(ctx, p, stream);
+    return launch<T, 512, 1>(ctx, p, stream);
+}
+
+}  // namespace
+}  // namespace msnh
+
+using namespace msnh;
+
+extern "C" int msnh_b200_token_scores(MsnhB200Ctx *ctx, const MsnhB200TokenScores *a, void *stream) try {
+    if (!ctx || !a) return MSNH_B200_ERR_ARG;
+    if (!is_float_type(a->dtype)) return fail(ctx, MSNH_B200_ERR_UNSUPPORTED, "token_scores: logits of type %d", a->dtype);
+    if (a->rows < 0 || a->cols < 1 || a->top < 0 || a->top > a->cols) return fail(ctx, MSNH_B200_ERR_ARG, "token_scores: the %d best of rows of %d logits", a->top, a->cols);
+    if (a->top > MSNH_B200_SCORES_MAX_TOP) return fail(ctx, MSNH_B200_ERR_UNSUPPORTED, "token_scores: the %d best (at most %d are given)", a->top, MSNH_B200_SCORES_MAX_TOP);
+    if (a->cols > 1 << 30) return fail(ctx, MSNH_B200_ERR_UNSUPPORTED, "token_scores: rows of %d logits (at most 2^30 are taken)", a->cols);
+    if (a->rows == 0) return MSNH_B200_OK;
+    if (!a->logits || (a->logprob && !a->ids) || (a->top && (!a->top_logprobs || !a->top_ids))) return fail(ctx, MSNH_B200_ERR_ARG, "token_scores: null logits, ids, top_logprobs or top_ids");
+    if (a->logits_stride < 0) return fail(ctx, MSNH_B200_ERR_ARG, "token_scores: a stride is negative");
+    DeviceScope scope(ctx->device);
+    CUDA_TRY(ctx, scope.status);
+    const ScoreParams p = {static_cast<const uint8_t *>(a->logits), reinterpret_cast<const long long *>(a->ids), a->logprob, a->entropy, a->top_logprobs,
+                           reinterpret_cast<long long *>(a->top_ids), a->rows, a->logits_stride, a->cols, a->top};
+    CUDA_TRY(ctx, a->dtype == MSNH_B200_F32 ? launch_by_size<float>(ctx, p, stream) : a->dtype == MSNH_B200_F16 ? launch_by_size<__half>(ctx, p, stream)
+                                                                                                              : launch_by_size<__nv_bfloat16>(ctx, p, stream));
+    return MSNH_B200_OK;
+} catch (...) { return caught(ctx); }

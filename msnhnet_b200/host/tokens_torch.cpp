@@ -13,6 +13,7 @@
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <algorithm>
 #include <cmath>
 #include <exception>
 #include <string>
@@ -212,6 +213,65 @@ PyObject *w4_linear(PyObject *, PyObject *const *args, Py_ssize_t n) {
     });
 }
 
+// x, positions, the table's turns, whether planes are interleaved, magnitude, out or None
+PyObject *rotary(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        const Args a(args, n, 8);
+        const at::Tensor &x = a.tensor(2, "x"), &positions = a.tensor(3, "positions"), &turns = a.tensor(4, "the table");
+        const auto type = x.scalar_type();
+        if (x.dim() != 3 || !is_float(type) || (x.stride(2) != 1 && x.size(2) > 1)) wrong("x: [tokens, heads, head_dim] of a floating type, the values of a head side by side");
+        const int64_t tokens = x.size(0), heads = x.size(1), dim = x.size(2);
+        if (heads > INT32_MAX || dim > INT32_MAX) wrong("x: too many heads or values");
+        if (positions.scalar_type() != at::kLong) vector_of(positions, tokens, at::kInt, "positions");
+        else vector_of(positions, tokens, at::kLong, "positions");
+        vector_of(turns, turns.numel(), at::kLong, "the table");
+        const at::Tensor *given = a.maybe(7, "out");
+        if (given && (given->sizes() != x.sizes() || given->scalar_type() != type || (given->stride(2) != 1 && dim > 1))) wrong("out: x's shape and type");
+        const at::Tensor out = given ? *given : a.empty(x.sizes(), type);
+        const int interleaved = PyObject_IsTrue(args[5]);
+        const MsnhB200Rotary call = {x.const_data_ptr(), out.mutable_data_ptr(), positions.const_data_ptr(), static_cast<const int64_t *>(turns.const_data_ptr()), tokens,
+                                     static_cast<int32_t>(heads), static_cast<int32_t>(dim), static_cast<int32_t>(std::min<int64_t>(2 * turns.numel(), INT32_MAX - 1)), type_of(type),
+                                     interleaved, positions.scalar_type() == at::kLong, x.stride(0), x.stride(1), out.stride(0), out.stride(1), static_cast<float>(a.number(6))};
+        check(a.ctx, msnh_b200_rotary(a.ctx, &call, a.stream()));
+        if (given) a.writes(*given);
+        return wrap(out);
+    });
+}
+
+// logits, ids or None, how many of the likeliest
+PyObject *token_scores(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        const Args a(args, n, 5);
+        const at::Tensor &logits = a.tensor(2, "logits");
+        const auto type = logits.scalar_type();
+        if (logits.dim() != 2 || !is_float(type) || (logits.stride(1) != 1 && logits.size(1) > 1)) wrong("logits: rows of floating values side by side");
+        const int64_t rows = logits.size(0), cols = logits.size(1);
+        if (cols > INT32_MAX) wrong("logits: rows that are too long");
+        const at::Tensor *ids = a.maybe(3, "ids");
+        if (ids) vector_of(*ids, rows, at::kLong, "ids");
+        const long long top = a.whole(4);
+        if (top > INT32_MAX || top < INT32_MIN) wrong("top: out of range");
+        const at::Tensor entropy = a.empty({rows}, at::kFloat);
+        at::Tensor logprob, top_logprobs, top_ids;
+        if (ids) logprob = a.empty({rows}, at::kFloat);
+        if (top > 0 && top <= MSNH_B200_SCORES_MAX_TOP) {
+            top_logprobs = a.empty({rows, top}, at::kFloat);
+            top_ids = a.empty({rows, top}, at::kLong);
+        }
+        const MsnhB200TokenScores call = {logits.const_data_ptr(), ids ? static_cast<const int64_t *>(ids->const_data_ptr()) : nullptr,
+                                          ids ? static_cast<float *>(logprob.mutable_data_ptr()) : nullptr, static_cast<float *>(entropy.mutable_data_ptr()),
+                                          top_logprobs.defined() ? static_cast<float *>(top_logprobs.mutable_data_ptr()) : nullptr,
+                                          top_ids.defined() ? static_cast<int64_t *>(top_ids.mutable_data_ptr()) : nullptr, rows, logits.stride(0),
+                                          static_cast<int32_t>(cols), type_of(type), static_cast<int32_t>(top)};
+        check(a.ctx, msnh_b200_token_scores(a.ctx, &call, a.stream()));
+        const auto or_none = [](const at::Tensor &t) -> PyObject * {
+            if (t.defined()) return wrap(t);
+            Py_RETURN_NONE;
+        };
+        return Py_BuildValue("(NNNN)", or_none(logprob), wrap(entropy), or_none(top_logprobs), or_none(top_ids));
+    });
+}
+
 // q, address of the cache's struct, its k_pages, seqs or None, scale or None, window, out or None, whether lse is wanted
 PyObject *attn_decode(PyObject *, PyObject *const *args, Py_ssize_t n) {
     return guarded([&]() -> PyObject * {
@@ -352,7 +412,8 @@ template <PyObject *(*f)(PyObject *, PyObject *const *, Py_ssize_t)> PyMethodDef
 }
 PyMethodDef kMethods[] = {method<rms_norm>("rms_norm"),   method<w4_linear>("w4_linear"),   method<attn_decode>("attn_decode"),
                           method<kv_append>("kv_append"), method<kv_fork>("kv_fork"),       method<kv_free>("kv_free"),
-                          method<kv_compact>("kv_compact"), method<kv_copy_pages>("kv_copy_pages"), {nullptr, nullptr, 0, nullptr}};
+                          method<kv_compact>("kv_compact"), method<kv_copy_pages>("kv_copy_pages"),
+                          method<rotary>("rotary"),       method<token_scores>("token_scores"), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_tokens", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

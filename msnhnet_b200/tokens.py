@@ -14,6 +14,7 @@ none, and their results would be cut off unnoticed. What the library refuses rai
 (host/tokens_torch.cpp): in Python they took longer than the kernels of one token.
 """
 import ctypes as C
+import math
 
 import torch
 
@@ -39,6 +40,14 @@ class W4Weights:
         self.args = _ffi.W4(packed.data_ptr() if packed is not None else None, n, k, group, _DTYPE[scale_dtype], int(has_zeros))
         self.ref = C.byref(self.args)
         self.address = C.addressof(self.args)
+
+
+class RotaryTable:
+    """What TokenOps.rotary turns by (TokenOps.rotary_table): `turns`, the whole turns a position of each plane as 64-bit fractions (int64 on the
+    GPU), whether planes are interleaved, and the factor of what is turned."""
+
+    def __init__(self, turns, interleaved, magnitude):
+        self.turns, self.interleaved, self.magnitude = turns, interleaved, magnitude
 
 
 class PagedCache:
@@ -130,6 +139,44 @@ class TokenOps:
         """x [rows, k] times the weights' transpose: [rows, n], at most 64 rows. x of float8_e4m3fn gives float16 unless out_dtype says
         otherwise; x_scale: float32 [rows]; bias: float32 [n]."""
         return _tokens.w4_linear(self._ctx, self._index, x, weights.address, weights.packed, bias, x_scale, out_dtype, out)
+
+    def rotary_table(self, dim, base=10000.0, interleaved=False, stretch=None, factor=1.0, trained=8192, low=1.0, high=4.0, magnitude=1.0):
+        """Frequencies for rotary: the first `dim` values of a head are turned, plane i by base ** (-2 i / dim) radians a position; planes are
+        the values (i, i + dim / 2) or, interleaved, (2i, 2i + 1). What is turned is taken times `magnitude`.
+
+        For texts `factor` times as long as the `trained` positions a model knows, stretch slows planes down: "all" of them by the factor; by a
+        larger "base" (base * factor ** (dim / (dim - 2)): the slowest plane by the factor, the fastest not at all); or "slow" ones: those that
+        turn `low` times or less within the trained positions by the factor, those that turn `high` times or more not, in between a mixture."""
+        if dim < 2 or dim % 2 or not base > 0 or not factor > 0 or not high > low or trained < 1:
+            raise ValueError(f"rotary_table: dim {dim} (even, 2 at least), base {base}, factor {factor}, {low} to {high} turns of {trained} positions")
+        if stretch not in (None, "all", "base", "slow"):
+            raise ValueError(f"stretch {stretch!r}: None, 'all', 'base' or 'slow'")
+        if stretch == "base":
+            base = base * factor ** (dim / max(dim - 2, 1))
+        turns = []
+        for i in range(dim // 2):
+            turn = base ** (-2 * i / dim) / (2 * math.pi)
+            if stretch == "all":
+                turn /= factor
+            elif stretch == "slow":
+                kept = min(max((trained * turn - low) / (high - low), 0.0), 1.0)
+                turn *= kept + (1 - kept) / factor
+            fraction = int(turn * 2.0 ** 64) % 2 ** 64
+            turns.append(fraction - 2 ** 64 if fraction >= 2 ** 63 else fraction)
+        return RotaryTable(torch.tensor(turns, dtype=torch.int64, device=self.device), bool(interleaved), float(magnitude))
+
+    def rotary(self, x, positions, table, out=None):
+        """Turns the heads of x [tokens, heads, head_dim] (queries and keys side by side, if you like) by positions [tokens] (int32 or int64, of any
+        size and sign) and a table of rotary_table. out may be x: turned in place."""
+        return _tokens.rotary(self._ctx, self._index, x, positions, table.turns, table.interleaved, table.magnitude, out)
+
+    def token_scores(self, logits, ids=None, top=0):
+        """(logprob, entropy, top_logprobs, top_ids) of softmax(logits), for rows of logits; what is not asked for is None.
+
+        logprob: float32 [rows], of the tokens ids (int64 [rows]; NaN where one is none). entropy: float32 [rows]. top_logprobs, top_ids:
+        float32 and int64 [rows, top], the likeliest tokens (at most 32), the lowest id first among equal ones. A row that is no distribution
+        (a NaN, +infinity, or only -infinity) has NaN throughout, and ids of -1."""
+        return _tokens.token_scores(self._ctx, self._index, logits, ids, top)
 
     def new_cache(self, n_pages, page_size, n_kv_heads, head_dim, n_seqs, max_pages, dtype=torch.float16):
         """A fresh cache with memory of its own."""
