@@ -431,7 +431,10 @@ int  msnh_b200_token_scores(MsnhB200Ctx *ctx, const MsnhB200TokenScores *args, v
  * place t % page_size. Sequences may share full pages (refs counts the sequences that hold a page; 0 = free); a page that is not
  * full belongs to one sequence. All of it is the caller's memory; a fresh cache has lengths and refs of 0.
  * An operation that finds no free page, no place left in a table row, or a sequence number that is none leaves that sequence
- * as it was and adds one to *refused. */
+ * as it was and adds one to *refused.
+ * A cache of type E4M3 holds 8-bit codes and, for every scale_block tokens of a page (a divisor of page_size) and head, a scale: a value
+ * is its code times its scale. Appending writes scales that are powers of two, the smallest by which a block's values are at most 448;
+ * other finite ones of the caller are read as they are. The last three members are looked at in such a cache only. */
 typedef struct MsnhB200KvCache {
     void *k_pages, *v_pages;           /* [n_pages][page_size][n_kv_heads][head_dim] in the order of the strides */
     int64_t k_page_stride, k_token_stride, k_head_stride;
@@ -442,15 +445,19 @@ typedef struct MsnhB200KvCache {
     int32_t *refused;                  /* one counter                                              */
     int64_t table_stride;
     int32_t n_pages, page_size, n_kv_heads, head_dim, n_seqs, max_pages;
-    int32_t dtype;                     /* F32, F16, BF16                                           */
+    int32_t dtype;                     /* F32, F16, BF16, E4M3                                     */
+    float *k_scales, *v_scales;        /* [n_pages][n_kv_heads][page_size / scale_block]            */
+    int32_t scale_block;
 } MsnhB200KvCache;
 
 /* Attention of one query token a row over the cached tokens of its sequence: out[row][h] = sum_t p_t v_t, p = softmax(scale *
  * q[row][h] . k_t) over the sequence's last `window` tokens (0: all), with keys and values of kv head h / (n_heads / n_kv_heads).
  * Statistics and sums are fp32. Table entries outside [0, n_pages) are holes: their tokens are left out. Where no token is
- * left, out is 0 and lse -infinity. head_dim: a multiple of 16 bytes, at most 256 values; the pages' rows 16-byte aligned. */
+ * left, out is 0 and lse -infinity. head_dim: a multiple of 16 bytes, at most 256 values; the pages' rows 16-byte aligned.
+ * q and out have the cache's type; over a cache of E4M3 they have `dtype`, and a key or value is code times scale in the sums, with
+ * nothing rounded in between (queries of F32 and BF16 to 2^-24, and to 2^-39 of the largest in their head). */
 typedef struct MsnhB200AttnDecode {
-    const void *q;                     /* [rows][n_heads][head_dim], the cache's type              */
+    const void *q;                     /* [rows][n_heads][head_dim]                                */
     void *out;                         /* same shape and type                                      */
     float *lse;                        /* [rows][n_heads] log of the softmax's sum, or NULL         */
     const int32_t *seqs;               /* [rows] sequence of each row, or NULL: row i is sequence i */
@@ -460,6 +467,7 @@ typedef struct MsnhB200AttnDecode {
     int32_t window;
     void   *workspace;                 /* attn_decode_workspace bytes, 16-byte aligned; NULL if 0   */
     size_t  workspace_bytes;
+    int32_t dtype;                     /* of q and out over a cache of E4M3: F32, F16, BF16         */
 } MsnhB200AttnDecode;
 int  msnh_b200_attn_decode_workspace(MsnhB200Ctx *ctx, const MsnhB200KvCache *cache, const MsnhB200AttnDecode *args, size_t *bytes);
 int  msnh_b200_attn_decode(MsnhB200Ctx *ctx, const MsnhB200KvCache *cache, const MsnhB200AttnDecode *args, void *stream);
@@ -475,11 +483,23 @@ int  msnh_b200_attn_decode(MsnhB200Ctx *ctx, const MsnhB200KvCache *cache, const
  *   compact: the i-th free page below the number of live pages takes the i-th live page from there on, contents, refs and
  *            table entries; afterwards live pages are 0..live-1. table_out / refs_out: where the new table (rows
  *            table_stride apart) and refs go, the cache's own or memory beside them (all entries are written)
- *   copy   : page src[i] to page dst[i]; no page is dst twice or src and dst */
+ *   copy   : page src[i] to page dst[i]; no page is dst twice or src and dst
+ *   read   : tokens first[i] and on (NULL: from 0) of sequence seqs[i] (NULL: i) to rows starts[i] to starts[i + 1] (n + 1 offsets, in
+ *            order) of k_out / v_out, as out_dtype (F32, F16, BF16); rows of no sequence, no token or a hole are 0. All n_rows rows are
+ *            written. It changes nothing of the cache.
+ * append_as takes k_new and v_new as new_dtype, which is the cache's type or, in a cache of E4M3, F32, F16 or BF16. There a block's scale is
+ * the smallest power of two by which the call's values of it are at most 448, or the one it has where that is larger; older codes of a block whose scale
+ * grows are rounded again, to the new one (which loses nothing but of codes that become less than 2^-6). A NaN or infinity is the code NaN
+ * and does not count for the scale. A block of zeros has scale 0. */
 int  msnh_b200_kv_workspace(MsnhB200Ctx *ctx, const MsnhB200KvCache *cache, int n, size_t *bytes);
 int  msnh_b200_kv_append(MsnhB200Ctx *ctx, const MsnhB200KvCache *cache, const int32_t *seqs, const int32_t *starts, int n,
                          const void *k_new, const void *v_new, int64_t new_token_stride, int64_t new_head_stride, int n_tokens,
                          void *workspace, size_t workspace_bytes, void *stream);
+int  msnh_b200_kv_append_as(MsnhB200Ctx *ctx, const MsnhB200KvCache *cache, const int32_t *seqs, const int32_t *starts, int n,
+                            const void *k_new, const void *v_new, int new_dtype, int64_t new_token_stride, int64_t new_head_stride, int n_tokens,
+                            void *workspace, size_t workspace_bytes, void *stream);
+int  msnh_b200_kv_read(MsnhB200Ctx *ctx, const MsnhB200KvCache *cache, const int32_t *seqs, const int32_t *starts, const int32_t *first, int n,
+                       void *k_out, void *v_out, int out_dtype, int64_t out_token_stride, int64_t out_head_stride, int n_rows, void *stream);
 int  msnh_b200_kv_fork(MsnhB200Ctx *ctx, const MsnhB200KvCache *cache, const int32_t *src, const int32_t *dst, int n,
                        void *workspace, size_t workspace_bytes, void *stream);
 int  msnh_b200_kv_free(MsnhB200Ctx *ctx, const MsnhB200KvCache *cache, const int32_t *seqs, int n, void *stream);

@@ -98,14 +98,15 @@ class KvCache(C.Structure):
     _fields_ = [("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("k_page_stride", C.c_int64), ("k_token_stride", C.c_int64), ("k_head_stride", C.c_int64),
                 ("v_page_stride", C.c_int64), ("v_token_stride", C.c_int64), ("v_head_stride", C.c_int64), ("page_table", C.c_void_p), ("lengths", C.c_void_p),
                 ("refs", C.c_void_p), ("refused", C.c_void_p), ("table_stride", C.c_int64), ("n_pages", C.c_int32), ("page_size", C.c_int32),
-                ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("n_seqs", C.c_int32), ("max_pages", C.c_int32), ("dtype", C.c_int32)]
+                ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("n_seqs", C.c_int32), ("max_pages", C.c_int32), ("dtype", C.c_int32), ("k_scales", C.c_void_p),
+                ("v_scales", C.c_void_p), ("scale_block", C.c_int32)]
 
 
 class AttnDecode(C.Structure):
     """MsnhB200AttnDecode"""
     _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p), ("seqs", C.c_void_p), ("rows", C.c_int32), ("n_heads", C.c_int32),
                 ("q_row_stride", C.c_int64), ("q_head_stride", C.c_int64), ("out_row_stride", C.c_int64), ("out_head_stride", C.c_int64), ("scale", C.c_float),
-                ("window", C.c_int32), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+                ("window", C.c_int32), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("dtype", C.c_int32)]
 
 
 class Rotary(C.Structure):
@@ -183,6 +184,8 @@ def kernel_lib():
     lib.msnh_b200_attn_decode.argtypes = [vp, C.POINTER(KvCache), C.POINTER(AttnDecode), vp]
     lib.msnh_b200_kv_workspace.argtypes = [vp, C.POINTER(KvCache), i32, szp]
     lib.msnh_b200_kv_append.argtypes = [vp, C.POINTER(KvCache), vp, vp, i32, vp, vp, i64, i64, i32, vp, C.c_size_t, vp]
+    lib.msnh_b200_kv_append_as.argtypes = [vp, C.POINTER(KvCache), vp, vp, i32, vp, vp, i32, i64, i64, i32, vp, C.c_size_t, vp]
+    lib.msnh_b200_kv_read.argtypes = [vp, C.POINTER(KvCache), vp, vp, vp, i32, vp, vp, i32, i64, i64, i32, vp]
     lib.msnh_b200_kv_fork.argtypes = [vp, C.POINTER(KvCache), vp, vp, i32, vp, C.c_size_t, vp]
     lib.msnh_b200_kv_free.argtypes = [vp, C.POINTER(KvCache), vp, i32, vp]
     lib.msnh_b200_kv_compact.argtypes = [vp, C.POINTER(KvCache), vp, vp, vp, C.c_size_t, vp]
@@ -207,7 +210,7 @@ KERNEL_SYMBOLS = [
     "msnh_b200_rms_norm", "msnh_b200_w4_pack_bytes", "msnh_b200_w4_pack", "msnh_b200_w4_linear_workspace", "msnh_b200_w4_linear",
     "msnh_b200_attn_decode_workspace", "msnh_b200_attn_decode", "msnh_b200_kv_workspace", "msnh_b200_kv_append", "msnh_b200_kv_fork",
     "msnh_b200_kv_free", "msnh_b200_kv_compact", "msnh_b200_kv_copy_pages",
-    "msnh_b200_rotary", "msnh_b200_token_scores",
+    "msnh_b200_kv_append_as", "msnh_b200_kv_read", "msnh_b200_rotary", "msnh_b200_token_scores",
 ]
 
 

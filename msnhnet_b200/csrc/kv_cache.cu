@@ -1,4 +1,4 @@
-// Upkeep of a paged cache of keys and values: append, fork, free, compact, copy (msnh_b200_kv_*).
+// Upkeep of a paged cache of keys and values: append, fork, free, compact, copy, read (msnh_b200_kv_*).
 //
 // Append, fork and compact are two launches: one block decides (which pages, in what order: the lowest free ones first, by a scan
 // over the page counts, so the result does not depend on timing) and writes its decisions into the workspace, then a grid moves the
@@ -77,15 +77,17 @@ __device__ int lowest_free(const KvParams &c, int need, int *list) {
 }
 
 // What append decides for a sequence of the call.
-struct AppendWork { int first, need, had, start; };              // first of its pages in the list; start: the length before, -1: refused
+struct AppendWork { int first, need, had, start, block; };       // first of its pages in the list; start: the length before, -1: refused;
+                                                                 // block: the blocks of scales that sequences before it write to (codes only)
 
 __global__ void kv_append_decide_kernel(KvParams c, const int *seqs, const int *starts, int n, int n_tokens, AppendWork *work, int *list) {
     pdl_enter();
-    int all = 0;
+    int all = 0, all_blocks = 0;
     bool down = false;                                           // starts that are not in order: then no token's sequence is certain
     for (int base = 0; base < n; base += kDecide) {
         const int i = base + threadIdx.x;
-        AppendWork w = {0, 0, 0, -1};
+        AppendWork w = {0, 0, 0, -1, 0};
+        int blocks = 0;
         if (i < n) {
             const int s = seqs ? seqs[i] : i;
             const long long from = starts ? starts[i] : i, to = starts ? starts[i + 1] : i + 1;
@@ -93,13 +95,20 @@ __global__ void kv_append_decide_kernel(KvParams c, const int *seqs, const int *
             if (s >= 0 && s < c.n_seqs && from >= 0 && to >= from && to <= n_tokens) {
                 const long long len = max(c.lengths[s], 0), had = (len + c.page_size - 1) / c.page_size;
                 const long long want = (len + to - from + c.page_size - 1) / c.page_size;
-                if (want <= c.max_pages) w = {0, static_cast<int>(want - had), static_cast<int>(had), static_cast<int>(len)};
+                if (want <= c.max_pages) {
+                    w = {0, static_cast<int>(want - had), static_cast<int>(had), static_cast<int>(len), 0};
+                    if (c.block && to > from) blocks = static_cast<int>((len + to - from - 1) / c.block - len / c.block + 1);
+                }
             }
         }
         int total;
         w.first = all + block_scan(w.need, &total);
-        if (i < n) work[i] = w;
         all += total;
+        if (c.block && starts) {
+            w.block = all_blocks + block_scan(blocks, &total);
+            all_blocks += total;
+        }
+        if (i < n) work[i] = w;
     }
     const int found = lowest_free(c, all, list);
     if (starts) down = __syncthreads_or(down);
@@ -153,6 +162,255 @@ __global__ void kv_append_write_kernel(KvParams c, const int *seqs, const int *s
         const int place = at % c.page_size;
         reinterpret_cast<Unit *>(c.k)[page * c.k_page + place * c.k_token + head * c.k_head + unit] = k_new[token * token_stride + head * head_stride + unit];
         reinterpret_cast<Unit *>(c.v)[page * c.v_page + place * c.v_token + head * c.v_head + unit] = v_new[token * token_stride + head * head_stride + unit];
+    }
+}
+
+// The last of n sequences whose number at(i) is not above x, for a whole warp: at(0), at(1), ... do not fall. Always one of them.
+template <typename At> __device__ __forceinline__ int last_not_above(int n, int x, int lane, At at) {
+    int low = 0, range = n;
+    while (range > 1) {
+        const int step = (range + 31) / 32, probe = low + lane * step;
+        const unsigned below = __ballot_sync(~0u, lane * step < range && at(probe) <= x);
+        const int which = below ? 31 - __clz(below) : 0;
+        low += which * step;
+        range = min(step, range - which * step);
+    }
+    return low;
+}
+
+template <int kVec> __device__ __forceinline__ void store_codes(uint8_t *to, const float (&x)[kVec]) {
+    if constexpr (kVec == 1) {
+        to[0] = static_cast<uint8_t>(to_e4m3x2(x[0], 0.f));
+    } else {
+        uint32_t words[kVec / 4];
+#pragma unroll
+        for (int i = 0; i < kVec / 4; ++i) words[i] = to_e4m3x2(x[4 * i], x[4 * i + 1]) | static_cast<uint32_t>(to_e4m3x2(x[4 * i + 2], x[4 * i + 3])) << 16;
+        if constexpr (kVec == 8) *reinterpret_cast<uint2 *>(to) = make_uint2(words[0], words[1]);
+        else *reinterpret_cast<uint32_t *>(to) = words[0];
+    }
+}
+// kVec values side by side, and as many codes
+template <typename T, int kVec> struct Piece {
+    alignas(16) T v[kVec];
+    __device__ __forceinline__ void load(const T *from) {
+        if constexpr (kVec > 1) *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(from);
+        else v[0] = from[0];
+    }
+    // the larger one of `before` and the magnitudes' bits, of all or of finite ones
+    __device__ __forceinline__ uint32_t top(uint32_t before, bool all) const {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+            const uint32_t bits = __float_as_uint(to_float(v[i])) & 0x7fffffffu;
+            if (all || bits < 0x7f800000u) before = max(before, bits);
+        }
+        return before;
+    }
+    template <typename Code> __device__ __forceinline__ void store(uint8_t *to, Code code) const {
+        float x[kVec];
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) x[i] = code(to_float(v[i]));
+        store_codes<kVec>(to, x);
+    }
+};
+template <int kVec> struct Codes {
+    alignas(8) __nv_fp8_e4m3 v[kVec];
+    __device__ __forceinline__ void load(const uint8_t *from) {
+        if constexpr (kVec == 8) *reinterpret_cast<uint2 *>(v) = *reinterpret_cast<const uint2 *>(from);
+        else if constexpr (kVec == 4) *reinterpret_cast<uint32_t *>(v) = *reinterpret_cast<const uint32_t *>(from);
+        else v[0].__x = *from;
+    }
+    template <typename Code> __device__ __forceinline__ void store(uint8_t *to, Code code) const {
+        float x[kVec];
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) x[i] = code(to_float(v[i]));
+        store_codes<kVec>(to, x);
+    }
+};
+
+// The smallest power of two by which a magnitude (its bits) is at most 448 = 1.75 * 2^8, from 2^-126 on; 0 for 0.
+__device__ __forceinline__ float scale_of(uint32_t top) {
+    if (top == 0) return 0.f;
+    const int exponent = static_cast<int>((top + 0x1fffffu) >> 23) - 8;      // (biased; mantissas above 1.75 carry)
+    return __uint_as_float(static_cast<uint32_t>(max(exponent, 1)) << 23);
+}
+// Whether x / scale is x times the scale's reciprocal, exactly.
+__device__ __forceinline__ bool is_power(float scale) {
+    const uint32_t bits = __float_as_uint(scale);
+    return (bits & 0x807fffffu) == 0 && bits >= 0x00800000u && bits <= 0x7e800000u;
+}
+
+constexpr int kHeld = 8;               // pieces of new values that a lane keeps between the maximum and the codes
+
+// A warp for the call's tokens in one block of scales of one head, keys or values: their largest magnitude, the scale, the block's older
+// codes by the new scale where that has grown, the new codes.
+template <typename T, int kVec>
+__global__ void __launch_bounds__(256) kv_append_codes_kernel(KvParams c, const int *seqs, const int *starts, int n, const AppendWork *work, const T *k_new, const T *v_new,
+                                                              long long token_stride, long long head_stride, long long most_blocks) {
+    pdl_enter();
+    const int lane = threadIdx.x % 32, vecs = c.dim / kVec, down = 32 / vecs, right = 32 % vecs;
+    const long long total = most_blocks * c.heads * 2;
+    for (long long w = (blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x) / 32; w < total; w += static_cast<long long>(gridDim.x) * blockDim.x / 32) {
+        const long long pair = w / c.heads;
+        const int head = static_cast<int>(w - pair * c.heads), unit = static_cast<int>(pair / 2);
+        const bool values = pair % 2;
+        const int i = starts ? last_not_above(n, unit, lane, [&](int at) { return work[at].block; }) : unit;
+        const int before = work[i].start, first = starts ? starts[i] : i, count = starts ? starts[i + 1] - first : 1;
+        if (before < 0 || count <= 0) continue;
+        const long long block = before / c.block + (starts ? unit - work[i].block : 0), begin = block * c.block;
+        const long long last = min(begin + c.block, before + static_cast<long long>(count));
+        if (last <= begin) continue;                             // (the bound on blocks is not reached)
+        const int from = static_cast<int>(max(begin, static_cast<long long>(before))), to = static_cast<int>(last);
+        const int page = c.table[(seqs ? seqs[i] : i) * c.table_stride + from / c.page_size];
+        if (page < 0 || page >= c.n_pages) continue;
+        const int place = from % c.page_size, older = from - static_cast<int>(begin);
+        const long long token_step = values ? c.v_token : c.k_token;
+        uint8_t *codes = values ? c.v + page * c.v_page + head * c.v_head + place * c.v_token : c.k + page * c.k_page + head * c.k_head + place * c.k_token;
+        float *scale_at = (values ? c.v_scales : c.k_scales) + (static_cast<long long>(page) * c.heads + head) * c.blocks + place / c.block;
+        const float had = older ? *scale_at : 0.f;
+        const T *source = (values ? v_new : k_new) + (first + from - before) * token_stride + head * head_stride;
+        const int pieces = (to - from) * vecs;
+
+        Piece<T, kVec> held[kHeld];
+        const int row0 = lane / vecs, column0 = lane - row0 * vecs;
+        int row = row0, column = column0;
+        const auto step = [&] {
+            row += down;
+            column += right;
+            if (column >= vecs) { column -= vecs; ++row; }
+        };
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) {
+            if (lane + 32 * j < pieces) held[j].load(source + row * token_stride + column * kVec);
+            step();
+        }
+        const int row_more = row, column_more = column;
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j)
+            if (lane + 32 * j < pieces) top = held[j].top(top, true);
+        for (int at = lane + 32 * kHeld; at < pieces; at += 32) {
+            Piece<T, kVec> p;
+            p.load(source + row * token_stride + column * kVec);
+            top = p.top(top, true);
+            step();
+        }
+        top = __reduce_max_sync(~0u, top);
+        const bool odd = top >= 0x7f800000u;                     // a NaN or infinity: once more without them
+        if (odd) {
+            top = 0;
+            row = row0;
+            column = column0;
+            for (int at = lane; at < pieces; at += 32) {
+                Piece<T, kVec> p;
+                p.load(source + row * token_stride + column * kVec);
+                top = p.top(top, false);
+                step();
+            }
+            top = __reduce_max_sync(~0u, top);
+        }
+        const float scale = fmaxf(had, scale_of(top));
+        const bool power = is_power(scale);
+        const float inverse = power ? 1.f / scale : 0.f;
+        if (older && scale != had) {
+            const auto again = [&](float x) { return power ? x * had * inverse : x * had / scale; };
+            uint8_t *old = codes - older * token_step;
+            row = row0;
+            column = column0;
+            for (int at = lane; at < older * vecs; at += 32) {
+                uint8_t *one = old + row * token_step + column * kVec;
+                Codes<kVec> p;
+                p.load(one);
+                p.store(one, again);
+                step();
+            }
+        }
+        const auto code = [&](float x) {
+            if (odd && !isfinite(x)) return __uint_as_float(0x7fffffffu);
+            return power ? x * inverse : scale == 0.f ? 0.f * x : x / scale;
+        };
+        row = row0;
+        column = column0;
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) {
+            if (lane + 32 * j < pieces) held[j].store(codes + row * token_step + column * kVec, code);
+            step();
+        }
+        row = row_more;
+        column = column_more;
+        for (int at = lane + 32 * kHeld; at < pieces; at += 32) {
+            Piece<T, kVec> p;
+            p.load(source + row * token_stride + column * kVec);
+            p.store(codes + row * token_step + column * kVec, code);
+            step();
+        }
+        if (lane == 0) *scale_at = scale;
+    }
+}
+
+// kVec values side by side of one type to another, times a scale
+template <typename In, typename Out, int kVec> __device__ __forceinline__ void convert(Out *to, const In *from, float scale) {
+    alignas(16) In in[kVec];
+    alignas(16) Out out[kVec];
+    if constexpr (kVec == 1) {
+        in[0] = from[0];
+    } else if constexpr (sizeof(in) == 8) {
+        *reinterpret_cast<uint2 *>(in) = *reinterpret_cast<const uint2 *>(from);
+    } else {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(in)) / 16; ++i) reinterpret_cast<uint4 *>(in)[i] = reinterpret_cast<const uint4 *>(from)[i];
+    }
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) out[i] = from_float<Out>(sizeof(In) == 1 ? to_float(in[i]) * scale : to_float(in[i]));
+    if constexpr (kVec == 1) {
+        to[0] = out[0];
+    } else {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(out)) / 16; ++i) reinterpret_cast<uint4 *>(to)[i] = reinterpret_cast<const uint4 *>(out)[i];
+    }
+}
+
+// A warp a row of the output: keys and values of all heads of one token.
+template <typename In, typename Out, int kVec>
+__global__ void __launch_bounds__(256) kv_read_kernel(KvParams c, const int *seqs, const int *starts, const int *firsts, int n, Out *k_out, Out *v_out, long long token_stride,
+                                                      long long head_stride, int n_rows) {
+    pdl_enter();
+    const int lane = threadIdx.x % 32, vecs = c.dim / kVec;
+    for (long long row = (blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x) / 32; row < n_rows; row += static_cast<long long>(gridDim.x) * blockDim.x / 32) {
+        int page = -1;
+        long long at = 0;
+        if (n > 0) {
+            const int r = static_cast<int>(row), i = last_not_above(n, r, lane, [&](int at) { return starts[at]; });
+            const int s = seqs ? seqs[i] : i;
+            if (r >= starts[i] && r < starts[i + 1] && s >= 0 && s < c.n_seqs) {
+                at = static_cast<long long>(r) - starts[i] + (firsts ? firsts[i] : 0);
+                if (at >= 0 && at < min(static_cast<long long>(c.lengths[s]), static_cast<long long>(c.max_pages) * c.page_size)) page = c.table[s * c.table_stride + at / c.page_size];
+            }
+        }
+        const bool there = page >= 0 && page < c.n_pages;
+        const int place = there ? static_cast<int>(at % c.page_size) : 0;
+        const In *k = reinterpret_cast<const In *>(c.k) + (there ? page * c.k_page + place * c.k_token : 0), *v = reinterpret_cast<const In *>(c.v) + (there ? page * c.v_page + place * c.v_token : 0);
+        Out *k_to = k_out + row * token_stride, *v_to = v_out + row * token_stride;
+        const long long scales = sizeof(In) == 1 && there ? static_cast<long long>(page) * c.heads * c.blocks + place / c.block : 0;
+        for (int u = lane; u < c.heads * vecs; u += 32) {
+            const int head = u / vecs, d = (u - head * vecs) * kVec;
+            if (there) {
+                convert<In, Out, kVec>(k_to + head * head_stride + d, k + head * c.k_head + d, sizeof(In) == 1 ? c.k_scales[scales + static_cast<long long>(head) * c.blocks] : 1.f);
+                convert<In, Out, kVec>(v_to + head * head_stride + d, v + head * c.v_head + d, sizeof(In) == 1 ? c.v_scales[scales + static_cast<long long>(head) * c.blocks] : 1.f);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kVec; ++i) k_to[head * head_stride + d + i] = v_to[head * head_stride + d + i] = from_float<Out>(0.f);
+            }
+        }
+    }
+}
+
+// The scales of the first `blocks` blocks of page src to page dst, by threads first, first + step, ...
+__device__ __forceinline__ void copy_scales(const KvParams &c, int src, int dst, int blocks, int first, int step) {
+    const long long from = static_cast<long long>(src) * c.heads * c.blocks, to = static_cast<long long>(dst) * c.heads * c.blocks;
+    for (int i = first; i < c.heads * blocks; i += step) {
+        const int at = i / blocks * c.blocks + i % blocks;
+        c.k_scales[to + at] = c.k_scales[from + at];
+        c.v_scales[to + at] = c.v_scales[from + at];
     }
 }
 
@@ -251,7 +509,10 @@ __global__ void kv_fork_copy_kernel(KvParams c, const int *src, const int *dst, 
         c.table[b + j] = page;
         if (page >= 0 && page < c.n_pages) atomicAdd(&c.refs[page], 1);
     }
-    if (w.to >= 0) copy_units<Unit>(c, w.from, w.to, units, first, step, w.rows * c.heads * units);
+    if (w.to >= 0) {
+        copy_units<Unit>(c, w.from, w.to, units, first, step, w.rows * c.heads * units);
+        if (c.block) copy_scales(c, w.from, w.to, (w.rows + c.block - 1) / c.block, first, step);
+    }
 }
 
 __global__ void kv_free_kernel(KvParams c, const int *seqs) {
@@ -347,6 +608,7 @@ __global__ void kv_compact_move_kernel(KvParams c, int *work, int *table_out, in
             refs_out[to] = c.refs[from];
             refs_out[from] = 0;
         }
+        if (first == 0 && c.block) copy_scales(c, from, to, c.blocks, threadIdx.x, blockDim.x);
         copy_units<Unit>(c, from, to, units, first + threadIdx.x, blockDim.x, min(total, first + kPiece));
     }
 }
@@ -361,6 +623,7 @@ __global__ void kv_copy_pages_kernel(KvParams c, const int *src, const int *dst,
             continue;
         }
         copy_units<Unit>(c, a, b, units, threadIdx.x, blockDim.x, c.page_size * c.heads * units);
+        if (c.block) copy_scales(c, a, b, c.blocks, threadIdx.x, blockDim.x);
     }
 }
 
@@ -402,9 +665,16 @@ int msnh_b200_kv_workspace(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, int n, si
 } catch (...) { return caught(ctx); }
 
 int msnh_b200_kv_append(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, const int32_t *seqs, const int32_t *starts, int n, const void *k_new, const void *v_new,
-                        int64_t new_token_stride, int64_t new_head_stride, int n_tokens, void *workspace, size_t workspace_bytes, void *stream) try {
+                        int64_t new_token_stride, int64_t new_head_stride, int n_tokens, void *workspace, size_t workspace_bytes, void *stream) {
+    return msnh_b200_kv_append_as(ctx, c, seqs, starts, n, k_new, v_new, c ? c->dtype : 0, new_token_stride, new_head_stride, n_tokens, workspace, workspace_bytes, stream);
+}
+
+int msnh_b200_kv_append_as(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, const int32_t *seqs, const int32_t *starts, int n, const void *k_new, const void *v_new, int new_dtype,
+                           int64_t new_token_stride, int64_t new_head_stride, int n_tokens, void *workspace, size_t workspace_bytes, void *stream) try {
     if (!ctx || !c) return MSNH_B200_ERR_ARG;
     if (const int rc = check_cache(ctx, c, true, "kv_append")) return rc;
+    const bool codes = c->dtype == MSNH_B200_E4M3;
+    if (codes ? !is_float_type(new_dtype) : new_dtype != c->dtype) return fail(ctx, MSNH_B200_ERR_ARG, "kv_append: values of type %d for a cache of type %d", new_dtype, c->dtype);
     if (n < 0 || n_tokens < 0) return fail(ctx, MSNH_B200_ERR_ARG, "kv_append: %d sequences, %d tokens", n, n_tokens);
     if (!starts && n_tokens != n) return fail(ctx, MSNH_B200_ERR_ARG, "kv_append: %d tokens for %d sequences without starts", n_tokens, n);
     if (!seqs && n > c->n_seqs) return fail(ctx, MSNH_B200_ERR_ARG, "kv_append: %d sequences of %d", n, c->n_seqs);
@@ -412,6 +682,9 @@ int msnh_b200_kv_append(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, const int32_
     if (n_tokens > 0 && (!k_new || !v_new)) return fail(ctx, MSNH_B200_ERR_ARG, "kv_append: null k_new or v_new");
     if (new_token_stride < 0 || new_head_stride < 0) return fail(ctx, MSNH_B200_ERR_ARG, "kv_append: a stride is negative");
     if (const int rc = check_workspace(ctx, *c, n, workspace, workspace_bytes, "kv_append")) return rc;
+    // blocks of scales that n_tokens tokens of n sequences lie in, at most
+    const long long most_blocks = codes ? starts ? n_tokens / c->scale_block + 2LL * std::min(n, n_tokens) : n : 0;
+    if (most_blocks > 0x7fffffff) return fail(ctx, MSNH_B200_ERR_UNSUPPORTED, "kv_append: 2^31 blocks of scales and more");
     DeviceScope scope(ctx->device);
     CUDA_TRY(ctx, scope.status);
     AppendWork *work = static_cast<AppendWork *>(workspace);
@@ -419,8 +692,24 @@ int msnh_b200_kv_append(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, const int32_
     const KvParams p = kv_params(*c);
     CUDA_TRY(ctx, launch_token_kernel(kv_append_decide_kernel, dim3(1), kDecide, 0, stream, ctx->pdl, p, seqs, starts, n, n_tokens, work, list));
     if (n_tokens == 0) return MSNH_B200_OK;
-    const size_t size = dtype_size(c->dtype);
-    const bool wide = kv_rows_multiple_of(*c, 16) && aligned16(k_new) && aligned16(v_new) && new_token_stride * size % 16 == 0 && new_head_stride * size % 16 == 0;
+    const size_t size = dtype_size(new_dtype);
+    const bool aligned = aligned16(k_new) && aligned16(v_new) && new_token_stride * size % 16 == 0 && new_head_stride * size % 16 == 0;
+    if (codes) {
+        const dim3 grid(blocks_for(ctx, most_blocks * c->n_kv_heads * 2, 8));
+        const auto write = [&](auto type, auto vec) {
+            using T = decltype(type);
+            constexpr int kVec = decltype(vec)::value;
+            return launch_token_kernel(kv_append_codes_kernel<T, kVec>, grid, 256, 0, stream, ctx->pdl, p, seqs, starts, n, work, static_cast<const T *>(k_new), static_cast<const T *>(v_new),
+                                       new_token_stride, new_head_stride, most_blocks);
+        };
+        const bool wide = aligned && kv_rows_multiple_of(*c, 16 / size);
+        const auto by_type = [&](auto type) {
+            return wide ? write(type, std::integral_constant<int, 16 / sizeof(type)>()) : write(type, std::integral_constant<int, 1>());
+        };
+        CUDA_TRY(ctx, new_dtype == MSNH_B200_F32 ? by_type(float()) : new_dtype == MSNH_B200_F16 ? by_type(__half()) : by_type(__nv_bfloat16()));
+        return MSNH_B200_OK;
+    }
+    const bool wide = aligned && kv_rows_multiple_of(*c, 16);
     int units;
     const KvParams q = in_units(p, size, wide ? 16 : size, &units);
     const long long per = wide ? static_cast<long long>(16 / size) : 1;
@@ -431,6 +720,35 @@ int msnh_b200_kv_append(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, const int32_
                                    static_cast<const Unit *>(v_new), new_token_stride / per, new_head_stride / per, units);
     };
     CUDA_TRY(ctx, wide ? write(uint4()) : size == 4 ? write(uint32_t()) : write(uint16_t()));
+    return MSNH_B200_OK;
+} catch (...) { return caught(ctx); }
+
+int msnh_b200_kv_read(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, const int32_t *seqs, const int32_t *starts, const int32_t *first, int n, void *k_out, void *v_out, int out_dtype,
+                      int64_t out_token_stride, int64_t out_head_stride, int n_rows, void *stream) try {
+    if (!ctx || !c) return MSNH_B200_ERR_ARG;
+    if (const int rc = check_cache(ctx, c, false, "kv_read")) return rc;
+    if (!is_float_type(out_dtype)) return fail(ctx, MSNH_B200_ERR_UNSUPPORTED, "kv_read: values of type %d", out_dtype);
+    if (n < 0 || n_rows < 0) return fail(ctx, MSNH_B200_ERR_ARG, "kv_read: %d sequences, %d rows", n, n_rows);
+    if (!seqs && n > c->n_seqs) return fail(ctx, MSNH_B200_ERR_ARG, "kv_read: %d sequences of %d", n, c->n_seqs);
+    if (n_rows == 0) return MSNH_B200_OK;
+    if (!k_out || !v_out || (n && !starts)) return fail(ctx, MSNH_B200_ERR_ARG, "kv_read: null k_out, v_out or starts");
+    if ((n_rows > 1 && out_token_stride < c->head_dim) || (c->n_kv_heads > 1 && out_head_stride < c->head_dim)) return fail(ctx, MSNH_B200_ERR_ARG, "kv_read: rows of the output overlap");
+    DeviceScope scope(ctx->device);
+    CUDA_TRY(ctx, scope.status);
+    const KvParams p = kv_params(*c);
+    const size_t size = dtype_size(out_dtype);
+    constexpr int kVec = 8;
+    const bool wide = c->head_dim % kVec == 0 && aligned16(k_out) && aligned16(v_out) && out_token_stride * size % 16 == 0 && out_head_stride * size % 16 == 0 &&
+                      kv_rows_multiple_of(*c, c->dtype == MSNH_B200_E4M3 ? 8 : 16);
+    const dim3 grid(blocks_for(ctx, n_rows, 8));
+    const auto read = [&](auto in, auto out) {
+        using In = decltype(in);
+        using Out = decltype(out);
+        return launch_token_kernel(wide ? kv_read_kernel<In, Out, kVec> : kv_read_kernel<In, Out, 1>, grid, 256, 0, stream, ctx->pdl, p, seqs, starts, first, n, static_cast<Out *>(k_out),
+                                   static_cast<Out *>(v_out), out_token_stride, out_head_stride, n_rows);
+    };
+    const auto from = [&](auto in) { return out_dtype == MSNH_B200_F32 ? read(in, float()) : out_dtype == MSNH_B200_F16 ? read(in, __half()) : read(in, __nv_bfloat16()); };
+    CUDA_TRY(ctx, c->dtype == MSNH_B200_F32 ? from(float()) : c->dtype == MSNH_B200_F16 ? from(__half()) : c->dtype == MSNH_B200_BF16 ? from(__nv_bfloat16()) : from(__nv_fp8_e4m3()));
     return MSNH_B200_OK;
 } catch (...) { return caught(ctx); }
 
@@ -454,7 +772,7 @@ int msnh_b200_kv_fork(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, const int32_t 
     const KvParams q = in_units(p, size, wide ? 16 : size, &units);
     const dim3 grid(n, std::max(1, std::min(8, 2 * ctx->sm_count / n)));
     const auto copy = [&](auto unit) { return launch_token_kernel(kv_fork_copy_kernel<decltype(unit)>, grid, 256, 0, stream, ctx->pdl, q, src, dst, work, units); };
-    CUDA_TRY(ctx, wide ? copy(uint4()) : size == 4 ? copy(uint32_t()) : copy(uint16_t()));
+    CUDA_TRY(ctx, wide ? copy(uint4()) : size == 4 ? copy(uint32_t()) : size == 2 ? copy(uint16_t()) : copy(uint8_t()));
     return MSNH_B200_OK;
 } catch (...) { return caught(ctx); }
 
@@ -487,7 +805,7 @@ int msnh_b200_kv_compact(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, int32_t *ta
     const KvParams q = in_units(p, size, wide ? 16 : size, &units);
     const dim3 grid(blocks_for(ctx, std::max<long long>(c->n_pages, static_cast<long long>(c->n_seqs) * c->max_pages / 256), 1));
     const auto move = [&](auto unit) { return launch_token_kernel(kv_compact_move_kernel<decltype(unit)>, grid, 256, 0, stream, ctx->pdl, q, work, table_out, refs_out, units); };
-    CUDA_TRY(ctx, wide ? move(uint4()) : size == 4 ? move(uint32_t()) : move(uint16_t()));
+    CUDA_TRY(ctx, wide ? move(uint4()) : size == 4 ? move(uint32_t()) : size == 2 ? move(uint16_t()) : move(uint8_t()));
     return MSNH_B200_OK;
 } catch (...) { return caught(ctx); }
 
@@ -505,7 +823,7 @@ int msnh_b200_kv_copy_pages(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, const in
     const KvParams q = in_units(kv_params(*c), size, wide ? 16 : size, &units);
     const dim3 grid(blocks_for(ctx, n, 1));
     const auto copy = [&](auto unit) { return launch_token_kernel(kv_copy_pages_kernel<decltype(unit)>, grid, 256, 0, stream, ctx->pdl, q, src, dst, n, units); };
-    CUDA_TRY(ctx, wide ? copy(uint4()) : size == 4 ? copy(uint32_t()) : copy(uint16_t()));
+    CUDA_TRY(ctx, wide ? copy(uint4()) : size == 4 ? copy(uint32_t()) : size == 2 ? copy(uint16_t()) : copy(uint8_t()));
     return MSNH_B200_OK;
 } catch (...) { return caught(ctx); }
 

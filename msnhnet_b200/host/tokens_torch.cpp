@@ -17,6 +17,7 @@
 #include <cmath>
 #include <exception>
 #include <string>
+#include <vector>
 
 #include "msnh_b200.h"
 
@@ -272,15 +273,18 @@ PyObject *token_scores(PyObject *, PyObject *const *args, Py_ssize_t n) {
     });
 }
 
+// The type that values beside a cache have: the cache's own, or any floating one beside 8-bit codes.
+at::ScalarType fitting(at::ScalarType cache, at::ScalarType given) { return cache == at::kFloat8_e4m3fn && is_float(given) ? given : cache; }
+
 // q, address of the cache's struct, its k_pages, seqs or None, scale or None, window, out or None, whether lse is wanted
 PyObject *attn_decode(PyObject *, PyObject *const *args, Py_ssize_t n) {
     return guarded([&]() -> PyObject * {
         const Args a(args, n, 10);
         const at::Tensor &q = a.tensor(2, "q"), &pages = a.tensor(4, "the cache");
         const MsnhB200KvCache *cache = a.pointer<MsnhB200KvCache>(3);
-        const auto type = pages.scalar_type();
-        if (q.dim() != 3 || q.size(2) != cache->head_dim || q.scalar_type() != type || (q.stride(2) != 1 && q.size(2) > 1))
-            wrong("q: [rows, n_heads, " + std::to_string(cache->head_dim) + "] of the cache's type " + c10::toString(type));
+        const auto type = fitting(pages.scalar_type(), q.scalar_type());
+        if (q.dim() != 3 || q.size(2) != cache->head_dim || q.scalar_type() != type || !is_float(type) || (q.stride(2) != 1 && q.size(2) > 1))
+            wrong("q: [rows, n_heads, " + std::to_string(cache->head_dim) + "] of the cache's type " + c10::toString(pages.scalar_type()) + " (of a floating one over 8 bits)");
         const int64_t rows = q.size(0), heads = q.size(1);
         if (rows > INT32_MAX || heads > INT32_MAX) wrong("q: too many rows or heads");
         const at::Tensor *seqs = a.maybe(5, "seqs"), *given = a.maybe(8, "out");
@@ -295,7 +299,7 @@ PyObject *attn_decode(PyObject *, PyObject *const *args, Py_ssize_t n) {
                                    seqs ? static_cast<const int32_t *>(seqs->const_data_ptr()) : nullptr, static_cast<int32_t>(rows), static_cast<int32_t>(heads),
                                    q.stride(0), q.stride(1), out.stride(0), out.stride(1),
                                    args[6] == Py_None ? 1.f / std::sqrt(static_cast<float>(cache->head_dim)) : static_cast<float>(a.number(6)),
-                                   static_cast<int32_t>(window), nullptr, 0};
+                                   static_cast<int32_t>(window), nullptr, 0, type_of(type)};
         check(a.ctx, msnh_b200_attn_decode_workspace(a.ctx, cache, &call, &call.workspace_bytes));
         at::Tensor scratch;
         if (call.workspace_bytes) {
@@ -322,9 +326,10 @@ PyObject *kv_append(PyObject *, PyObject *const *args, Py_ssize_t n) {
         const Args a(args, n, 9);
         const MsnhB200KvCache *cache = a.pointer<MsnhB200KvCache>(2);
         const at::Tensor &pages = a.tensor(3, "the cache"), &k = a.tensor(5, "k"), &v = a.tensor(6, "v");
-        if (k.dim() != 3 || v.sizes() != k.sizes() || k.size(1) != cache->n_kv_heads || k.size(2) != cache->head_dim || k.scalar_type() != pages.scalar_type() ||
-            v.scalar_type() != k.scalar_type())
-            wrong("k, v: [tokens, " + std::to_string(cache->n_kv_heads) + ", " + std::to_string(cache->head_dim) + "] of the cache's type " + c10::toString(pages.scalar_type()));
+        if (k.dim() != 3 || v.sizes() != k.sizes() || k.size(1) != cache->n_kv_heads || k.size(2) != cache->head_dim || k.scalar_type() != fitting(pages.scalar_type(), k.scalar_type()) ||
+            v.scalar_type() != k.scalar_type() || !is_float(k.scalar_type()))
+            wrong("k, v: [tokens, " + std::to_string(cache->n_kv_heads) + ", " + std::to_string(cache->head_dim) + "] of the cache's type " + c10::toString(pages.scalar_type()) +
+                  " (of a floating one for 8 bits)");
         if (v.strides() != k.strides() || (k.stride(2) != 1 && k.size(2) > 1)) wrong("k, v: the same strides, the values of a head side by side");
         const at::Tensor *seqs = a.maybe(7, "seqs"), *starts = a.maybe(8, "starts");
         const int64_t tokens = k.size(0), count = !starts ? tokens : starts->dim() == 1 && starts->size(0) ? starts->size(0) - 1 : -1;
@@ -333,10 +338,43 @@ PyObject *kv_append(PyObject *, PyObject *const *args, Py_ssize_t n) {
         if (seqs) vector_of(*seqs, count, at::kInt, "seqs");
         if (tokens > INT32_MAX) wrong("k, v: too many tokens");
         const at::Tensor scratch = kv_scratch(a, cache, count);
-        check(a.ctx, msnh_b200_kv_append(a.ctx, cache, seqs ? ints(*seqs) : nullptr, starts ? ints(*starts) : nullptr, static_cast<int>(count), k.const_data_ptr(),
-                                         v.const_data_ptr(), k.stride(0), k.stride(1), static_cast<int>(tokens), scratch.mutable_data_ptr(), scratch.numel(), a.stream()));
+        check(a.ctx, msnh_b200_kv_append_as(a.ctx, cache, seqs ? ints(*seqs) : nullptr, starts ? ints(*starts) : nullptr, static_cast<int>(count), k.const_data_ptr(),
+                                            v.const_data_ptr(), type_of(k.scalar_type()), k.stride(0), k.stride(1), static_cast<int>(tokens), scratch.mutable_data_ptr(), scratch.numel(),
+                                            a.stream()));
         a.writes_cache(4);
         Py_RETURN_NONE;
+    });
+}
+
+// address of the cache's struct, its k_pages, starts, the number of rows, seqs or None, first or None, dtype or None, k_out or None, v_out or None
+PyObject *kv_read(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        const Args a(args, n, 11);
+        const MsnhB200KvCache *cache = a.pointer<MsnhB200KvCache>(2);
+        const at::Tensor &pages = a.tensor(3, "the cache"), &starts = a.tensor(4, "starts");
+        const int64_t rows = a.whole(5), count = starts.dim() == 1 && starts.size(0) ? starts.size(0) - 1 : -1;
+        if (count < 0) wrong("starts: one more than sequences");
+        vector_of(starts, count + 1, at::kInt, "starts");
+        if (rows < 0 || rows > INT32_MAX || count > INT32_MAX) wrong("kv_read: the number of tokens or sequences is out of range");
+        const at::Tensor *seqs = a.maybe(6, "seqs"), *first = a.maybe(7, "first"), *k = a.maybe(9, "out"), *v = a.maybe(10, "out");
+        if (seqs) vector_of(*seqs, count, at::kInt, "seqs");
+        if (first) vector_of(*first, count, at::kInt, "first");
+        if (!k != !v) wrong("out: keys and values");
+        const auto type = a.dtype(8, k ? k->scalar_type() : is_float(pages.scalar_type()) ? pages.scalar_type() : at::kHalf);
+        if (!is_float(type)) wrong(std::string("kv_read: a floating type is wanted, not ") + c10::toString(type));
+        const std::vector<int64_t> shape = {rows, cache->n_kv_heads, cache->head_dim};
+        if (k && (k->sizes() != shape || v->sizes() != shape || k->scalar_type() != type || v->scalar_type() != type || k->strides() != v->strides() ||
+                  (k->stride(2) != 1 && cache->head_dim > 1)))
+            wrong("out: keys and values [" + std::to_string(rows) + ", " + std::to_string(cache->n_kv_heads) + ", " + std::to_string(cache->head_dim) + "] of type " + c10::toString(type) +
+                  " and the same strides, the values of a head side by side");
+        const at::Tensor k_out = k ? *k : a.empty(shape, type), v_out = v ? *v : a.empty(shape, type);
+        check(a.ctx, msnh_b200_kv_read(a.ctx, cache, seqs ? ints(*seqs) : nullptr, ints(starts), first ? ints(*first) : nullptr, static_cast<int>(count), k_out.mutable_data_ptr(),
+                                       v_out.mutable_data_ptr(), type_of(type), k_out.stride(0), k_out.stride(1), static_cast<int>(rows), a.stream()));
+        if (k) {
+            a.writes(*k);
+            a.writes(*v);
+        }
+        return Py_BuildValue("(NN)", wrap(k_out), wrap(v_out));
     });
 }
 
@@ -413,7 +451,7 @@ template <PyObject *(*f)(PyObject *, PyObject *const *, Py_ssize_t)> PyMethodDef
 PyMethodDef kMethods[] = {method<rms_norm>("rms_norm"),   method<w4_linear>("w4_linear"),   method<attn_decode>("attn_decode"),
                           method<kv_append>("kv_append"), method<kv_fork>("kv_fork"),       method<kv_free>("kv_free"),
                           method<kv_compact>("kv_compact"), method<kv_copy_pages>("kv_copy_pages"),
-                          method<rotary>("rotary"),       method<token_scores>("token_scores"), {nullptr, nullptr, 0, nullptr}};
+                          method<rotary>("rotary"),       method<token_scores>("token_scores"), method<kv_read>("kv_read"), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_tokens", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -53,12 +53,14 @@ class RotaryTable:
 class PagedCache:
     """Keys and values in pages (MsnhB200KvCache), over tensors of the caller:
 
-    k_pages, v_pages  [n_pages, page_size, n_kv_heads, head_dim] (any strides but the last), float32, float16 or bfloat16
+    k_pages, v_pages  [n_pages, page_size, n_kv_heads, head_dim] (any strides but the last), float32, float16, bfloat16 or float8_e4m3fn
     page_table        int32 [n_seqs, max_pages]; lengths int32 [n_seqs]; refs int32 [n_pages]; all of them 0 in a fresh cache
+    k_scales, v_scales  for pages of float8_e4m3fn: float32 [n_pages, n_kv_heads, page_size / scale_block], what a code of a block of
+                      scale_block tokens of a page and head is taken times
     """
 
-    def __init__(self, k_pages, v_pages, page_table, lengths, refs):
-        if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype or k_pages.dtype not in _FLOATS:
+    def __init__(self, k_pages, v_pages, page_table, lengths, refs, k_scales=None, v_scales=None):
+        if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype or k_pages.dtype not in _DTYPE:
             raise ValueError("k_pages and v_pages: [n_pages, page_size, n_kv_heads, head_dim] of one floating type")
         if k_pages.stride(3) != 1 or v_pages.stride(3) != 1:
             raise ValueError("k_pages and v_pages: the values of a head lie side by side")
@@ -69,19 +71,34 @@ class PagedCache:
                 raise ValueError("page_table, lengths and refs are int32")
         if not lengths.is_contiguous() or not refs.is_contiguous():
             raise ValueError("lengths and refs are contiguous")
-        _no_gradient(k_pages, v_pages)
+        scales = (k_scales, v_scales)
+        self.scale_block = 0
+        if k_pages.dtype not in _FLOATS:
+            n_pages, page_size, heads, _ = k_pages.shape
+            if any(t is None or t.dim() != 3 or t.shape[:2] != (n_pages, heads) or t.shape != k_scales.shape or t.dtype != torch.float32 or not t.is_contiguous() for t in scales):
+                raise ValueError("k_scales and v_scales: contiguous float32 [n_pages, n_kv_heads, blocks of a page] beside 8-bit pages")
+            blocks = k_scales.shape[2]
+            if blocks < 1 or page_size % blocks:
+                raise ValueError(f"k_scales and v_scales: {blocks} blocks in pages of {page_size} tokens")
+            self.scale_block = page_size // blocks
+        elif any(t is not None for t in scales):
+            raise ValueError("k_scales and v_scales are of 8-bit pages")
+        scales = tuple(t for t in scales if t is not None)
+        _no_gradient(k_pages, v_pages, *scales)
         self.device = k_pages.device
-        if not k_pages.is_cuda or any(t.device != self.device for t in (v_pages, page_table, lengths, refs)):
+        if not k_pages.is_cuda or any(t.device != self.device for t in (v_pages, page_table, lengths, refs, *scales)):
             raise ValueError("the cache's tensors are on one GPU")
         self.k_pages, self.v_pages, self.page_table, self.lengths, self.refs = k_pages, v_pages, page_table, lengths, refs
+        self.k_scales, self.v_scales = k_scales, v_scales
         self.refused_count = torch.zeros(1, dtype=torch.int32, device=self.device)
-        self.tensors = k_pages, v_pages, page_table, lengths, refs, self.refused_count
+        self.tensors = k_pages, v_pages, page_table, lengths, refs, self.refused_count, *scales
         self.dtype = k_pages.dtype
         self.n_pages, self.page_size, self.n_kv_heads, self.head_dim = k_pages.shape
         self.n_seqs, self.max_pages = page_table.shape
         self.args = _ffi.KvCache(k_pages.data_ptr(), v_pages.data_ptr(), *k_pages.stride()[:3], *v_pages.stride()[:3], page_table.data_ptr(),
                                  lengths.data_ptr(), refs.data_ptr(), self.refused_count.data_ptr(), page_table.stride(0), self.n_pages,
-                                 self.page_size, self.n_kv_heads, self.head_dim, self.n_seqs, self.max_pages, _DTYPE[self.dtype])
+                                 self.page_size, self.n_kv_heads, self.head_dim, self.n_seqs, self.max_pages, _DTYPE[self.dtype],
+                                 *((k_scales.data_ptr(), v_scales.data_ptr(), self.scale_block) if scales else (None, None, 0)))
         self.ref = C.byref(self.args)
         self.address = C.addressof(self.args)
 
@@ -178,21 +195,40 @@ class TokenOps:
         (a NaN, +infinity, or only -infinity) has NaN throughout, and ids of -1."""
         return _tokens.token_scores(self._ctx, self._index, logits, ids, top)
 
-    def new_cache(self, n_pages, page_size, n_kv_heads, head_dim, n_seqs, max_pages, dtype=torch.float16):
-        """A fresh cache with memory of its own."""
+    def new_cache(self, n_pages, page_size, n_kv_heads, head_dim, n_seqs, max_pages, dtype=torch.float16, scale_block=None):
+        """A fresh cache with memory of its own. dtype float8_e4m3fn: half the memory, with a scale for each scale_block tokens of a page and head
+        (a divisor of page_size; without it the largest one of 16 that is)."""
+        if dtype == torch.float8_e4m3fn:
+            scale_block = math.gcd(16, page_size) if scale_block is None else scale_block
+            if scale_block < 1 or page_size % scale_block:
+                raise ValueError(f"scales of {scale_block} tokens in pages of {page_size}")
+        elif scale_block is not None:
+            raise ValueError("scale_block is of 8-bit pages")
         pages = [torch.zeros(n_pages, page_size, n_kv_heads, head_dim, dtype=dtype, device=self.device) for _ in range(2)]
         ints = [torch.zeros(*shape, dtype=torch.int32, device=self.device) for shape in ((n_seqs, max_pages), (n_seqs,), (n_pages,))]
-        return PagedCache(*pages, *ints)
+        if dtype != torch.float8_e4m3fn:
+            return PagedCache(*pages, *ints)
+        return PagedCache(*pages, *ints, *(torch.zeros(n_pages, n_kv_heads, page_size // scale_block, device=self.device) for _ in range(2)))
 
     def attn_decode(self, q, cache, seqs=None, scale=None, window=0, out=None, return_lse=False):
         """One query token a row: q [rows, n_heads, head_dim] over the cached tokens of sequence seqs[row] (int32; row without seqs); its last
-        `window` ones only where that is not 0. scale: 1 / sqrt(head_dim). Returns out, or (out, lse float32 [rows, n_heads])."""
+        `window` ones only where that is not 0. scale: 1 / sqrt(head_dim). Returns out, or (out, lse float32 [rows, n_heads]). q has the cache's
+        type; over 8 bits it may have any floating one, and out is of the same."""
         return _tokens.attn_decode(self._ctx, self._index, q, cache.address, cache.k_pages, seqs, scale, window, out, return_lse)
 
     def kv_append(self, cache, k, v, seqs=None, starts=None):
         """Tokens behind their sequences' own: k, v [tokens, n_kv_heads, head_dim]; one token for each of seqs (int32; without it for
-        sequences 0, 1, ...), or rows starts[i] to starts[i + 1] (int32, one more than sequences) for sequence seqs[i]."""
+        sequences 0, 1, ...), or rows starts[i] to starts[i + 1] (int32, one more than sequences) for sequence seqs[i]. k and v have the cache's
+        type; for 8 bits any floating one: they are quantised, by the smallest power of two that brings the values of a block of tokens and head
+        to 448 at most. A block that was begun keeps its scale, or takes a larger one with its older codes rounded again."""
         _tokens.kv_append(self._ctx, self._index, cache.address, cache.k_pages, cache.tensors, k, v, seqs, starts)
+
+    def kv_read(self, cache, starts, tokens, seqs=None, first=None, dtype=None, out=None):
+        """Keys and values as the cache holds them, (k, v) [tokens, n_kv_heads, head_dim]: rows starts[i] to starts[i + 1] (int32, one more than
+        sequences) are those of sequence seqs[i] (int32; i without it) from its token first[i] (int32; 0 without it) on. Rows of no sequence or
+        token are 0. dtype: the cache's, float16 for 8 bits; out: (k, v) to write into."""
+        k, v = (None, None) if out is None else out
+        return _tokens.kv_read(self._ctx, self._index, cache.address, cache.k_pages, starts, tokens, seqs, first, dtype, k, v)
 
     def kv_fork(self, cache, src, dst):
         """Sequences dst (int32, empty before) become copies of sequences src."""
