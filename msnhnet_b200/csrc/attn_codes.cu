@@ -32,12 +32,121 @@ __device__ __forceinline__ float load_shared(uint32_t at) {
     return v;
 }
 
-// Lane l holds, of a tile's scores, tokens l / 4 and l / 4 + 8 of heads 2 (l % 4) and + 1; of a block of 16 value columns the same two heads of
+// A warp's ring of tiles of 32 tokens: the codes of keys and values in rows of kDim bytes, then a scale for each key and value. A row's 16-byte pieces
+// are exchanged by its number, so that eight rows at one column lie in all the banks. What is not there is 0. Where eight tokens in a row lie in one page and are all seen (a run), a
+// lane works out where that run's rows are, for eight tiles at a time; a tile then takes a few shuffles.
+template <int kDim, int kStages> struct CodeRing {
+    static constexpr int kTile = kCodeTile, kRuns = kTile / 8, kAhead = 32 / kRuns;
+    static constexpr int kSide = kTile * kDim, kStage = 2 * kSide + 2 * kTile * 4, kBytes = kStages * kStage;
+    static constexpr int kPieces = kDim / 16;
+
+    // The piece of a row in which its column-th one lies.
+    static __device__ __forceinline__ int piece_of(int row, int column) {
+        return column ^ (kPieces % 8 == 0 ? row & 7 : kPieces % 4 == 0 ? row >> 1 & 3 : row >> 2 & 1);
+    }
+
+    const KvParams &c;
+    int *masks;                              // [kStages] bit t: token t of the tile takes part
+    uint32_t base;
+    int lane;
+    const uint8_t *k = nullptr, *v = nullptr;                    // of the key head
+    const float *k_scales = nullptr, *v_scales = nullptr;
+    const int *table = nullptr;              // of the sequence
+    int first = 0, last = 0, origin = 0;     // tokens that are seen; token of the piece's first tile
+    int next = -1;                           // a lane's page of one of the next runs, -1: no run
+    int page = -1, place = 0;                // of one of this time's runs
+    long long at_k = 0, at_v = 0;
+    unsigned runs = 0;                       // lanes that have one
+
+    __device__ __forceinline__ CodeRing(const KvParams &c_, int *masks_, uint32_t base_, int lane_) : c(c_), masks(masks_), base(base_), lane(lane_) {}
+
+    __device__ __forceinline__ void start(int head, const int *table_, int first_, int last_, int first_tile) {
+        k = c.k + head * c.k_head;
+        v = c.v + head * c.v_head;
+        k_scales = c.k_scales + static_cast<long long>(head) * c.blocks;
+        v_scales = c.v_scales + static_cast<long long>(head) * c.blocks;
+        table = table_;
+        first = first_;
+        last = last_;
+        origin = (first / kTile + first_tile) * kTile;
+    }
+    __device__ __forceinline__ void look_ahead(int first_tile, int tiles) {
+        next = -1;
+        const int token = origin + first_tile * kTile + lane * 8;
+        if (first_tile + lane / kRuns < tiles && c.page_size % 8 == 0 && token >= first && token + 8 <= last) {
+            next = table[token / c.page_size];
+            if (next >= c.n_pages) next = -1;
+        }
+    }
+    __device__ __forceinline__ void take_pages(int first_tile) {
+        page = next;
+        place = (origin + first_tile * kTile + lane * 8) % c.page_size;
+        at_k = page * c.k_page + place * c.k_token;
+        at_v = page * c.v_page + place * c.v_token;
+        runs = __ballot_sync(~0u, page >= 0);
+    }
+    __device__ __forceinline__ int block_of(int token_place) const {
+        return (c.block & (c.block - 1)) == 0 ? token_place >> (31 - __clz(c.block)) : token_place / c.block;
+    }
+    __device__ __forceinline__ void copy(int stage, int tile) const {
+        const uint32_t to = base + stage * kStage, to_scales = to + 2 * kSide + lane * 4;
+        const int from = tile % kAhead * kRuns;
+        if ((runs >> from & ((1u << kRuns) - 1)) == (1u << kRuns) - 1) {
+            const uint8_t *k_run[kRuns], *v_run[kRuns];
+#pragma unroll
+            for (int r = 0; r < kRuns; ++r) {
+                k_run[r] = k + __shfl_sync(~0u, at_k, from + r);
+                v_run[r] = v + __shfl_sync(~0u, at_v, from + r);
+            }
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                const int row = (lane + 32 * i) / kPieces, column = (lane + 32 * i) % kPieces;
+                constexpr int kRow = 8 * kPieces;                // pieces of a run
+                const int low = 32 * i / kRow, high = (32 * i + 31) / kRow;
+                const int inside = min(column, c.dim / 16 - 1) * 16;
+                const int bytes = column < c.dim / 16 ? 16 : 0;
+                const uint32_t at = to + row * kDim + piece_of(row, column) * 16;
+                copy16(at, (row / 8 == low ? k_run[low] : k_run[high]) + row % 8 * c.k_token + inside, bytes);
+                copy16(at + kSide, (row / 8 == low ? v_run[low] : v_run[high]) + row % 8 * c.v_token + inside, bytes);
+            }
+            const int its_page = __shfl_sync(~0u, page, from + lane / 8), its_place = __shfl_sync(~0u, place, from + lane / 8) + lane % 8;
+            const long long scale = static_cast<long long>(its_page) * (c.heads * c.blocks) + block_of(its_place);
+            copy4(to_scales, k_scales + scale, 4);
+            copy4(to_scales + kTile * 4, v_scales + scale, 4);
+            if (lane == 0) masks[stage] = -1;
+            return;
+        }
+        // any tile: a row's place from the lane that has its token
+        const int token = origin + tile * kTile + lane;
+        int its_page = -1;
+        if (token >= first && token < last) its_page = table[token / c.page_size];
+        const bool there = its_page >= 0 && its_page < c.n_pages;
+        const int its_place = token % c.page_size;
+        const long long row_k = there ? its_page * c.k_page + its_place * c.k_token : 0, row_v = there ? its_page * c.v_page + its_place * c.v_token : 0;
+        const long long scale = there ? static_cast<long long>(its_page) * (c.heads * c.blocks) + block_of(its_place) : 0;
+        copy4(to_scales, k_scales + scale, there ? 4 : 0);
+        copy4(to_scales + kTile * 4, v_scales + scale, there ? 4 : 0);
+        const unsigned mask = __ballot_sync(~0u, there);
+        if (lane == 0) masks[stage] = static_cast<int>(mask);
+#pragma unroll 1
+        for (int i = 0; i < kPieces; ++i) {
+            const int row = (lane + 32 * i) / kPieces, column = (lane + 32 * i) % kPieces;
+            const long long from_k = __shfl_sync(~0u, row_k, row), from_v = __shfl_sync(~0u, row_v, row);
+            const int inside = min(column, c.dim / 16 - 1) * 16;
+            const int bytes = column < c.dim / 16 && (mask >> row & 1) ? 16 : 0;
+            const uint32_t at = to + row * kDim + piece_of(row, column) * 16;
+            copy16(at, k + from_k + inside, bytes);
+            copy16(at + kSide, v + from_v + inside, bytes);
+        }
+    }
+};
+
+// Lane l holds, of a tile's scores, tokens l / 4, + 8, + 16 and + 24 of heads 2 (l % 4) and + 1; of a block of 16 value columns the same two heads of
 // columns 2 (l / 4) and + 1. A head's values are contracted in an order of the codes' own: a lane's four codes of a token lie side by side,
 // two of them are the fragment's lower columns and two its upper ones, and so it is with the queries.
 template <typename T, int kDim_, int kGroups_, int kStages_, int kWarps_, int kBlocks_> struct CodeHeads {
     using Type = T;
-    using Cache = __nv_fp8_e4m3;
+    using Ring = CodeRing<kDim_, kStages_>;
     static constexpr int kDim = kDim_, kStages = kStages_, kGroups = kGroups_, kWarps = kWarps_, kBlocks = kBlocks_;
     static constexpr int kParts = std::is_same<T, float>::value ? 2 : 1;       // fp16 parts of a query's value
     static constexpr float kLift = 14.f;                                       // factors are taken times 2^14: they are below 2, and fp16 goes to 2^16
@@ -103,52 +212,66 @@ template <typename T, int kDim_, int kGroups_, int kStages_, int kWarps_, int kB
         return v;
     }
     __device__ __forceinline__ void tile(uint32_t keys, uint32_t values, int mask, int lane, int, float *) {
-        using R = Ring<Cache, kDim, kStages>;
-        constexpr int kPitch = R::kPitch;
-        const uint32_t scales = keys + 2 * R::kSide + lane / 4 * 4;
-        float key_scale[2], factor[2], power[2];                               // of tokens l / 4 and + 8; a value's scale is factor * 2^power
+        constexpr int kFour = Ring::kTile / 8;                                  // tokens of a lane
+        const uint32_t scales = keys + 2 * Ring::kSide + lane / 4 * 4;
+        float key_scale[kFour], factor[kFour], power[kFour];                   // a value's scale is factor * 2^power
+        bool even = mask == -1;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < kFour; ++t) {
             key_scale[t] = load_shared(scales + t * 32);
-            const float v = load_shared(scales + 64 + t * 32);
+            const float v = load_shared(scales + kFour * 32 + t * 32);
             const int exponent = max(static_cast<int>(__float_as_uint(v) >> 23 & 255), 1);
             power[t] = static_cast<float>(exponent - 127);
             factor[t] = exponent < 254 ? v * __uint_as_float(static_cast<uint32_t>(254 - exponent) << 23) : v * 1.17549435e-38f * 0.5f;
+            even &= power[t] == power[0];
         }
         // whether all of the tile's values have one power: then the largest factor is the one of the largest score
         const float first_power = __shfl_sync(~0u, power[0], 0);
-        const bool even = __all_sync(~0u, power[0] == first_power && power[1] == first_power) && mask == 0xffff;
-        // two sums, of even and odd steps: a product waits for the one before the last
-        float s[kGroups][2][4] = {};
-        const uint32_t at_k = keys + lane % 16 * kPitch + lane / 16 * 16;
+        even = __all_sync(~0u, even && power[0] == first_power);
+        float s[kGroups][kFour / 2][4] = {};
+        const uint32_t at_k = keys + lane % 16 * kDim;
 #pragma unroll
-        for (int i = 0; i < kDim / 32; ++i) {
-            uint32_t c[4];
-            ldmatrix(c, at_k + i * 32);
+        for (int i = 0; i < kDim / 32; ++i)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const uint32_t a[4] = {halves_low(c[2 * j]), halves_low(c[2 * j + 1]), halves_high(c[2 * j]), halves_high(c[2 * j + 1])};
+            for (int u = 0; u < kFour / 2; ++u) {
+                uint32_t c[4];
+                ldmatrix(c, at_k + u * 16 * kDim + Ring::piece_of(lane % 16, 2 * i + lane / 16) * 16);
 #pragma unroll
-                for (int n = 0; n < kGroups; ++n)
+                for (int j = 0; j < 2; ++j) {
+                    const uint32_t a[4] = {halves_low(c[2 * j]), halves_low(c[2 * j + 1]), halves_high(c[2 * j]), halves_high(c[2 * j + 1])};
 #pragma unroll
-                    for (int part = 0; part < kParts; ++part) mma<__half>(s[n][j], a, q[part][n][2 * i + j][0], q[part][n][2 * i + j][1]);
+                    for (int n = 0; n < kGroups; ++n)
+#pragma unroll
+                        for (int part = 0; part < kParts; ++part) mma<__half>(s[n][u], a, q[part][n][2 * i + j][0], q[part][n][2 * i + j][1]);
+                }
             }
-        }
-        uint32_t high[kGroups][2], low[kGroups][2];
+        uint32_t high[kGroups][kFour], low[kGroups][kFour];
         bool grown = false;
         float keep[kGroups][2];
 #pragma unroll
         for (int n = 0; n < kGroups; ++n) {
             float base[2], from[2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                s[n][0][i] = (s[n][0][i] + s[n][1][i]) * (scale[n][i % 2] * key_scale[i / 2]);
-                if (mask != 0xffff && !(mask >> (lane / 4 + i / 2 * 8) & 1)) s[n][0][i] = -INFINITY;
-            }
+            for (int t = 0; t < kFour; ++t)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float &x = s[n][t / 2][t % 2 * 2 + h];
+                    x *= scale[n][h] * key_scale[t];
+                    if (mask != -1 && !(mask >> (lane / 4 + t * 8) & 1)) x = -INFINITY;
+                }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const float most = warp_max(fmaxf(s[n][0][h], s[n][0][h + 2]));
-                const float most_factor = even ? most + power[0] : warp_max(fmaxf(s[n][0][h] + power[0], s[n][0][h + 2] + power[1]));
+                float most = -INFINITY, most_factor = -INFINITY;
+#pragma unroll
+                for (int t = 0; t < kFour; ++t) most = fmaxf(most, s[n][t / 2][t % 2 * 2 + h]);
+                most = warp_max(most);
+                if (even) {
+                    most_factor = most + first_power;
+                } else {
+#pragma unroll
+                    for (int t = 0; t < kFour; ++t) most_factor = fmaxf(most_factor, s[n][t / 2][t % 2 * 2 + h] + power[t]);
+                    most_factor = warp_max(most_factor);
+                }
                 const float now = fmaxf(ceilf(most), top[n][h]), now_factor = fmaxf(ceilf(most_factor), best[n][h]);
                 base[h] = now == -INFINITY ? 0.f : now;
                 from[h] = now_factor == -INFINITY ? 0.f : now_factor - kLift;
@@ -157,11 +280,14 @@ template <typename T, int kDim_, int kGroups_, int kStages_, int kWarps_, int kB
                 grown |= now_factor != best[n][h];
                 top[n][h] = now;
                 best[n][h] = now_factor;
-                sum[n][h] += pow2(s[n][0][h] - base[h]) + pow2(s[n][0][h + 2] - base[h]);
+                float more = 0.f;
+#pragma unroll
+                for (int t = 0; t < kFour; ++t) more += pow2(s[n][t / 2][t % 2 * 2 + h] - base[h]);
+                sum[n][h] += more;
             }
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {                        // tokens l / 4 (+ 8): two heads of a token to two tokens of a head
-                const float a = pow2(s[n][0][2 * t] - (from[0] - power[t])) * factor[t], b = pow2(s[n][0][2 * t + 1] - (from[1] - power[t])) * factor[t];
+            for (int t = 0; t < kFour; ++t) {                    // two heads of a token to two tokens of a head
+                const float a = pow2(s[n][t / 2][t % 2 * 2] - (from[0] - power[t])) * factor[t], b = pow2(s[n][t / 2][t % 2 * 2 + 1] - (from[1] - power[t])) * factor[t];
                 const uint32_t pair = pack2<__half>(a, b);
                 float high_a, high_b;
                 unpack2<__half>(pair, high_a, high_b);
@@ -177,23 +303,25 @@ template <typename T, int kDim_, int kGroups_, int kStages_, int kWarps_, int kB
 #pragma unroll
                     for (int c = 0; c < 4; ++c) acc[n][i][c] *= keep[n][c % 2];
         }
-        const uint32_t at_v = values + lane % 16 * kPitch + lane / 16 * 16;
+        const uint32_t at_v = values + lane % 16 * kDim;
 #pragma unroll
-        for (int i = 0; i < kDim / 32; ++i) {
-            uint32_t c[4];
-            ldmatrix_trans(c, at_v + i * 32);
+        for (int i = 0; i < kDim / 32; ++i)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                // two columns of two tokens each: the columns apart
-                const uint32_t one = __byte_perm(c[2 * j], 0, 0x3120), two = __byte_perm(c[2 * j + 1], 0, 0x3120);
-                const uint32_t a[4] = {halves_low(one), halves_high(one), halves_low(two), halves_high(two)};
+            for (int u = 0; u < kFour / 2; ++u) {
+                uint32_t c[4];
+                ldmatrix_trans(c, at_v + u * 16 * kDim + Ring::piece_of(lane % 16, 2 * i + lane / 16) * 16);
 #pragma unroll
-                for (int n = 0; n < kGroups; ++n) {
-                    mma<__half>(acc[n][2 * i + j], a, high[n][0], high[n][1]);
-                    mma<__half>(acc[n][2 * i + j], a, low[n][0], low[n][1]);
+                for (int j = 0; j < 2; ++j) {
+                    // two columns of two tokens each: the columns apart
+                    const uint32_t one = __byte_perm(c[2 * j], 0, 0x3120), two = __byte_perm(c[2 * j + 1], 0, 0x3120);
+                    const uint32_t a[4] = {halves_low(one), halves_high(one), halves_low(two), halves_high(two)};
+#pragma unroll
+                    for (int n = 0; n < kGroups; ++n) {
+                        mma<__half>(acc[n][2 * i + j], a, high[n][2 * u], high[n][2 * u + 1]);
+                        mma<__half>(acc[n][2 * i + j], a, low[n][2 * u], low[n][2 * u + 1]);
+                    }
                 }
             }
-        }
     }
     // done(head, maximum, sum) once for every head, which gives the factor of its values; then put(head, d, value)
     template <typename Done, typename Put> __device__ __forceinline__ void finish(int heads, int dim, int lane, Done done, Put put) {
@@ -224,11 +352,11 @@ cudaError_t launch_type(const MsnhB200Ctx *ctx, const AttnParams &p, int blocks,
     constexpr int kMany = std::is_same<T, float>::value ? 1 : 2;               // (a pair has 8 heads of fp32 queries at most)
     const bool few = p.chunk <= 8;
     if (p.c.dim <= 32) return few ? launch<CodeHeads<T, 32, 1, 8, 4, 2>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 32, kMany, 8, 4, 2>>(ctx, p, blocks, stream);
-    if (p.c.dim <= 64) return few ? launch<CodeHeads<T, 64, 1, 8, 4, 2>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 64, kMany, 8, 4, 2>>(ctx, p, blocks, stream);
-    if (p.c.dim <= 96) return few ? launch<CodeHeads<T, 96, 1, 6, 4, 2>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 96, kMany, 6, 4, 2>>(ctx, p, blocks, stream);
-    if (p.c.dim <= 128) return few ? launch<CodeHeads<T, 128, 1, 5, 4, 2>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 128, kMany, 5, 4, 2>>(ctx, p, blocks, stream);
-    if (p.c.dim <= 192) return few ? launch<CodeHeads<T, 192, 1, 6, 4, 1>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 192, kMany, 6, 4, 1>>(ctx, p, blocks, stream);
-    return few ? launch<CodeHeads<T, 256, 1, 5, 4, 1>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 256, kMany, 5, 4, 1>>(ctx, p, blocks, stream);
+    if (p.c.dim <= 64) return few ? launch<CodeHeads<T, 64, 1, 6, 4, 2>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 64, kMany, 6, 4, 2>>(ctx, p, blocks, stream);
+    if (p.c.dim <= 96) return few ? launch<CodeHeads<T, 96, 1, 4, 4, 2>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 96, kMany, 4, 4, 2>>(ctx, p, blocks, stream);
+    if (p.c.dim <= 128) return few ? launch<CodeHeads<T, 128, 1, 3, 4, 2>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 128, kMany, 3, 4, 2>>(ctx, p, blocks, stream);
+    if (p.c.dim <= 192) return few ? launch<CodeHeads<T, 192, 1, 4, 4, 1>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 192, kMany, 4, 4, 1>>(ctx, p, blocks, stream);
+    return few ? launch<CodeHeads<T, 256, 1, 3, 4, 1>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 256, kMany, 3, 4, 1>>(ctx, p, blocks, stream);
 }
 
 }  // namespace

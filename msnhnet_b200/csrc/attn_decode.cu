@@ -35,7 +35,7 @@ constexpr int kWholeTiles = 8;
 // and l / 4 + 8 of heads 2 (l % 4) and + 1; of a block of 16 value columns the same two heads of columns l / 4 and l / 4 + 8.
 template <typename T, int kDim_, int kGroups_, int kStages_, int kBlocks_> struct TensorHeads {
     using Type = T;
-    using Cache = T;
+    using Ring = attn::Ring<T, kDim_, kStages_>;
     static constexpr int kDim = kDim_, kStages = kStages_, kGroups = kGroups_, kWarps = 4, kBlocks = kBlocks_;
     // fp16 weights are taken times 2^14, so that a weight of 2^-29 of the largest is still a normal number (sum and values carry the
     // same factor); what a weight loses when it is rounded to the cache's type goes into a second product. Both parts are above 0 where the
@@ -69,7 +69,7 @@ template <typename T, int kDim_, int kGroups_, int kStages_, int kBlocks_> struc
         scale = p.scale * kLog2e;
     }
     __device__ __forceinline__ void tile(uint32_t keys, uint32_t values, int mask, int lane, int, float *) {
-        constexpr int kPitch = Ring<T, kDim, kStages>::kPitch;
+        constexpr int kPitch = Ring::kPitch;
         // two sums, of even and odd steps: a product waits for the one before the last
         float s[kGroups][2][4] = {};
         const uint32_t at_k = keys + lane % 16 * kPitch + lane / 16 * 16;
@@ -162,8 +162,8 @@ template <typename T, int kDim_, int kGroups_, int kStages_, int kBlocks_> struc
 // kDim / 32 columns a lane.
 template <int kDim_, int kHeads_, int kStages_, int kWarps_> struct PlainHeads {
     using Type = float;
-    using Cache = float;
-    static constexpr int kDim = kDim_, kStages = kStages_, kWarps = kWarps_, kHeads = kHeads_, kBlocks = 1;
+    using Ring = attn::Ring<float, kDim_, kStages_>;
+    static constexpr int kDim = kDim_, kStages = kStages_, kWarps = kWarps_, kHeads = kHeads_, kBlocks = 1, kTile = Ring::kTile;
     static constexpr int kColumns = kDim / 32, kVec = kColumns % 4 == 0 ? 4 : kColumns % 2 == 0 ? 2 : 1;
 
     float acc[kHeads][kColumns], top[kHeads], sum[kHeads];
@@ -192,7 +192,7 @@ template <int kDim_, int kHeads_, int kStages_, int kWarps_> struct PlainHeads {
         return v;
     }
     __device__ __forceinline__ void tile(uint32_t keys, uint32_t values, int mask, int lane, int, float *scratch) {
-        constexpr int kPitch = Ring<float, kDim, kStages>::kPitch;
+        constexpr int kPitch = Ring::kPitch;
         float *weights = scratch + kHeads * kDim;
         const float4 *q = reinterpret_cast<const float4 *>(scratch) + lane / 16 * (kDim / 8);
         float s[kHeads] = {};
@@ -355,7 +355,8 @@ AttnPlan plan_of(const MsnhB200Ctx *ctx, const MsnhB200KvCache &c, const MsnhB20
     const BlockShape shape = block_shape(c.dtype, c.head_dim);
     const long long blocks = static_cast<long long>(ctx->sm_count) * shape.of_sm;
     const long long most_tokens = static_cast<long long>(c.max_pages) * c.page_size, seen = a.window > 0 ? std::min<long long>(most_tokens, a.window) : most_tokens;
-    const long long tiles = (seen + kTile - 1) / kTile + (a.window > 0);        // (a window may start inside a tile)
+    const int tile = c.dtype == MSNH_B200_E4M3 ? kCodeTile : 16;
+    const long long tiles = (seen + tile - 1) / tile + (a.window > 0);        // (a window may start inside a tile)
     l.tiles = tiles;
     l.whole = tiles <= kWholeTiles;
     const long long row_tiles = (tiles + kStart) * c.n_kv_heads * l.chunks;

@@ -7,7 +7,6 @@
 namespace msnh {
 namespace attn {
 
-constexpr int kTile = 16;                    // tokens of a tile
 constexpr int kMaxRows = 256;                // rows of a launch: what they see is kept in shared memory
 // Tiles that a pair's start counts for, and tiles of a share, where there are as many. fp16, 32 heads over 8, with kStart 1, 3 and 6: one row
 // of 500 tokens 9.7, 10.8 and 13.1 us, 16 of them 17.2, 16.5 and 18.0, one of 65536 beside 63 of 100 76.7, 75.2 and 75.7, one of 4000 14.2,
@@ -39,7 +38,7 @@ __device__ __forceinline__ Row row_of(const AttnParams &p, int row) {
     r.first = p.window > 0 ? max(0, r.last - p.window) : 0;
     return r;
 }
-__device__ __forceinline__ int tiles_of(const Row &r) { return r.last > r.first ? (r.last - 1) / kTile - r.first / kTile + 1 : 0; }
+template <int kTile> __device__ __forceinline__ int tiles_of(const Row &r) { return r.last > r.first ? (r.last - 1) / kTile - r.first / kTile + 1 : 0; }
 
 // The share of a warp, in tiles of the line. (A launch's line has less than 2^30 tiles: code for longer ones is a microsecond of reading
 // instructions alone.)
@@ -64,21 +63,51 @@ __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_gr
 template <int kLeft> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
 
 // A warp's ring: kStages tiles of keys and values. Rows are 16 bytes longer than kDim values: eight rows at one column then lie in all
-// the banks. Pieces of tokens that are not there, and keys' columns beyond dim, are filled with zeros: a weight of 0 meets a 0. A tile of 8-bit
-// codes is followed by a scale for each of its keys and values.
+// the banks. Pieces of tokens that are not there, and keys' columns beyond dim, are filled with zeros: a weight of 0 meets a 0.
 template <typename T, int kDim, int kStages> struct Ring {
+    static constexpr int kTile = 16, kAhead = 32;                // tokens of a tile; tiles whose pages are looked up together
     static constexpr int kPitch = kDim * sizeof(T) + 16;
-    static constexpr bool kCodes = sizeof(T) == 1;
-    static constexpr int kSide = kTile * kPitch, kStage = 2 * kSide + (kCodes ? 2 * kTile * 4 : 0), kBytes = kStages * kStage;
+    static constexpr int kSide = kTile * kPitch, kStage = 2 * kSide, kBytes = kStages * kStage;
     static constexpr int kPieces = kDim * sizeof(T) / 16, kValues = 16 / sizeof(T);
 
     const KvParams &c;
-    const T *k, *v;                          // of the key head
-    const float *scales[2];                  // the same, of codes: of keys, of values
-    const int *table;                        // of the sequence
     int *masks;                              // [kStages] bit t: token t of the tile takes part
     uint32_t base;
-    int first, last, lane;                   // tokens that are seen; lane of the warp
+    int lane;
+    const T *k = nullptr, *v = nullptr;      // of the key head
+    const int *table = nullptr;              // of the sequence
+    int first = 0, last = 0, origin = 0;     // tokens that are seen; token of the piece's first tile
+    int low_page = -1, high_page = -1, next_low = -1, next_high = -1;         // a lane's pages of one of 32 tiles, and of one of the 32 behind them
+
+    __device__ __forceinline__ Ring(const KvParams &c_, int *masks_, uint32_t base_, int lane_) : c(c_), masks(masks_), base(base_), lane(lane_) {}
+
+    __device__ __forceinline__ void start(int head, const int *table_, int first_, int last_, int first_tile) {
+        k = reinterpret_cast<const T *>(c.k) + head * c.k_head;
+        v = reinterpret_cast<const T *>(c.v) + head * c.v_head;
+        table = table_;
+        first = first_;
+        last = last_;
+        origin = (first / kTile + first_tile) * kTile;
+    }
+    // Asks for the pages of the tiles from first_tile on.
+    __device__ __forceinline__ void look_ahead(int first_tile, int tiles) {
+        next_low = next_high = -1;
+        if (first_tile + lane < tiles) {
+            const int token = origin + (first_tile + lane) * kTile;
+            next_low = page_of(token);
+            next_high = page_of(token + 8);
+        }
+    }
+    // What has been asked for is of the tiles from here on.
+    __device__ __forceinline__ void take_pages(int) {
+        low_page = next_low;
+        high_page = next_high;
+    }
+    __device__ __forceinline__ void copy(int stage, int tile) const {
+        const int a = __shfl_sync(~0u, low_page, tile % 32), b = __shfl_sync(~0u, high_page, tile % 32);
+        if ((a | b) >= 0) issue(stage, origin + tile * kTile, a, b);
+        else issue_any(stage, origin + tile * kTile);
+    }
 
     // The page of a run of eight tokens that are all seen, in a cache whose pages are multiples of eight; -1 otherwise.
     __device__ __forceinline__ int page_of(int token) const {
@@ -86,33 +115,10 @@ template <typename T, int kDim, int kStages> struct Ring {
         const int page = table[token / c.page_size];
         return page < c.n_pages ? page : -1;
     }
-    // The scale of the token that lane % 16 stands for: of its key (lanes 0 to 15) or its value; 0 where it is not there.
-    __device__ __forceinline__ void copy_scale(uint32_t to, long long page, int place, bool there) const {
-        const float *from = lane < kTile ? scales[0] : scales[1];
-        if (there) from += page * c.heads * c.blocks + place / c.block;
-        copy4(to + 2 * kSide + lane * 4, from, there ? 4 : 0);
-    }
     // A tile of two such runs.
     __device__ __forceinline__ void issue(int stage, int token, int page_low, int page_high) const {
         const uint32_t to = base + stage * kStage;
         if (lane == 0) masks[stage] = 0xffff;
-        if constexpr (kCodes) {
-            const int place_low = token % c.page_size, place_high = (token + 8) % c.page_size;
-            const T *low_k = k + page_low * c.k_page + place_low * c.k_token, *low_v = v + page_low * c.v_page + place_low * c.v_token;
-            const T *high_k = k + page_high * c.k_page + (place_high - 8) * c.k_token, *high_v = v + page_high * c.v_page + (place_high - 8) * c.v_token;
-#pragma unroll
-            for (int i = 0; i < kPieces / 2; ++i) {
-                const int piece = lane + 32 * i, row = piece / kPieces, column = piece % kPieces;
-                const bool inside = column < c.dim / kValues;
-                const T *from_k = row < 8 ? low_k : high_k, *from_v = row < 8 ? low_v : high_v;
-                const uint32_t at = to + row * kPitch + column * 16;
-                copy16(at, inside ? from_k + row * c.k_token + column * kValues : k, inside ? 16 : 0);
-                copy16(at + kSide, inside ? from_v + row * c.v_token + column * kValues : v, inside ? 16 : 0);
-            }
-            const int t = lane % kTile;
-            copy_scale(to, t < 8 ? page_low : page_high, t < 8 ? place_low + t : place_high + t - 8, true);
-            return;
-        }
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             const long long page = half ? page_high : page_low, place = (token + 8 * half) % c.page_size;
@@ -153,11 +159,6 @@ template <typename T, int kDim, int kStages> struct Ring {
         const unsigned mask = __ballot_sync(~0u, there);
         if (lane == 0) masks[stage] = static_cast<int>(mask);
         const uint32_t to = base + stage * kStage;
-        if constexpr (kCodes) {
-            const int from = lane % kTile;
-            const int its_page = __shfl_sync(~0u, page, from), its_place = __shfl_sync(~0u, static_cast<int>(place), from);
-            copy_scale(to, its_page, its_place, mask >> from & 1);
-        }
 #pragma unroll 1
         for (int i = 0; i < kTile * kPieces / 32; ++i) {
             const int piece = lane + 32 * i, row = piece / kPieces, column = piece % kPieces;
@@ -222,6 +223,7 @@ template <typename Heads> struct Side {
 
 // A warp's walk along its share: pieces of pairs, one after the other.
 template <typename Heads> struct Walk {
+    static constexpr int kTile = Heads::Ring::kTile;
     const AttnParams &p;
     const Side<Heads> &side;
     int left;                                                    // of the share
@@ -261,8 +263,7 @@ template <typename Heads> struct Walk {
 template <typename Heads>
 __global__ void __launch_bounds__(Heads::kWarps * 32, Heads::kBlocks) attn_decode_kernel(const __grid_constant__ AttnParams p) {
     using T = typename Heads::Type;
-    using Cache = typename Heads::Cache;
-    using R = Ring<Cache, Heads::kDim, Heads::kStages>;
+    using R = typename Heads::Ring;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ Side<Heads> side;
     constexpr int kWarps = Heads::kWarps, kThreads = kWarps * 32, kStages = Heads::kStages;
@@ -278,7 +279,7 @@ __global__ void __launch_bounds__(Heads::kWarps * 32, Heads::kBlocks) attn_decod
             side.first[i] = r.first;
             side.last[i] = r.last;
         }
-        const int tiles = tiles_of(r);
+        const int tiles = tiles_of<R::kTile>(r);
         const int mine = tiles == 0 ? 0 : (p.whole ? 1 : tiles + kStart) * pairs;
         int sum = mine;
 #pragma unroll
@@ -324,45 +325,24 @@ __global__ void __launch_bounds__(Heads::kWarps * 32, Heads::kBlocks) attn_decod
     ahead.at = unit - side.prefix[low] - ahead.pair * ahead.length;
     Walk<Heads> walk = ahead;
 
-    // the copies' side: the piece they are at, its next tile, and a lane's page of one of the next 32 tiles
+    // the copies' side: the piece they are at, and its next tile
     typename Walk<Heads>::Piece from;
-    R ring = {p.c, nullptr, nullptr, {nullptr, nullptr}, nullptr, side.masks[warp], static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * R::kBytes, 0, 0, lane};
-    int tile = 0, tiles = 0, origin = 0, low_page = -1, high_page = -1, next_low = -1, next_high = -1, filled = 0, queued = 0;
-    const auto pages_from = [&](int first_tile) {
-        next_low = next_high = -1;
-        if (first_tile + lane < tiles) {
-            const int token = origin + (first_tile + lane) * kTile;
-            next_low = ring.page_of(token);
-            next_high = ring.page_of(token + 8);
-        }
-    };
+    R ring(p.c, side.masks[warp], static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * R::kBytes, lane);
+    int tile = 0, tiles = 0, filled = 0, queued = 0;
     const auto advance = [&] {                                   // to the next piece; its pages are on their way when this returns
         if (!ahead.next(from)) { tiles = 0; return; }
-        const int kv = from.pair / p.chunks;
-        ring.k = reinterpret_cast<const Cache *>(p.c.k) + kv * p.c.k_head;
-        ring.v = reinterpret_cast<const Cache *>(p.c.v) + kv * p.c.v_head;
-        if constexpr (R::kCodes) {
-            ring.scales[0] = p.c.k_scales + static_cast<long long>(kv) * p.c.blocks;
-            ring.scales[1] = p.c.v_scales + static_cast<long long>(kv) * p.c.blocks;
-        }
-        ring.table = p.c.table + side.seq[from.row] * p.c.table_stride;
-        ring.first = side.first[from.row];
-        ring.last = side.last[from.row];
-        origin = (ring.first / kTile + from.begin) * kTile;
+        ring.start(from.pair / p.chunks, p.c.table + side.seq[from.row] * p.c.table_stride, side.first[from.row], side.last[from.row], from.begin);
         tile = 0;
         tiles = from.end - from.begin;
-        pages_from(0);
+        ring.look_ahead(0, tiles);
     };
     const auto copy_next = [&] {
         if (tile >= tiles) return;
-        if (tile % 32 == 0) {
-            low_page = next_low;
-            high_page = next_high;
-            if (tile + 32 < tiles) pages_from(tile + 32);
+        if (tile % R::kAhead == 0) {
+            ring.take_pages(tile);
+            if (tile + R::kAhead < tiles) ring.look_ahead(tile + R::kAhead, tiles);
         }
-        const int a = __shfl_sync(~0u, low_page, tile % 32), b = __shfl_sync(~0u, high_page, tile % 32);
-        if ((a | b) >= 0) ring.issue(filled, origin + tile * kTile, a, b);
-        else ring.issue_any(filled, origin + tile * kTile);
+        ring.copy(filled, tile);
         copy_commit();
         filled = filled == kStages - 1 ? 0 : filled + 1;
         ++queued;
@@ -415,15 +395,16 @@ inline cudaError_t launch(const MsnhB200Ctx *ctx, const AttnParams &p, int block
     static std::atomic<uint64_t> done{0};
     const uint64_t bit = 1ull << (ctx->device & 63);
     if (!(done.load(std::memory_order_acquire) & bit)) {
-        const cudaError_t e = cudaFuncSetAttribute(attn_decode_kernel<Heads>, cudaFuncAttributeMaxDynamicSharedMemorySize, Heads::kWarps * Ring<typename Heads::Cache, Heads::kDim, Heads::kStages>::kBytes);
+        const cudaError_t e = cudaFuncSetAttribute(attn_decode_kernel<Heads>, cudaFuncAttributeMaxDynamicSharedMemorySize, Heads::kWarps * Heads::Ring::kBytes);
         if (e != cudaSuccess) return e;
         done.fetch_or(bit, std::memory_order_release);
     }
-    return launch_token_kernel(attn_decode_kernel<Heads>, dim3(blocks), Heads::kWarps * 32, Heads::kWarps * Ring<typename Heads::Cache, Heads::kDim, Heads::kStages>::kBytes, stream, ctx->pdl, p);
+    return launch_token_kernel(attn_decode_kernel<Heads>, dim3(blocks), Heads::kWarps * 32, Heads::kWarps * Heads::Ring::kBytes, stream, ctx->pdl, p);
 }
 
 struct BlockShape { int warps, of_sm; };
-// Caches of 8-bit codes (attn_codes.cu); dtype: of queries and output.
+// Caches of 8-bit codes (attn_codes.cu): tokens of a tile; dtype: of queries and output.
+constexpr int kCodeTile = 32;
 BlockShape block_shape_codes(int dim);
 cudaError_t launch_codes(const MsnhB200Ctx *ctx, const AttnParams &p, int dtype, int blocks, void *stream);
 
