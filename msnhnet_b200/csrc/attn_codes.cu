@@ -15,17 +15,6 @@ namespace msnh {
 namespace attn {
 namespace {
 
-// two codes to two fp16 values
-__device__ __forceinline__ uint32_t halves_low(uint32_t codes) {
-    uint32_t r;
-    asm("{ .reg .b16 low, high; mov.b32 {low, high}, %1; cvt.rn.f16x2.e4m3x2 %0, low; }" : "=r"(r) : "r"(codes));
-    return r;
-}
-__device__ __forceinline__ uint32_t halves_high(uint32_t codes) {
-    uint32_t r;
-    asm("{ .reg .b16 low, high; mov.b32 {low, high}, %1; cvt.rn.f16x2.e4m3x2 %0, high; }" : "=r"(r) : "r"(codes));
-    return r;
-}
 __device__ __forceinline__ float load_shared(uint32_t at) {
     float v;
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");

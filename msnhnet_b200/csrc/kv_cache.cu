@@ -189,19 +189,38 @@ template <int kVec> __device__ __forceinline__ void store_codes(uint8_t *to, con
         else *reinterpret_cast<uint32_t *>(to) = words[0];
     }
 }
-// kVec values side by side, and as many codes
+// kVec values side by side
 template <typename T, int kVec> struct Piece {
     alignas(16) T v[kVec];
     __device__ __forceinline__ void load(const T *from) {
         if constexpr (kVec > 1) *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(from);
         else v[0] = from[0];
     }
-    // the larger one of `before` and the magnitudes' bits, of all or of finite ones
-    __device__ __forceinline__ uint32_t top(uint32_t before, bool all) const {
+    // The larger one of `before` and the magnitudes' bits; 16-bit values in two halves, which last() joins.
+    __device__ __forceinline__ uint32_t top(uint32_t before) const {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) before = max(before, __float_as_uint(v[i]) & 0x7fffffffu);
+        } else if constexpr (kVec == 1) {
+            before = max(before, reinterpret_cast<const uint16_t *>(v)[0] & 0x7fffu);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kVec / 2; ++i) before = __vmaxu2(before, reinterpret_cast<const uint32_t *>(v)[i] & 0x7fff7fffu);
+        }
+        return before;
+    }
+    // The largest magnitude as an fp32 number's bits.
+    static __device__ __forceinline__ uint32_t last(uint32_t top) {
+        if constexpr (sizeof(T) == 4) return top;
+        const uint16_t bits = static_cast<uint16_t>(max(top & 0xffffu, top >> 16));
+        return __float_as_uint(to_float(reinterpret_cast<const T &>(bits)));
+    }
+    // The same of what is finite.
+    __device__ __forceinline__ uint32_t finite_top(uint32_t before) const {
 #pragma unroll
         for (int i = 0; i < kVec; ++i) {
             const uint32_t bits = __float_as_uint(to_float(v[i])) & 0x7fffffffu;
-            if (all || bits < 0x7f800000u) before = max(before, bits);
+            if (bits < 0x7f800000u) before = max(before, bits);
         }
         return before;
     }
@@ -239,15 +258,31 @@ __device__ __forceinline__ bool is_power(float scale) {
     return (bits & 0x807fffffu) == 0 && bits >= 0x00800000u && bits <= 0x7e800000u;
 }
 
+// A lane's walk over the pieces of some rows, 32 pieces a step.
+struct RowWalk {
+    int vecs, right, column;
+    long long step, wrap;                                        // between pieces; more where the step passes a row's end
+    __device__ __forceinline__ RowWalk(int vecs_, int lane, int per_vec, long long row_step) : vecs(vecs_), right(32 % vecs_), column(lane % vecs_) {
+        step = 32 / vecs * row_step + right * per_vec;
+        wrap = row_step - static_cast<long long>(vecs) * per_vec;
+    }
+    template <typename P> __device__ __forceinline__ void next(P *&at) {
+        at += step;
+        column += right;
+        if (column >= vecs) { column -= vecs; at += wrap; }
+    }
+};
+
 constexpr int kHeld = 8;               // pieces of new values that a lane keeps between the maximum and the codes
 
 // A warp for the call's tokens in one block of scales of one head, keys or values: their largest magnitude, the scale, the block's older
 // codes by the new scale where that has grown, the new codes.
 template <typename T, int kVec>
-__global__ void __launch_bounds__(256) kv_append_codes_kernel(KvParams c, const int *seqs, const int *starts, int n, const AppendWork *work, const T *k_new, const T *v_new,
-                                                              long long token_stride, long long head_stride, long long most_blocks) {
+__global__ void __launch_bounds__(256, kVec > 1 ? 3 : 1) kv_append_codes_kernel(KvParams c, const int *seqs, const int *starts, int n, const AppendWork *work, const T *k_new,
+                                                                                 const T *v_new, long long token_stride, long long head_stride, long long most_blocks) {
+    using Pieces = Piece<T, kVec>;
     pdl_enter();
-    const int lane = threadIdx.x % 32, vecs = c.dim / kVec, down = 32 / vecs, right = 32 % vecs;
+    const int lane = threadIdx.x % 32, vecs = c.dim / kVec;
     const long long total = most_blocks * c.heads * 2;
     for (long long w = (blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x) / 32; w < total; w += static_cast<long long>(gridDim.x) * blockDim.x / 32) {
         const long long pair = w / c.heads;
@@ -270,41 +305,39 @@ __global__ void __launch_bounds__(256) kv_append_codes_kernel(KvParams c, const 
         const T *source = (values ? v_new : k_new) + (first + from - before) * token_stride + head * head_stride;
         const int pieces = (to - from) * vecs;
 
-        Piece<T, kVec> held[kHeld];
-        const int row0 = lane / vecs, column0 = lane - row0 * vecs;
-        int row = row0, column = column0;
-        const auto step = [&] {
-            row += down;
-            column += right;
-            if (column >= vecs) { column -= vecs; ++row; }
-        };
+        Pieces held[kHeld];
         uint32_t top = 0;
+        {
+            RowWalk walk(vecs, lane, kVec, token_stride);
+            const T *at = source + lane / vecs * token_stride + walk.column * kVec;
 #pragma unroll
-        for (int j = 0; j < kHeld; ++j) {
-            if (lane + 32 * j < pieces) held[j].load(source + row * token_stride + column * kVec);
-            step();
-        }
-        const int row_more = row, column_more = column;
+            for (int j = 0; j < kHeld; ++j) {
+                if (lane + 32 * j < pieces) held[j].load(at);
+                walk.next(at);
+            }
 #pragma unroll
-        for (int j = 0; j < kHeld; ++j)
-            if (lane + 32 * j < pieces) top = held[j].top(top, true);
-        for (int at = lane + 32 * kHeld; at < pieces; at += 32) {
-            Piece<T, kVec> p;
-            p.load(source + row * token_stride + column * kVec);
-            top = p.top(top, true);
-            step();
+            for (int j = 0; j < kHeld; ++j)
+                if (lane + 32 * j < pieces) top = held[j].top(top);
+#pragma unroll 1
+            for (int u = lane + 32 * kHeld; u < pieces; u += 32) {
+                Pieces p;
+                p.load(at);
+                top = p.top(top);
+                walk.next(at);
+            }
         }
-        top = __reduce_max_sync(~0u, top);
+        top = __reduce_max_sync(~0u, Pieces::last(top));
         const bool odd = top >= 0x7f800000u;                     // a NaN or infinity: once more without them
         if (odd) {
             top = 0;
-            row = row0;
-            column = column0;
-            for (int at = lane; at < pieces; at += 32) {
-                Piece<T, kVec> p;
-                p.load(source + row * token_stride + column * kVec);
-                top = p.top(top, false);
-                step();
+            RowWalk walk(vecs, lane, kVec, token_stride);
+            const T *at = source + lane / vecs * token_stride + walk.column * kVec;
+#pragma unroll 1
+            for (int u = lane; u < pieces; u += 32) {
+                Pieces p;
+                p.load(at);
+                top = p.finite_top(top);
+                walk.next(at);
             }
             top = __reduce_max_sync(~0u, top);
         }
@@ -313,68 +346,102 @@ __global__ void __launch_bounds__(256) kv_append_codes_kernel(KvParams c, const 
         const float inverse = power ? 1.f / scale : 0.f;
         if (older && scale != had) {
             const auto again = [&](float x) { return power ? x * had * inverse : x * had / scale; };
-            uint8_t *old = codes - older * token_step;
-            row = row0;
-            column = column0;
-            for (int at = lane; at < older * vecs; at += 32) {
-                uint8_t *one = old + row * token_step + column * kVec;
+            RowWalk walk(vecs, lane, kVec, token_step);
+            uint8_t *at = codes + (lane / vecs - older) * token_step + walk.column * kVec;
+#pragma unroll 1
+            for (int u = lane; u < older * vecs; u += 32) {
                 Codes<kVec> p;
-                p.load(one);
-                p.store(one, again);
-                step();
+                p.load(at);
+                p.store(at, again);
+                walk.next(at);
             }
         }
-        const auto code = [&](float x) {
-            if (odd && !isfinite(x)) return __uint_as_float(0x7fffffffu);
-            return power ? x * inverse : scale == 0.f ? 0.f * x : x / scale;
-        };
-        row = row0;
-        column = column0;
+        RowWalk walk(vecs, lane, kVec, token_step);
+        uint8_t *at = codes + lane / vecs * token_step + walk.column * kVec;
+        if (power && !odd) {
+            const auto code = [&](float x) { return x * inverse; };
 #pragma unroll
-        for (int j = 0; j < kHeld; ++j) {
-            if (lane + 32 * j < pieces) held[j].store(codes + row * token_step + column * kVec, code);
-            step();
-        }
-        row = row_more;
-        column = column_more;
-        for (int at = lane + 32 * kHeld; at < pieces; at += 32) {
-            Piece<T, kVec> p;
-            p.load(source + row * token_stride + column * kVec);
-            p.store(codes + row * token_step + column * kVec, code);
-            step();
+            for (int j = 0; j < kHeld; ++j) {
+                if (lane + 32 * j < pieces) held[j].store(at, code);
+                walk.next(at);
+            }
+            if (pieces > 32 * kHeld) {
+                RowWalk again(vecs, lane, kVec, token_stride);
+                const T *from_new = source + lane / vecs * token_stride + again.column * kVec;
+                for (int j = 0; j < kHeld; ++j) again.next(from_new);
+#pragma unroll 1
+                for (int u = lane + 32 * kHeld; u < pieces; u += 32) {
+                    Pieces p;
+                    p.load(from_new);
+                    p.store(at, code);
+                    again.next(from_new);
+                    walk.next(at);
+                }
+            }
+        } else {
+            const auto code = [&](float x) {
+                if (!isfinite(x)) return __uint_as_float(0x7fffffffu);
+                return scale == 0.f ? 0.f * x : x / scale;
+            };
+            RowWalk again(vecs, lane, kVec, token_stride);
+            const T *from_new = source + lane / vecs * token_stride + again.column * kVec;
+#pragma unroll 1
+            for (int u = lane; u < pieces; u += 32) {
+                Pieces p;
+                p.load(from_new);
+                p.store(at, code);
+                again.next(from_new);
+                walk.next(at);
+            }
         }
         if (lane == 0) *scale_at = scale;
     }
 }
 
-// kVec values side by side of one type to another, times a scale
-template <typename In, typename Out, int kVec> __device__ __forceinline__ void convert(Out *to, const In *from, float scale) {
-    alignas(16) In in[kVec];
-    alignas(16) Out out[kVec];
-    if constexpr (kVec == 1) {
-        in[0] = from[0];
-    } else if constexpr (sizeof(in) == 8) {
-        *reinterpret_cast<uint2 *>(in) = *reinterpret_cast<const uint2 *>(from);
-    } else {
+// kVec values side by side, and what they are as another type, times a scale
+template <typename In, int kVec> struct Values {
+    alignas(16) In v[kVec];
+    __device__ __forceinline__ void load(const In *from) {
+        if constexpr (kVec == 1) {
+            v[0] = from[0];
+        } else if constexpr (sizeof(v) == 8) {
+            *reinterpret_cast<uint2 *>(v) = *reinterpret_cast<const uint2 *>(from);
+        } else {
 #pragma unroll
-        for (int i = 0; i < static_cast<int>(sizeof(in)) / 16; ++i) reinterpret_cast<uint4 *>(in)[i] = reinterpret_cast<const uint4 *>(from)[i];
+            for (int i = 0; i < static_cast<int>(sizeof(v)) / 16; ++i) reinterpret_cast<uint4 *>(v)[i] = reinterpret_cast<const uint4 *>(from)[i];
+        }
     }
+    template <typename Out> __device__ __forceinline__ void store(Out *to, float scale) const {
+        alignas(16) Out out[kVec];
+        if constexpr (sizeof(In) == 1 && kVec > 1) {
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) out[i] = from_float<Out>(sizeof(In) == 1 ? to_float(in[i]) * scale : to_float(in[i]));
-    if constexpr (kVec == 1) {
-        to[0] = out[0];
-    } else {
+            for (int i = 0; i < kVec / 4; ++i) {
+                float x[4];
+                to_floats(reinterpret_cast<const uint32_t *>(v)[i], x);
 #pragma unroll
-        for (int i = 0; i < static_cast<int>(sizeof(out)) / 16; ++i) reinterpret_cast<uint4 *>(to)[i] = reinterpret_cast<const uint4 *>(out)[i];
+                for (int j = 0; j < 4; ++j) out[4 * i + j] = from_float<Out>(x[j] * scale);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) out[i] = from_float<Out>(sizeof(In) == 1 ? to_float(v[i]) * scale : to_float(v[i]));
+        }
+        if constexpr (kVec == 1) {
+            to[0] = out[0];
+        } else {
+#pragma unroll
+            for (int i = 0; i < static_cast<int>(sizeof(out)) / 16; ++i) reinterpret_cast<uint4 *>(to)[i] = reinterpret_cast<const uint4 *>(out)[i];
+        }
     }
-}
+};
 
-// A warp a row of the output: keys and values of all heads of one token.
+// A warp a row of the output: keys and values of all heads of one token, kTurn pieces of each on their way together.
 template <typename In, typename Out, int kVec>
 __global__ void __launch_bounds__(256) kv_read_kernel(KvParams c, const int *seqs, const int *starts, const int *firsts, int n, Out *k_out, Out *v_out, long long token_stride,
                                                       long long head_stride, int n_rows) {
+    constexpr bool kCodes = sizeof(In) == 1;
+    constexpr int kTurn = kVec > 1 && sizeof(In) <= 2 ? 4 : 2;
     pdl_enter();
-    const int lane = threadIdx.x % 32, vecs = c.dim / kVec;
+    const int lane = threadIdx.x % 32, vecs = c.dim / kVec, total = c.heads * vecs, head_step = 32 / vecs, head0 = lane / vecs;
     for (long long row = (blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x) / 32; row < n_rows; row += static_cast<long long>(gridDim.x) * blockDim.x / 32) {
         int page = -1;
         long long at = 0;
@@ -387,18 +454,45 @@ __global__ void __launch_bounds__(256) kv_read_kernel(KvParams c, const int *seq
             }
         }
         const bool there = page >= 0 && page < c.n_pages;
-        const int place = there ? static_cast<int>(at % c.page_size) : 0;
-        const In *k = reinterpret_cast<const In *>(c.k) + (there ? page * c.k_page + place * c.k_token : 0), *v = reinterpret_cast<const In *>(c.v) + (there ? page * c.v_page + place * c.v_token : 0);
-        Out *k_to = k_out + row * token_stride, *v_to = v_out + row * token_stride;
-        const long long scales = sizeof(In) == 1 && there ? static_cast<long long>(page) * c.heads * c.blocks + place / c.block : 0;
-        for (int u = lane; u < c.heads * vecs; u += 32) {
-            const int head = u / vecs, d = (u - head * vecs) * kVec;
-            if (there) {
-                convert<In, Out, kVec>(k_to + head * head_stride + d, k + head * c.k_head + d, sizeof(In) == 1 ? c.k_scales[scales + static_cast<long long>(head) * c.blocks] : 1.f);
-                convert<In, Out, kVec>(v_to + head * head_stride + d, v + head * c.v_head + d, sizeof(In) == 1 ? c.v_scales[scales + static_cast<long long>(head) * c.blocks] : 1.f);
-            } else {
+        RowWalk walk_k(vecs, lane, kVec, c.k_head), walk_v(vecs, lane, kVec, c.v_head), walk_out(vecs, lane, kVec, head_stride);
+        const int place = there ? static_cast<int>(static_cast<unsigned>(at) % c.page_size) : 0;
+        const In *k = reinterpret_cast<const In *>(c.k) + (there ? page * c.k_page + place * c.k_token : 0) + head0 * c.k_head + walk_k.column * kVec;
+        const In *v = reinterpret_cast<const In *>(c.v) + (there ? page * c.v_page + place * c.v_token : 0) + head0 * c.v_head + walk_v.column * kVec;
+        long long to = row * token_stride + head0 * head_stride + walk_out.column * kVec;
+        const long long scales = kCodes && there ? static_cast<long long>(page) * c.heads * c.blocks + place / c.block : 0;
+        int head = head0;
+        for (int u = lane; u < total; u += 32 * kTurn) {
+            Values<In, kVec> a[kTurn], b[kTurn];
+            float scale_a[kTurn], scale_b[kTurn];
 #pragma unroll
-                for (int i = 0; i < kVec; ++i) k_to[head * head_stride + d + i] = v_to[head * head_stride + d + i] = from_float<Out>(0.f);
+            for (int j = 0; j < kTurn; ++j) {
+                scale_a[j] = scale_b[j] = 0.f;
+                if (there && u + 32 * j < total) {
+                    a[j].load(k);
+                    b[j].load(v);
+                    if (kCodes) {
+                        scale_a[j] = c.k_scales[scales + head * c.blocks];
+                        scale_b[j] = c.v_scales[scales + head * c.blocks];
+                    }
+                }
+                head += head_step + (walk_k.column + walk_k.right >= vecs);
+                walk_k.next(k);
+                walk_v.next(v);
+            }
+#pragma unroll
+            for (int j = 0; j < kTurn; ++j) {
+                if (u + 32 * j < total) {
+                    if (there) {
+                        a[j].store(k_out + to, scale_a[j]);
+                        b[j].store(v_out + to, scale_b[j]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < kVec; ++i) k_out[to + i] = v_out[to + i] = from_float<Out>(0.f);
+                    }
+                }
+                const Out *next = k_out + to;
+                walk_out.next(next);
+                to = next - k_out;
             }
         }
     }

@@ -15,7 +15,18 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kTable = 1024;             // planes of a block's tokens at most
-constexpr int kAhead = 4;                // vector pairs of a thread on their way together
+constexpr int kAhead = 2;                // vector pairs of a thread on their way together
+
+// Division of numbers below 2^31 by a number that the launch knows: (high half of n * factor + n) >> shift.
+struct Divisor {
+    uint32_t by, factor;
+    int shift;
+    explicit Divisor(uint32_t d) : by(d), shift(0) {
+        while (1ull << shift < d) ++shift;
+        factor = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+    }
+    __device__ __forceinline__ int quotient(int n) const { return static_cast<int>((__umulhi(static_cast<uint32_t>(n), factor) + static_cast<uint32_t>(n)) >> shift); }
+};
 
 struct RotaryParams {
     const uint8_t *x;
@@ -25,6 +36,7 @@ struct RotaryParams {
     long long tokens, x_token, x_head, y_token, y_head;
     int heads, dim, half, wide_positions, tokens_of_block, heads_of_block;
     float magnitude;
+    Divisor per_head, heads_in, kept;                            // items of a head, heads of a block, vectors of a head that are not turned (1: none)
 };
 
 // V values side by side (V = 1: of tensors without 16-byte alignment)
@@ -35,7 +47,7 @@ template <typename T, int V> __device__ __forceinline__ void copy_values(T *to, 
 
 // An item is V planes of a head of a token: values i.. and half + i.. of it, or, interleaved, 2 V values side by side.
 template <typename T, int V, bool kInterleaved>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
+__global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const __grid_constant__ RotaryParams p) {
     __shared__ __align__(16) float cosine[kTable], sine[kTable];
     pdl_enter();
     const long long first_token = static_cast<long long>(blockIdx.x) * p.tokens_of_block;
@@ -43,7 +55,8 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
     const int first_head = blockIdx.y * p.heads_of_block, heads = min(p.heads_of_block, p.heads - first_head);
     const T *x = reinterpret_cast<const T *>(p.x) + first_token * p.x_token + first_head * p.x_head;
     T *y = reinterpret_cast<T *>(p.y) + first_token * p.y_token + first_head * p.y_head;
-    const int per_head = p.half / V, per_token = per_head * heads, items = per_token * tokens;
+    // (the last block's heads may be fewer: items are counted as if they were not, and left out)
+    const int per_head = static_cast<int>(p.per_head.by), items = per_head * static_cast<int>(p.heads_in.by) * tokens;
     const int apart = kInterleaved ? V : p.half;
     bool made = false;
     for (int base = threadIdx.x; !made || base - static_cast<int>(threadIdx.x) < items; base += kThreads * kAhead) {
@@ -53,11 +66,11 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
             const int item = base + u * kThreads;
-            if (item >= items) break;
-            const int token = item / per_token, rest = item - token * per_token, head = rest / per_head, i = (rest - head * per_head) * V;
+            const int row = p.per_head.quotient(item), token = p.heads_in.quotient(row), head = row - token * static_cast<int>(p.heads_in.by), i = (item - row * per_head) * V;
+            plane[u] = item < items && head < heads ? token * p.half + i : -1;
+            if (plane[u] < 0) continue;
             const int at = kInterleaved ? 2 * i : i;
             const T *from = x + token * p.x_token + head * p.x_head + at;
-            plane[u] = token * p.half + i;
             to[u] = token * p.y_token + head * p.y_head + at;
             copy_values<T, V>(pair[u].v, from);
             copy_values<T, V>(pair[u].v + V, from + apart);
@@ -78,7 +91,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
         }
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            if (base + u * kThreads >= items) break;
+            if (plane[u] < 0) continue;
             float c[V], s[V];
             if constexpr (V == 1) {
                 c[0] = cosine[plane[u]];
@@ -103,20 +116,22 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
         }
     }
     // what is not turned
-    const int kept = (p.dim - 2 * p.half) / V;
-    if (kept == 0 || (p.x == p.y && p.x_token == p.y_token && p.x_head == p.y_head)) return;
-    const int kept_of_token = kept * heads;
-    for (int item = threadIdx.x; item < kept_of_token * tokens; item += kThreads) {
-        const int token = item / kept_of_token, rest = item - token * kept_of_token, head = rest / kept, i = 2 * p.half + (rest - head * kept) * V;
-        copy_values<T, V>(y + token * p.y_token + head * p.y_head + i, x + token * p.x_token + head * p.x_head + i);
+    if (p.dim == 2 * p.half || (p.x == p.y && p.x_token == p.y_token && p.x_head == p.y_head)) return;
+    const int kept = static_cast<int>(p.kept.by);
+    for (int item = threadIdx.x; item < kept * static_cast<int>(p.heads_in.by) * tokens; item += kThreads) {
+        const int row = p.kept.quotient(item), token = p.heads_in.quotient(row), head = row - token * static_cast<int>(p.heads_in.by), i = 2 * p.half + (item - row * kept) * V;
+        if (head < heads) copy_values<T, V>(y + token * p.y_token + head * p.y_head + i, x + token * p.x_token + head * p.x_head + i);
     }
 }
 
 template <typename T>
-cudaError_t launch(const MsnhB200Ctx *ctx, const MsnhB200Rotary &a, const RotaryParams &p, dim3 grid, void *stream) {
+cudaError_t launch(const MsnhB200Ctx *ctx, const MsnhB200Rotary &a, RotaryParams p, dim3 grid, void *stream) {
     constexpr int V = 16 / sizeof(T);
     bool wide = p.half % V == 0 && p.dim % V == 0 && aligned16(a.x) && aligned16(a.y);
     for (const long long stride : {p.x_token, p.x_head, p.y_token, p.y_head}) wide = wide && stride % V == 0;
+    p.per_head = Divisor(p.half / (wide ? V : 1));
+    p.heads_in = Divisor(p.heads_of_block);
+    p.kept = Divisor(std::max(1, (p.dim - 2 * p.half) / (wide ? V : 1)));
     if (wide) return a.interleaved ? launch_token_kernel(rotary_kernel<T, V, true>, grid, kThreads, 0, stream, ctx->pdl, p)
                                    : launch_token_kernel(rotary_kernel<T, V, false>, grid, kThreads, 0, stream, ctx->pdl, p);
     return a.interleaved ? launch_token_kernel(rotary_kernel<T, 1, true>, grid, kThreads, 0, stream, ctx->pdl, p)
@@ -143,7 +158,7 @@ extern "C" int msnh_b200_rotary(MsnhB200Ctx *ctx, const MsnhB200Rotary *a, void 
     CUDA_TRY(ctx, scope.status);
     RotaryParams p = {static_cast<const uint8_t *>(a->x), static_cast<uint8_t *>(a->y), a->positions, reinterpret_cast<const unsigned long long *>(a->turns), a->tokens,
                       a->x_token_stride, a->x_head_stride, a->y_token_stride, a->y_head_stride, a->heads, a->dim, a->rotary_dim / 2, a->wide_positions, 1, a->heads,
-                      a->magnitude};
+                      a->magnitude, Divisor(1), Divisor(1), Divisor(1)};
     // A block's tokens: as many as there are threads for their planes, up to eight, where that leaves every SM some blocks. Few tokens: their heads in
     // parts, as long as a part has an item for each thread.
     const long long most = std::max(1, std::min(8, kThreads / p.half));

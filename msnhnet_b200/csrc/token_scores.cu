@@ -76,6 +76,60 @@ struct Sums {
     }
 };
 
+// Two fp32 numbers in a register pair, and their arithmetic in one instruction.
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pair_of(float a, float b) {
+    Pair r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void parts_of(Pair p, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ Pair add(Pair a, Pair b) {
+    Pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Pair multiply(Pair a, Pair b) {
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Pair multiply_add(Pair a, Pair b, Pair c) {
+    Pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+// The largest (NaN where one is) and the smallest value of a 16-byte chunk.
+template <typename T> struct Range;
+template <> struct Range<float> {
+    float low, high;
+    __device__ __forceinline__ explicit Range(const uint4 &raw) {
+        const float a = __uint_as_float(raw.x), b = __uint_as_float(raw.y), c = __uint_as_float(raw.z), d = __uint_as_float(raw.w);
+        high = max_or_nan(max_or_nan(a, b), max_or_nan(c, d));
+        low = fminf(fminf(a, b), fminf(c, d));
+    }
+};
+template <typename T2> __device__ __forceinline__ T2 two_of(uint32_t word) { return reinterpret_cast<const T2 &>(word); }
+template <> struct Range<__half> {
+    float low, high;
+    __device__ __forceinline__ explicit Range(const uint4 &raw) {
+        const __half2 a = two_of<__half2>(raw.x), b = two_of<__half2>(raw.y), c = two_of<__half2>(raw.z), d = two_of<__half2>(raw.w);
+        const __half2 top = __hmax2_nan(__hmax2_nan(a, b), __hmax2_nan(c, d)), least = __hmin2(__hmin2(a, b), __hmin2(c, d));
+        high = max_or_nan(__low2float(top), __high2float(top));
+        low = fminf(__low2float(least), __high2float(least));
+    }
+};
+template <> struct Range<__nv_bfloat16> {
+    float low, high;
+    __device__ __forceinline__ explicit Range(const uint4 &raw) {
+        const __nv_bfloat162 a = two_of<__nv_bfloat162>(raw.x), b = two_of<__nv_bfloat162>(raw.y), c = two_of<__nv_bfloat162>(raw.z), d = two_of<__nv_bfloat162>(raw.w);
+        const __nv_bfloat162 top = __hmax2_nan(__hmax2_nan(a, b), __hmax2_nan(c, d)), least = __hmin2(__hmin2(a, b), __hmin2(c, d));
+        high = max_or_nan(__low2float(top), __high2float(top));
+        low = fminf(__low2float(least), __high2float(least));
+    }
+};
+
 // Across a warp's lanes: the larger keys of a pair at distance `o` to the lower lanes.
 __device__ __forceinline__ Key exchange(Key mine, int o, bool larger) {
     const Key other = __shfl_xor_sync(~0u, mine, o);
@@ -125,14 +179,13 @@ template <typename T> struct Row {
     __device__ __forceinline__ bool whole(int chunk) const { return (chunk > 0 || shift == 0) && first_of(chunk) <= cols - kVec; }
     __device__ __forceinline__ uint4 load_whole(int chunk) const { return *reinterpret_cast<const uint4 *>(at + first_of(chunk)); }
     // places that are not the row's hold `none`
-    __device__ __forceinline__ void load(int chunk, float (&v)[kVec], float none) const {
-        if (whole(chunk)) {
-            Vec16<T>::unpack(load_whole(chunk), v);
-        } else {
-            const int first = first_of(chunk);
+    __device__ __forceinline__ uint4 load(int chunk, float none) const {
+        if (whole(chunk)) return load_whole(chunk);
+        const int first = first_of(chunk);
+        uint4 raw;
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) v[i] = first + i >= 0 && first + i < cols ? to_float(at[first + i]) : none;
-        }
+        for (int i = 0; i < kVec; ++i) reinterpret_cast<T *>(&raw)[i] = first + i >= 0 && first + i < cols ? at[first + i] : from_float<T>(none);
+        return raw;
     }
 };
 
@@ -153,39 +206,63 @@ __global__ void __launch_bounds__(kThreads) token_scores_kernel(const __grid_con
         const int per_part = (row.chunks + kCluster - 1) / kCluster, begin = min(part * per_part, row.chunks), end = min(begin + per_part, row.chunks);
         Sums mine = {-INFINITY, 0.f, 0.f};
         int best = begin + threadIdx.x;                          // the first chunk that has the maximum
-        const auto take = [&](const float (&v)[kVec], int chunk) {
-            float top = v[0];
+        // kCount chunks of the thread, kThreads apart
+        const auto take = [&](const auto &raw, int chunk) {
+            constexpr int kCount = sizeof(raw) / sizeof(uint4);
+            float high[kCount], top, low;
 #pragma unroll
-            for (int i = 1; i < kVec; ++i) top = max_or_nan(top, v[i]);
+            for (int u = 0; u < kCount; ++u) {
+                const Range<T> range(raw[u]);
+                high[u] = range.high;
+                top = u == 0 ? range.high : max_or_nan(top, range.high);
+                low = u == 0 ? range.low : fminf(low, range.low);
+            }
             if (!(top <= mine.top)) {
                 mine.lift(top);
                 best = chunk;
+#pragma unroll
+                for (int u = kCount - 1; u >= 0; --u)
+                    if (high[u] == top) best = chunk + u * kThreads;
             }
             if (mine.top == -INFINITY) return;                   // (nothing but -infinity so far)
+            const bool near = low >= mine.top - kFar;
+            const Pair minus = pair_of(-1.f, -1.f), scale = pair_of(-kLog2e, -kLog2e), reference = pair_of(mine.top, mine.top);
+            Pair sum = 0, more = 0;
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) {
-                const float d = fminf(mine.top - v[i], kFar), e = pow2(d * -kLog2e);
-                mine.sum += e;
-                mine.more = fmaf(e, d, mine.more);
+            for (int u = 0; u < kCount; ++u) {
+                float v[kVec];
+                Vec16<T>::unpack(raw[u], v);
+#pragma unroll
+                for (int i = 0; i < kVec; i += 2) {
+                    Pair d = multiply_add(pair_of(v[i], v[i + 1]), minus, reference);
+                    float a, b;
+                    if (!near) {
+                        parts_of(d, a, b);
+                        d = pair_of(fminf(a, kFar), fminf(b, kFar));
+                    }
+                    parts_of(multiply(d, scale), a, b);
+                    const Pair e = pair_of(pow2(a), pow2(b));
+                    sum = add(sum, e);
+                    more = multiply_add(e, d, more);
+                }
             }
+            float a, b;
+            parts_of(sum, a, b);
+            mine.sum += a + b;
+            parts_of(more, a, b);
+            mine.more += a + b;
         };
         for (int c = begin + threadIdx.x; c < end; c += kThreads * kAhead) {
             if (row.whole(c) && c + kThreads * (kAhead - 1) < end && row.whole(c + kThreads * (kAhead - 1))) {
                 uint4 raw[kAhead];
 #pragma unroll
                 for (int u = 0; u < kAhead; ++u) raw[u] = row.load_whole(c + u * kThreads);
-#pragma unroll
-                for (int u = 0; u < kAhead; ++u) {
-                    float v[kVec];
-                    Vec16<T>::unpack(raw[u], v);
-                    take(v, c + u * kThreads);
-                }
+                take(raw, c);
             } else {
 #pragma unroll 1
                 for (int u = 0; u < kAhead && c + u * kThreads < end; ++u) {
-                    float v[kVec];
-                    row.load(c + u * kThreads, v, -INFINITY);
-                    take(v, c + u * kThreads);
+                    const uint4 raw[1] = {row.load(c + u * kThreads, -INFINITY)};
+                    take(raw, c + u * kThreads);
                 }
             }
         }
@@ -205,7 +282,7 @@ __global__ void __launch_bounds__(kThreads) token_scores_kernel(const __grid_con
                 for (int base = first; base < end; base += kThreads * 32) {
                     const int c = base + lane * kThreads;
                     float v[kVec];
-                    if (c < end) row.load(c, v, __uint_as_float(0x7fffffffu));
+                    if (c < end) Vec16<T>::unpack(row.load(c, __uint_as_float(0x7fffffffu)), v);
 #pragma unroll
                     for (int i = 0; i < kVec; ++i) {
                         // (what is not of the row is NaN here, and so not above the threshold; neither is a NaN of the row, whose ids are -1 anyway)
@@ -288,7 +365,8 @@ cudaError_t launch(const MsnhB200Ctx *ctx, const ScoreParams &p, void *stream) {
     return cudaLaunchKernelEx(&config, token_scores_kernel<T, kThreads, kCluster>, p);
 }
 
-// Blocks of a row: as many as leave every SM two, each with 4096 logits at least. Short rows: 128 threads.
+// Blocks of a row: as many as leave every SM two, each with 4096 logits at least. Short rows: 128 threads; rows that a block has to itself: 256,
+// since what follows the pass over the logits grows with the warps.
 template <typename T>
 cudaError_t launch_by_size(const MsnhB200Ctx *ctx, const ScoreParams &p, void *stream) {
     if (p.cols <= 4096) return launch<T, 128, 1>(ctx, p, stream);
@@ -296,7 +374,7 @@ cudaError_t launch_by_size(const MsnhB200Ctx *ctx, const ScoreParams &p, void *s
     if (parts >= 8) return launch<T, 512, 8>(ctx, p, stream);
     if (parts >= 4) return launch<T, 512, 4>(ctx, p, stream);
     if (parts >= 2) return launch<T, 512, 2>(ctx, p, stream);
-    return launch<T, 512, 1>(ctx, p, stream);
+    return launch<T, 256, 1>(ctx, p, stream);
 }
 
 }  // namespace

@@ -30,6 +30,23 @@ __device__ __forceinline__ uint16_t to_e4m3x2(float a, float b) {
     return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }
 
+// two of four codes to two fp16 values, which hold all codes
+__device__ __forceinline__ uint32_t halves_low(uint32_t codes) {
+    uint32_t r;
+    asm("{ .reg .b16 low, high; mov.b32 {low, high}, %1; cvt.rn.f16x2.e4m3x2 %0, low; }" : "=r"(r) : "r"(codes));
+    return r;
+}
+__device__ __forceinline__ uint32_t halves_high(uint32_t codes) {
+    uint32_t r;
+    asm("{ .reg .b16 low, high; mov.b32 {low, high}, %1; cvt.rn.f16x2.e4m3x2 %0, high; }" : "=r"(r) : "r"(codes));
+    return r;
+}
+__device__ __forceinline__ void to_floats(uint32_t codes, float (&v)[4]) {
+    const uint32_t low = halves_low(codes), high = halves_high(codes);
+    const float2 a = __half22float2(reinterpret_cast<const __half2 &>(low)), b = __half22float2(reinterpret_cast<const __half2 &>(high));
+    v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+}
+
 // kVec values of T in 16 bytes
 template <typename T> struct Vec16 {
     static constexpr int kVec = 16 / sizeof(T);
