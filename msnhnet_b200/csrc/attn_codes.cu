@@ -136,6 +136,7 @@ template <int kDim, int kStages> struct CodeRing {
 template <typename T, int kDim_, int kGroups_, int kStages_, int kWarps_, int kBlocks_> struct CodeHeads {
     using Type = T;
     using Ring = CodeRing<kDim_, kStages_>;
+    static constexpr bool kEarly = false;
     static constexpr int kDim = kDim_, kStages = kStages_, kGroups = kGroups_, kWarps = kWarps_, kBlocks = kBlocks_;
     static constexpr int kParts = std::is_same<T, float>::value ? 2 : 1;       // fp16 parts of a query's value
     static constexpr float kLift = 14.f;                                       // factors are taken times 2^14: they are below 2, and fp16 goes to 2^16
@@ -340,9 +341,9 @@ template <typename T>
 cudaError_t launch_type(const MsnhB200Ctx *ctx, const AttnParams &p, int blocks, void *stream) {
     constexpr int kMany = std::is_same<T, float>::value ? 1 : 2;               // (a pair has 8 heads of fp32 queries at most)
     const bool few = p.chunk <= 8;
-    if (p.c.dim <= 32) return few ? launch<CodeHeads<T, 32, 1, 8, 4, 2>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 32, kMany, 8, 4, 2>>(ctx, p, blocks, stream);
-    if (p.c.dim <= 64) return few ? launch<CodeHeads<T, 64, 1, 6, 4, 2>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 64, kMany, 6, 4, 2>>(ctx, p, blocks, stream);
-    if (p.c.dim <= 96) return few ? launch<CodeHeads<T, 96, 1, 4, 4, 2>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 96, kMany, 4, 4, 2>>(ctx, p, blocks, stream);
+    if (p.c.dim <= 32) return few ? launch<CodeHeads<T, 32, 1, 7, 4, 3>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 32, kMany, 7, 4, 3>>(ctx, p, blocks, stream);
+    if (p.c.dim <= 64) return few ? launch<CodeHeads<T, 64, 1, 4, 4, 3>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 64, kMany, 4, 4, 3>>(ctx, p, blocks, stream);
+    if (p.c.dim <= 96) return few ? launch<CodeHeads<T, 96, 1, 2, 4, 3>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 96, kMany, 2, 4, 3>>(ctx, p, blocks, stream);
     if (p.c.dim <= 128) return few ? launch<CodeHeads<T, 128, 1, 3, 4, 2>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 128, kMany, 3, 4, 2>>(ctx, p, blocks, stream);
     if (p.c.dim <= 192) return few ? launch<CodeHeads<T, 192, 1, 4, 4, 1>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 192, kMany, 4, 4, 1>>(ctx, p, blocks, stream);
     return few ? launch<CodeHeads<T, 256, 1, 3, 4, 1>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 256, kMany, 3, 4, 1>>(ctx, p, blocks, stream);
@@ -350,7 +351,7 @@ cudaError_t launch_type(const MsnhB200Ctx *ctx, const AttnParams &p, int blocks,
 
 }  // namespace
 
-BlockShape block_shape_codes(int dim) { return {4, dim <= 128 ? 2 : 1}; }
+BlockShape block_shape_codes(int dim) { return {4, dim < 128 ? 3 : dim == 128 ? 2 : 1}; }
 
 cudaError_t launch_codes(const MsnhB200Ctx *ctx, const AttnParams &p, int dtype, int blocks, void *stream) {
     return dtype == MSNH_B200_F32 ? launch_type<float>(ctx, p, blocks, stream) : dtype == MSNH_B200_F16 ? launch_type<__half>(ctx, p, blocks, stream)

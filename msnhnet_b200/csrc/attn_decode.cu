@@ -36,6 +36,7 @@ constexpr int kWholeTiles = 8;
 template <typename T, int kDim_, int kGroups_, int kStages_, int kBlocks_> struct TensorHeads {
     using Type = T;
     using Ring = attn::Ring<T, kDim_, kStages_>;
+    static constexpr bool kEarly = true;
     static constexpr int kDim = kDim_, kStages = kStages_, kGroups = kGroups_, kWarps = 4, kBlocks = kBlocks_;
     // fp16 weights are taken times 2^14, so that a weight of 2^-29 of the largest is still a normal number (sum and values carry the
     // same factor); what a weight loses when it is rounded to the cache's type goes into a second product. Both parts are above 0 where the
@@ -163,6 +164,7 @@ template <typename T, int kDim_, int kGroups_, int kStages_, int kBlocks_> struc
 template <int kDim_, int kHeads_, int kStages_, int kWarps_> struct PlainHeads {
     using Type = float;
     using Ring = attn::Ring<float, kDim_, kStages_>;
+    static constexpr bool kEarly = true;
     static constexpr int kDim = kDim_, kStages = kStages_, kWarps = kWarps_, kHeads = kHeads_, kBlocks = 1, kTile = Ring::kTile;
     static constexpr int kColumns = kDim / 32, kVec = kColumns % 4 == 0 ? 4 : kColumns % 2 == 0 ? 2 : 1;
 

@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(Heads::kWarps * 32, Heads::kBlocks) attn_decod
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ Side<Heads> side;
     constexpr int kWarps = Heads::kWarps, kThreads = kWarps * 32, kStages = Heads::kStages;
-    pdl_enter();
+    if (Heads::kEarly) pdl_enter(); else pdl_wait();
     const int pairs = p.c.heads * p.chunks, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     int line = 0;
     for (int base = 0; base < p.rows; base += kThreads) {
@@ -387,6 +387,7 @@ __global__ void __launch_bounds__(Heads::kWarps * 32, Heads::kBlocks) attn_decod
         }
         more = walk.next(piece);
     }
+    if (!Heads::kEarly) pdl_launch_dependents();
 }
 
 template <typename Heads>
