@@ -344,14 +344,14 @@ cudaError_t launch_type(const MsnhB200Ctx *ctx, const AttnParams &p, int blocks,
     if (p.c.dim <= 32) return few ? launch<CodeHeads<T, 32, 1, 7, 4, 3>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 32, kMany, 7, 4, 3>>(ctx, p, blocks, stream);
     if (p.c.dim <= 64) return few ? launch<CodeHeads<T, 64, 1, 4, 4, 3>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 64, kMany, 4, 4, 3>>(ctx, p, blocks, stream);
     if (p.c.dim <= 96) return few ? launch<CodeHeads<T, 96, 1, 2, 4, 3>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 96, kMany, 2, 4, 3>>(ctx, p, blocks, stream);
-    if (p.c.dim <= 128) return few ? launch<CodeHeads<T, 128, 1, 3, 4, 2>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 128, kMany, 3, 4, 2>>(ctx, p, blocks, stream);
+    if (p.c.dim <= 128) return few ? launch<CodeHeads<T, 128, 1, 2, 4, 3>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 128, kMany, 2, 4, 3>>(ctx, p, blocks, stream);
     if (p.c.dim <= 192) return few ? launch<CodeHeads<T, 192, 1, 4, 4, 1>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 192, kMany, 4, 4, 1>>(ctx, p, blocks, stream);
     return few ? launch<CodeHeads<T, 256, 1, 3, 4, 1>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 256, kMany, 3, 4, 1>>(ctx, p, blocks, stream);
 }
 
 }  // namespace
 
-BlockShape block_shape_codes(int dim) { return {4, dim < 128 ? 3 : dim == 128 ? 2 : 1}; }
+BlockShape block_shape_codes(int dim) { return {4, dim <= 128 ? 3 : 1}; }
 
 cudaError_t launch_codes(const MsnhB200Ctx *ctx, const AttnParams &p, int dtype, int blocks, void *stream) {
     return dtype == MSNH_B200_F32 ? launch_type<float>(ctx, p, blocks, stream) : dtype == MSNH_B200_F16 ? launch_type<__half>(ctx, p, blocks, stream)
