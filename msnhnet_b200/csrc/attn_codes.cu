@@ -27,7 +27,7 @@ __device__ __forceinline__ float load_shared(uint32_t at) {
 template <int kDim, int kStages> struct CodeRing {
     static constexpr int kTile = kCodeTile, kRuns = kTile / 8, kAhead = 32 / kRuns;
     static constexpr int kSide = kTile * kDim, kStage = 2 * kSide + 2 * kTile * 4, kBytes = kStages * kStage;
-    static constexpr int kPieces = kDim / 16;
+    static constexpr int kPieces = kDim / 16, kRows = 32 % kPieces == 0 ? 32 / kPieces : 0;
 
     // The piece of a row in which its column-th one lies.
     static __device__ __forceinline__ int piece_of(int row, int column) {
@@ -62,7 +62,7 @@ template <int kDim, int kStages> struct CodeRing {
     __device__ __forceinline__ void look_ahead(int first_tile, int tiles) {
         next = -1;
         const int token = origin + first_tile * kTile + lane * 8;
-        if (first_tile + lane / kRuns < tiles && c.page_size % 8 == 0 && token >= first && token + 8 <= last) {
+        if (first_tile + lane / kRuns < tiles && c.page_size % 8 == 0 && token >= first && token + 8 <= last && c.k_token < 1 << 27 && c.v_token < 1 << 27) {
             next = table[token / c.page_size];
             if (next >= c.n_pages) next = -1;
         }
@@ -81,22 +81,39 @@ template <int kDim, int kStages> struct CodeRing {
         const uint32_t to = base + stage * kStage, to_scales = to + 2 * kSide + lane * 4;
         const int from = tile % kAhead * kRuns;
         if ((runs >> from & ((1u << kRuns) - 1)) == (1u << kRuns) - 1) {
+            // (rows of a run are less than 2^31 bytes apart, or it is none)
             const uint8_t *k_run[kRuns], *v_run[kRuns];
 #pragma unroll
             for (int r = 0; r < kRuns; ++r) {
                 k_run[r] = k + __shfl_sync(~0u, at_k, from + r);
                 v_run[r] = v + __shfl_sync(~0u, at_v, from + r);
             }
+            const int k_token = static_cast<int>(c.k_token), v_token = static_cast<int>(c.v_token);
+            if constexpr (kRows > 0 && kRows <= 8) {             // a warp copies kRows whole rows at a time
+                const int row0 = lane / kPieces, column = lane % kPieces;
+                const int inside = min(column, c.dim / 16 - 1) * 16, bytes = column < c.dim / 16 ? 16 : 0;
+                const int off_k = row0 * k_token + inside, off_v = row0 * v_token + inside;
+                const uint32_t at = to + row0 * kDim;
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i) {
-                const int row = (lane + 32 * i) / kPieces, column = (lane + 32 * i) % kPieces;
-                constexpr int kRow = 8 * kPieces;                // pieces of a run
-                const int low = 32 * i / kRow, high = (32 * i + 31) / kRow;
-                const int inside = min(column, c.dim / 16 - 1) * 16;
-                const int bytes = column < c.dim / 16 ? 16 : 0;
-                const uint32_t at = to + row * kDim + piece_of(row, column) * 16;
-                copy16(at, (row / 8 == low ? k_run[low] : k_run[high]) + row % 8 * c.k_token + inside, bytes);
-                copy16(at + kSide, (row / 8 == low ? v_run[low] : v_run[high]) + row % 8 * c.v_token + inside, bytes);
+                for (int i = 0; i < kPieces; ++i) {
+                    constexpr int kStep = kRows > 0 ? kRows : 1;
+                    const int more = i * kStep % 8, run = i * kStep / 8;
+                    const uint32_t there = at + i * kStep * kDim + piece_of(row0 + more, column) * 16;
+                    copy16(there, k_run[run] + (off_k + more * k_token), bytes);
+                    copy16(there + kSide, v_run[run] + (off_v + more * v_token), bytes);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i) {
+                    const int row = (lane + 32 * i) / kPieces, column = (lane + 32 * i) % kPieces;
+                    constexpr int kRow = 8 * kPieces;            // pieces of a run
+                    const int low = 32 * i / kRow, high = (32 * i + 31) / kRow;
+                    const int inside = min(column, c.dim / 16 - 1) * 16;
+                    const int bytes = column < c.dim / 16 ? 16 : 0;
+                    const uint32_t at = to + row * kDim + piece_of(row, column) * 16;
+                    copy16(at, (row / 8 == low ? k_run[low] : k_run[high]) + (row % 8 * k_token + inside), bytes);
+                    copy16(at + kSide, (row / 8 == low ? v_run[low] : v_run[high]) + (row % 8 * v_token + inside), bytes);
+                }
             }
             const int its_page = __shfl_sync(~0u, page, from + lane / 8), its_place = __shfl_sync(~0u, place, from + lane / 8) + lane % 8;
             const long long scale = static_cast<long long>(its_page) * (c.heads * c.blocks) + block_of(its_place);
@@ -130,13 +147,25 @@ template <int kDim, int kStages> struct CodeRing {
     }
 };
 
+// A value's scale: factor * 2^power, the factor's magnitude from 1 to 2 (0 for 0).
+struct Scale {
+    float power, factor;
+    __device__ __forceinline__ explicit Scale(float v) {
+        const int exponent = max(static_cast<int>(__float_as_uint(v) >> 23 & 255), 1);
+        power = static_cast<float>(exponent - 127);
+        factor = exponent < 254 ? v * __uint_as_float(static_cast<uint32_t>(254 - exponent) << 23) : v * 1.17549435e-38f * 0.5f;
+    }
+    __device__ __forceinline__ float times(float more) const { return factor * pow2(power + more); }
+};
+
 // Lane l holds, of a tile's scores, tokens l / 4, + 8, + 16 and + 24 of heads 2 (l % 4) and + 1; of a block of 16 value columns the same two heads of
 // columns 2 (l / 4) and + 1. A head's values are contracted in an order of the codes' own: a lane's four codes of a token lie side by side,
 // two of them are the fragment's lower columns and two its upper ones, and so it is with the queries.
 template <typename T, int kDim_, int kGroups_, int kStages_, int kWarps_, int kBlocks_> struct CodeHeads {
     using Type = T;
     using Ring = CodeRing<kDim_, kStages_>;
-    static constexpr bool kEarly = false;
+    static constexpr bool kEarly = false;                                      // (the joining launch's blocks would take the room of a next call's)
+    static constexpr int kBegin = kCodeStart;
     static constexpr int kDim = kDim_, kStages = kStages_, kGroups = kGroups_, kWarps = kWarps_, kBlocks = kBlocks_;
     static constexpr int kParts = std::is_same<T, float>::value ? 2 : 1;       // fp16 parts of a query's value
     static constexpr float kLift = 14.f;                                       // factors are taken times 2^14: they are below 2, and fp16 goes to 2^16
@@ -204,20 +233,20 @@ template <typename T, int kDim_, int kGroups_, int kStages_, int kWarps_, int kB
     __device__ __forceinline__ void tile(uint32_t keys, uint32_t values, int mask, int lane, int, float *) {
         constexpr int kFour = Ring::kTile / 8;                                  // tokens of a lane
         const uint32_t scales = keys + 2 * Ring::kSide + lane / 4 * 4;
-        float key_scale[kFour], factor[kFour], power[kFour];                   // a value's scale is factor * 2^power
-        bool even = mask == -1;
+        float key_scale[kFour], value_scale[kFour];
 #pragma unroll
         for (int t = 0; t < kFour; ++t) {
             key_scale[t] = load_shared(scales + t * 32);
-            const float v = load_shared(scales + kFour * 32 + t * 32);
-            const int exponent = max(static_cast<int>(__float_as_uint(v) >> 23 & 255), 1);
-            power[t] = static_cast<float>(exponent - 127);
-            factor[t] = exponent < 254 ? v * __uint_as_float(static_cast<uint32_t>(254 - exponent) << 23) : v * 1.17549435e-38f * 0.5f;
-            even &= power[t] == power[0];
+            value_scale[t] = load_shared(scales + kFour * 32 + t * 32);
         }
-        // whether all of the tile's values have one power: then the largest factor is the one of the largest score
-        const float first_power = __shfl_sync(~0u, power[0], 0);
-        even = __all_sync(~0u, even && power[0] == first_power);
+        // Whether the tile's halves of 16 values have one scale each, and powers that are near one another (blocks of 16 tokens and more, mostly): then
+        // a factor is a weight times one of two numbers.
+        const float scale_low = __shfl_sync(~0u, value_scale[0], 0), scale_high = __shfl_sync(~0u, value_scale[kFour / 2], 0);
+        bool even = mask == -1;
+#pragma unroll
+        for (int t = 0; t < kFour; ++t) even &= value_scale[t] == (t < kFour / 2 ? scale_low : scale_high);
+        const Scale parts[2] = {Scale(scale_low), Scale(scale_high)};
+        even = __all_sync(~0u, even) && fabsf(parts[0].power - parts[1].power) <= 4.f;
         float s[kGroups][kFour / 2][4] = {};
         const uint32_t at_k = keys + lane % 16 * kDim;
 #pragma unroll
@@ -240,49 +269,75 @@ template <typename T, int kDim_, int kGroups_, int kStages_, int kWarps_, int kB
         float keep[kGroups][2];
 #pragma unroll
         for (int n = 0; n < kGroups; ++n) {
-            float base[2], from[2];
 #pragma unroll
             for (int t = 0; t < kFour; ++t)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float &x = s[n][t / 2][t % 2 * 2 + h];
-                    x *= scale[n][h] * key_scale[t];
-                    if (mask != -1 && !(mask >> (lane / 4 + t * 8) & 1)) x = -INFINITY;
-                }
+                for (int h = 0; h < 2; ++h) s[n][t / 2][t % 2 * 2 + h] *= scale[n][h] * key_scale[t];
+            if (mask != -1) {
+#pragma unroll
+                for (int t = 0; t < kFour; ++t)
+                    if (!(mask >> (lane / 4 + t * 8) & 1)) s[n][t / 2][t % 2 * 2] = s[n][t / 2][t % 2 * 2 + 1] = -INFINITY;
+            }
+            float factors[kFour][2], now_best[2];
+            bool near = even;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                float most = -INFINITY, most_factor = -INFINITY;
+                float most = s[n][0][h];
 #pragma unroll
-                for (int t = 0; t < kFour; ++t) most = fmaxf(most, s[n][t / 2][t % 2 * 2 + h]);
-                most = warp_max(most);
-                if (even) {
-                    most_factor = most + first_power;
-                } else {
-#pragma unroll
-                    for (int t = 0; t < kFour; ++t) most_factor = fmaxf(most_factor, s[n][t / 2][t % 2 * 2 + h] + power[t]);
-                    most_factor = warp_max(most_factor);
-                }
-                const float now = fmaxf(ceilf(most), top[n][h]), now_factor = fmaxf(ceilf(most_factor), best[n][h]);
-                base[h] = now == -INFINITY ? 0.f : now;
-                from[h] = now_factor == -INFINITY ? 0.f : now_factor - kLift;
+                for (int t = 1; t < kFour; ++t) most = fmaxf(most, s[n][t / 2][t % 2 * 2 + h]);
+                const float here = ceilf(warp_max(most)), now = fmaxf(here, top[n][h]), base = now == -INFINITY ? 0.f : now;
                 sum[n][h] *= now == top[n][h] ? 1.f : pow2(top[n][h] - now);
-                keep[n][h] = now_factor == best[n][h] ? 1.f : pow2(best[n][h] - now_factor);
-                grown |= now_factor != best[n][h];
+                now_best[h] = here + fmaxf(parts[0].power, parts[1].power);
+                near &= now - here <= 64.f;                      // (not where a score is no number)
                 top[n][h] = now;
-                best[n][h] = now_factor;
                 float more = 0.f;
 #pragma unroll
-                for (int t = 0; t < kFour; ++t) more += pow2(s[n][t / 2][t % 2 * 2 + h] - base[h]);
+                for (int t = 0; t < kFour; ++t) more += factors[t][h] = pow2(s[n][t / 2][t % 2 * 2 + h] - base);
                 sum[n][h] += more;
+            }
+            if (__all_sync(~0u, near)) {
+                // weights relative to the scores' reference become factors relative to their own: what is 0 of them here is 0 there, too, since the
+                // references are less than 2^64 apart
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float now = fmaxf(now_best[h], best[n][h]), from = top[n][h] - now + kLift;
+                    const float low_part = parts[0].times(from), high_part = parts[1].times(from);
+#pragma unroll
+                    for (int t = 0; t < kFour; ++t) factors[t][h] *= t < kFour / 2 ? low_part : high_part;
+                    now_best[h] = now;
+                }
+            } else {
+                float power[kFour], factor[kFour];
+#pragma unroll
+                for (int t = 0; t < kFour; ++t) {
+                    const Scale v(value_scale[t]);
+                    power[t] = v.power;
+                    factor[t] = v.factor;
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float most = -INFINITY;
+#pragma unroll
+                    for (int t = 0; t < kFour; ++t) most = fmaxf(most, s[n][t / 2][t % 2 * 2 + h] + power[t]);
+                    now_best[h] = fmaxf(ceilf(warp_max(most)), best[n][h]);
+                    const float from = now_best[h] == -INFINITY ? 0.f : now_best[h] - kLift;
+#pragma unroll
+                    for (int t = 0; t < kFour; ++t) factors[t][h] = pow2(s[n][t / 2][t % 2 * 2 + h] - (from - power[t])) * factor[t];
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                keep[n][h] = now_best[h] == best[n][h] ? 1.f : pow2(best[n][h] - now_best[h]);
+                grown |= now_best[h] != best[n][h];
+                best[n][h] = now_best[h];
             }
 #pragma unroll
             for (int t = 0; t < kFour; ++t) {                    // two heads of a token to two tokens of a head
-                const float a = pow2(s[n][t / 2][t % 2 * 2] - (from[0] - power[t])) * factor[t], b = pow2(s[n][t / 2][t % 2 * 2 + 1] - (from[1] - power[t])) * factor[t];
-                const uint32_t pair = pack2<__half>(a, b);
+                const uint32_t pair = pack2<__half>(factors[t][0], factors[t][1]);
                 float high_a, high_b;
                 unpack2<__half>(pair, high_a, high_b);
                 high[n][t] = transposed(pair);
-                low[n][t] = transposed(pack2<__half>(a - high_a, b - high_b));
+                low[n][t] = transposed(pack2<__half>(factors[t][0] - high_a, factors[t][1] - high_b));
             }
         }
         if (__any_sync(~0u, grown)) {

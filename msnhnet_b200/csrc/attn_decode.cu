@@ -37,6 +37,7 @@ template <typename T, int kDim_, int kGroups_, int kStages_, int kBlocks_> struc
     using Type = T;
     using Ring = attn::Ring<T, kDim_, kStages_>;
     static constexpr bool kEarly = true;
+    static constexpr int kBegin = kStart;
     static constexpr int kDim = kDim_, kStages = kStages_, kGroups = kGroups_, kWarps = 4, kBlocks = kBlocks_;
     // fp16 weights are taken times 2^14, so that a weight of 2^-29 of the largest is still a normal number (sum and values carry the
     // same factor); what a weight loses when it is rounded to the cache's type goes into a second product. Both parts are above 0 where the
@@ -165,6 +166,7 @@ template <int kDim_, int kHeads_, int kStages_, int kWarps_> struct PlainHeads {
     using Type = float;
     using Ring = attn::Ring<float, kDim_, kStages_>;
     static constexpr bool kEarly = true;
+    static constexpr int kBegin = kStart;
     static constexpr int kDim = kDim_, kStages = kStages_, kWarps = kWarps_, kHeads = kHeads_, kBlocks = 1, kTile = Ring::kTile;
     static constexpr int kColumns = kDim / 32, kVec = kColumns % 4 == 0 ? 4 : kColumns % 2 == 0 ? 2 : 1;
 
@@ -291,8 +293,8 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_co
     const int pairs = p.c.heads * p.chunks, dim = p.c.dim;
     const int before = p.prefix[row], after = p.prefix[row + 1], line = p.prefix[p.rows], length = (after - before) / pairs;
     if (length == 0) return;
-    const int share = share_of(line, workers), unit = before + (kv * p.chunks + chunk) * length;
-    const int first = (unit + kStart) / share, last = (unit + length - 1) / share;
+    const int share = share_of(line, workers, p.start), unit = before + (kv * p.chunks + chunk) * length;
+    const int first = (unit + p.start) / share, last = (unit + length - 1) / share;
     if (first == last) return;                                   // (finished by its warp)
     const int parts = last - first + 1, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     float top = -INFINITY, sum = 0.f;
@@ -361,7 +363,7 @@ AttnPlan plan_of(const MsnhB200Ctx *ctx, const MsnhB200KvCache &c, const MsnhB20
     const long long tiles = (seen + tile - 1) / tile + (a.window > 0);        // (a window may start inside a tile)
     l.tiles = tiles;
     l.whole = tiles <= kWholeTiles;
-    const long long row_tiles = (tiles + kStart) * c.n_kv_heads * l.chunks;
+    const long long row_tiles = (tiles + (c.dtype == MSNH_B200_E4M3 ? kCodeStart : kStart)) * c.n_kv_heads * l.chunks;
     l.rows = static_cast<int>(std::min<long long>(std::min(a.rows, kMaxRows), ((1LL << 30) - 1) / row_tiles));
     if (l.rows == 0) return l;                                   // (a row alone is too long)
     const long long pairs = static_cast<long long>(l.rows) * c.n_kv_heads * l.chunks;
@@ -406,7 +408,7 @@ constexpr int kManyParts = 32;
 template <typename T>
 cudaError_t launch_join(const MsnhB200Ctx *ctx, const AttnParams &p, int workers, long long tiles, void *stream) {
     const dim3 grid(p.rows, p.n_heads);
-    const long long parts = std::min<long long>(workers / (static_cast<long long>(p.rows) * p.c.heads * p.chunks), (tiles + kStart) / (kStart + kLeast));
+    const long long parts = std::min<long long>(workers / (static_cast<long long>(p.rows) * p.c.heads * p.chunks), (tiles + p.start) / (p.start + kLeast));
     return parts < kManyParts ? launch_token_kernel(attn_join_kernel<T, kJoinFew>, grid, kJoinFew, 0, stream, ctx->pdl, p, workers)
                               : launch_token_kernel(attn_join_kernel<T, kJoinMany>, grid, kJoinMany, 0, stream, ctx->pdl, p, workers);
 }
@@ -451,7 +453,7 @@ int msnh_b200_attn_decode(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, const Msnh
     CUDA_TRY(ctx, scope.status);
     uint8_t *work = static_cast<uint8_t *>(a->workspace);
     AttnParams p = {kv_params(*c), static_cast<const uint8_t *>(a->q), static_cast<uint8_t *>(a->out), a->lse, a->seqs, a->q_row_stride, a->q_head_stride,
-                    a->out_row_stride, a->out_head_stride, 0, a->n_heads, l.each, l.chunk, l.chunks, a->window, 0, l.whole, a->scale,
+                    a->out_row_stride, a->out_head_stride, 0, a->n_heads, l.each, l.chunk, l.chunks, a->window, 0, l.whole, c->dtype == MSNH_B200_E4M3 ? kCodeStart : kStart, a->scale,
                     reinterpret_cast<int *>(work), reinterpret_cast<float2 *>(work + l.ml_at), reinterpret_cast<float *>(work + l.part_at)};
     for (int row = 0; row < a->rows; row += l.rows) {
         p.first_row = row;

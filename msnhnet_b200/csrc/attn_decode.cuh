@@ -12,6 +12,9 @@ constexpr int kMaxRows = 256;                // rows of a launch: what they see 
 // of 500 tokens 9.7, 10.8 and 13.1 us, 16 of them 17.2, 16.5 and 18.0, one of 65536 beside 63 of 100 76.7, 75.2 and 75.7, one of 4000 14.2,
 // 14.8 and 16.1; 16 of 4000 and more tokens are the same within 1 %.
 constexpr int kStart = 3, kLeast = 2;
+// The same of 8-bit codes, whose tiles are of 32 tokens and go by faster than a pair's start does: 48 rows of up to 8192 tokens (and two of up to 131072)
+// take 46.4, 41.5, 36.4, 34.4 and 36.3 us (62.9, 62.7, 62.7, 62.8 and 60.1) with 1, 2, 3, 5 and 8.
+constexpr int kCodeStart = 5;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct AttnParams {
@@ -23,7 +26,7 @@ struct AttnParams {
     long long q_row, q_head, out_row, out_head;
     int rows, n_heads, each, chunk, chunks, window;      // each: query heads of a key head; chunk: how many of them a pair has
     int first_row;                                       // of this launch
-    int whole;
+    int whole, start;                                    // start: tiles that a pair's start counts for
     float scale;
     int *prefix;                                         // workspace: the line's tiles before each row (rows + 1), then the parts
     float2 *part_ml;                                     // [slot][chunk] maximum and sum
@@ -42,8 +45,8 @@ template <int kTile> __device__ __forceinline__ int tiles_of(const Row &r) { ret
 
 // The share of a warp, in tiles of the line. (A launch's line has less than 2^30 tiles: code for longer ones is a microsecond of reading
 // instructions alone.)
-__device__ __forceinline__ int share_of(int line, int workers) {
-    return max((line + workers - 1) / workers, kStart + kLeast);
+__device__ __forceinline__ int share_of(int line, int workers, int start) {
+    return max((line + workers - 1) / workers, start + kLeast);
 }
 
 // 16 bytes to shared memory, of which the first `bytes` are copied (16 or none) and the others are 0
@@ -223,14 +226,14 @@ template <typename Heads> struct Side {
 
 // A warp's walk along its share: pieces of pairs, one after the other.
 template <typename Heads> struct Walk {
-    static constexpr int kTile = Heads::Ring::kTile;
+    static constexpr int kTile = Heads::Ring::kTile, kBegin = Heads::kBegin;
     const AttnParams &p;
     const Side<Heads> &side;
     int left;                                                    // of the share
     int row, pair, pairs, at, length;                            // where it stands: row (of the launch), pair, tile of the line within it
     int worker;
 
-    __device__ __forceinline__ int length_of(int r) const { return p.whole ? 1 : (side.last[r] - 1) / kTile - side.first[r] / kTile + 1 + kStart; }
+    __device__ __forceinline__ int length_of(int r) const { return p.whole ? 1 : (side.last[r] - 1) / kTile - side.first[r] / kTile + 1 + kBegin; }
     // tiles [begin, end) of the row's tiles; slot of the workspace or -1
     struct Piece { int row, pair, begin, end, slot; };
     __device__ __forceinline__ bool next(Piece &piece) {
@@ -243,8 +246,8 @@ template <typename Heads> struct Walk {
                 piece.end = (side.last[row] - 1) / kTile - side.first[row] / kTile + 1;
                 piece.slot = -1;
             } else {
-                piece.begin = max(0, at - kStart);
-                piece.end = to - kStart;
+                piece.begin = max(0, at - kBegin);
+                piece.end = to - kBegin;
                 piece.slot = piece.begin == 0 && to == length ? -1 : 2 * worker + (piece.begin == 0);
             }
             left -= to - at;
@@ -280,7 +283,7 @@ __global__ void __launch_bounds__(Heads::kWarps * 32, Heads::kBlocks) attn_decod
             side.last[i] = r.last;
         }
         const int tiles = tiles_of<R::kTile>(r);
-        const int mine = tiles == 0 ? 0 : (p.whole ? 1 : tiles + kStart) * pairs;
+        const int mine = tiles == 0 ? 0 : (p.whole ? 1 : tiles + Heads::kBegin) * pairs;
         int sum = mine;
 #pragma unroll
         for (int o = 1; o < 32; o *= 2) {
@@ -311,7 +314,7 @@ __global__ void __launch_bounds__(Heads::kWarps * 32, Heads::kBlocks) attn_decod
         }
     // the share; neighbours in the line are in different blocks, so that a short line is spread over the SMs
     const int workers = gridDim.x * kWarps, worker = warp * gridDim.x + blockIdx.x;
-    const int share = p.whole ? (line + workers - 1) / workers : share_of(line, workers), unit = worker * share;
+    const int share = p.whole ? (line + workers - 1) / workers : share_of(line, workers, Heads::kBegin), unit = worker * share;
     if (unit >= line) return;
     int low = 0;                                                 // the last row that begins at or before the share
     for (int step = kMaxRows / 32; step; step = step == kMaxRows / 32 ? 1 : 0) {
