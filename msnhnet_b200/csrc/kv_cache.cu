@@ -258,8 +258,8 @@ __device__ __forceinline__ bool is_power(float scale) {
     return (bits & 0x807fffffu) == 0 && bits >= 0x00800000u && bits <= 0x7e800000u;
 }
 
-// A lane's walk over the pieces of some rows, 32 pieces a step.
-struct RowWalk {
+// A lane's walk over the pieces of some rows, 32 pieces a step. kWhole: a step is whole rows.
+template <bool kWhole> struct RowWalk {
     int vecs, right, column;
     long long step, wrap;                                        // between pieces; more where the step passes a row's end
     __device__ __forceinline__ RowWalk(int vecs_, int lane, int per_vec, long long row_step) : vecs(vecs_), right(32 % vecs_), column(lane % vecs_) {
@@ -268,39 +268,42 @@ struct RowWalk {
     }
     template <typename P> __device__ __forceinline__ void next(P *&at) {
         at += step;
-        column += right;
-        if (column >= vecs) { column -= vecs; at += wrap; }
+        if constexpr (!kWhole) {
+            column += right;
+            if (column >= vecs) { column -= vecs; at += wrap; }
+        }
     }
 };
+// What the append's warps divide by.
+struct AppendDivisors { Divisor heads, block, page; };
 
 constexpr int kHeld = 8;               // pieces of new values that a lane keeps between the maximum and the codes
 
 // A warp for the call's tokens in one block of scales of one head, keys or values: their largest magnitude, the scale, the block's older
 // codes by the new scale where that has grown, the new codes.
-template <typename T, int kVec>
+template <typename T, int kVec, bool kWhole>
 __global__ void __launch_bounds__(256, kVec > 1 ? 3 : 1) kv_append_codes_kernel(KvParams c, const int *seqs, const int *starts, int n, const AppendWork *work, const T *k_new,
-                                                                                 const T *v_new, long long token_stride, long long head_stride, long long most_blocks) {
+                                                                                 const T *v_new, long long token_stride, long long head_stride, int total, AppendDivisors by) {
     using Pieces = Piece<T, kVec>;
+    using Walk = RowWalk<kWhole>;
     pdl_enter();
     const int lane = threadIdx.x % 32, vecs = c.dim / kVec;
-    const long long total = most_blocks * c.heads * 2;
-    for (long long w = (blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x) / 32; w < total; w += static_cast<long long>(gridDim.x) * blockDim.x / 32) {
-        const long long pair = w / c.heads;
-        const int head = static_cast<int>(w - pair * c.heads), unit = static_cast<int>(pair / 2);
+    for (long long at_w = (blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x) / 32; at_w < total; at_w += static_cast<long long>(gridDim.x) * blockDim.x / 32) {
+        const int w = static_cast<int>(at_w), pair = by.heads.quotient(w), head = w - pair * c.heads, unit = pair / 2;
         const bool values = pair % 2;
         const int i = starts ? last_not_above(n, unit, lane, [&](int at) { return work[at].block; }) : unit;
         const int before = work[i].start, first = starts ? starts[i] : i, count = starts ? starts[i + 1] - first : 1;
         if (before < 0 || count <= 0) continue;
-        const long long block = before / c.block + (starts ? unit - work[i].block : 0), begin = block * c.block;
+        const long long block = by.block.quotient(before) + (starts ? unit - work[i].block : 0), begin = block * c.block;
         const long long last = min(begin + c.block, before + static_cast<long long>(count));
         if (last <= begin) continue;                             // (the bound on blocks is not reached)
         const int from = static_cast<int>(max(begin, static_cast<long long>(before))), to = static_cast<int>(last);
-        const int page = c.table[(seqs ? seqs[i] : i) * c.table_stride + from / c.page_size];
+        const int nth = by.page.quotient(from), page = c.table[(seqs ? seqs[i] : i) * c.table_stride + nth];
         if (page < 0 || page >= c.n_pages) continue;
-        const int place = from % c.page_size, older = from - static_cast<int>(begin);
+        const int place = from - nth * c.page_size, older = from - static_cast<int>(begin);
         const long long token_step = values ? c.v_token : c.k_token;
         uint8_t *codes = values ? c.v + page * c.v_page + head * c.v_head + place * c.v_token : c.k + page * c.k_page + head * c.k_head + place * c.k_token;
-        float *scale_at = (values ? c.v_scales : c.k_scales) + (static_cast<long long>(page) * c.heads + head) * c.blocks + place / c.block;
+        float *scale_at = (values ? c.v_scales : c.k_scales) + (static_cast<long long>(page) * c.heads + head) * c.blocks + by.block.quotient(place);
         const float had = older ? *scale_at : 0.f;
         const T *source = (values ? v_new : k_new) + (first + from - before) * token_stride + head * head_stride;
         const int pieces = (to - from) * vecs;
@@ -308,7 +311,7 @@ __global__ void __launch_bounds__(256, kVec > 1 ? 3 : 1) kv_append_codes_kernel(
         Pieces held[kHeld];
         uint32_t top = 0;
         {
-            RowWalk walk(vecs, lane, kVec, token_stride);
+            Walk walk(vecs, lane, kVec, token_stride);
             const T *at = source + lane / vecs * token_stride + walk.column * kVec;
 #pragma unroll
             for (int j = 0; j < kHeld; ++j) {
@@ -330,7 +333,7 @@ __global__ void __launch_bounds__(256, kVec > 1 ? 3 : 1) kv_append_codes_kernel(
         const bool odd = top >= 0x7f800000u;                     // a NaN or infinity: once more without them
         if (odd) {
             top = 0;
-            RowWalk walk(vecs, lane, kVec, token_stride);
+            Walk walk(vecs, lane, kVec, token_stride);
             const T *at = source + lane / vecs * token_stride + walk.column * kVec;
 #pragma unroll 1
             for (int u = lane; u < pieces; u += 32) {
@@ -346,7 +349,7 @@ __global__ void __launch_bounds__(256, kVec > 1 ? 3 : 1) kv_append_codes_kernel(
         const float inverse = power ? 1.f / scale : 0.f;
         if (older && scale != had) {
             const auto again = [&](float x) { return power ? x * had * inverse : x * had / scale; };
-            RowWalk walk(vecs, lane, kVec, token_step);
+            Walk walk(vecs, lane, kVec, token_step);
             uint8_t *at = codes + (lane / vecs - older) * token_step + walk.column * kVec;
 #pragma unroll 1
             for (int u = lane; u < older * vecs; u += 32) {
@@ -356,7 +359,7 @@ __global__ void __launch_bounds__(256, kVec > 1 ? 3 : 1) kv_append_codes_kernel(
                 walk.next(at);
             }
         }
-        RowWalk walk(vecs, lane, kVec, token_step);
+        Walk walk(vecs, lane, kVec, token_step);
         uint8_t *at = codes + lane / vecs * token_step + walk.column * kVec;
         if (power && !odd) {
             const auto code = [&](float x) { return x * inverse; };
@@ -366,7 +369,7 @@ __global__ void __launch_bounds__(256, kVec > 1 ? 3 : 1) kv_append_codes_kernel(
                 walk.next(at);
             }
             if (pieces > 32 * kHeld) {
-                RowWalk again(vecs, lane, kVec, token_stride);
+                Walk again(vecs, lane, kVec, token_stride);
                 const T *from_new = source + lane / vecs * token_stride + again.column * kVec;
                 for (int j = 0; j < kHeld; ++j) again.next(from_new);
 #pragma unroll 1
@@ -383,7 +386,7 @@ __global__ void __launch_bounds__(256, kVec > 1 ? 3 : 1) kv_append_codes_kernel(
                 if (!isfinite(x)) return __uint_as_float(0x7fffffffu);
                 return scale == 0.f ? 0.f * x : x / scale;
             };
-            RowWalk again(vecs, lane, kVec, token_stride);
+            Walk again(vecs, lane, kVec, token_stride);
             const T *from_new = source + lane / vecs * token_stride + again.column * kVec;
 #pragma unroll 1
             for (int u = lane; u < pieces; u += 32) {
@@ -435,9 +438,9 @@ template <typename In, int kVec> struct Values {
 };
 
 // A warp a row of the output: keys and values of all heads of one token, kTurn pieces of each on their way together.
-template <typename In, typename Out, int kVec>
+template <typename In, typename Out, int kVec, bool kWhole>
 __global__ void __launch_bounds__(256) kv_read_kernel(KvParams c, const int *seqs, const int *starts, const int *firsts, int n, Out *k_out, Out *v_out, long long token_stride,
-                                                      long long head_stride, int n_rows) {
+                                                      long long head_stride, int n_rows, Divisor by_page, Divisor by_block) {
     constexpr bool kCodes = sizeof(In) == 1;
     constexpr int kTurn = kVec > 1 && sizeof(In) <= 2 ? 4 : 2;
     pdl_enter();
@@ -450,16 +453,20 @@ __global__ void __launch_bounds__(256) kv_read_kernel(KvParams c, const int *seq
             const int s = seqs ? seqs[i] : i;
             if (r >= starts[i] && r < starts[i + 1] && s >= 0 && s < c.n_seqs) {
                 at = static_cast<long long>(r) - starts[i] + (firsts ? firsts[i] : 0);
-                if (at >= 0 && at < min(static_cast<long long>(c.lengths[s]), static_cast<long long>(c.max_pages) * c.page_size)) page = c.table[s * c.table_stride + at / c.page_size];
+                if (at >= 0 && at < min(static_cast<long long>(c.lengths[s]), static_cast<long long>(c.max_pages) * c.page_size)) {
+                    const int nth = by_page.quotient(static_cast<int>(at));
+                    page = c.table[s * c.table_stride + nth];
+                    at -= static_cast<long long>(nth) * c.page_size;
+                }
             }
         }
         const bool there = page >= 0 && page < c.n_pages;
-        RowWalk walk_k(vecs, lane, kVec, c.k_head), walk_v(vecs, lane, kVec, c.v_head), walk_out(vecs, lane, kVec, head_stride);
-        const int place = there ? static_cast<int>(static_cast<unsigned>(at) % c.page_size) : 0;
+        RowWalk<kWhole> walk_k(vecs, lane, kVec, c.k_head), walk_v(vecs, lane, kVec, c.v_head), walk_out(vecs, lane, kVec, head_stride);
+        const int place = there ? static_cast<int>(at) : 0;
         const In *k = reinterpret_cast<const In *>(c.k) + (there ? page * c.k_page + place * c.k_token : 0) + head0 * c.k_head + walk_k.column * kVec;
         const In *v = reinterpret_cast<const In *>(c.v) + (there ? page * c.v_page + place * c.v_token : 0) + head0 * c.v_head + walk_v.column * kVec;
         long long to = row * token_stride + head0 * head_stride + walk_out.column * kVec;
-        const long long scales = kCodes && there ? static_cast<long long>(page) * c.heads * c.blocks + place / c.block : 0;
+        const long long scales = kCodes && there ? static_cast<long long>(page) * c.heads * c.blocks + by_block.quotient(place) : 0;
         int head = head0;
         for (int u = lane; u < total; u += 32 * kTurn) {
             Values<In, kVec> a[kTurn], b[kTurn];
@@ -475,7 +482,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(KvParams c, const int *seq
                         scale_b[j] = c.v_scales[scales + head * c.blocks];
                     }
                 }
-                head += head_step + (walk_k.column + walk_k.right >= vecs);
+                head += head_step + (!kWhole && walk_k.column + walk_k.right >= vecs);
                 walk_k.next(k);
                 walk_v.next(v);
             }
@@ -778,7 +785,7 @@ int msnh_b200_kv_append_as(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, const int
     if (const int rc = check_workspace(ctx, *c, n, workspace, workspace_bytes, "kv_append")) return rc;
     // blocks of scales that n_tokens tokens of n sequences lie in, at most
     const long long most_blocks = codes ? starts ? n_tokens / c->scale_block + 2LL * std::min(n, n_tokens) : n : 0;
-    if (most_blocks > 0x7fffffff) return fail(ctx, MSNH_B200_ERR_UNSUPPORTED, "kv_append: 2^31 blocks of scales and more");
+    if (most_blocks > 0x7fffffff / 2 / c->n_kv_heads) return fail(ctx, MSNH_B200_ERR_UNSUPPORTED, "kv_append: 2^31 scales and more");
     DeviceScope scope(ctx->device);
     CUDA_TRY(ctx, scope.status);
     AppendWork *work = static_cast<AppendWork *>(workspace);
@@ -789,16 +796,16 @@ int msnh_b200_kv_append_as(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, const int
     const size_t size = dtype_size(new_dtype);
     const bool aligned = aligned16(k_new) && aligned16(v_new) && new_token_stride * size % 16 == 0 && new_head_stride * size % 16 == 0;
     if (codes) {
-        const dim3 grid(blocks_for(ctx, most_blocks * c->n_kv_heads * 2, 8));
-        const auto write = [&](auto type, auto vec) {
-            using T = decltype(type);
-            constexpr int kVec = decltype(vec)::value;
-            return launch_token_kernel(kv_append_codes_kernel<T, kVec>, grid, 256, 0, stream, ctx->pdl, p, seqs, starts, n, work, static_cast<const T *>(k_new), static_cast<const T *>(v_new),
-                                       new_token_stride, new_head_stride, most_blocks);
-        };
+        const int total = static_cast<int>(most_blocks * c->n_kv_heads * 2);
+        const dim3 grid(blocks_for(ctx, total, 8));
+        const AppendDivisors by = {Divisor(c->n_kv_heads), Divisor(c->scale_block), Divisor(c->page_size)};
         const bool wide = aligned && kv_rows_multiple_of(*c, 16 / size);
+        const bool whole = wide && 32 % (c->head_dim * size / 16) == 0;
         const auto by_type = [&](auto type) {
-            return wide ? write(type, std::integral_constant<int, 16 / sizeof(type)>()) : write(type, std::integral_constant<int, 1>());
+            using T = decltype(type);
+            constexpr int kVec = 16 / sizeof(T);
+            return launch_token_kernel(!wide ? kv_append_codes_kernel<T, 1, false> : whole ? kv_append_codes_kernel<T, kVec, true> : kv_append_codes_kernel<T, kVec, false>, grid, 256, 0,
+                                       stream, ctx->pdl, p, seqs, starts, n, work, static_cast<const T *>(k_new), static_cast<const T *>(v_new), new_token_stride, new_head_stride, total, by);
         };
         CUDA_TRY(ctx, new_dtype == MSNH_B200_F32 ? by_type(float()) : new_dtype == MSNH_B200_F16 ? by_type(__half()) : by_type(__nv_bfloat16()));
         return MSNH_B200_OK;
@@ -838,8 +845,9 @@ int msnh_b200_kv_read(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, const int32_t 
     const auto read = [&](auto in, auto out) {
         using In = decltype(in);
         using Out = decltype(out);
-        return launch_token_kernel(wide ? kv_read_kernel<In, Out, kVec> : kv_read_kernel<In, Out, 1>, grid, 256, 0, stream, ctx->pdl, p, seqs, starts, first, n, static_cast<Out *>(k_out),
-                                   static_cast<Out *>(v_out), out_token_stride, out_head_stride, n_rows);
+        return launch_token_kernel(!wide ? kv_read_kernel<In, Out, 1, false> : 32 % (c->head_dim / kVec) == 0 ? kv_read_kernel<In, Out, kVec, true> : kv_read_kernel<In, Out, kVec, false>, grid,
+                                   256, 0, stream, ctx->pdl, p, seqs, starts, first, n, static_cast<Out *>(k_out), static_cast<Out *>(v_out), out_token_stride, out_head_stride, n_rows,
+                                   Divisor(c->page_size), Divisor(p.block ? p.block : 1));
     };
     const auto from = [&](auto in) { return out_dtype == MSNH_B200_F32 ? read(in, float()) : out_dtype == MSNH_B200_F16 ? read(in, __half()) : read(in, __nv_bfloat16()); };
     CUDA_TRY(ctx, c->dtype == MSNH_B200_F32 ? from(float()) : c->dtype == MSNH_B200_F16 ? from(__half()) : c->dtype == MSNH_B200_BF16 ? from(__nv_bfloat16()) : from(__nv_fp8_e4m3()));

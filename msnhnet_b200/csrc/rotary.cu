@@ -17,17 +17,6 @@ constexpr int kThreads = 256;
 constexpr int kTable = 1024;             // planes of a block's tokens at most
 constexpr int kAhead = 2;                // vector pairs of a thread on their way together
 
-// Division of numbers below 2^31 by a number that the launch knows: (high half of n * factor + n) >> shift.
-struct Divisor {
-    uint32_t by, factor;
-    int shift;
-    explicit Divisor(uint32_t d) : by(d), shift(0) {
-        while (1ull << shift < d) ++shift;
-        factor = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
-    }
-    __device__ __forceinline__ int quotient(int n) const { return static_cast<int>((__umulhi(static_cast<uint32_t>(n), factor) + static_cast<uint32_t>(n)) >> shift); }
-};
-
 struct RotaryParams {
     const uint8_t *x;
     uint8_t *y;

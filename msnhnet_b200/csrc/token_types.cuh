@@ -15,6 +15,18 @@ __device__ __forceinline__ void pdl_enter() {
     pdl_launch_dependents();
 }
 
+// Division of numbers below 2^31 by a number that the launch knows: (high half of n * factor + n) >> shift.
+struct Divisor {
+    uint32_t by, factor;
+    int shift;
+    Divisor() = default;
+    explicit Divisor(uint32_t d) : by(d), shift(0) {
+        while (1ull << shift < d) ++shift;
+        factor = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+    }
+    __device__ __forceinline__ int quotient(int n) const { return static_cast<int>((__umulhi(static_cast<uint32_t>(n), factor) + static_cast<uint32_t>(n)) >> shift); }
+};
+
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
