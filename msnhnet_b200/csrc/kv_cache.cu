@@ -277,126 +277,182 @@ template <bool kWhole> struct RowWalk {
 // What the append's warps divide by.
 struct AppendDivisors { Divisor heads, block, page; };
 
-constexpr int kHeld = 8;               // pieces of new values that a lane keeps between the maximum and the codes
+// The call's tokens in one block of scales: where they go, and where they come from.
+struct BlockOfScales {
+    bool there;
+    int page, place, older, count;                               // place of the first new token, older tokens of the block before it, new ones
+    long long first;                                             // row of the first new one
+};
+// For whole warps: every lane has the answer.
+__device__ __forceinline__ BlockOfScales block_of_scales(const KvParams &c, const int *seqs, const int *starts, int n, const AppendWork *work, int unit, int lane,
+                                                         const AppendDivisors &by) {
+    BlockOfScales b = {false, 0, 0, 0, 0, 0};
+    const int i = starts ? last_not_above(n, unit, lane, [&](int at) { return work[at].block; }) : unit;
+    const int before = work[i].start, row = starts ? starts[i] : i, count = starts ? starts[i + 1] - row : 1;
+    if (before < 0 || count <= 0) return b;
+    const long long begin = (by.block.quotient(before) + static_cast<long long>(starts ? unit - work[i].block : 0)) * c.block;
+    const long long last = min(begin + c.block, before + static_cast<long long>(count));
+    if (last <= begin) return b;                                 // (the bound on blocks is not reached)
+    const int from = static_cast<int>(max(begin, static_cast<long long>(before))), nth = by.page.quotient(from);
+    b.page = c.table[(seqs ? seqs[i] : i) * c.table_stride + nth];
+    b.there = b.page >= 0 && b.page < c.n_pages;
+    b.place = from - nth * c.page_size;
+    b.older = from - static_cast<int>(begin);
+    b.count = static_cast<int>(last) - from;
+    b.first = static_cast<long long>(row) + from - before;
+    return b;
+}
 
-// A warp for the call's tokens in one block of scales of one head, keys or values: their largest magnitude, the scale, the block's older
-// codes by the new scale where that has grown, the new codes.
-template <typename T, int kVec, bool kWhole>
-__global__ void __launch_bounds__(256, kVec > 1 ? 3 : 1) kv_append_codes_kernel(KvParams c, const int *seqs, const int *starts, int n, const AppendWork *work, const T *k_new,
-                                                                                 const T *v_new, long long token_stride, long long head_stride, int total, AppendDivisors by) {
-    using Pieces = Piece<T, kVec>;
-    using Walk = RowWalk<kWhole>;
+constexpr int kColumns = 128;          // threads of an appending block
+constexpr int kHeld = 16;              // tokens whose pieces a thread keeps between the maximum and the codes
+
+// A block of threads for one block of scales of some heads, keys and values: a thread has a 16-byte column of a head and goes down the tokens, all of
+// its reads on their way together. The head's largest magnitude, from its columns' threads; the scale; the block's older codes by the new
+// scale where that has grown; the new codes. kWarp: a head's columns are threads of one warp, a power of two of them.
+template <typename T, bool kWarp>
+__global__ void __launch_bounds__(kColumns, 512 / kColumns) kv_append_codes_kernel(KvParams c, const int *seqs, const int *starts, int n, const AppendWork *work, const T *k_new, const T *v_new,
+                                                                 long long token_stride, long long head_stride, int items, Divisor groups, int heads_of_block, AppendDivisors by) {
+    constexpr int kVec = 16 / sizeof(T);
+    using Column = Piece<T, kVec>;
+    __shared__ uint32_t tops[kColumns];
     pdl_enter();
-    const int lane = threadIdx.x % 32, vecs = c.dim / kVec;
-    for (long long at_w = (blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x) / 32; at_w < total; at_w += static_cast<long long>(gridDim.x) * blockDim.x / 32) {
-        const int w = static_cast<int>(at_w), pair = by.heads.quotient(w), head = w - pair * c.heads, unit = pair / 2;
-        const bool values = pair % 2;
-        const int i = starts ? last_not_above(n, unit, lane, [&](int at) { return work[at].block; }) : unit;
-        const int before = work[i].start, first = starts ? starts[i] : i, count = starts ? starts[i + 1] - first : 1;
-        if (before < 0 || count <= 0) continue;
-        const long long block = by.block.quotient(before) + (starts ? unit - work[i].block : 0), begin = block * c.block;
-        const long long last = min(begin + c.block, before + static_cast<long long>(count));
-        if (last <= begin) continue;                             // (the bound on blocks is not reached)
-        const int from = static_cast<int>(max(begin, static_cast<long long>(before))), to = static_cast<int>(last);
-        const int nth = by.page.quotient(from), page = c.table[(seqs ? seqs[i] : i) * c.table_stride + nth];
-        if (page < 0 || page >= c.n_pages) continue;
-        const int place = from - nth * c.page_size, older = from - static_cast<int>(begin);
+    const int lane = threadIdx.x % 32, vecs = c.dim / kVec, mine = threadIdx.x / vecs, column = threadIdx.x - mine * vecs;
+    BlockOfScales next = block_of_scales(c, seqs, starts, n, work, groups.quotient(blockIdx.x), lane, by);
+    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+        const BlockOfScales b = next;
+        const int unit = groups.quotient(item), both = (item - unit * static_cast<int>(groups.by)) * heads_of_block + mine;      // a head of the keys, then of the values
+        const bool active = mine < heads_of_block && both < 2 * c.heads, values = both >= c.heads;
+        const int head = values ? both - c.heads : both;
         const long long token_step = values ? c.v_token : c.k_token;
-        uint8_t *codes = values ? c.v + page * c.v_page + head * c.v_head + place * c.v_token : c.k + page * c.k_page + head * c.k_head + place * c.k_token;
-        float *scale_at = (values ? c.v_scales : c.k_scales) + (static_cast<long long>(page) * c.heads + head) * c.blocks + by.block.quotient(place);
-        const float had = older ? *scale_at : 0.f;
-        const T *source = (values ? v_new : k_new) + (first + from - before) * token_stride + head * head_stride;
-        const int pieces = (to - from) * vecs;
+        uint8_t *codes = (values ? c.v + b.page * c.v_page + head * c.v_head + b.place * c.v_token : c.k + b.page * c.k_page + head * c.k_head + b.place * c.k_token) + column * kVec;
+        float *scale_at = (values ? c.v_scales : c.k_scales) + (static_cast<long long>(b.page) * c.heads + head) * c.blocks + by.block.quotient(b.place);
+        const T *source = (values ? v_new : k_new) + b.first * token_stride + head * head_stride + column * kVec;
+        const int count = active && b.there ? b.count : 0;
 
-        Pieces held[kHeld];
+        Column held[kHeld];
+        const float had = active && b.there && b.older ? *scale_at : 0.f;
+#pragma unroll
+        for (int t = 0; t < kHeld; ++t)
+            if (t < count) held[t].load(source + t * token_stride);
+        // (where the next one is, is looked up while these are on their way)
+        if (item + static_cast<int>(gridDim.x) < items) next = block_of_scales(c, seqs, starts, n, work, groups.quotient(item + gridDim.x), lane, by);
+        if (!b.there) continue;
         uint32_t top = 0;
-        {
-            Walk walk(vecs, lane, kVec, token_stride);
-            const T *at = source + lane / vecs * token_stride + walk.column * kVec;
 #pragma unroll
-            for (int j = 0; j < kHeld; ++j) {
-                if (lane + 32 * j < pieces) held[j].load(at);
-                walk.next(at);
-            }
-#pragma unroll
-            for (int j = 0; j < kHeld; ++j)
-                if (lane + 32 * j < pieces) top = held[j].top(top);
-#pragma unroll 1
-            for (int u = lane + 32 * kHeld; u < pieces; u += 32) {
-                Pieces p;
-                p.load(at);
-                top = p.top(top);
-                walk.next(at);
-            }
+        for (int t = 0; t < kHeld; ++t)
+            if (t < count) top = held[t].top(top);
+#pragma unroll 4
+        for (int t = kHeld; t < count; ++t) {
+            Column p;
+            p.load(source + t * token_stride);
+            top = p.top(top);
         }
-        top = __reduce_max_sync(~0u, Pieces::last(top));
-        const bool odd = top >= 0x7f800000u;                     // a NaN or infinity: once more without them
-        if (odd) {
-            top = 0;
-            Walk walk(vecs, lane, kVec, token_stride);
-            const T *at = source + lane / vecs * token_stride + walk.column * kVec;
-#pragma unroll 1
-            for (int u = lane; u < pieces; u += 32) {
-                Pieces p;
-                p.load(at);
-                top = p.finite_top(top);
-                walk.next(at);
+        top = Column::last(top);
+        const auto over_head = [&](uint32_t top) {               // the head's largest one
+            if constexpr (kWarp) {
+                for (int o = vecs / 2; o; o >>= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
+                return top;
+            } else {
+                __syncthreads();                                 // (what was there has been read)
+                if (column == 0) tops[mine] = 0;
+                __syncthreads();
+                atomicMax(&tops[mine], top);
+                __syncthreads();
+                return tops[mine];
             }
-            top = __reduce_max_sync(~0u, top);
+        };
+        top = over_head(top);
+        const bool odd = top >= 0x7f800000u;                     // a NaN or infinity: once more without them
+        if (__syncthreads_or(odd)) {
+            uint32_t finite = 0;
+            for (int t = 0; t < count; ++t) {
+                Column p;
+                p.load(source + t * token_stride);
+                finite = p.finite_top(finite);
+            }
+            finite = over_head(finite);
+            if (odd) top = finite;
         }
         const float scale = fmaxf(had, scale_of(top));
         const bool power = is_power(scale);
         const float inverse = power ? 1.f / scale : 0.f;
-        if (older && scale != had) {
+        if (active && b.older && scale != had) {
             const auto again = [&](float x) { return power ? x * had * inverse : x * had / scale; };
-            Walk walk(vecs, lane, kVec, token_step);
-            uint8_t *at = codes + (lane / vecs - older) * token_step + walk.column * kVec;
-#pragma unroll 1
-            for (int u = lane; u < older * vecs; u += 32) {
-                Codes<kVec> p;
-                p.load(at);
-                p.store(at, again);
-                walk.next(at);
+            constexpr int kTurn = 8;                             // of them on their way together
+            for (int first = -b.older; first < 0; first += kTurn) {
+                Codes<kVec> p[kTurn];
+#pragma unroll
+                for (int t = 0; t < kTurn; ++t)
+                    if (first + t < 0) p[t].load(codes + (first + t) * token_step);
+#pragma unroll
+                for (int t = 0; t < kTurn; ++t)
+                    if (first + t < 0) p[t].store(codes + (first + t) * token_step, again);
             }
         }
-        Walk walk(vecs, lane, kVec, token_step);
-        uint8_t *at = codes + lane / vecs * token_step + walk.column * kVec;
         if (power && !odd) {
             const auto code = [&](float x) { return x * inverse; };
 #pragma unroll
-            for (int j = 0; j < kHeld; ++j) {
-                if (lane + 32 * j < pieces) held[j].store(at, code);
-                walk.next(at);
-            }
-            if (pieces > 32 * kHeld) {
-                Walk again(vecs, lane, kVec, token_stride);
-                const T *from_new = source + lane / vecs * token_stride + again.column * kVec;
-                for (int j = 0; j < kHeld; ++j) again.next(from_new);
-#pragma unroll 1
-                for (int u = lane + 32 * kHeld; u < pieces; u += 32) {
-                    Pieces p;
-                    p.load(from_new);
-                    p.store(at, code);
-                    again.next(from_new);
-                    walk.next(at);
-                }
+            for (int t = 0; t < kHeld; ++t)
+                if (t < count) held[t].store(codes + t * token_step, code);
+#pragma unroll 4
+            for (int t = kHeld; t < count; ++t) {
+                Column p;
+                p.load(source + t * token_stride);
+                p.store(codes + t * token_step, code);
             }
         } else {
             const auto code = [&](float x) {
                 if (!isfinite(x)) return __uint_as_float(0x7fffffffu);
                 return scale == 0.f ? 0.f * x : x / scale;
             };
-            Walk again(vecs, lane, kVec, token_stride);
-            const T *from_new = source + lane / vecs * token_stride + again.column * kVec;
-#pragma unroll 1
-            for (int u = lane; u < pieces; u += 32) {
-                Pieces p;
-                p.load(from_new);
-                p.store(at, code);
-                again.next(from_new);
-                walk.next(at);
+            for (int t = 0; t < count; ++t) {
+                Column p;
+                p.load(source + t * token_stride);
+                p.store(codes + t * token_step, code);
             }
         }
+        if (active && column == 0) *scale_at = scale;
+    }
+}
+
+// The same for rows of any alignment and length, a value at a time: a warp for a head.
+template <typename T>
+__global__ void __launch_bounds__(256) kv_append_values_kernel(KvParams c, const int *seqs, const int *starts, int n, const AppendWork *work, const T *k_new, const T *v_new,
+                                                               long long token_stride, long long head_stride, int total, AppendDivisors by) {
+    pdl_enter();
+    const int lane = threadIdx.x % 32;
+    for (long long w = (blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x) / 32; w < total; w += static_cast<long long>(gridDim.x) * blockDim.x / 32) {
+        const int pair = by.heads.quotient(static_cast<int>(w)), head = static_cast<int>(w) - pair * c.heads;
+        const bool values = pair % 2;
+        const BlockOfScales b = block_of_scales(c, seqs, starts, n, work, pair / 2, lane, by);
+        if (!b.there) continue;
+        const long long token_step = values ? c.v_token : c.k_token;
+        uint8_t *codes = values ? c.v + b.page * c.v_page + head * c.v_head + b.place * c.v_token : c.k + b.page * c.k_page + head * c.k_head + b.place * c.k_token;
+        float *scale_at = (values ? c.v_scales : c.k_scales) + (static_cast<long long>(b.page) * c.heads + head) * c.blocks + by.block.quotient(b.place);
+        const float had = b.older ? *scale_at : 0.f;
+        const T *source = (values ? v_new : k_new) + b.first * token_stride + head * head_stride;
+        uint32_t top = 0;
+        for (int t = 0; t < b.count; ++t)
+            for (int d = lane; d < c.dim; d += 32) {
+                const uint32_t bits = __float_as_uint(to_float(source[t * token_stride + d])) & 0x7fffffffu;
+                if (bits < 0x7f800000u) top = max(top, bits);
+            }
+        const float scale = fmaxf(had, scale_of(__reduce_max_sync(~0u, top)));
+        for (int t = -b.older; t < b.count; ++t)
+            for (int d = lane; d < c.dim; d += 32) {
+                uint8_t &code = codes[t * token_step + d];
+                float x;
+                if (t < 0) {
+                    if (scale == had) continue;
+                    __nv_fp8_e4m3 old;
+                    old.__x = code;
+                    x = to_float(old) * had / scale;
+                } else {
+                    x = to_float(source[t * token_stride + d]);
+                    x = !isfinite(x) ? __uint_as_float(0x7fffffffu) : scale == 0.f ? 0.f * x : x / scale;
+                }
+                code = static_cast<uint8_t>(to_e4m3x2(x, 0.f));
+            }
         if (lane == 0) *scale_at = scale;
     }
 }
@@ -796,16 +852,19 @@ int msnh_b200_kv_append_as(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, const int
     const size_t size = dtype_size(new_dtype);
     const bool aligned = aligned16(k_new) && aligned16(v_new) && new_token_stride * size % 16 == 0 && new_head_stride * size % 16 == 0;
     if (codes) {
-        const int total = static_cast<int>(most_blocks * c->n_kv_heads * 2);
-        const dim3 grid(blocks_for(ctx, total, 8));
         const AppendDivisors by = {Divisor(c->n_kv_heads), Divisor(c->scale_block), Divisor(c->page_size)};
-        const bool wide = aligned && kv_rows_multiple_of(*c, 16 / size);
-        const bool whole = wide && 32 % (c->head_dim * size / 16) == 0;
+        // a block has as many heads as its threads are columns of
+        const int vecs = static_cast<int>(c->head_dim * size / 16);
+        const bool wide = aligned && kv_rows_multiple_of(*c, 16 / size) && vecs >= 1 && vecs <= kColumns, warps = wide && vecs <= 32 && (vecs & (vecs - 1)) == 0;
+        const int total = static_cast<int>(most_blocks * c->n_kv_heads * 2), heads_of_block = wide ? std::min(kColumns / vecs, 2 * c->n_kv_heads) : 1;
+        const int groups = (2 * c->n_kv_heads + heads_of_block - 1) / heads_of_block, items = static_cast<int>(most_blocks * groups);
         const auto by_type = [&](auto type) {
             using T = decltype(type);
-            constexpr int kVec = 16 / sizeof(T);
-            return launch_token_kernel(!wide ? kv_append_codes_kernel<T, 1, false> : whole ? kv_append_codes_kernel<T, kVec, true> : kv_append_codes_kernel<T, kVec, false>, grid, 256, 0,
-                                       stream, ctx->pdl, p, seqs, starts, n, work, static_cast<const T *>(k_new), static_cast<const T *>(v_new), new_token_stride, new_head_stride, total, by);
+            const T *k = static_cast<const T *>(k_new), *v = static_cast<const T *>(v_new);
+            if (!wide) return launch_token_kernel(kv_append_values_kernel<T>, dim3(blocks_for(ctx, total, 8)), 256, 0, stream, ctx->pdl, p, seqs, starts, n, work, k, v, new_token_stride,
+                                                  new_head_stride, total, by);
+            return launch_token_kernel(warps ? kv_append_codes_kernel<T, true> : kv_append_codes_kernel<T, false>, dim3(blocks_for(ctx, items, 1)), kColumns, 0, stream, ctx->pdl, p, seqs,
+                                       starts, n, work, k, v, new_token_stride, new_head_stride, items, Divisor(groups), heads_of_block, by);
         };
         CUDA_TRY(ctx, new_dtype == MSNH_B200_F32 ? by_type(float()) : new_dtype == MSNH_B200_F16 ? by_type(__half()) : by_type(__nv_bfloat16()));
         return MSNH_B200_OK;
