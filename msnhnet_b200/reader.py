@@ -4,7 +4,8 @@ The net's last feature map is the prefix, one token a cell; every cell sees ever
 before it: norm (with the residual's addition, activations in 8 bits), 4-bit products, the cache, attention. Weights are seeded stand-ins, as the
 nets' are.
 
-    python -m msnhnet_b200.reader [--images N] [--tokens N]      # reads the features of ResNet-18, 224 x 224
+    python -m msnhnet_b200.reader [--images N] [--tokens N] [--cache f16|e4m3] [--positions learned|rotary] [--scores]
+                                                                 # reads the features of ResNet-18, 224 x 224
 """
 import argparse
 import time
@@ -19,11 +20,15 @@ E4M3 = torch.float8_e4m3fn
 class Reader:
     """A decoder of `layers` layers: width features, heads query heads over kv_heads key heads of head_dim, ffn hidden values, vocab tokens.
     At most n_seqs sequences of max_tokens (features and tokens) each, MAX_ROWS of them in a call. What cannot fit raises ValueError
-    before anything is launched."""
+    before anything is launched. cache_dtype: float16, or float8_e4m3fn for half the memory. positions: "learned" ones, added to what is looked at
+    and read, or "rotary": queries and keys are turned by where they are (rotary: further arguments of TokenOps.rotary_table)."""
 
     MAX_ROWS = 64                            # of w4_linear
 
-    def __init__(self, ops, channels=512, width=512, layers=2, heads=8, kv_heads=2, head_dim=64, ffn=1024, vocab=1000, n_seqs=8, max_tokens=256, page=16, seed=1):
+    def __init__(self, ops, channels=512, width=512, layers=2, heads=8, kv_heads=2, head_dim=64, ffn=1024, vocab=1000, n_seqs=8, max_tokens=256, page=16, seed=1,
+                 cache_dtype=torch.float16, positions="learned", rotary=None):
+        if positions not in ("learned", "rotary") or (rotary and positions != "rotary"):
+            raise ValueError(f"positions {positions!r}: 'learned', or 'rotary' with arguments of its own")
         self.ops, self.width, self.heads, self.kv_heads, self.head_dim, self.layers = ops, width, heads, kv_heads, head_dim, layers
         self.vocab, self.n_seqs, self.max_tokens = vocab, n_seqs, max_tokens
         # Tokens of each sequence, at most: the sequences' numbers lie on the GPU, so a step counts for all of them. Where a count reaches
@@ -58,11 +63,18 @@ class Reader:
         self.last_norm = norm()
         self.embedding = (0.5 * normal(vocab, width)).half()
         self.position = (0.5 * normal(max_tokens, width)).half()
+        # (rotary positions turn keys and queries, and nothing is added to what is looked at and read)
+        self.turns = ops.rotary_table(head_dim, **(rotary or {})) if positions == "rotary" else None
         pages = -(-max_tokens // page)
-        self.caches = [ops.new_cache(n_seqs * pages, page, kv_heads, head_dim, n_seqs, pages) for _ in range(layers)]
+        more = {} if cache_dtype == torch.float16 else {"dtype": cache_dtype}
+        self.caches = [ops.new_cache(n_seqs * pages, page, kv_heads, head_dim, n_seqs, pages, **more) for _ in range(layers)]
 
-    def _decode(self, x, seqs, append):
-        """Rows of values through the layers; append(cache, k, v) puts their keys and values down. Returns the logits."""
+    def _placed(self, x, at):
+        """Rows of values with their learned positions; as they are where positions are rotary."""
+        return x + self.position[at] if self.turns is None else x
+
+    def _decode(self, x, seqs, append, at):
+        """Rows of values at positions `at` (int32) through the layers; append(cache, k, v) puts their keys and values down. Returns the logits."""
         ops, rows, h = self.ops, x.shape[0], x
         delta = None
         for w, cache in zip(self.weights, self.caches):
@@ -71,6 +83,9 @@ class Reader:
             else:
                 y, scale, h = ops.rms_norm(delta, w["norm1"], residual=h, residual_out=h, out_dtype=E4M3)
             qkv = ops.w4_linear(y, w["qkv"], x_scale=scale).view(rows, -1, self.head_dim)
+            if self.turns is not None:
+                turned = qkv[:, :self.heads + self.kv_heads]
+                ops.rotary(turned, at, self.turns, out=turned)
             append(cache, qkv[:, self.heads:self.heads + self.kv_heads], qkv[:, self.heads + self.kv_heads:])
             seen = ops.attn_decode(qkv[:, :self.heads], cache, seqs=seqs)
             delta = ops.w4_linear(seen.view(rows, -1), w["out"])
@@ -107,10 +122,11 @@ class Reader:
             raise ValueError(f"{n} cells for sequence {seq}: 1 to {self.MAX_ROWS} cells, {self.n_seqs} sequences")
         self._empty([seq])
         self._take(n, None, [seq])
-        x = self.ops.w4_linear(features.half(), self.project) + self.position[:n]
+        x = self._placed(self.ops.w4_linear(features.half(), self.project), slice(n))
+        at = None if self.turns is None else torch.arange(n, dtype=torch.int32, device=x.device)
         one = torch.tensor([seq], dtype=torch.int32, device=x.device)
         starts = torch.tensor([0, n], dtype=torch.int32, device=x.device)
-        return self._decode(x, one.expand(n).contiguous(), lambda cache, k, v: self.ops.kv_append(cache, k, v, seqs=one, starts=starts))
+        return self._decode(x, one.expand(n).contiguous(), lambda cache, k, v: self.ops.kv_append(cache, k, v, seqs=one, starts=starts), at)
 
     def step(self, ids, seqs):
         """One token (ids: int64 [n], at most 64) behind each of the sequences seqs (int32 [n]); the logits of what follows. A row whose
@@ -122,14 +138,14 @@ class Reader:
             raise ValueError(f"{len(ids)} tokens for {len(seqs)} sequences: as many, and at most {self.MAX_ROWS}")
         self._take(1, seqs, named)
         if named is not None:                                        # (all of them known to be in range)
-            return self._decode(self.embedding[ids] + self.position[self.caches[0].lengths[seqs.long()].long()], seqs,
-                                lambda cache, k, v: self.ops.kv_append(cache, k, v, seqs=seqs))
+            at = self.caches[0].lengths[seqs.long()]
+            return self._decode(self._placed(self.embedding[ids], at.long()), seqs, lambda cache, k, v: self.ops.kv_append(cache, k, v, seqs=seqs), at)
         # (indexes are kept in range: one that is not would end the process's use of the GPU)
         seq, token = seqs.clamp(0, self.n_seqs - 1), ids.clamp(0, self.vocab - 1)
         there = (seq == seqs) & (token == ids)
         at = self.caches[0].lengths.index_select(0, seq).clamp_(0, self.max_tokens - 1)
         seqs = torch.where(there, seqs, -1)
-        logits = self._decode(self.embedding.index_select(0, token) + self.position.index_select(0, at), seqs, lambda cache, k, v: self.ops.kv_append(cache, k, v, seqs=seqs))
+        logits = self._decode(self._placed(self.embedding.index_select(0, token), at), seqs, lambda cache, k, v: self.ops.kv_append(cache, k, v, seqs=seqs), at)
         return torch.where(there[:, None], logits, float("nan"))
 
     def fork(self, src, dst):
@@ -146,26 +162,86 @@ class Reader:
         for cache in self.caches:
             self.ops.kv_compact(cache)
 
-    def read(self, features, n_tokens):
+    def read(self, features, n_tokens, scores=False):
         """The likeliest tokens, one after the other, for each of a list of feature maps [cells, channels]: int64 [maps, n_tokens]. Takes
-        sequences 0, 1, ..., which have to be empty, and forgets them again."""
+        sequences 0, 1, ..., which have to be empty, and forgets them again. With scores: (tokens, logprobs, entropies), both float32
+        [maps, n_tokens]: how likely each token was among all, and how undecided the reader (a token is -1, and its scores NaN, where logits are no
+        numbers)."""
         if not 0 < len(features) <= min(self.n_seqs, self.MAX_ROWS) or n_tokens < 1:
             raise ValueError(f"{n_tokens} tokens for {len(features)} maps: at least one of each, {min(self.n_seqs, self.MAX_ROWS)} maps at most")
         for f in features:
-            if not 0 < f.shape[0] <= self.MAX_ROWS or f.shape[0] + n_tokens - 1 > self.max_tokens:
-                raise ValueError(f"{f.shape[0]} cells and {n_tokens} tokens: at most {self.MAX_ROWS} cells, {self.max_tokens} of both")
+            self._fits(f.shape[0], n_tokens)
         named = list(range(len(features)))
         self._empty(named)
         seqs = torch.arange(len(features), dtype=torch.int32, device=self.position.device)
-        ids = torch.stack([self.look(f, i)[-1].argmax() for i, f in enumerate(features)])
-        said = [ids]
-        for _ in range(n_tokens - 1):
-            ids = self._step(ids, seqs, named).argmax(-1)
-            said.append(ids)
+        logits = torch.stack([self.look(f, i)[-1] for i, f in enumerate(features)])
+        said = []
+        for i in range(n_tokens):
+            if i:
+                logits = self._step(ids, seqs, named)
+            if scores:
+                _, entropy, logprob, best = self.ops.token_scores(logits, top=1)
+                ids = best[:, 0].clamp(min=0)                        # (one that is none is no index)
+                said.append((best[:, 0], logprob[:, 0], entropy))
+            else:
+                ids = logits.argmax(-1)
+                said.append((ids,))
+        self._forgotten(seqs, named)
+        out = tuple(torch.stack(column, 1) for column in zip(*said))
+        return out if scores else out[0]
+
+    def score(self, features, ids, alternatives=0):
+        """How likely the reader takes a text to be: ids [n] behind a feature map [cells, channels]. (logprobs float32 [n], entropies float32
+        [n], top_logprobs, top_ids [n, alternatives] or None), as TokenOps.token_scores gives them. Takes sequence 0, which has to be empty, and
+        forgets it again."""
+        ids = torch.as_tensor(ids, dtype=torch.int64, device=self.position.device)
+        if ids.dim() != 1 or len(ids) < 1:
+            raise ValueError("ids: [n], one token at least")
+        if not 0 <= alternatives <= min(tokens.TokenOps.MAX_TOP, self.vocab):
+            raise ValueError(f"{alternatives} alternatives: at most {min(tokens.TokenOps.MAX_TOP, self.vocab)}")
+        self._fits(features.shape[0], len(ids))
+        self._empty([0])
+        seqs = torch.zeros(1, dtype=torch.int32, device=self.position.device)
+        rows = [self.look(features, 0)[-1:]]
+        for i in range(len(ids) - 1):
+            rows.append(self.step(ids[i:i + 1], seqs))
+        self._forgotten(seqs, [0])
+        return self.ops.token_scores(torch.cat(rows), ids, top=alternatives)
+
+    def save(self, seq):
+        """What the caches hold of a sequence, to be kept elsewhere: a list of (keys, values) [tokens, kv_heads, head_dim], one of each layer
+        (waits for the GPU). Values of an 8-bit cache are float32, which holds them as they are."""
+        if not 0 <= seq < self.n_seqs:
+            raise ValueError(f"sequence {seq} of {self.n_seqs}")
+        n = int(self.caches[0].lengths[seq])
+        device = self.position.device
+        one, starts = (torch.tensor(v, dtype=torch.int32, device=device) for v in ([seq], [0, n]))
+        kept = torch.float32 if self.caches[0].dtype == E4M3 else None
+        return [self.ops.kv_read(cache, starts, n, seqs=one, dtype=kept) for cache in self.caches]
+
+    def restore(self, seq, saved):
+        """Makes the empty sequence `seq` what save gave (of this reader or one of the same shape; on any device)."""
+        if not 0 <= seq < self.n_seqs or len(saved) != self.layers:
+            raise ValueError(f"{len(saved)} layers for sequence {seq}: {self.layers} layers, {self.n_seqs} sequences")
+        n = saved[0][0].shape[0]
+        if any(t.shape != (n, self.kv_heads, self.head_dim) for pair in saved for t in pair):
+            raise ValueError("keys and values of all layers: as many tokens, and the reader's heads")
+        self._empty([seq])
+        self._take(n, None, [seq])
+        device = self.position.device
+        one, starts = (torch.tensor(v, dtype=torch.int32, device=device) for v in ([seq], [0, n]))
+        kind = torch.float32 if self.caches[0].dtype == E4M3 else self.caches[0].dtype
+        for cache, (k, v) in zip(self.caches, saved):
+            self.ops.kv_append(cache, k.to(device, kind).contiguous(), v.to(device, kind).contiguous(), seqs=one, starts=starts)
+
+    def _fits(self, cells, n_tokens):
+        if not 0 < cells <= self.MAX_ROWS or cells + n_tokens - 1 > self.max_tokens:
+            raise ValueError(f"{cells} cells and {n_tokens} tokens: at most {self.MAX_ROWS} cells, {self.max_tokens} of both")
+
+    def _forgotten(self, seqs, named):
         self.forget(seqs)
         for i in named:
             self.most[i] = 0
-        return torch.stack(said, 1)
 
 
 def features_of(net, images, cells=49):
@@ -182,6 +258,9 @@ def main():
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     ap.add_argument("--images", type=int, default=2)
     ap.add_argument("--tokens", type=int, default=24)
+    ap.add_argument("--cache", choices=["f16", "e4m3"], default="f16")
+    ap.add_argument("--positions", choices=["learned", "rotary"], default="learned")
+    ap.add_argument("--scores", action="store_true", help="how likely each token was, and how undecided the reader")
     a = ap.parse_args()
     from . import _ffi, synth, topologies
     from .net import Net
@@ -189,14 +268,20 @@ def main():
     net = Net(text, synth.make_blob(text, synth.load_factors("resnet18")), fp16=True, batch=a.images, flags=_ffi.PLAN_KEEP_ALL)
     features = features_of(net, synth.make_images(a.images, 3, 224, 224))
     net.close()
-    reader = Reader(tokens.TokenOps(), n_seqs=a.images, max_tokens=max(256, features.shape[1] + a.tokens))
+    reader = Reader(tokens.TokenOps(), n_seqs=a.images, max_tokens=max(256, features.shape[1] + a.tokens),
+                    cache_dtype=E4M3 if a.cache == "e4m3" else torch.float16, positions=a.positions)
     reader.read(list(features), 2)
     torch.cuda.synchronize()
     began = time.perf_counter()
-    said = reader.read(list(features), a.tokens).tolist()
-    for i, ids in enumerate(said):
+    said = reader.read(list(features), a.tokens, scores=a.scores)
+    torch.cuda.synchronize()
+    took = time.perf_counter() - began
+    for i, ids in enumerate((said[0] if a.scores else said).tolist()):
         print(f"image {i}:", *ids)
-    print(f"{(time.perf_counter() - began) / a.tokens * 1e3:.2f} ms a token and image batch")
+        if a.scores:
+            print("   log p:", *(f"{x:.2f}" for x in said[1][i].tolist()))
+            print("   entropy:", *(f"{x:.2f}" for x in said[2][i].tolist()))
+    print(f"{took / a.tokens * 1e3:.2f} ms a token and image batch")
 
 
 if __name__ == "__main__":

@@ -110,6 +110,8 @@ class PagedCache:
 class TokenOps:
     """The operators of one device (a context of the kernel library)."""
 
+    MAX_TOP = 32                             # of token_scores
+
     def __init__(self, device=None):
         self.device = torch.device("cuda", torch.cuda.current_device() if device is None else device)
         self.ctx = _ffi.Context(self.device.index)
