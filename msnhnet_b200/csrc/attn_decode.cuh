@@ -270,7 +270,9 @@ __global__ void __launch_bounds__(Heads::kWarps * 32, Heads::kBlocks) attn_decod
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ Side<Heads> side;
     constexpr int kWarps = Heads::kWarps, kThreads = kWarps * 32, kStages = Heads::kStages;
-    if (Heads::kEarly) pdl_enter(); else pdl_wait();
+    const bool early = Heads::kEarly || p.whole;                 // (nothing is joined after whole pairs)
+    pdl_wait();
+    if (early) pdl_launch_dependents();
     const int pairs = p.c.heads * p.chunks, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     int line = 0;
     for (int base = 0; base < p.rows; base += kThreads) {
@@ -390,7 +392,7 @@ __global__ void __launch_bounds__(Heads::kWarps * 32, Heads::kBlocks) attn_decod
         }
         more = walk.next(piece);
     }
-    if (!Heads::kEarly) pdl_launch_dependents();
+    if (!early) pdl_launch_dependents();
 }
 
 template <typename Heads>
