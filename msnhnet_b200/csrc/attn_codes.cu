@@ -9,6 +9,12 @@
 // A weight and its value's scale, 2^(s_t - m) vs_t, are one factor, which has a running reference of its own: it goes to fp16 in two parts (22
 // bits) relative to the largest factor, whatever the scales are. The sum of weights is fp32 and knows nothing of the scales. Both references
 // are whole numbers, the largest exponent rounded up: what has been summed is then rescaled by powers of two, exactly, and seldom.
+//
+// Measured, both launches, 32 heads over 8 of 128: two fp16 rows of up to 131072 tokens (270 MB) 60.7 us, 4.4 TB/s; 48 bf16 rows of up to 8192 (99 MB)
+// 34.2; one of 37 in a short table 7.4. Copying alone takes 57 of the first (the joining launch is 7), computing alone 46: three warps a scheduler, each
+// waiting five cycles for an instruction, hide most of one behind the other. Tiles of 16 tokens, as in 16 bits, had 83 and 49 us; two blocks an SM with three tiles
+// on their way 67.2 and 39.4; rows asked for a tile earlier (to L2) 66.4. Lengths that are multiples of a share, so that the heads of a token are read at
+// the same time, are 7 % faster: DRAM's share of it.
 #include "attn_decode.cuh"
 
 namespace msnh {
@@ -164,7 +170,8 @@ struct Scale {
 template <typename T, int kDim_, int kGroups_, int kStages_, int kWarps_, int kBlocks_> struct CodeHeads {
     using Type = T;
     using Ring = CodeRing<kDim_, kStages_>;
-    static constexpr bool kEarly = false;                                      // (the joining launch's blocks would take the room of a next call's)
+    // (let in early, the joining launch's blocks take the room of the next call's: 48 rows 47.5 us instead of 35.3, one call behind the other)
+    static constexpr bool kEarly = false;
     static constexpr int kBegin = kCodeStart;
     static constexpr int kDim = kDim_, kStages = kStages_, kGroups = kGroups_, kWarps = kWarps_, kBlocks = kBlocks_;
     static constexpr int kParts = std::is_same<T, float>::value ? 2 : 1;       // fp16 parts of a query's value
@@ -394,19 +401,24 @@ template <typename T, int kDim_, int kGroups_, int kStages_, int kWarps_, int kB
 
 template <typename T>
 cudaError_t launch_type(const MsnhB200Ctx *ctx, const AttnParams &p, int blocks, void *stream) {
-    constexpr int kMany = std::is_same<T, float>::value ? 1 : 2;               // (a pair has 8 heads of fp32 queries at most)
+    constexpr int kMany = std::is_same<T, float>::value ? 1 : 2;               // (a pair has 8 heads of fp32 queries at most, see most_heads_codes)
     const bool few = p.chunk <= 8;
     if (p.c.dim <= 32) return few ? launch<CodeHeads<T, 32, 1, 7, 4, 3>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 32, kMany, 7, 4, 3>>(ctx, p, blocks, stream);
     if (p.c.dim <= 64) return few ? launch<CodeHeads<T, 64, 1, 4, 4, 3>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 64, kMany, 4, 4, 3>>(ctx, p, blocks, stream);
     if (p.c.dim <= 96) return few ? launch<CodeHeads<T, 96, 1, 2, 4, 3>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 96, kMany, 2, 4, 3>>(ctx, p, blocks, stream);
-    if (p.c.dim <= 128) return few ? launch<CodeHeads<T, 128, 1, 2, 4, 3>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 128, kMany, 2, 4, 3>>(ctx, p, blocks, stream);
+    if (p.c.dim <= 128) return few ? launch<CodeHeads<T, 128, 1, 2, 4, 3>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 128, kMany, 3, 4, 2>>(ctx, p, blocks, stream);
     if (p.c.dim <= 192) return few ? launch<CodeHeads<T, 192, 1, 4, 4, 1>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 192, kMany, 4, 4, 1>>(ctx, p, blocks, stream);
-    return few ? launch<CodeHeads<T, 256, 1, 3, 4, 1>>(ctx, p, blocks, stream) : launch<CodeHeads<T, 256, kMany, 3, 4, 1>>(ctx, p, blocks, stream);
+    return launch<CodeHeads<T, 256, 1, 3, 4, 1>>(ctx, p, blocks, stream);
 }
 
 }  // namespace
 
-BlockShape block_shape_codes(int dim) { return {4, dim <= 128 ? 3 : 1}; }
+// Three blocks an SM where a pair's values have registers for it: two rows of 65536 tokens, heads of 96 and 16 of them a key head 82.6 us instead of 91.1 with two,
+// heads of 128 118 instead of 84.3, which is why those have two; four blocks were slower throughout (heads of 64, 4 a key head: 104 us instead of 71).
+BlockShape block_shape_codes(int dim, int chunk) { return {4, dim <= 96 || (dim <= 128 && chunk <= 8) ? 3 : dim <= 128 ? 2 : 1}; }
+// fp32 queries are two parts, and heads of more than 192 values have no registers for 16 of them (294 us for two rows of 65536 tokens, 16 heads a key head; in
+// two pairs, which read the cache twice, 216).
+int most_heads_codes(int dtype, int dim) { return dtype == MSNH_B200_F32 || dim > 192 ? 8 : 16; }
 
 cudaError_t launch_codes(const MsnhB200Ctx *ctx, const AttnParams &p, int dtype, int blocks, void *stream) {
     return dtype == MSNH_B200_F32 ? launch_type<float>(ctx, p, blocks, stream) : dtype == MSNH_B200_F16 ? launch_type<__half>(ctx, p, blocks, stream)

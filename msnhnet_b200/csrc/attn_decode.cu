@@ -347,16 +347,16 @@ struct AttnPlan {
     size_t ml_at, part_at, bytes;
 };
 
-BlockShape block_shape(int dtype, int dim) {
-    return dtype == MSNH_B200_E4M3 ? block_shape_codes(dim) : dtype == MSNH_B200_F32 ? BlockShape{dim <= 128 ? 4 : 2, 1} : BlockShape{4, dim <= 128 ? 2 : 1};
+BlockShape block_shape(int dtype, int dim, int chunk) {
+    return dtype == MSNH_B200_E4M3 ? block_shape_codes(dim, chunk) : dtype == MSNH_B200_F32 ? BlockShape{dim <= 128 ? 4 : 2, 1} : BlockShape{4, dim <= 128 ? 2 : 1};
 }
 
 AttnPlan plan_of(const MsnhB200Ctx *ctx, const MsnhB200KvCache &c, const MsnhB200AttnDecode &a) {
     AttnPlan l = {};
     l.each = a.n_heads / c.n_kv_heads;
-    l.chunk = std::min(l.each, (c.dtype == MSNH_B200_E4M3 ? a.dtype : c.dtype) == MSNH_B200_F32 ? 8 : 16);
+    l.chunk = std::min(l.each, c.dtype == MSNH_B200_E4M3 ? most_heads_codes(a.dtype, c.head_dim) : c.dtype == MSNH_B200_F32 ? 8 : 16);
     l.chunks = (l.each + l.chunk - 1) / l.chunk;
-    const BlockShape shape = block_shape(c.dtype, c.head_dim);
+    const BlockShape shape = block_shape(c.dtype, c.head_dim, l.chunk);
     const long long blocks = static_cast<long long>(ctx->sm_count) * shape.of_sm;
     const long long most_tokens = static_cast<long long>(c.max_pages) * c.page_size, seen = a.window > 0 ? std::min<long long>(most_tokens, a.window) : most_tokens;
     const int tile = c.dtype == MSNH_B200_E4M3 ? kCodeTile : 16;

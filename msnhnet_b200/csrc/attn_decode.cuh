@@ -411,7 +411,8 @@ inline cudaError_t launch(const MsnhB200Ctx *ctx, const AttnParams &p, int block
 struct BlockShape { int warps, of_sm; };
 // Caches of 8-bit codes (attn_codes.cu): tokens of a tile; dtype: of queries and output.
 constexpr int kCodeTile = 32;
-BlockShape block_shape_codes(int dim);
+BlockShape block_shape_codes(int dim, int chunk);         // chunk: query heads of a pair
+int most_heads_codes(int dtype, int dim);                // of a pair
 cudaError_t launch_codes(const MsnhB200Ctx *ctx, const AttnParams &p, int dtype, int blocks, void *stream);
 
 }  // namespace attn

@@ -8,6 +8,11 @@
 // values (107 MB) they take 17 (6.3 TB/s). The rest is the deciding block: a few reads that wait for one another and two scans; it is
 // one block because every page's place depends on all counts before it. A step of a beam search of 256 sequences (fork, append, free: five
 // launches, 15.9 MB) takes 20 us, 4 a launch.
+//
+// In a cache of 8-bit codes append quantises: a block of tokens and head has one scale, a power of two, so that a scale can grow under older codes
+// without a second rounding (a shift of their exponents; only codes below 2^-6 lose bits). Read is the way back, for any cache. Both are bound by their
+// bytes, read and written once: prompts of 26200 bf16 tokens, 8 heads of 128 (161 MB) are written in 42 us (31 the codes' launch by itself, 5.2 TB/s; the deciding block
+// is most of the rest) and read in 31.5 (5.1 TB/s).
 #include "kv_cache.h"
 #include "token_types.cuh"
 
@@ -303,8 +308,10 @@ __device__ __forceinline__ BlockOfScales block_of_scales(const KvParams &c, cons
     return b;
 }
 
-constexpr int kColumns = 128;          // threads of an appending block
-constexpr int kHeld = 16;              // tokens whose pieces a thread keeps between the maximum and the codes
+// Threads of an appending block, and tokens whose pieces a thread keeps between the maximum and the codes. The prompts above: 42.0 us, with blocks of 256 threads 46.0,
+// of 64 43.5; with a warp for a block of one head, eight pieces a lane, 48.0. What is looked up of the next block waits for nothing: 46 instead of 59.
+constexpr int kColumns = 128;
+constexpr int kHeld = 16;
 
 // A block of threads for one block of scales of some heads, keys and values: a thread has a 16-byte column of a head and goes down the tokens, all of
 // its reads on their way together. The head's largest magnitude, from its columns' threads; the scale; the block's older codes by the new

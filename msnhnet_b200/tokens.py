@@ -4,9 +4,11 @@
     y, h = ops.rms_norm(x, weight, residual=h)           # h: the sum, for the next residual
     w = ops.w4_pack(codes, scales)                       # once; then, every step:
     qkv = ops.w4_linear(y, w)
-    cache = ops.new_cache(n_pages, page_size, n_kv_heads, head_dim, n_seqs, max_pages, dtype)
+    cache = ops.new_cache(n_pages, page_size, n_kv_heads, head_dim, n_seqs, max_pages, dtype)     # float8_e4m3fn: half the memory
+    ops.rotary(x, positions, table, out=x)               # queries and keys by their positions; table = ops.rotary_table(head_dim)
     ops.kv_append(cache, k, v)
     out = ops.attn_decode(q, cache)
+    logprob, entropy, best, ids = ops.token_scores(logits, top=5)
 
 Calls enqueue on torch's current stream of the tensors' device and do not wait; nothing here computes anything. Wrong types, shapes or
 devices raise ValueError before the call, and so does a tensor that requires a gradient where torch records gradients: the operators have
@@ -228,7 +230,7 @@ class TokenOps:
     def kv_read(self, cache, starts, tokens, seqs=None, first=None, dtype=None, out=None):
         """Keys and values as the cache holds them, (k, v) [tokens, n_kv_heads, head_dim]: rows starts[i] to starts[i + 1] (int32, one more than
         sequences) are those of sequence seqs[i] (int32; i without it) from its token first[i] (int32; 0 without it) on. Rows of no sequence or
-        token are 0. dtype: the cache's, float16 for 8 bits; out: (k, v) to write into."""
+        token are 0. dtype: the cache's, float16 for 8 bits (what is beyond a type's range is infinite); out: (k, v) to write into."""
         k, v = (None, None) if out is None else out
         return _tokens.kv_read(self._ctx, self._index, cache.address, cache.k_pages, starts, tokens, seqs, first, dtype, k, v)
 

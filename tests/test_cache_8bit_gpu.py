@@ -121,7 +121,7 @@ def used_cache(n_pages, page, heads, dim, n_seqs, max_pages, block, seed, heads_
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("page,block,heads,dim,heads_first,front", [(16, 16, 2, 64, False, 0), (16, 4, 3, 128, False, 0), (8, 1, 2, 80, True, 0), (12, 6, 1, 24, False, 0), (64, 64, 1, 256, False, 0),
-                                                                    (5, 5, 2, 7, False, 0), (16, 16, 2, 64, False, 3), (32, 8, 1, 40, True, 8), (1, 1, 4, 16, False, 0), (32, 32, 2, 12, False, 4)])
+                                                                    (5, 5, 2, 7, False, 0), (16, 16, 2, 64, False, 3), (32, 8, 1, 40, True, 8), (1, 1, 4, 16, False, 0), (32, 32, 2, 12, False, 4), (16, 8, 1, 264, False, 0), (20, 20, 1, 1032, False, 0)])
 def test_append_follows_the_model(ops, dtype, page, block, heads, dim, heads_first, front):
     rng = random.Random(page * 100 + block)
     cache = used_cache(90, page, heads, dim, 6, -(-150 // page), block, 1, heads_first, front)
@@ -322,6 +322,16 @@ def test_read_of_parts_holes_and_rows_of_nothing(ops):
     assert bool((ops.kv_read(cache, ints(0), 3)[0] == 0).all())
     assert ops.kv_read(cache, ints(0, 0), 0)[1].shape == (0, 2, 64)
     cache.page_table[4, 2] = hole
+
+
+def test_read_of_values_beyond_the_output_type(ops):
+    cache = ops.new_cache(2, 16, 1, 16, 1, 1, dtype=E4M3)
+    x = torch.full((2, 1, 16), 1e6, device="cuda")
+    x[1] = 1e-9
+    ops.kv_append(cache, x, -x, starts=ints(0, 2))
+    k, v = ops.kv_read(cache, ints(0, 2), 2, dtype=F16)
+    assert bool((k[0] == INF).all()) and bool((v[0] == -INF).all()) and bool((k[1] == 0).all())
+    assert bool(((ops.kv_read(cache, ints(0, 2), 2, dtype=F32)[0][0] - 1e6).abs() <= 1e6 / 16).all())
 
 
 def test_read_back_and_append_again_gives_the_same_codes(ops):
