@@ -11,8 +11,8 @@
 // A row is one block's or, where there are fewer rows than SMs, one cluster's: its blocks hand their sums and lists to the first one
 // through distributed shared memory, so that there is one launch and no workspace.
 //
-// Measured: 2000 rows of 50000 bf16 logits (200 MB) with the best 8 in 50.5 us, 4.0 TB/s; instructions bound it (eight a logit, one of them 2^x at 16 a
-// cycle and SM, which alone would take 22 us).
+// Measured: 2000 rows of 50000 bf16 logits (200 MB) with the best 8 in 50.5 us, 4.0 TB/s; instructions bound it (eleven a logit, one of them 2^x at 16
+// a cycle and SM, which alone would take 22 us).
 #include <cooperative_groups.h>
 #include "token_ops.h"
 #include "token_types.cuh"
