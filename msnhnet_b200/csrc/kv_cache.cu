@@ -85,7 +85,10 @@ __device__ int lowest_free(const KvParams &c, int need, int *list) {
 struct AppendWork { int first, need, had, start, block; };       // first of its pages in the list; start: the length before, -1: refused;
                                                                  // block: the blocks of scales that sequences before it write to (codes only)
 
-__global__ void kv_append_decide_kernel(KvParams c, const int *seqs, const int *starts, int n, int n_tokens, AppendWork *work, int *list) {
+// What an append's kernels divide by.
+struct AppendDivisors { Divisor heads, block, page; };
+
+__global__ void kv_append_decide_kernel(KvParams c, const int *seqs, const int *starts, int n, int n_tokens, AppendWork *work, int *list, AppendDivisors by) {
     pdl_enter();
     int all = 0, all_blocks = 0;
     bool down = false;                                           // starts that are not in order: then no token's sequence is certain
@@ -98,11 +101,16 @@ __global__ void kv_append_decide_kernel(KvParams c, const int *seqs, const int *
             const long long from = starts ? starts[i] : i, to = starts ? starts[i + 1] : i + 1;
             down |= to < from;
             if (s >= 0 && s < c.n_seqs && from >= 0 && to >= from && to <= n_tokens) {
-                const long long len = max(c.lengths[s], 0), had = (len + c.page_size - 1) / c.page_size;
-                const long long want = (len + to - from + c.page_size - 1) / c.page_size;
-                if (want <= c.max_pages) {
-                    w = {0, static_cast<int>(want - had), static_cast<int>(had), static_cast<int>(len), 0};
-                    if (c.block && to > from) blocks = static_cast<int>((len + to - from - 1) / c.block - len / c.block + 1);
+                const int len = max(c.lengths[s], 0);
+                if (len + to - from <= static_cast<long long>(c.max_pages) * c.page_size) {
+                    const int after = static_cast<int>(len + to - from);
+                    const auto pages_of = [&](int tokens) {
+                        const int whole = by.page.quotient(tokens);
+                        return whole + (whole * c.page_size < tokens);
+                    };
+                    const int had = pages_of(len);
+                    w = {0, pages_of(after) - had, had, len, 0};
+                    if (c.block && after > len) blocks = by.block.quotient(after - 1) - by.block.quotient(len) + 1;
                 }
             }
         }
@@ -279,8 +287,6 @@ template <bool kWhole> struct RowWalk {
         }
     }
 };
-// What the append's warps divide by.
-struct AppendDivisors { Divisor heads, block, page; };
 
 // The call's tokens in one block of scales: where they go, and where they come from.
 struct BlockOfScales {
@@ -854,12 +860,12 @@ int msnh_b200_kv_append_as(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, const int
     AppendWork *work = static_cast<AppendWork *>(workspace);
     int *list = reinterpret_cast<int *>(work + n);
     const KvParams p = kv_params(*c);
-    CUDA_TRY(ctx, launch_token_kernel(kv_append_decide_kernel, dim3(1), kDecide, 0, stream, ctx->pdl, p, seqs, starts, n, n_tokens, work, list));
+    const AppendDivisors by = {Divisor(c->n_kv_heads), Divisor(codes ? c->scale_block : 1), Divisor(c->page_size)};
+    CUDA_TRY(ctx, launch_token_kernel(kv_append_decide_kernel, dim3(1), kDecide, 0, stream, ctx->pdl, p, seqs, starts, n, n_tokens, work, list, by));
     if (n_tokens == 0) return MSNH_B200_OK;
     const size_t size = dtype_size(new_dtype);
     const bool aligned = aligned16(k_new) && aligned16(v_new) && new_token_stride * size % 16 == 0 && new_head_stride * size % 16 == 0;
     if (codes) {
-        const AppendDivisors by = {Divisor(c->n_kv_heads), Divisor(c->scale_block), Divisor(c->page_size)};
         // a block has as many heads as its threads are columns of
         const int vecs = static_cast<int>(c->head_dim * size / 16);
         const bool wide = aligned && kv_rows_multiple_of(*c, 16 / size) && vecs >= 1 && vecs <= kColumns, warps = wide && vecs <= 32 && (vecs & (vecs - 1)) == 0;
