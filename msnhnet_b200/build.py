@@ -80,7 +80,7 @@ def build_tokens(force=False):
     libs = os.path.join(os.path.dirname(torch.__file__), "lib")
     cmd = [_host_cxx(), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
     cmd += [x for i in includes for x in ("-isystem", i)] + ["-o", TOKENS_LIB, TOKENS_SOURCE, "-L", HERE, "-lmsnh_b200", "-Wl,-rpath,$ORIGIN",
-                                                            "-L", libs, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+                                                            "-L", libs, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"]
     subprocess.run(cmd, check=True)
     return TOKENS_LIB
 

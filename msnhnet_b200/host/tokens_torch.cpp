@@ -10,6 +10,7 @@
 #include <torch/csrc/DynamicTypes.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -108,7 +109,8 @@ struct Args {
         if (PyErr_Occurred()) throw Refused();
         return static_cast<T *>(p);
     }
-    at::Tensor empty(at::IntArrayRef sizes, at::ScalarType type) const { return at::empty(sizes, at::TensorOptions().dtype(type).device(device)); }
+    // (torch's allocator without its dispatcher: 0.25 us less a tensor; what is allocated here is written whole, or is a workspace)
+    at::Tensor empty(at::IntArrayRef sizes, at::ScalarType type) const { return at::Tensor(at::detail::empty_cuda(sizes, type, device, std::nullopt)); }
 };
 
 template <typename F> PyObject *guarded(F f) noexcept {
