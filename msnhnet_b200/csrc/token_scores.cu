@@ -11,7 +11,7 @@
 // A row is one block's or, where there are fewer rows than SMs, one cluster's: its blocks hand their sums and lists to the first one
 // through distributed shared memory, so that there is one launch and no workspace.
 //
-// Measured: 2000 rows of 50000 bf16 logits (200 MB) with the best 8 in 50.5 us, 4.0 TB/s; instructions bound it (eleven a logit, one of them 2^x at 16
+// Measured: 2000 rows of 50000 bf16 logits (200 MB) with the best 8 in 51 us, 3.9 TB/s; instructions bound it (eleven a logit, one of them 2^x at 16
 // a cycle and SM, which alone would take 22 us).
 #include <cooperative_groups.h>
 #include "token_ops.h"
@@ -322,10 +322,13 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 7 : 1) token_score
             // (their order depends on timing; the keys of what they hold do not)
             Key found = 0;
             const float least_value = least ? unordered(least) : -INFINITY;
-            for (int j = warp; j < shared.count; j += kWarps) {
-                const int first = begin + shared.threads[j];
-                for (int base = first; base < end; base += kThreads * 32) {
-                    const int c = base + lane * kThreads;
+            // (so many lanes for a thread as it has chunks, up to all of them)
+            const int each = (end - begin + kThreads - 1) / kThreads, bits = each >= 32 ? 5 : each > 1 ? 32 - __clz(each - 1) : 0, width = 1 << bits;
+            const int at_once = 32 >> bits, count = shared.count;
+            for (int j = warp * at_once; j < count; j += kWarps * at_once) {
+                const int its = j + (lane >> bits), first = its < count ? begin + shared.threads[its] : end;
+                for (int base = 0; base < each; base += width) {
+                    const int c = min(first + (base + (lane & (width - 1))) * kThreads, end);
                     float v[kVec];
                     if (c < end) Vec16<T>::unpack(row.load(c, __uint_as_float(0x7fffffffu)), v);
 #pragma unroll
@@ -356,17 +359,21 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 7 : 1) token_score
             if (lane == 0) shared.all = all;
         }
         if constexpr (kCluster > 1) cg::this_cluster().sync();
+        Key best = 0;
+        if (p.top > 0 && part == 0) {
+            best = shared.keys[lane];
+            if constexpr (kCluster > 1) {                        // a list of another block for each warp
+                static_assert(kWarps >= kCluster, "a warp for each block of a cluster");
+                if (warp > 0) best = warp < kCluster ? cg::this_cluster().map_shared_rank(&shared, warp)->keys[lane] : 0;
+                best = merge_block<kWarps>(best, shared.list, warp, lane);
+            }
+        }
         if (part == 0 && warp == 0) {
             __syncwarp();
             Sums all = shared.all;
-            Key key = p.top > 0 ? shared.keys[lane] : 0;
             if constexpr (kCluster > 1) {
-#pragma unroll 1
-                for (int o = 1; o < kCluster; ++o) {
-                    const ScoreShared<kWarps> *other = cg::this_cluster().map_shared_rank(&shared, o);
-                    all.join(other->all);
-                    if (p.top > 0) key = merge_warp(key, other->keys[31 - lane], lane);
-                }
+                all = lane < kCluster ? cg::this_cluster().map_shared_rank(&shared, lane)->all : Sums{-INFINITY, 0.f, 0.f};
+                all.join_warp();
             }
             const float nan = __uint_as_float(0x7fffffffu);
             // (a maximum of +infinity has sums of 0 or NaN)
@@ -380,8 +387,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 7 : 1) token_score
                 }
             }
             if (lane < p.top) {
-                p.top_ids[r * p.top + lane] = good ? static_cast<long long>(index_of(key)) : -1;
-                p.top_logprobs[r * p.top + lane] = good ? unordered(static_cast<uint32_t>(key >> 32)) - all.top - log_sum : nan;
+                p.top_ids[r * p.top + lane] = good ? static_cast<long long>(index_of(best)) : -1;
+                p.top_logprobs[r * p.top + lane] = good ? unordered(static_cast<uint32_t>(best >> 32)) - all.top - log_sum : nan;
             }
         }
         if constexpr (kCluster > 1) cg::this_cluster().sync();
@@ -411,10 +418,10 @@ cudaError_t launch(const MsnhB200Ctx *ctx, const ScoreParams &p, void *stream) {
     return cudaLaunchKernelEx(&config, token_scores_kernel<T, kThreads, kCluster>, p);
 }
 
-// Blocks of a row: as many as leave every SM two, each with 4096 logits at least, of 256 threads (with 512, whose clusters find less room, 16 rows of 50000
-// bf16 logits take 17.4 us and not 9.8, 60 of 32000 fp32 ones 14.6 and not 8.6; three of 128000 fp16 ones 10.2 and not 11.1). A row that is one
-// block's has 128 threads, since what follows the pass over the logits grows with the warps, and seven such blocks an SM have registers for the
-// next chunks (2000 rows of 50000: 50.5 us; 51.5 with eight, 69 with nine).
+// Blocks of a row: as many as leave every SM two, each with 4096 logits at least, of 256 threads (clusters of 512 find less room: 16 rows of 50000 bf16 logits took
+// 17.4 us and not 9.8; now 8.0, three of 128000 fp16 ones 8.3, 120 of 128000 14.3). A row that is one block's has 128 threads, since what follows the pass over
+// the logits grows with the warps, and seven such blocks an SM have registers for the next chunks (2000 rows of 50000: 51 us; a microsecond more with eight, 18 more
+// with nine).
 template <typename T>
 cudaError_t launch_by_size(const MsnhB200Ctx *ctx, const ScoreParams &p, void *stream) {
     const long long parts = std::min<long long>(2LL * ctx->sm_count / p.rows, p.cols / 4096);
