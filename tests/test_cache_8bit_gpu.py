@@ -248,6 +248,35 @@ def test_fork_copy_and_compact_take_scales_along(ops, block, dim, heads_first):
         assert torch.equal(now[0], kept[0]) and torch.equal(now[1], kept[1])
 
 
+def test_append_and_read_of_many_sequences(ops):
+    # more sequences than a warp looks through at once, and than the deciding block has threads; many without a token
+    rng = random.Random(16)
+    n = 3000
+    cache = used_cache(6000, 8, 1, 16, n, 4, 4, 17)
+    m = Model(cache)
+    order = rng.sample(range(n), n)
+    for _ in range(2):
+        counts = [rng.choice([0, 0, 1, 2, 5, 9]) for _ in range(n)]
+        tokens = sum(counts)
+        k, v = randn(tokens, 1, 16, seed=18, dtype=F16), randn(tokens, 1, 16, seed=19, dtype=F16) * 8
+        starts = ints(0, *torch.tensor(counts).cumsum(0).tolist())
+        ops.kv_append(cache, k, v, seqs=ints(*order), starts=starts)
+        m.append(order, counts, k, v)
+    m.same()
+    assert cache.refused() == 0
+    lengths = [m.lengths[s] for s in order]
+    starts = ints(0, *torch.tensor(lengths).cumsum(0).tolist())
+    k, v = ops.kv_read(cache, starts, sum(lengths), seqs=ints(*order), dtype=F32)
+    at, table = 0, cache.page_table.tolist()
+    for s, length in zip(order, lengths):
+        for t in range(length):
+            page, place = table[s][t // 8], t % 8
+            for side, out in ((0, k), (1, v)):
+                if s % 50 == 0:
+                    assert torch.equal(out[at + t, 0].cpu().double(), m.codes[side][page, place, 0].double() * m.scales[side][page, 0, place // 4])
+        at += length
+
+
 def test_append_refuses_on_the_device(ops):
     cache = used_cache(3, 4, 1, 16, 2, 2, 2, 14)
     m = Model(cache)
@@ -598,6 +627,34 @@ def test_on_another_stream_and_in_a_graph(ops):
     assert all(torch.equal(a, b) for a, b in zip(got, want)) and all(torch.equal(a.float(), b.float()) for a, b in zip(cache.tensors, after))
     graph.replay()                                                    # one more token each
     assert cache.lengths.tolist() == [32, 72, 7, 2]
+
+
+def test_two_streams_at_once(ops):
+    caches = []
+    for i in range(2):
+        cache = ops.new_cache(300, 16, 2, 128, 8, 40, dtype=E4M3)
+        fill(ops, cache, [500, 3, 0, 77, 400, 1, 20, 600], 90 + i)
+        caches.append(cache)
+    q, new = randn(8, 8, 128, seed=92, dtype=F16), randn(8, 2, 128, seed=93, dtype=F16)
+    logits = randn(8, 50000, seed=94)
+
+    def step(cache):
+        ops.kv_append(cache, new, new)
+        return ops.attn_decode(q, cache), *ops.token_scores(logits, top=3)[1:]
+    kept = [[t.clone() for t in c.tensors] for c in caches]
+    want = [[step(c) for _ in range(5)] for c in caches]
+    for c, old in zip(caches, kept):
+        for t, o in zip(c.tensors, old):
+            t.copy_(o)
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in caches], [[], []]
+    for _ in range(5):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(step(caches[i]))
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(x, y) for one, other in zip(a, b) for x, y in zip(one, other))
 
 
 def test_writes_are_known_to_torch(ops):
