@@ -11,7 +11,7 @@
 // are whole numbers, the largest exponent rounded up: what has been summed is then rescaled by powers of two, exactly, and seldom.
 //
 // Measured, both launches, 32 heads over 8 of 128: two fp16 rows of up to 131072 tokens (270 MB) 60.7 us, 4.4 TB/s; 48 bf16 rows of up to 8192 (99 MB)
-// 34.2; one of 37 in a short table 7.4. Copying alone takes 57 of the first (the joining launch is 7), computing alone 46: three warps a scheduler, each
+// 31.8; one of 37 in a short table 7.3. Copying alone takes 57 of the first (the joining launch is 7), computing alone 46: three warps a scheduler, each
 // waiting five cycles for an instruction, hide most of one behind the other. Tiles of 16 tokens, as in 16 bits, had 83 and 49 us; two blocks an SM with three tiles
 // on their way 67.2 and 39.4; rows asked for a tile earlier (to L2) 66.4. Lengths that are multiples of a share, so that the heads of a token are read at
 // the same time, are 7 % faster: DRAM's share of it.
@@ -182,19 +182,39 @@ template <typename T, int kDim_, int kGroups_, int kStages_, int kWarps_, int kB
     uint32_t q[kParts][kGroups][kDim / 16][2];
 
     __device__ __forceinline__ void start(const AttnParams &p, int row, int head, int heads, int lane, float *) {
+        using Four = std::conditional_t<sizeof(T) == 4, uint4, uint2>;
         const T *from = reinterpret_cast<const T *>(p.q) + row * p.q_row + head * p.q_head;
 #pragma unroll
         for (int n = 0; n < kGroups; ++n) {
             const int r = n * 8 + lane / 4;
+            // values s * 16 + 4 (l % 4) and the three behind it: one load of four where
+            // they are aligned, all of a head's loads under way before the first is
+            // used. Two values a load, and read again for the largest magnitude: 48
+            // bf16 rows 34.6 us instead of 31.8, four rows of heads of 256 23.5 for 20.2
+            alignas(16) T v[kDim / 16][4];
+            const T *mine = from + r * p.q_head + lane % 4 * 4;
+            const int left = r < heads ? p.c.dim - lane % 4 * 4 : 0;
+            if (p.wide_q) {
+#pragma unroll
+                for (int s = 0; s < kDim / 16; ++s) {
+                    Four x{};
+                    if (s * 16 < left) x = *reinterpret_cast<const Four *>(mine + s * 16);
+                    *reinterpret_cast<Four *>(v[s]) = x;
+                }
+            } else {
+#pragma unroll
+                for (int s = 0; s < kDim / 16; ++s)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[s][i] = s * 16 < left ? mine[s * 16 + i] : T(0.f);
+            }
             float factor = 1.f, back = 1.f;
             if constexpr (!std::is_same<T, __half>::value) {
                 // the head's largest magnitude to between 2^14 and 2^15
                 uint32_t most = 0;
 #pragma unroll
-                for (int d = lane % 4 * 4; d < kDim; d += 16)
+                for (int s = 0; s < kDim / 16; ++s)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (r < heads && d + i < p.c.dim) most = max(most, __float_as_uint(to_float(from[r * p.q_head + d + i])) & 0x7fffffffu);
+                    for (int i = 0; i < 4; ++i) most = max(most, __float_as_uint(to_float(v[s][i])) & 0x7fffffffu);
                 most = max(most, __shfl_xor_sync(~0u, most, 1));
                 most = max(most, __shfl_xor_sync(~0u, most, 2));
                 if (most > 0 && most < 0x7f800000u) {
@@ -207,12 +227,7 @@ template <typename T, int kDim_, int kGroups_, int kStages_, int kWarps_, int kB
             for (int s = 0; s < kDim / 16; ++s)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const int d = s * 16 + lane % 4 * 4 + i * 2;
-                    float a = 0.f, b = 0.f;
-                    if (r < heads && d < p.c.dim) {
-                        a = to_float(from[r * p.q_head + d]) * factor;
-                        b = to_float(from[r * p.q_head + d + 1]) * factor;
-                    }
+                    float a = to_float(v[s][2 * i]) * factor, b = to_float(v[s][2 * i + 1]) * factor;
 #pragma unroll
                     for (int part = 0; part < kParts; ++part) {
                         q[part][n][s][i] = pack2<__half>(a, b);

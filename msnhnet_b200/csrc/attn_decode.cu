@@ -455,6 +455,8 @@ int msnh_b200_attn_decode(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, const Msnh
     AttnParams p = {kv_params(*c), static_cast<const uint8_t *>(a->q), static_cast<uint8_t *>(a->out), a->lse, a->seqs, a->q_row_stride, a->q_head_stride,
                     a->out_row_stride, a->out_head_stride, 0, a->n_heads, l.each, l.chunk, l.chunks, a->window, 0, l.whole, c->dtype == MSNH_B200_E4M3 ? kCodeStart : kStart, a->scale,
                     reinterpret_cast<int *>(work), reinterpret_cast<float2 *>(work + l.ml_at), reinterpret_cast<float *>(work + l.part_at)};
+    const size_t q_size = dtype_size(c->dtype == MSNH_B200_E4M3 ? a->dtype : c->dtype);
+    p.wide_q = reinterpret_cast<uintptr_t>(a->q) % (4 * q_size) == 0 && a->q_row_stride % 4 == 0 && a->q_head_stride % 4 == 0;
     for (int row = 0; row < a->rows; row += l.rows) {
         p.first_row = row;
         p.rows = std::min(l.rows, a->rows - row);

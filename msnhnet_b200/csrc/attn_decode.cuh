@@ -31,6 +31,7 @@ struct AttnParams {
     int *prefix;                                         // workspace: the line's tiles before each row (rows + 1), then the parts
     float2 *part_ml;                                     // [slot][chunk] maximum and sum
     float *part;                                         // [slot][chunk][dim]
+    int wide_q;                                          // four values of a query, from every fourth one on, are aligned (8-bit caches)
 };
 
 struct Row { int seq, first, last; };

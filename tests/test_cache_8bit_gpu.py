@@ -520,6 +520,20 @@ def test_attention_layouts_and_rows(ops, dtype, heads_first):
     check_attn(got, lse, q, [none if s is None else keys[s] for s in pick], [none if s is None else values[s] for s in pick], 0.125)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("front,stride", [(0, 64), (1, 64), (2, 64), (3, 65), (4, 64), (0, 66), (4, 68), (6, 70), (4, 67)])
+@pytest.mark.parametrize("dim", [48, 64])
+def test_attention_of_queries_that_start_anywhere(ops, dtype, front, stride, dim):
+    cache, _, _ = code_cache([70, 5, 130], 16, 2, dim, 16, 68)
+    q = randn(3, 6, dim, seed=69, dtype=dtype)
+    room = torch.full((8 + 3 * 6 * stride,), NAN, device="cuda", dtype=dtype)
+    there = room[front:].as_strided((3, 6, dim), (6 * stride, stride, 1))
+    there.copy_(q)
+    expected, lse = ops.attn_decode(q, cache, return_lse=True)
+    got, got_lse = ops.attn_decode(there, cache, return_lse=True)
+    assert torch.equal(got, expected) and torch.equal(got_lse, lse)
+
+
 @pytest.mark.parametrize("dtype,size", [(F32, 1e30), (F32, 1e-30), (F32, 1.0), (BF16, 1e30), (BF16, 1e-30), (F16, 2.0 ** -20), (F16, 3e4)])
 def test_attention_of_queries_of_all_sizes(ops, dtype, size):
     cache, keys, values = code_cache([90, 300], 16, 1, 64, 16, 66)
