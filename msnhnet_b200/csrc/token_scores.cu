@@ -261,7 +261,7 @@ template <int kWarps> struct ScoreShared {
 };
 
 template <typename T, int kThreads, int kCluster>
-__global__ void __launch_bounds__(kThreads, kThreads == 128 ? 7 : 1) token_scores_kernel(const __grid_constant__ ScoreParams p) {
+__global__ void __launch_bounds__(kThreads, kThreads == 128 ? 7 : kThreads == 32 ? 28 : 1) token_scores_kernel(const __grid_constant__ ScoreParams p) {
     constexpr int kVec = 16 / sizeof(T), kWarps = kThreads / 32, kAhead = kCluster > 1 ? 2 : 4;
     __shared__ ScoreShared<kWarps> shared;
     pdl_enter();
@@ -421,13 +421,19 @@ cudaError_t launch(const MsnhB200Ctx *ctx, const ScoreParams &p, void *stream) {
 // Blocks of a row: as many as leave every SM two, each with 4096 logits at least, of 256 threads (clusters of 512 find less room: 16 rows of 50000 bf16 logits took
 // 17.4 us and not 9.8; now 8.0, three of 128000 fp16 ones 8.3, 120 of 128000 14.3). A row that is one block's has 128 threads, since what follows the pass over
 // the logits grows with the warps, and seven such blocks an SM have registers for the next chunks (2000 rows of 50000: 51 us; a microsecond more with eight, 18 more
-// with nine).
+// with nine). Narrow rows are one warp's each, without other warps' lists to join, where there are more than the SMs hold at 128 threads a row, and always where a
+// warp has a row in one chunk a lane: 4000 bf16 rows of 1000 with the best 5 8.5 us instead of 20.9, 1200 of 4000 9.4 instead of 12.9, 20000 of 500 32.0 instead of 95.6. A
+// warp looks at more chunks again the more logits are wanted, hence the bounds (1200 rows of 8000 with the best 8 would take 16.3 instead of 14.7, of 1000
+// fp32 ones with the best 32 16.0 instead of 11.6).
 template <typename T>
 cudaError_t launch_by_size(const MsnhB200Ctx *ctx, const ScoreParams &p, void *stream) {
     const long long parts = std::min<long long>(2LL * ctx->sm_count / p.rows, p.cols / 4096);
     if (parts >= 8) return launch<T, 256, 8>(ctx, p, stream);
     if (parts >= 4) return launch<T, 256, 4>(ctx, p, stream);
     if (parts >= 2) return launch<T, 256, 2>(ctx, p, stream);
+    const long long warps = 7LL * ctx->sm_count;
+    const int narrow = p.rows < warps ? 0 : (p.top > 8 ? 512 : 4096) * (p.rows < 3 * warps ? 1 : 2);
+    if (p.cols <= std::max<int>(narrow, 32 * 16 / sizeof(T))) return launch<T, 32, 1>(ctx, p, stream);
     return launch<T, 128, 1>(ctx, p, stream);
 }
 

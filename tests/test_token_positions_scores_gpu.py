@@ -172,7 +172,7 @@ def test_rotary_tells_torch_of_its_writes(ops):
 
 # ---- scores of tokens -----------------------------------------------------------------------------------------------
 
-def check_scores(got, logits, ids, top):
+def check_scores(got, logits, ids, top, lanes=128):
     logprob, entropy, top_logprobs, top_ids = got
     z = logits.double()
     cols = z.shape[1]
@@ -184,9 +184,9 @@ def check_scores(got, logits, ids, top):
     p = torch.exp(-d - log_s[:, None])
     far = torch.where(p > 0, d, torch.zeros_like(d))
     mean, square = (p * far).sum(-1), (p * far * far).sum(-1)
-    # e^-d: the distance is rounded (2^-24 d), times log2 e (2^-24 d), 2^x to two units; a thread adds its logits one by one, at most one in 128 of them,
+    # e^-d: the distance is rounded (2^-24 d), times log2 e (2^-24 d), 2^x to two units; a thread adds its logits one by one, at most one in `lanes` of them,
     # (and its maximum's growth rescales them, ten times at most in what is bound here); then the threads are joined (nine steps)
-    n = 2.0 ** -24 * (cols / 128 + 60)
+    n = 2.0 ** -24 * (cols / lanes + 60)
     rel = n + 2.0 ** -23 * (2 * mean + 4)
     bound_log = rel + 2.0 ** -22 * log_s
 
@@ -222,6 +222,33 @@ def test_scores_match_the_formula(ops, dtype, rows, cols, top):
     if cols == 1000:
         check_scores(ops.token_scores(z, top=top), z, None, top)
         check_scores(ops.token_scores(z, ids), z, ids, 0)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rows,cols,top", [(1300, 1, 1), (1300, 30, 30), (1300, 128, 32), (1300, 129, 32), (1300, 257, 20), (1300, 512, 32), (1300, 513, 32), (1300, 1000, 8), (1300, 4096, 8), (1300, 4097, 8),
+                                           (2000, 3001, 0), (4500, 1024, 32), (4500, 1025, 9), (4500, 8191, 8), (4500, 8192, 1), (4500, 8193, 8)])
+def test_scores_of_many_narrow_rows(ops, dtype, rows, cols, top):
+    z = (randn(rows, cols, seed=120) * 3).to(dtype)
+    z[5::7, ::2] = -INF
+    z[6::7, cols // 2] = NAN
+    z[7::70] = -INF
+    z[8::70] = 1.0
+    ids = torch.randint(0, cols, (rows,), generator=gen(121), device="cuda")
+    check_scores(ops.token_scores(z, ids, top=top), z, ids, top, lanes=32)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("cols", [60, 500, 4000])
+@pytest.mark.parametrize("extra,front", [(0, 1), (3, 0), (1, 5)])
+def test_scores_of_many_narrow_rows_that_start_anywhere(ops, dtype, cols, extra, front):
+    rows = 1100
+    raw = torch.full((front + rows * (cols + extra),), NAN, device="cuda").to(dtype)
+    z = raw[front:].view(rows, cols + extra)[:, :cols]
+    z.copy_((randn(rows, cols, seed=122) * 2).to(dtype))
+    z[::3, cols - 1] = 30.0
+    ids = torch.randint(0, cols, (rows,), generator=gen(123), device="cuda")
+    for top in (0, 1, 6):
+        check_scores(ops.token_scores(z, ids, top=top), z, ids, top, lanes=32)
 
 
 @pytest.mark.parametrize("dtype", [F32, F16])
