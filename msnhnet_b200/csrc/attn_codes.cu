@@ -172,7 +172,7 @@ template <typename T, int kDim_, int kGroups_, int kStages_, int kWarps_, int kB
     using Ring = CodeRing<kDim_, kStages_>;
     // (let in early, the joining launch's blocks take the room of the next call's: 48 rows 47.5 us instead of 35.3, one call behind the other)
     static constexpr bool kEarly = false;
-    static constexpr int kBegin = kCodeStart;
+    static constexpr int kBegin = kCodeStart, kSmallest = kCodeSmallest;
     static constexpr int kDim = kDim_, kStages = kStages_, kGroups = kGroups_, kWarps = kWarps_, kBlocks = kBlocks_;
     static constexpr int kParts = std::is_same<T, float>::value ? 2 : 1;       // fp16 parts of a query's value
     static constexpr float kLift = 14.f;                                       // factors are taken times 2^14: they are below 2, and fp16 goes to 2^16

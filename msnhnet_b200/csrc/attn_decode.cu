@@ -37,7 +37,7 @@ template <typename T, int kDim_, int kGroups_, int kStages_, int kBlocks_> struc
     using Type = T;
     using Ring = attn::Ring<T, kDim_, kStages_>;
     static constexpr bool kEarly = true;
-    static constexpr int kBegin = kStart;
+    static constexpr int kBegin = kStart, kSmallest = attn::kSmallest;
     static constexpr int kDim = kDim_, kStages = kStages_, kGroups = kGroups_, kWarps = 4, kBlocks = kBlocks_;
     // fp16 weights are taken times 2^14, so that a weight of 2^-29 of the largest is still a normal number (sum and values carry the
     // same factor); what a weight loses when it is rounded to the cache's type goes into a second product. Both parts are above 0 where the
@@ -166,7 +166,7 @@ template <int kDim_, int kHeads_, int kStages_, int kWarps_> struct PlainHeads {
     using Type = float;
     using Ring = attn::Ring<float, kDim_, kStages_>;
     static constexpr bool kEarly = true;
-    static constexpr int kBegin = kStart;
+    static constexpr int kBegin = kStart, kSmallest = attn::kSmallest;
     static constexpr int kDim = kDim_, kStages = kStages_, kWarps = kWarps_, kHeads = kHeads_, kBlocks = 1, kTile = Ring::kTile;
     static constexpr int kColumns = kDim / 32, kVec = kColumns % 4 == 0 ? 4 : kColumns % 2 == 0 ? 2 : 1;
 
@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_co
     const int pairs = p.c.heads * p.chunks, dim = p.c.dim;
     const int before = p.prefix[row], after = p.prefix[row + 1], line = p.prefix[p.rows], length = (after - before) / pairs;
     if (length == 0) return;
-    const int share = share_of(line, workers, p.start), unit = before + (kv * p.chunks + chunk) * length;
+    const int share = share_of(line, workers, p.smallest), unit = before + (kv * p.chunks + chunk) * length;
     const int first = (unit + p.start) / share, last = (unit + length - 1) / share;
     if (first == last) return;                                   // (finished by its warp)
     const int parts = last - first + 1, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -408,7 +408,7 @@ constexpr int kManyParts = 32;
 template <typename T>
 cudaError_t launch_join(const MsnhB200Ctx *ctx, const AttnParams &p, int workers, long long tiles, void *stream) {
     const dim3 grid(p.rows, p.n_heads);
-    const long long parts = std::min<long long>(workers / (static_cast<long long>(p.rows) * p.c.heads * p.chunks), (tiles + p.start) / (p.start + kLeast));
+    const long long parts = std::min<long long>(workers / (static_cast<long long>(p.rows) * p.c.heads * p.chunks), (tiles + p.start) / p.smallest);
     return parts < kManyParts ? launch_token_kernel(attn_join_kernel<T, kJoinFew>, grid, kJoinFew, 0, stream, ctx->pdl, p, workers)
                               : launch_token_kernel(attn_join_kernel<T, kJoinMany>, grid, kJoinMany, 0, stream, ctx->pdl, p, workers);
 }
@@ -453,7 +453,8 @@ int msnh_b200_attn_decode(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, const Msnh
     CUDA_TRY(ctx, scope.status);
     uint8_t *work = static_cast<uint8_t *>(a->workspace);
     AttnParams p = {kv_params(*c), static_cast<const uint8_t *>(a->q), static_cast<uint8_t *>(a->out), a->lse, a->seqs, a->q_row_stride, a->q_head_stride,
-                    a->out_row_stride, a->out_head_stride, 0, a->n_heads, l.each, l.chunk, l.chunks, a->window, 0, l.whole, c->dtype == MSNH_B200_E4M3 ? kCodeStart : kStart, a->scale,
+                    a->out_row_stride, a->out_head_stride, 0, a->n_heads, l.each, l.chunk, l.chunks, a->window, 0, l.whole, c->dtype == MSNH_B200_E4M3 ? kCodeStart : kStart,
+                    c->dtype == MSNH_B200_E4M3 ? kCodeSmallest : kSmallest, a->scale,
                     reinterpret_cast<int *>(work), reinterpret_cast<float2 *>(work + l.ml_at), reinterpret_cast<float *>(work + l.part_at)};
     const size_t q_size = dtype_size(c->dtype == MSNH_B200_E4M3 ? a->dtype : c->dtype);
     p.wide_q = reinterpret_cast<uintptr_t>(a->q) % (4 * q_size) == 0 && a->q_row_stride % 4 == 0 && a->q_head_stride % 4 == 0;

@@ -8,13 +8,14 @@ namespace msnh {
 namespace attn {
 
 constexpr int kMaxRows = 256;                // rows of a launch: what they see is kept in shared memory
-// Tiles that a pair's start counts for, and tiles of a share, where there are as many. fp16, 32 heads over 8, with kStart 1, 3 and 6: one row
-// of 500 tokens 9.7, 10.8 and 13.1 us, 16 of them 17.2, 16.5 and 18.0, one of 65536 beside 63 of 100 76.7, 75.2 and 75.7, one of 4000 14.2,
+// Tiles that a pair's start counts for, and the smallest share, a start and two tiles, where there are as many. fp16, 32 heads over 8, with kStart 1, 3 and
+// 6: one row of 500 tokens 9.7, 10.8 and 13.1 us, 16 of them 17.2, 16.5 and 18.0, one of 65536 beside 63 of 100 76.7, 75.2 and 75.7, one of 4000 14.2,
 // 14.8 and 16.1; 16 of 4000 and more tokens are the same within 1 %.
-constexpr int kStart = 3, kLeast = 2;
-// The same of 8-bit codes, whose tiles are of 32 tokens and go by faster than a pair's start does: 48 rows of up to 8192 tokens (and two of up to 131072)
-// take 46.4, 41.5, 36.4, 34.4 and 36.3 us (62.9, 62.7, 62.7, 62.8 and 60.1) with 1, 2, 3, 5 and 8.
-constexpr int kCodeStart = 5;
+constexpr int kStart = 3, kSmallest = 5;
+// The same of 8-bit codes, whose tiles are of 32 tokens. With a start of 1, 2, 3 and 5: 48 rows of up to 8192 tokens 37.9, 31.7, 31.7 and 31.7 us, five of up to
+// 20000 25.2, 23.0, 23.2 and 26.5, 16 of up to 1000 15.2, 16.9, 17.6 and 18.4, one of 500 12.0, 12.1, 12.7 and 15.4, one of 65536 beside 63 of 100 65.8, 66.6, 62.5
+// and 63.5. With one tile at least and a start of 2: 31.7, 23.1, 15.1, 11.2 and 65.2; four of up to 1418 with heads of 256 14.4 and not 16.0.
+constexpr int kCodeStart = 2, kCodeSmallest = 3;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct AttnParams {
@@ -26,7 +27,7 @@ struct AttnParams {
     long long q_row, q_head, out_row, out_head;
     int rows, n_heads, each, chunk, chunks, window;      // each: query heads of a key head; chunk: how many of them a pair has
     int first_row;                                       // of this launch
-    int whole, start;                                    // start: tiles that a pair's start counts for
+    int whole, start, smallest;                          // start: tiles that a pair's start counts for; smallest: share of a warp
     float scale;
     int *prefix;                                         // workspace: the line's tiles before each row (rows + 1), then the parts
     float2 *part_ml;                                     // [slot][chunk] maximum and sum
@@ -46,8 +47,8 @@ template <int kTile> __device__ __forceinline__ int tiles_of(const Row &r) { ret
 
 // The share of a warp, in tiles of the line. (A launch's line has less than 2^30 tiles: code for longer ones is a microsecond of reading
 // instructions alone.)
-__device__ __forceinline__ int share_of(int line, int workers, int start) {
-    return max((line + workers - 1) / workers, start + kLeast);
+__device__ __forceinline__ int share_of(int line, int workers, int smallest) {
+    return max((line + workers - 1) / workers, smallest);
 }
 
 // 16 bytes to shared memory, of which the first `bytes` are copied (16 or none) and the others are 0
@@ -317,7 +318,7 @@ __global__ void __launch_bounds__(Heads::kWarps * 32, Heads::kBlocks) attn_decod
         }
     // the share; neighbours in the line are in different blocks, so that a short line is spread over the SMs
     const int workers = gridDim.x * kWarps, worker = warp * gridDim.x + blockIdx.x;
-    const int share = p.whole ? (line + workers - 1) / workers : share_of(line, workers, Heads::kBegin), unit = worker * share;
+    const int share = p.whole ? (line + workers - 1) / workers : share_of(line, workers, Heads::kSmallest), unit = worker * share;
     if (unit >= line) return;
     int low = 0;                                                 // the last row that begins at or before the share
     for (int step = kMaxRows / 32; step; step = step == kMaxRows / 32 ? 1 : 0) {
