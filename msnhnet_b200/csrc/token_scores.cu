@@ -376,11 +376,12 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 7 : kThreads == 32
                 all.join_warp();
             }
             const float nan = __uint_as_float(0x7fffffffu);
-            // (a maximum of +infinity has sums of 0 or NaN)
-            const bool good = all.top > -INFINITY && all.top < INFINITY && all.sum >= 1.f;
-            const float log_sum = good ? logf(all.sum) : nan;
+            // (a NaN has sums that are NaN, a maximum of +infinity ones of 0 or NaN. A good row's sum is 1 or more and its second one 0 or more, but for
+            // their roundings: the maximum's own term may come out as 1 - 2^-24, and where one token has all of the probability there is little else)
+            const bool good = all.top > -INFINITY && all.top < INFINITY && all.sum > 0.f;
+            const float sum = fmaxf(all.sum, 1.f), log_sum = good ? logf(sum) : nan;
             if (lane == 0) {
-                if (p.entropy) p.entropy[r] = good ? log_sum + all.more / all.sum : nan;
+                if (p.entropy) p.entropy[r] = good ? log_sum + fmaxf(all.more, 0.f) / sum : nan;
                 if (p.logprob) {
                     const long long id = p.ids[r];
                     p.logprob[r] = good && id >= 0 && id < p.cols ? to_float(row.at[id]) - all.top - log_sum : nan;
