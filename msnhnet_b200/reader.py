@@ -192,8 +192,8 @@ class Reader:
 
     def score(self, features, ids, alternatives=0):
         """How likely the reader takes a text to be: ids [n] behind a feature map [cells, channels]. (logprobs float32 [n], entropies float32
-        [n], top_logprobs, top_ids [n, alternatives] or None), as TokenOps.token_scores gives them. Takes sequence 0, which has to be empty, and
-        forgets it again."""
+        [n], top_logprobs, top_ids [n, alternatives] or None), as TokenOps.token_scores gives them. An id that is no token has a log probability of NaN, and
+        whatever follows it has NaN throughout (and ids of -1). Takes sequence 0, which has to be empty, and forgets it again."""
         ids = torch.as_tensor(ids, dtype=torch.int64, device=self.position.device)
         if ids.dim() != 1 or len(ids) < 1:
             raise ValueError("ids: [n], one token at least")
@@ -206,7 +206,10 @@ class Reader:
         for i in range(len(ids) - 1):
             rows.append(self.step(ids[i:i + 1], seqs))
         self._forgotten(seqs, [0])
-        return self.ops.token_scores(torch.cat(rows), ids, top=alternatives)
+        # (a step leaves the sequence as it was where a token is none: what came behind it would be scored as if it were not there)
+        follows = ((ids >= 0) & (ids < self.vocab)).roll(1).index_fill(0, ids.new_zeros(1), True).cumprod(0).bool()
+        logits = torch.where(follows[:, None], torch.cat(rows), float("nan"))
+        return self.ops.token_scores(logits, ids, top=alternatives)
 
     def save(self, seq):
         """What the caches hold of a sequence, to be kept elsewhere: a list of (keys, values) [tokens, kv_heads, head_dim], one of each layer
