@@ -397,7 +397,8 @@ int  msnh_b200_w4_linear(MsnhB200Ctx *ctx, const MsnhB200W4 *weights, const Msnh
  * (2i, 2i + 1), i = 0 .. rotary_dim / 2 - 1, and times `magnitude`; the others are copied:
  *   y_a = magnitude * (x_a cos t - x_b sin t), y_b = magnitude * (x_a sin t + x_b cos t), t = 2 pi * position * turns[i] / 2^64
  * turns[i] is the plane's frequency in whole turns a position, as a 64-bit fraction (negative: the other way round). Positions may be
- * negative and as large as their type: angles do not lose precision by them. y may be x with the same strides. */
+ * negative and as large as their type: angles do not lose precision by them. y may be x with the same strides; where rows of it share memory
+ * with one another, or with x otherwise, the call is refused. */
 typedef struct MsnhB200Rotary {
     const void *x;                     /* [tokens][heads][dim]: F32, F16, BF16                     */
     void *y;                           /* same shape and type                                      */

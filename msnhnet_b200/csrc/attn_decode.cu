@@ -18,6 +18,7 @@
 // Blocks in equal parts of a sequence instead of shares by warp had 115, 140 and 35 us; two to eight times as many blocks, taken up as SMs
 // come free, 114 to 144 us for the first: a warp's start costs 3.5 us.
 #include "attn_decode.cuh"
+#include "row_overlap.h"
 
 namespace msnh {
 using namespace attn;
@@ -444,7 +445,9 @@ int msnh_b200_attn_decode(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, const Msnh
     if (const int rc = check_attn(ctx, c, a, "attn_decode")) return rc;
     if (a->rows == 0) return MSNH_B200_OK;
     if (!a->q || !a->out) return fail(ctx, MSNH_B200_ERR_ARG, "attn_decode: null q or out");
-    if (a->q_row_stride < 0 || a->q_head_stride < 0 || (a->n_heads > 1 && a->out_head_stride < c->head_dim) || (a->rows > 1 && a->out_row_stride < c->head_dim))
+    const size_t q_size = dtype_size(c->dtype == MSNH_B200_E4M3 ? a->dtype : c->dtype);
+    const int64_t size = static_cast<int64_t>(q_size);
+    if (a->q_row_stride < 0 || a->q_head_stride < 0 || rows_overlap(Rows(a->rows, a->n_heads, a->out_row_stride * size, a->out_head_stride * size, c->head_dim * size)))
         return fail(ctx, MSNH_B200_ERR_ARG, "attn_decode: a stride of q is negative, or rows of out overlap");
     const AttnPlan l = plan_of(ctx, *c, *a);
     if (l.bytes && (!a->workspace || a->workspace_bytes < l.bytes || !aligned16(a->workspace)))
@@ -456,7 +459,6 @@ int msnh_b200_attn_decode(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, const Msnh
                     a->out_row_stride, a->out_head_stride, 0, a->n_heads, l.each, l.chunk, l.chunks, a->window, 0, l.whole, c->dtype == MSNH_B200_E4M3 ? kCodeStart : kStart,
                     c->dtype == MSNH_B200_E4M3 ? kCodeSmallest : kSmallest, a->scale,
                     reinterpret_cast<int *>(work), reinterpret_cast<float2 *>(work + l.ml_at), reinterpret_cast<float *>(work + l.part_at)};
-    const size_t q_size = dtype_size(c->dtype == MSNH_B200_E4M3 ? a->dtype : c->dtype);
     p.wide_q = reinterpret_cast<uintptr_t>(a->q) % (4 * q_size) == 0 && a->q_row_stride % 4 == 0 && a->q_head_stride % 4 == 0;
     for (int row = 0; row < a->rows; row += l.rows) {
         p.first_row = row;

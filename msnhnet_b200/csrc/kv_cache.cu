@@ -14,6 +14,7 @@
 // bytes, read and written once: prompts of 26200 bf16 tokens, 8 heads of 128 (161 MB) are written in 42 us (31 the codes' launch by itself, 5.2 TB/s; the deciding block
 // is most of the rest) and read in 31.5 (5.1 TB/s).
 #include "kv_cache.h"
+#include "row_overlap.h"
 #include "token_types.cuh"
 
 namespace msnh {
@@ -905,7 +906,9 @@ int msnh_b200_kv_read(MsnhB200Ctx *ctx, const MsnhB200KvCache *c, const int32_t 
     if (!seqs && n > c->n_seqs) return fail(ctx, MSNH_B200_ERR_ARG, "kv_read: %d sequences of %d", n, c->n_seqs);
     if (n_rows == 0) return MSNH_B200_OK;
     if (!k_out || !v_out || (n && !starts)) return fail(ctx, MSNH_B200_ERR_ARG, "kv_read: null k_out, v_out or starts");
-    if ((n_rows > 1 && out_token_stride < c->head_dim) || (c->n_kv_heads > 1 && out_head_stride < c->head_dim)) return fail(ctx, MSNH_B200_ERR_ARG, "kv_read: rows of the output overlap");
+    const int64_t out_size = static_cast<int64_t>(dtype_size(out_dtype));
+    const Rows rows(n_rows, c->n_kv_heads, out_token_stride * out_size, out_head_stride * out_size, c->head_dim * out_size);
+    if (rows_overlap(rows) || rows_meet(k_out, rows, v_out, rows)) return fail(ctx, MSNH_B200_ERR_ARG, "kv_read: rows of the output overlap");
     DeviceScope scope(ctx->device);
     CUDA_TRY(ctx, scope.status);
     const KvParams p = kv_params(*c);

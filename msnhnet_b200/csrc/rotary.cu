@@ -9,6 +9,7 @@
 // (into shared memory, while its first values are on their way) and turns all heads by them, two vectors of 16 bytes at a time. 4100 bf16 tokens of 40
 // heads of 128 (84 MB) take 16.3 us, 5.1 TB/s; one token a launch (1.9 us in a graph, 3.9 between calls). With four pairs of vectors on their way and
 // divisions instead of multiplications: 21.3 us, two blocks an SM.
+#include "row_overlap.h"
 #include "token_ops.h"
 #include "token_types.cuh"
 
@@ -143,8 +144,12 @@ extern "C" int msnh_b200_rotary(MsnhB200Ctx *ctx, const MsnhB200Rotary *a, void 
         return fail(ctx, MSNH_B200_ERR_UNSUPPORTED, "rotary: more than %d turned values of a head, or 2^27 values of a token", 2 * kTable);
     if (a->tokens == 0 || a->heads == 0) return MSNH_B200_OK;
     if (!a->x || !a->y || !a->positions || !a->turns) return fail(ctx, MSNH_B200_ERR_ARG, "rotary: null x, y, positions or turns");
-    if (a->x_token_stride < 0 || a->x_head_stride < 0 || (a->tokens > 1 && a->y_token_stride < a->dim) || (a->heads > 1 && a->y_head_stride < a->dim))
-        return fail(ctx, MSNH_B200_ERR_ARG, "rotary: a stride of x is negative, or rows of y overlap");
+    if (a->x_token_stride < 0 || a->x_head_stride < 0) return fail(ctx, MSNH_B200_ERR_ARG, "rotary: a stride of x is negative");
+    const int64_t size = dtype_size(a->dtype);
+    const Rows from(a->tokens, a->heads, a->x_token_stride * size, a->x_head_stride * size, a->dim * size), to(a->tokens, a->heads, a->y_token_stride * size, a->y_head_stride * size, a->dim * size);
+    if (rows_overlap(to)) return fail(ctx, MSNH_B200_ERR_ARG, "rotary: rows of y overlap");
+    const bool in_place = a->x == a->y && from.n_step == to.n_step && from.m_step == to.m_step;
+    if (!in_place && rows_meet(a->x, from, a->y, to)) return fail(ctx, MSNH_B200_ERR_ARG, "rotary: rows of x and y overlap, and y is not x");
     DeviceScope scope(ctx->device);
     CUDA_TRY(ctx, scope.status);
     RotaryParams p = {static_cast<const uint8_t *>(a->x), static_cast<uint8_t *>(a->y), a->positions, reinterpret_cast<const unsigned long long *>(a->turns), a->tokens,
