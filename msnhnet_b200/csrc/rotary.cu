@@ -2,8 +2,8 @@
 // position times the plane's frequency; the values behind them are kept.
 //
 // The angle is position * frequency without the whole turns. Frequencies are given in turns, as 64-bit fractions, so the product modulo
-// 2^64 is the exact fraction of a turn for any position: what is left of an angle's error is the frequency's own 2^-64 times the position,
-// and the 2^-25 of a turn's half that the fraction is rounded to in fp32.
+// 2^64 is the exact fraction of a turn for any position: what is left of an angle's error is the frequency's own 2^-65 of a turn times the
+// position, and the fraction's rounding to fp32, 2^-24 of an angle of up to half a turn.
 //
 // Every value is read and written once, and those bytes bound it. A block has some tokens' planes: it makes their sines and cosines once
 // (into shared memory, while its first values are on their way) and turns all heads by them, two vectors of 16 bytes at a time. 4100 bf16 tokens of 40
@@ -73,8 +73,8 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const __grid_consta
                 const long long position = p.wide_positions ? static_cast<const long long *>(p.positions)[token] : static_cast<const int *>(p.positions)[token];
                 const unsigned long long turned = static_cast<unsigned long long>(position) * p.turns[i % p.half];
                 float s, c;
-                // (the upper half as a signed number: from -1/2 to 1/2 of a turn, in units of 2^-32)
-                sincospif(static_cast<float>(static_cast<int>(turned >> 32)) * 4.656612873077393e-10f, &s, &c);
+                // (a signed number of half turns, from -1 to 1, in units of 2^-63: rounded once, so small angles keep 24 bits, too)
+                sincospif(static_cast<float>(static_cast<long long>(turned)) * 1.0842021724855044e-19f, &s, &c);
                 cosine[i] = c * p.magnitude;
                 sine[i] = s * p.magnitude;
             }
