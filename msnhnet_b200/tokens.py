@@ -16,6 +16,7 @@ none, and their results would be cut off unnoticed. What the library refuses rai
 (host/tokens_torch.cpp): in Python they took longer than the kernels of one token.
 """
 import ctypes as C
+import decimal
 import math
 
 import torch
@@ -27,6 +28,8 @@ from . import _tokens  # noqa: E402  (needs torch's and the kernel library's sym
 
 _DTYPE = {torch.float32: _ffi.F32, torch.float16: _ffi.F16, torch.bfloat16: _ffi.BF16, torch.float8_e4m3fn: _ffi.E4M3}
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+# (rotary tables: a fraction of 64 bits takes more than a float's 53)
+_TWO_PI = decimal.Decimal("6.28318530717958647692528676655900576839433879875021164194989")
 
 
 def _no_gradient(*tensors):
@@ -46,7 +49,7 @@ class W4Weights:
 
 class RotaryTable:
     """What TokenOps.rotary turns by (TokenOps.rotary_table): `turns`, the whole turns a position of each plane as 64-bit fractions (int64 on the
-    GPU), whether planes are interleaved, and the factor of what is turned."""
+    GPU; the nearest ones: off by 2^-65 of a turn, times the position for an angle), whether planes are interleaved, and the factor of what is turned."""
 
     def __init__(self, turns, interleaved, magnitude):
         self.turns, self.interleaved, self.magnitude = turns, interleaved, magnitude
@@ -172,18 +175,25 @@ class TokenOps:
             raise ValueError(f"rotary_table: dim {dim} (even, 2 at least), base {base}, factor {factor}, {low} to {high} turns of {trained} positions")
         if stretch not in (None, "all", "base", "slow"):
             raise ValueError(f"stretch {stretch!r}: None, 'all', 'base' or 'slow'")
-        if stretch == "base":
-            base = base * factor ** (dim / max(dim - 2, 1))
         turns = []
-        for i in range(dim // 2):
-            turn = base ** (-2 * i / dim) / (2 * math.pi)
-            if stretch == "all":
-                turn /= factor
-            elif stretch == "slow":
-                kept = min(max((trained * turn - low) / (high - low), 0.0), 1.0)
-                turn *= kept + (1 - kept) / factor
-            fraction = int(turn * 2.0 ** 64) % 2 ** 64
-            turns.append(fraction - 2 ** 64 if fraction >= 2 ** 63 else fraction)
+        # (without traps: infinite bases and factors are what they are in floats)
+        with decimal.localcontext(decimal.Context(prec=60, traps=[])) as numbers:
+            base, factor, trained, low, high, dim = (decimal.Decimal(float(v)) for v in (base, factor, trained, low, high, dim))
+            if stretch == "base":
+                base = base * factor ** (dim / max(dim - 2, 1))
+            # bases and factors below 1 give whole turns, whose digits come in front of the fraction's
+            numbers.prec += max(-base.adjusted(), 0) + max(-factor.adjusted(), 0)
+            ratio, plane = base ** (-2 / dim), 1 / _TWO_PI
+            for _ in range(int(dim) // 2):
+                turn = plane
+                plane *= ratio
+                if stretch == "all":
+                    turn /= factor
+                elif stretch == "slow":
+                    kept = min(max((trained * turn - low) / (high - low), 0), 1)
+                    turn *= kept + (1 - kept) / factor
+                fraction = int((turn % 1 * 2 ** 64).to_integral_value()) % 2 ** 64
+                turns.append(fraction - 2 ** 64 if fraction >= 2 ** 63 else fraction)
         return RotaryTable(torch.tensor(turns, dtype=torch.int64, device=self.device), bool(interleaved), float(magnitude))
 
     def rotary(self, x, positions, table, out=None):
