@@ -68,7 +68,7 @@ template <int kDim, int kStages> struct CodeRing {
     __device__ __forceinline__ void look_ahead(int first_tile, int tiles) {
         next = -1;
         const int token = origin + first_tile * kTile + lane * 8;
-        if (first_tile + lane / kRuns < tiles && c.page_size % 8 == 0 && token >= first && token + 8 <= last && c.k_token < 1 << 27 && c.v_token < 1 << 27) {
+        if (first_tile + lane / kRuns < tiles && c.page_size % 8 == 0 && token >= first && token <= last - 8 && c.k_token < 1 << 27 && c.v_token < 1 << 27) {
             next = table[token / c.page_size];
             if (next >= c.n_pages) next = -1;
         }

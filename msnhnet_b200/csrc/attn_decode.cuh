@@ -114,9 +114,10 @@ template <typename T, int kDim, int kStages> struct Ring {
         else issue_any(stage, origin + tile * kTile);
     }
 
-    // The page of a run of eight tokens that are all seen, in a cache whose pages are multiples of eight; -1 otherwise.
+    // The page of a run of eight tokens that are all seen, in a cache whose pages are multiples of eight; -1 otherwise. (Tokens go to
+    // 2^31 - 1: sums behind the last one would pass it.)
     __device__ __forceinline__ int page_of(int token) const {
-        if (c.page_size % 8 || token < first || token + 8 > last) return -1;
+        if (c.page_size % 8 || token < first || token > last - 8) return -1;
         const int page = table[token / c.page_size];
         return page < c.n_pages ? page : -1;
     }
