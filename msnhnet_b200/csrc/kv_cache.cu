@@ -332,8 +332,10 @@ __global__ void __launch_bounds__(kColumns, 512 / kColumns) kv_append_codes_kern
     pdl_enter();
     const int lane = threadIdx.x % 32, vecs = c.dim / kVec, mine = threadIdx.x / vecs, column = threadIdx.x - mine * vecs;
     BlockOfScales next = block_of_scales(c, seqs, starts, n, work, groups.quotient(blockIdx.x), lane, by);
-    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+    // (counted without a sign: items go up to 2^31 - 2, and what is behind the last one has to be behind it still)
+    for (uint32_t turn = blockIdx.x; turn < static_cast<uint32_t>(items); turn += gridDim.x) {
         const BlockOfScales b = next;
+        const int item = static_cast<int>(turn);
         const int unit = groups.quotient(item), both = (item - unit * static_cast<int>(groups.by)) * heads_of_block + mine;      // a head of the keys, then of the values
         const bool active = mine < heads_of_block && both < 2 * c.heads, values = both >= c.heads;
         const int head = values ? both - c.heads : both;
@@ -349,7 +351,7 @@ __global__ void __launch_bounds__(kColumns, 512 / kColumns) kv_append_codes_kern
         for (int t = 0; t < kHeld; ++t)
             if (t < count) held[t].load(source + t * token_stride);
         // (where the next one is, is looked up while these are on their way)
-        if (item + static_cast<int>(gridDim.x) < items) next = block_of_scales(c, seqs, starts, n, work, groups.quotient(item + gridDim.x), lane, by);
+        if (turn + gridDim.x < static_cast<uint32_t>(items)) next = block_of_scales(c, seqs, starts, n, work, groups.quotient(static_cast<int>(turn + gridDim.x)), lane, by);
         if (!b.there) continue;
         uint32_t top = 0;
 #pragma unroll
