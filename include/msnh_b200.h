@@ -490,7 +490,7 @@ int  msnh_b200_attn_decode(MsnhB200Ctx *ctx, const MsnhB200KvCache *cache, const
  *            order) of k_out / v_out, as out_dtype (F32, F16, BF16); rows of no sequence, no token or a hole are 0. All n_rows rows are
  *            written. It changes nothing of the cache.
  * append_as takes k_new and v_new as new_dtype, which is the cache's type or, in a cache of E4M3, F32, F16 or BF16. There a block's scale is
- * the smallest power of two by which the call's values of it are at most 448, or the one it has where that is larger; older codes of a block whose scale
+ * the smallest power of two by which the call's values of it are at most 448, or the one it has where that is larger in magnitude; older codes of a block whose scale
  * grows are rounded again, to the new one (which loses nothing but of codes that become less than 2^-6). A NaN or infinity is the code NaN
  * and does not count for the scale. A block of zeros has scale 0. */
 int  msnh_b200_kv_workspace(MsnhB200Ctx *ctx, const MsnhB200KvCache *cache, int n, size_t *bytes);

@@ -266,6 +266,8 @@ __device__ __forceinline__ float scale_of(uint32_t top) {
     const int exponent = static_cast<int>((top + 0x1fffffu) >> 23) - 8;      // (biased; mantissas above 1.75 carry)
     return __uint_as_float(static_cast<uint32_t>(max(exponent, 1)) << 23);
 }
+// A block's scale from the one it has (the caller's own may be negative: it is as good as its magnitude) and the least one that its new values take.
+__device__ __forceinline__ float larger_scale(float had, float least) { return fabsf(had) >= least ? had : least; }
 // Whether x / scale is x times the scale's reciprocal, exactly.
 __device__ __forceinline__ bool is_power(float scale) {
     const uint32_t bits = __float_as_uint(scale);
@@ -389,7 +391,7 @@ __global__ void __launch_bounds__(kColumns, 512 / kColumns) kv_append_codes_kern
             finite = over_head(finite);
             if (odd) top = finite;
         }
-        const float scale = fmaxf(had, scale_of(top));
+        const float scale = larger_scale(had, scale_of(top));
         const bool power = is_power(scale);
         const float inverse = power ? 1.f / scale : 0.f;
         if (active && b.older && scale != had) {
@@ -453,7 +455,7 @@ __global__ void __launch_bounds__(256) kv_append_values_kernel(KvParams c, const
                 const uint32_t bits = __float_as_uint(to_float(source[t * token_stride + d])) & 0x7fffffffu;
                 if (bits < 0x7f800000u) top = max(top, bits);
             }
-        const float scale = fmaxf(had, scale_of(__reduce_max_sync(~0u, top)));
+        const float scale = larger_scale(had, scale_of(__reduce_max_sync(~0u, top)));
         for (int t = -b.older; t < b.count; ++t)
             for (int d = lane; d < c.dim; d += 32) {
                 uint8_t &code = codes[t * token_step + d];
