@@ -192,31 +192,25 @@ template <typename At> __device__ __forceinline__ int last_not_above(int n, int 
     return low;
 }
 
+// (four values or eight: what 16 bytes of the new ones hold)
 template <int kVec> __device__ __forceinline__ void store_codes(uint8_t *to, const float (&x)[kVec]) {
-    if constexpr (kVec == 1) {
-        to[0] = static_cast<uint8_t>(to_e4m3x2(x[0], 0.f));
-    } else {
-        uint32_t words[kVec / 4];
+    uint32_t words[kVec / 4];
 #pragma unroll
-        for (int i = 0; i < kVec / 4; ++i) words[i] = to_e4m3x2(x[4 * i], x[4 * i + 1]) | static_cast<uint32_t>(to_e4m3x2(x[4 * i + 2], x[4 * i + 3])) << 16;
-        if constexpr (kVec == 8) *reinterpret_cast<uint2 *>(to) = make_uint2(words[0], words[1]);
-        else *reinterpret_cast<uint32_t *>(to) = words[0];
-    }
+    for (int i = 0; i < kVec / 4; ++i) words[i] = to_e4m3x2(x[4 * i], x[4 * i + 1]) | static_cast<uint32_t>(to_e4m3x2(x[4 * i + 2], x[4 * i + 3])) << 16;
+    if constexpr (kVec == 8) *reinterpret_cast<uint2 *>(to) = make_uint2(words[0], words[1]);
+    else *reinterpret_cast<uint32_t *>(to) = words[0];
 }
-// kVec values side by side
+// kVec values side by side, 16 bytes of them
 template <typename T, int kVec> struct Piece {
     alignas(16) T v[kVec];
     __device__ __forceinline__ void load(const T *from) {
-        if constexpr (kVec > 1) *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(from);
-        else v[0] = from[0];
+        *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(from);
     }
     // The larger one of `before` and the magnitudes' bits; 16-bit values in two halves, which last() joins.
     __device__ __forceinline__ uint32_t top(uint32_t before) const {
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
             for (int i = 0; i < kVec; ++i) before = max(before, __float_as_uint(v[i]) & 0x7fffffffu);
-        } else if constexpr (kVec == 1) {
-            before = max(before, reinterpret_cast<const uint16_t *>(v)[0] & 0x7fffu);
         } else {
 #pragma unroll
             for (int i = 0; i < kVec / 2; ++i) before = __vmaxu2(before, reinterpret_cast<const uint32_t *>(v)[i] & 0x7fff7fffu);
@@ -249,8 +243,7 @@ template <int kVec> struct Codes {
     alignas(8) __nv_fp8_e4m3 v[kVec];
     __device__ __forceinline__ void load(const uint8_t *from) {
         if constexpr (kVec == 8) *reinterpret_cast<uint2 *>(v) = *reinterpret_cast<const uint2 *>(from);
-        else if constexpr (kVec == 4) *reinterpret_cast<uint32_t *>(v) = *reinterpret_cast<const uint32_t *>(from);
-        else v[0].__x = *from;
+        else *reinterpret_cast<uint32_t *>(v) = *reinterpret_cast<const uint32_t *>(from);
     }
     template <typename Code> __device__ __forceinline__ void store(uint8_t *to, Code code) const {
         float x[kVec];
