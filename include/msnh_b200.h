@@ -456,7 +456,7 @@ typedef struct MsnhB200KvCache {
  * Statistics and sums are fp32. Table entries outside [0, n_pages) are holes: their tokens are left out. Where no token is
  * left, out is 0 and lse -infinity. head_dim: a multiple of 16 bytes, at most 256 values; the pages' rows 16-byte aligned.
  * q and out have the cache's type; over a cache of E4M3 they have `dtype`, and a key or value is code times scale in the sums, with
- * nothing rounded in between (queries of F32 and BF16 to 2^-24, and to 2^-39 of the largest in their head). There a weight times its
+ * nothing rounded in between (queries of F32 to 2^-23, and of F32 and BF16 to 2^-39 of the largest in their head or 2^-151). There a weight times its
  * value's scale is taken to 2^-22 and the sums are the tensor cores' fp32: an F32 result holds to about 1e-6 of its values' size. */
 typedef struct MsnhB200AttnDecode {
     const void *q;                     /* [rows][n_heads][head_dim]                                */

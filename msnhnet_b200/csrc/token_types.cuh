@@ -15,7 +15,8 @@ __device__ __forceinline__ void pdl_enter() {
     pdl_launch_dependents();
 }
 
-// Division of numbers below 2^31 by a number that the launch knows: (high half of n * factor + n) >> shift.
+// Division of numbers below 2^31 by a number that the launch knows: (high half of n * factor + n) >> shift (Granlund and Montgomery, Division by
+// Invariant Integers using Multiplication, 1994).
 struct Divisor {
     uint32_t by, factor;
     int shift;

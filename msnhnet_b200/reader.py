@@ -223,7 +223,9 @@ class Reader:
         return [self.ops.kv_read(cache, starts, n, seqs=one, dtype=kept) for cache in self.caches]
 
     def restore(self, seq, saved):
-        """Makes the empty sequence `seq` what save gave (of this reader or one of the same shape; on any device)."""
+        """Makes the empty sequence `seq` what save gave (of this reader or one of the same shape; on any device). Keys and values are the same ones; in an
+        8-bit cache a last block that is not full may have half the scale it had, where its largest value was rounded down to 224 of it, and tokens that
+        follow are then rounded by that."""
         if not 0 <= seq < self.n_seqs or len(saved) != self.layers:
             raise ValueError(f"{len(saved)} layers for sequence {seq}: {self.layers} layers, {self.n_seqs} sequences")
         n = saved[0][0].shape[0]
