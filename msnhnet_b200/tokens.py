@@ -177,13 +177,13 @@ class TokenOps:
             raise ValueError(f"stretch {stretch!r}: None, 'all', 'base' or 'slow'")
         turns = []
         # (without traps: infinite bases and factors are what they are in floats)
-        with decimal.localcontext(decimal.Context(prec=60, traps=[])) as numbers:
+        with decimal.localcontext(decimal.Context(prec=40, traps=[])) as numbers:
             base, factor, trained, low, high, dim = (decimal.Decimal(float(v)) for v in (base, factor, trained, low, high, dim))
             if stretch == "base":
                 base = base * factor ** (dim / max(dim - 2, 1))
             # bases and factors below 1 give whole turns, whose digits come in front of the fraction's
             numbers.prec += max(-base.adjusted(), 0) + max(-factor.adjusted(), 0)
-            ratio, plane = base ** (-2 / dim), 1 / _TWO_PI
+            ratio, plane = (base.ln() * -2 / dim).exp(), 1 / _TWO_PI
             for _ in range(int(dim) // 2):
                 turn = plane
                 plane *= ratio
@@ -192,8 +192,7 @@ class TokenOps:
                 elif stretch == "slow":
                     kept = min(max((trained * turn - low) / (high - low), 0), 1)
                     turn *= kept + (1 - kept) / factor
-                fraction = int((turn % 1 * 2 ** 64).to_integral_value()) % 2 ** 64
-                turns.append(fraction - 2 ** 64 if fraction >= 2 ** 63 else fraction)
+                turns.append((int((turn * 2 ** 64).to_integral_value()) + 2 ** 63) % 2 ** 64 - 2 ** 63)
         return RotaryTable(torch.tensor(turns, dtype=torch.int64, device=self.device), bool(interleaved), float(magnitude))
 
     def rotary(self, x, positions, table, out=None):
