@@ -10,9 +10,10 @@
 // bits) relative to the largest factor, whatever the scales are. The sum of weights is fp32 and knows nothing of the scales. Both references
 // are whole numbers, the largest exponent rounded up: what has been summed is then rescaled by powers of two, exactly, and seldom.
 //
-// Measured, both launches, 32 heads over 8 of 128: two fp16 rows of up to 131072 tokens (270 MB) 60.7 us, 4.4 TB/s; 48 bf16 rows of up to 8192 (99 MB)
-// 31.8; one of 37 in a short table 7.3. Copying alone takes 57 of the first (the joining launch is 7), computing alone 46: three warps a scheduler, each
-// waiting five cycles for an instruction, hide most of one behind the other. Tiles of 16 tokens, as in 16 bits, had 83 and 49 us; two blocks an SM with three tiles
+// Measured in graphs over three sets of inputs, both launches, 32 heads over 8 of 128: two fp16 rows of up to 131072 tokens (270 MB) 61.6 us, 4.4 TB/s; 48 bf16
+// rows of up to 8192 (99 MB) 31.3; one of 37 in a short table 7.3 (from Python 62, 32 and 7.6). With the copies alone the first two take 58 and 29, with the
+// arithmetic alone 45 and 27 (the joining launch, about 7, is in all of them): three warps a scheduler, each waiting five cycles for an instruction, hide most of
+// one behind the other. Tiles of 16 tokens, as in 16 bits, had 83 and 49 us; two blocks an SM with three tiles
 // on their way 67.2 and 39.4; rows asked for a tile earlier (to L2) 66.4. Lengths that are multiples of a share, so that the heads of a token are read at
 // the same time, are 7 % faster: DRAM's share of it.
 #include "attn_decode.cuh"

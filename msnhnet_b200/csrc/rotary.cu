@@ -7,8 +7,8 @@
 //
 // Every value is read and written once, and those bytes bound it. A block has some tokens' planes: it makes their sines and cosines once
 // (into shared memory, while its first values are on their way) and turns all heads by them, two vectors of 16 bytes at a time. 4100 bf16 tokens of 40
-// heads of 128 (84 MB) take 16.3 us, 5.1 TB/s; one token a launch (1.9 us in a graph, 3.9 between calls). With four pairs of vectors on their way and
-// divisions instead of multiplications: 21.3 us, two blocks an SM.
+// heads of 128 (84 MB) take 18.0 us with inputs that no cache holds (4.7 TB/s), 16.1 in a graph over three sets of them in turn; one token is bound by its
+// launch (1.8 us in a graph, 3.7 between calls). With four pairs of vectors on their way and divisions instead of multiplications: 21.3 us, two blocks an SM.
 #include "row_overlap.h"
 #include "token_ops.h"
 #include "token_types.cuh"

@@ -420,7 +420,7 @@ cudaError_t launch(const MsnhB200Ctx *ctx, const ScoreParams &p, void *stream) {
 }
 
 // Blocks of a row: as many as leave every SM two, each with 4096 logits at least, of 256 threads (clusters of 512 find less room: 16 rows of 50000 bf16 logits took
-// 17.4 us and not 9.8; now 8.0, three of 128000 fp16 ones 8.3, 120 of 128000 14.3). A row that is one block's has 128 threads, since what follows the pass over
+// 17.4 us and not 9.8; now 8.0, three of 128000 fp16 ones 8.3, 120 of 128000 16.2 with the best 8 and 12.7 without them). A row that is one block's has 128 threads, since what follows the pass over
 // the logits grows with the warps, and seven such blocks an SM have registers for the next chunks (2000 rows of 50000: 51 us; a microsecond more with eight, 18 more
 // with nine). Narrow rows are one warp's each, without other warps' lists to join, where there are more than the SMs hold at 128 threads a row, and always where a
 // warp has a row in one chunk a lane: 4000 bf16 rows of 1000 with the best 5 8.5 us instead of 20.9, 1200 of 4000 9.4 instead of 12.9, 20000 of 500 32.0 instead of 95.6. A
