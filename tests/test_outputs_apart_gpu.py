@@ -134,3 +134,12 @@ def test_attention_into_any_layout(ops, kind, strides, apart):
     else:
         with pytest.raises(_ffi.KernelError, match="overlap"):
             ops.attn_decode(q, cache, out=out)
+
+
+def test_outputs_that_are_given_are_what_comes_back(ops):
+    x, positions, table = randn(3, 2, D, seed=11), ints(3, 4, 5), ops.rotary_table(D)
+    want = ops.rotary(x, positions, table)
+    out = torch.zeros_like(x)
+    for given in (out, x):                                            # beside the input, then in its place
+        got = ops.rotary(x, positions, table, out=given)
+        assert got.data_ptr() == given.data_ptr() and got.stride() == given.stride() and torch.equal(got, want)
